@@ -12,14 +12,17 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfp4gemm.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
-SOURCES = ["capi.cu", "quantize.cu", "quantize_units.cu", "gemm_sm100.cu", "noalloc.cu", "selftest.cu", "peak.cu", "peer_barrier.cu"]
-HEADERS = ["fp4b_internal.h", "nvfp4_codec.cuh", "ptx_sm100.cuh", "quantize_core.cuh"]
+SOURCES = ["capi.cu", "quantize.cu", "quantize_units.cu", "gemm_sm100.cu", "noalloc.cu", "selftest.cu", "peak.cu", "peer_barrier.cu",
+           "kv_cache.cu", "decode_attention.cu", "gemv.cu"]
+HEADERS = ["decode_core.cuh", "fp4b_internal.h", "nvfp4_codec.cuh", "ptx_sm100.cuh", "quantize_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -48,12 +51,22 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
     if not force and up_to_date():
         return LIB
+    # One nvcc per source, as many at a time as there are cores, then the link.
+    cc = nvcc()
     tmp = LIB + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), f"-I{CSRC}", f"-I{INCLUDE}",
-           *[os.path.join(CSRC, f) for f in SOURCES], "-o", tmp]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    with tempfile.TemporaryDirectory(prefix="fp4b_build_") as work:
+        def compile_one(name: str) -> str:
+            obj = os.path.join(work, name + ".o")
+            cmd = [cc, *[f for f in NVCC_FLAGS if f != "-shared"], *(extra or []), f"-I{CSRC}", f"-I{INCLUDE}",
+                   "-c", os.path.join(CSRC, name), "-o", obj]
+            if verbose:
+                print(" ".join(cmd))
+            subprocess.check_call(cmd)
+            return obj
+
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            objs = list(pool.map(compile_one, SOURCES))
+        subprocess.check_call([cc, *NVCC_FLAGS, *objs, "-o", tmp])
     os.replace(tmp, LIB)
     return LIB
 

@@ -1,0 +1,129 @@
+// decode_core.cuh -- device code shared by the decode-side operators: the
+// paged key-value cache's formats, warp reductions, the error word.
+//
+// Cache layout (fp4b_kv_cache in fp4gemm.h): pages [num_pages, kv_heads,
+// page_size, head_dim], so that the keys of one head in one page are one
+// contiguous run.  A "row" is one (page, head, slot): head_dim elements, with
+//   bf16   2 * D bytes;
+//   fp8    D bytes of E4M3 and one fp32 scale;
+//   nvfp4  D / 2 bytes of E2M1 (even element in the low nibble) and D / 16
+//          UE4M3 scale bytes, the codec of the weight quantizer.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "fp4gemm.h"
+#include "nvfp4_codec.cuh"
+
+namespace fp4b {
+
+enum KvKind : int { kKvBf16 = FP4B_KV_BF16, kKvFp8 = FP4B_KV_FP8, kKvNvfp4 = FP4B_KV_NVFP4, kKvNone = -1 };
+
+// Codes in the device error word (fp4b_device_error) of indices that the
+// kernels found out of range; the access is left out.
+constexpr int kErrSlotRange = 11;
+constexpr int kErrPositionRange = 12;
+constexpr int kErrPageRange = 13;
+
+// |x|max below which a block takes the arithmetic rounding; larger, infinite
+// and NaN blocks take the codec's literal scan (as in the weight quantizer).
+constexpr uint32_t kFastAbsmaxF32Limit = kFastAbsmaxBf16Limit << 16;
+
+constexpr float kFp8Max = 448.0f;
+// Smallest absmax an fp8 row's scale stands for (2^-100): 448 / absmax and
+// absmax / 448 both stay normal, and a row of zeros needs no case of its own.
+constexpr float kFp8AbsmaxFloor = 7.888609052210118e-31f;
+
+namespace decode {
+
+__device__ __forceinline__ void report(int* err, int code) {
+    if (err) atomicCAS(err, 0, code);
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Two E2M1 codes (one byte) -> two fp16 values, exact.
+__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
+    uint32_t r;
+    asm("{\n.reg .b8 b;\ncvt.u8.u32 b, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(r) : "r"(byte));
+    return r;
+}
+
+// Two E4M3 codes -> two fp16 values, exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t two) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
+    return r;
+}
+
+__device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) { return __half22float2(*reinterpret_cast<__half2*>(&h)); }
+
+// One scaled value -> the fp32 stand-in whose hardware conversion to E2M1
+// (nearest even) equals the codec's rule (ties to the lower magnitude, sign
+// only below zero): the odd-bit float at or one ulp below its magnitude.  v
+// must be finite.
+__device__ __forceinline__ float e2m1_stand_in(float v) {
+    const uint32_t a = __float_as_uint(v) & 0x7FFFFFFFu;
+    const uint32_t m = (a - (a != 0u ? 1u : 0u)) | 1u;
+    return __uint_as_float(m | (v < 0.0f ? 0x80000000u : 0u));
+}
+
+// Four scaled values -> four E2M1 codes, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x4(float a, float b, float c, float d) {
+    uint16_t r;
+    asm("{\n"
+        ".reg .b8 b0, b1;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+        "mov.b16 %0, {b0, b1};\n"
+        "}"
+        : "=h"(r)
+        : "f"(e2m1_stand_in(a)), "f"(e2m1_stand_in(b)), "f"(e2m1_stand_in(c)), "f"(e2m1_stand_in(d)));
+    return r;
+}
+
+// Four fp32 values -> four E4M3 codes (nearest even, saturating).
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(lo) : "f"(a), "f"(b));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+template <int WIDTH>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <int WIDTH>
+__device__ __forceinline__ uint32_t group_umax(uint32_t v) {
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// UE4M3 byte -> fp32; the fp16 form is exact too (at most 480, at least 2^-9).
+__device__ __forceinline__ float ue4m3_float(uint32_t byte) { return ue4m3_decode((uint8_t)byte); }
+
+// Index `i` of an int32 or int64 array.
+__device__ __forceinline__ long load_index(const void* p, long i, int is64) {
+    return is64 ? (long)static_cast<const int64_t*>(p)[i] : (long)static_cast<const int32_t*>(p)[i];
+}
+
+}  // namespace decode
+
+// Host side: why a cache description cannot be used (nullptr if it can).
+const char* kv_cache_check(const fp4b_kv_cache* c);
+
+}  // namespace fp4b

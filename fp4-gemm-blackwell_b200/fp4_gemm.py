@@ -9,6 +9,7 @@ Same public names, argument meaning, return values and errors:
     FP4WeightCache(weight, bias=None)             quantize once, .forward(x, sync=True)
     fp4_quantize(weight, bias=None)               -> FP4WeightCache
     fp4_cached_matmul(A, cache), fp4_cached_linear(x, cache)
+    fp4_cached_gemv(x, cache)                     F.linear for few rows, BF16 activations as they are (additive)
     sync(), prealloc(max_M, max_N, max_K), cleanup(), SF_VEC_SIZE
 
 The work runs in ``libfp4gemm.so`` (beside this file, loaded through ctypes with
@@ -84,6 +85,7 @@ _bind("fp4b_ipc_close", _i, [_vp, ctypes.c_long])
 _bind("fp4b_mma_rate", _i, [_i, _i, _i, _i, _i, ctypes.POINTER(_i), _vp])
 _bind("fp4b_peer_barrier", _i, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_i), _i, _i, ctypes.c_ulonglong, _vp])
 _bind("fp4b_copy2d", _i, [_vp, ctypes.c_long, _vp, ctypes.c_long, ctypes.c_long, ctypes.c_long, _vp])
+_bind("fp4b_gemv_cached", _i, [_vp, _i, _i, ctypes.c_long, _vp, _i, _vp, ctypes.c_long, _vp, _vp])
 
 # Query scale factor vector size
 SF_VEC_SIZE = _lib.fp4_gemm_sf_vec_size()
@@ -559,6 +561,42 @@ def fp4_cached_linear(
     """F.linear(x, W, bias) with W (and its bias) stored in `cache`; x is [..., K],
     the result [..., N]."""
     return cache.forward(x)
+
+
+def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
+    """
+    F.linear(x, W, bias) for few rows, with the activations left in BF16: x [..., K] is multiplied as it is with the
+    cached NVFP4 weight, summed in fp32 and rounded once, after a BF16 bias of the cache was added (any other bias is
+    added to the BF16 result, which it promotes as in forward).  Returns [..., N]; queued on the current stream, nothing
+    synchronises.
+
+    For decoding: up to about 16 rows the time is that of reading the weight once.  It takes any number of rows, but
+    reads the weight again for every 16; forward() is the form for many rows (and quantizes the activations).
+    """
+    if cache._handle is None:
+        raise RuntimeError("FP4WeightCache has been freed")
+    k, n = cache.K_orig, cache.N_orig
+    if x.shape[-1] != k:
+        raise ValueError(f"Input K={x.shape[-1]} doesn't match weight K={k}")
+    assert x.is_cuda and cache.device.index in (None, x.device.index), "x must be on the cache's CUDA device"
+    if x.dtype != torch.bfloat16:
+        x = x.to(torch.bfloat16)
+    x_2d, ldx = _rows_view(x.reshape(-1, k))
+    m = x_2d.shape[0]
+    y = torch.empty(*x.shape[:-1], n, dtype=torch.bfloat16, device=x.device)
+    bias = cache.bias
+    fuse_bias = bias is not None and bias.dtype == torch.bfloat16 and bias.is_cuda
+    if m > 0:
+        if fuse_bias:
+            bias = bias.reshape(-1).contiguous()
+            if bias.numel() != n:
+                raise ValueError(f"the cache's bias has {bias.numel()} elements, not {n}")
+        with torch.cuda.device(x.device):
+            rc = _lib.fp4b_gemv_cached(x_2d.data_ptr(), m, k, ldx, cache._handle, n, y.data_ptr(), n,
+                                       bias.data_ptr() if fuse_bias else None, _stream_ptr(x.device))
+        if rc != 0:
+            raise RuntimeError(f"fp4_cached_gemv failed with error code {rc} ({_last_error()})")
+    return y + bias if bias is not None and not fuse_bias else y
 
 
 # ----------------------------------------------------------------------------

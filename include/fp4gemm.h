@@ -257,6 +257,80 @@ int fp4b_ipc_get_handle(const void* ptr, void* handle_out, long* offset_out);
 void* fp4b_ipc_open_handle(const void* handle, long offset);
 int fp4b_ipc_close(void* ptr, long offset);
 
+/* ----------------------------------------------------------------------------
+ * Decode-side operators (no counterpart in the reference): the matrix-vector
+ * product on a weight cache, and what lies between the QKV and the output
+ * linear of a decoder layer.  All asynchronous on `stream`; 0 ok, -1 bad
+ * arguments, -2 a geometry the kernels cannot take, -4 launch failure.  An
+ * index that only the GPU sees (slot, position, page, length) and that is out
+ * of range is left out and recorded in the device error word
+ * (fp4b_device_error): 11 slot, 12 position, 13 page or length.
+ * ------------------------------------------------------------------------- */
+
+/* y[m, n_out] = w_alpha * x @ W^T (+ bias) with x [m, k_in] BF16 as it is (not
+ * quantized), W the cached weight and bias [n_out] BF16 or NULL; fp32 sums, one
+ * rounding to BF16.  Any m >= 1; made for few rows, where the weight's bytes
+ * are the cost. */
+int fp4b_gemv_cached(const void* x_bf16, int m, int k_in, long ldx, const void* cache_handle, int n_out,
+                     void* y_bf16, long ldy, const void* bias_bf16, void* stream);
+
+/* Formats of a paged key-value cache. */
+enum { FP4B_KV_BF16 = 0, FP4B_KV_FP8 = 1, FP4B_KV_NVFP4 = 2 };
+
+/* A paged key-value cache.  Pages are [num_pages, kv_heads, page_size,
+ * head_dim]; the element at (page, head, slot) has `head_dim` BF16 values, or
+ * E4M3 bytes with one fp32 scale in [num_pages, kv_heads, page_size], or packed
+ * E2M1 with head_dim / 16 UE4M3 bytes in [num_pages, kv_heads, page_size,
+ * head_dim / 16].  page_size a power of two up to 1024, head_dim 64, 128 or
+ * 256, pages and scales 16-byte aligned.  A token's slot number is
+ * page * page_size + its place in the page. */
+typedef struct fp4b_kv_cache {
+    void* k;
+    void* v;
+    void* k_scale; /* NULL for BF16 */
+    void* v_scale;
+    int num_pages, kv_heads, page_size, head_dim;
+    int kind;
+} fp4b_kv_cache;
+
+/* Queries [tokens, q_heads, head_dim] and keys [tokens, kv_heads, head_dim]
+ * normed (weights [head_dim] BF16, NULL for none) and rotated (rope: fp32
+ * [rope_rows, rot], rot / 2 cosines then rot / 2 sines of each position; NULL
+ * for none; interleaved: pairs 2i, 2i + 1 instead of i, i + rot / 2), queries
+ * to q_out and keys to k_out, or with `cache` keys and values into the cache
+ * at `slots` (one a token; a negative slot skips the token).  Any of q, v may
+ * be NULL, k too without a cache.  *_st, *_sh: token and head strides in
+ * elements, multiples of 4; rows 8-byte aligned, elements contiguous; outputs
+ * contiguous.  positions and slots are int64 where pos64 / slot64, else int32. */
+int fp4b_kv_rows(const void* q, long q_st, long q_sh, const void* k, long k_st, long k_sh, const void* v, long v_st,
+                 long v_sh, int tokens, int q_heads, int kv_heads, int head_dim, const void* positions, int pos64,
+                 const float* rope, int rope_rows, int rot, int interleaved, const void* q_weight,
+                 const void* k_weight, float eps, void* q_out, void* k_out, const fp4b_kv_cache* cache,
+                 const void* slots, int slot64, void* stream);
+
+/* Keys and values of `count` slots as BF16 [count, kv_heads, head_dim] each;
+ * zeros for a negative slot. */
+int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int slot64, long count, void* k_out, void* v_out,
+                 void* stream);
+
+/* Attention of one new token a sequence: out[b, h] = sum_i p_i v_i with p the
+ * softmax of scale * q[b, h] . k_i over the keys i of [max(0, len - window),
+ * len) (window 0: all), len = seq_lens[b], found through page_table[b] (int32,
+ * row stride table_stride, table_width entries); query head h reads key head
+ * h / (q_heads / kv_heads).  sinks: fp32 [q_heads] or NULL, one more logit in
+ * each head's softmax that no value belongs to.  A sequence without keys gives
+ * zeros.  q: BF16, strides in elements (multiples of 4, rows 8-byte aligned);
+ * out BF16 [batch, q_heads, head_dim] contiguous; lse: fp32 [batch, q_heads],
+ * the log of the softmax's denominator (-inf where it is empty), or NULL.
+ * workspace: fp4b_decode_attention_workspace bytes of device memory, 16-byte
+ * aligned, zeroed before its first use and left zeroed where it has to be;
+ * calls that share it must be ordered. */
+long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int head_dim);
+int fp4b_decode_attention(const void* q, long q_sb, long q_sh, int batch, int q_heads, const fp4b_kv_cache* cache,
+                          const int* page_table, long table_stride, int table_width, const int* seq_lens,
+                          float scale, int window, const float* sinks, void* out, float* lse, void* workspace,
+                          long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
