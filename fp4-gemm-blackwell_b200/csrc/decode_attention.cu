@@ -1,128 +1,792 @@
 // decode_attention.cu -- attention of one new token a sequence over a paged
-// key-value cache.
+// key-value cache, split over the cache's length and joined in one launch.
 //
 //   out[b, h] = sum_i p_i v_i / l,  p_i = exp(scale * q . k_i - m),
-//   l = sum_i p_i (+ exp(sink_h - m)),  m = the running maximum
+//   l = sum_i p_i (+ exp(sink_h - m))
 //
-// over the keys i of [max(0, len - window), len), K and V decoded from the
-// cache's format as they are read.
+// over the keys i of [max(0, len - window), len).  Every cached byte is read
+// once for all query heads of its key head, so the floor is the cache's bytes
+// over the HBM rate; what has to stay below that is the work per key.
+//
+// Products.  Both run on mma.sync m16n8k16 with the keys (then the elements of
+// a value) as the 16 rows and up to 8 query heads as the 8 columns:
+//   S^T[16 keys, 8 heads]     = K[16, D] Q^T[D, 8]
+//   O^T[16 elements, 8 heads] += V^T[16 elements, 16 keys] P^T[16 keys, 8]
+// (tcgen05's 128 rows would need 128 query heads for each key head).  The order
+// of the contracted index is free as long as both operands agree, so a lane
+// reads the 16-byte runs of a row as they lie, and neither K nor V is
+// transposed through shared memory: V^T's register pairs, two keys of one
+// element, are byte permutes of two rows' words.  P^T comes from S^T's
+// accumulators by movmatrix.
+//
+// Formats.  bf16 multiplies in BF16, with p split in two BF16 terms (one would
+// round p to 8 bits, as large an error as the output's own rounding).  fp8 and
+// nvfp4 multiply in FP16, which holds their codes exactly (e2m1 * ue4m3 has 6
+// significant bits; the scale enters as 2^-8 of its value, a shift of its
+// byte), q times the power of two that puts its largest element into
+// [2^14, 2^15), and p rounded to 11 bits.  An fp8 row's scale multiplies the
+// score of its key and the weight of its value.
+//
+// Softmax.  In base 2 with a reference exponent per head instead of the exact
+// maximum: it moves (to the maximum less 4) only when a score passes it by
+// more than 10, so most steps need one vote and no rescaling; p stays below
+// 2^14.  For fp8 the reference follows the weighted scale, score + log2(value
+// scale), so that p times the scale is what stays in range.
+//
+// Split.  Sequence lengths are known on the GPU only.  A round is WARPS * TK
+// keys of one sequence and head unit, one step for each warp; the rounds of the
+// whole batch, in order, are dealt out evenly to the CTAs, each of which finds
+// its share by a prefix sum over the lengths.  Lengths of any unevenness fill
+// the GPU the same.  A share may end inside a sequence: such parts go to the
+// workspace, and the CTA that arrives last at a sequence's counter joins them,
+// in the order of their keys, so that results do not depend on the arrival.
+//
+// A warp streams its steps through a ring of its own in shared memory with
+// cp.async: no barrier in the loop.  Masked keys are zero-filled, not read.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <mutex>
 
 #include "decode_core.cuh"
 #include "fp4b_internal.h"
+#include "ptx_sm100.cuh"
 
 #define FP4B_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace fp4b {
 namespace {
 
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMaxCtasPerSm = 4;
+constexpr float kNoScore = -1e30f;    // reference exponent before any key
+constexpr float kHeadroom = 10.0f;    // a score may pass the reference by 2^10 ...
+constexpr float kBelowMax = 4.0f;     // ... which is set 2^4 below the maximum
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 struct AttentionParams {
     const uint16_t* q;
     long q_sb, q_sh;
     int batch, q_heads, group;
+    int group_tiles;  // head units of a key head: ceil(group / heads of a unit)
     fp4b_kv_cache cache;
     int page_shift;
     const int* table;
     long table_stride;
     int table_width;
     const int* lens;
-    float scale;
+    float scale2;  // scale * log2(e)
     int window;
     const float* sinks;
     uint16_t* out;
     float* lse;
     int* err;
+    uint32_t* counters;  // [grid], zero before and after
+    float* part_ml;      // [2 * grid][heads of a unit][2]
+    float* part_acc;     // [2 * grid][heads of a unit][D]
 };
 
-// Two neighbouring elements of a row.
-template <int KIND>
-__device__ __forceinline__ float2 read_two(const void* base, const void* scales, long row, int d, int e) {
-    if constexpr (KIND == kKvBf16) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(base) + (size_t)row * d + e);
-        return make_float2(decode::bf16_lo(w), decode::bf16_hi(w));
-    } else if constexpr (KIND == kKvFp8) {
-        const uint16_t w = *reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(base) + (size_t)row * d + e);
-        const float2 f = decode::f16x2_to_float2(decode::e4m3x2_to_f16x2(w));
-        const float s = static_cast<const float*>(scales)[row];
-        return make_float2(f.x * s, f.y * s);
-    } else {
-        const uint8_t w = static_cast<const uint8_t*>(base)[((size_t)row * d + e) >> 1];
-        const float2 f = decode::f16x2_to_float2(decode::e2m1x2_to_f16x2(w));
-        const float s = decode::ue4m3_float(static_cast<const uint8_t*>(scales)[((size_t)row * d + e) >> 4]);
-        return make_float2(f.x * s, f.y * s);
-    }
+template <int KIND, int D, int NT>
+struct Cfg {
+    static constexpr int RB = KIND == kKvBf16 ? 2 * D : KIND == kKvFp8 ? D : D / 2;  // bytes of a row
+    static constexpr int SB = KIND == kKvBf16 ? 0 : KIND == kKvFp8 ? 4 : D / 16;     // bytes of its scales
+    static constexpr int TK = RB <= 64 ? 32 : 16;   // keys of a step: at least 1 KB of K
+    static constexpr int KT = TK / 16;
+    static constexpr int HEADS = 8 * NT;
+    static constexpr int ROUND = kWarps * TK;
+    static constexpr int STAGE = 2 * TK * (RB + SB);
+    // About 24 KB of ring a warp where rows are wide, at least 4 stages where they are narrow.
+    static constexpr int STAGES = STAGE >= 16384 ? 3 : STAGE >= 8192 ? 3 : 4;
+    static constexpr int RING = STAGES * STAGE;
+    static constexpr int LD = D + 8;                // row stride of the merge area
+    static constexpr int MERGE = kWarps * HEADS * LD * 4;
+    static constexpr int SMEM = (kWarps * RING > MERGE ? kWarps * RING : MERGE);
+    // Elements of one of a lane's runs in a K row (4 lanes share the row) and in a V row (8 lanes).
+    static constexpr int EK = KIND == kKvBf16 ? 8 : KIND == kKvFp8 ? 16 : (D == 64 ? 16 : 32);
+    static constexpr int EV = KIND == kKvBf16 ? 8 : KIND == kKvFp8 ? (D == 64 ? 8 : 16) : D / 8;
+};
+
+// Shared-memory offset of 16-byte chunk c of row r: rows of 128 bytes or more
+// (and all V rows) are permuted so that the 8 or 16 lanes of one phase of the
+// reads below meet distinct banks.
+template <int RB>
+__device__ __forceinline__ int k_offset(int r, int c) {
+    return r * RB + 16 * (RB >= 128 ? c ^ ((r & 1) << 2) : c);
+}
+template <int RB>
+__device__ __forceinline__ int v_offset(int r, int c) {
+    if constexpr (RB == 32) return ((((r >> 1) & 3) | ((r & 1) << 2) | (r & 24)) * RB) + 16 * c;
+    else if constexpr (RB == 64) return ((((r >> 1) & 1) | ((r & 1) << 1) | (r & 28)) * RB) + 16 * (c ^ (((r >> 2) & 1) << 1));
+    else return r * RB + 16 * (c ^ (((r >> 1) & 3) << 1));
 }
 
-// One warp per (sequence, query head), one key at a time; lane l holds the
-// elements 2l, 2l + 1 of each run of 64.
-template <int KIND, int D>
-__global__ void __launch_bounds__(128) decode_attention_kernel(const __grid_constant__ AttentionParams p) {
-    const int lane = threadIdx.x & 31;
-    const long unit = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit >= (long)p.batch * p.q_heads) return;
-    const int b = (int)(unit / p.q_heads), h = (int)(unit - (long)b * p.q_heads), hk = h / p.group;
-    constexpr int R = D / 64;
-    float2 q[R], acc[R];
-    const uint16_t* qr = p.q + b * p.q_sb + h * p.q_sh;
-    for (int r = 0; r < R; ++r) {
-        q[r] = make_float2(__uint_as_float((uint32_t)qr[64 * r + 2 * lane] << 16), __uint_as_float((uint32_t)qr[64 * r + 2 * lane + 1] << 16));
-        acc[r] = make_float2(0.f, 0.f);
-    }
-    int len = p.lens[b];
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(live ? BYTES : 0)
+                     : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint2 lds64(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// A UE4M3 byte as 2^-8 of its value in both halves: the byte's exponent and
+// mantissa shifted into FP16's (exact, subnormals too).
+__device__ __forceinline__ uint32_t ue4m3_shifted(uint32_t byte) { return byte * 0x00800080u; }
+
+__device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
+
+// First key of a sequence's rounds, its clamped length and first visible key.
+struct Span {
+    int start, first, len, rounds;
+};
+template <int TK, int ROUND>
+__device__ __forceinline__ Span span_of(const AttentionParams& p, int b) {
+    Span s;
     const long most = (long)p.table_width << p.page_shift;
-    if (len < 0 || len > most) {
-        if (lane == 0) decode::report(p.err, kErrPageRange);
-        len = len < 0 ? 0 : (int)most;
+    s.len = p.lens[b];
+    if (s.len < 0 || s.len > most) {
+        decode::report(p.err, kErrPageRange);
+        s.len = s.len < 0 ? 0 : (int)most;
     }
-    const int first = p.window > 0 && len > p.window ? len - p.window : 0;
-    float m = -INFINITY, l = 0.0f;
-    for (int i = first; i < len; ++i) {
-        const int page = p.table[b * p.table_stride + (i >> p.page_shift)];
-        if (page < 0 || page >= p.cache.num_pages) {
-            if (lane == 0) decode::report(p.err, kErrPageRange);
+    s.first = p.window > 0 && s.len > p.window ? s.len - p.window : 0;
+    s.start = s.first & ~(TK - 1);
+    s.rounds = (int)(((long)s.len - s.start + ROUND - 1) / ROUND);
+    return s;
+}
+
+// One output row: divides by the softmax's denominator, the sink's share included.
+struct Finish {
+    float factor, lse;
+};
+__device__ __forceinline__ Finish finish(const AttentionParams& p, int head, float m, float l, float unit) {
+    float share = 1.0f;
+    if (p.sinks) {
+        const float sink = p.sinks[head] * kLog2e;
+        const float top = fmaxf(m, sink);
+        share = exp2_approx(m - top);
+        l = l * share + exp2_approx(sink - top);
+        m = top;
+    }
+    // l == 0: nothing was seen (m is kNoScore or the sink is -inf)
+    return Finish{l == 0.0f ? 0.0f : unit * share / l, l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2};
+}
+
+template <int KIND, int D, int NT>
+__global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid_constant__ AttentionParams p) {
+    using C = Cfg<KIND, D, NT>;
+    constexpr int TK = C::TK, KT = C::KT, RB = C::RB, SB = C::SB, MT = D / 16, HEADS = C::HEADS;
+    constexpr bool kBf16 = KIND == kKvBf16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long s_pre, s_total[kWarps];
+    __shared__ int s_b;
+    __shared__ float s_m[kWarps][HEADS], s_l[kWarps][HEADS];
+    __shared__ int s_last;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int units = p.cache.kv_heads * p.group_tiles;
+
+    // ---- this CTA's share [u0, u1) of the batch's rounds, and the sequence that it starts in
+    long total = 0, mine = 0, before = 0;
+    for (int base = 0; base < p.batch; base += kThreads) {
+        const int b = base + tid;
+        mine = b < p.batch ? (long)span_of<TK, C::ROUND>(p, b).rounds * units : 0;
+        long scan = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long other = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += other;
+        }
+        if (lane == 31) s_total[warp] = scan;
+        __syncthreads();
+        before = total + scan - mine;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_total[w];
+            total += s_total[w];
+        }
+        __syncthreads();
+    }
+    // Sequences without keys: their rows are the sink's alone.
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        if (span_of<TK, C::ROUND>(p, b).rounds > 0) continue;
+        for (int i = tid; i < p.q_heads * (D / 4); i += kThreads)
+            *reinterpret_cast<uint2*>(p.out + (size_t)b * p.q_heads * D + 4 * i) = make_uint2(0u, 0u);
+        if (p.lse)
+            for (int h = tid; h < p.q_heads; h += kThreads)
+                p.lse[(size_t)b * p.q_heads + h] = finish(p, h, kNoScore, 0.0f, 1.0f).lse;
+    }
+    if (total == 0) return;
+    const long ctas = min((long)gridDim.x, total);
+    if ((long)blockIdx.x >= ctas) return;
+    long u = total * blockIdx.x / ctas;
+    const long u1 = total * (blockIdx.x + 1) / ctas;
+    if (p.batch > kThreads) {  // the sums of the last chunk are the ones at hand: go over them again
+        long sum = 0;
+        for (int base = 0; base < p.batch; base += kThreads) {
+            const int b = base + tid;
+            mine = b < p.batch ? (long)span_of<TK, C::ROUND>(p, b).rounds * units : 0;
+            long scan = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long other = __shfl_up_sync(0xffffffffu, scan, o);
+                if (lane >= o) scan += other;
+            }
+            if (lane == 31) s_total[warp] = scan;
+            __syncthreads();
+            before = sum + scan - mine;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) before += s_total[w];
+                sum += s_total[w];
+            }
+            if (mine > 0 && before <= u && u < before + mine) {
+                s_b = b;
+                s_pre = before;
+            }
+            __syncthreads();
+            if (sum > u) break;
+        }
+    } else {
+        if (mine > 0 && before <= u && u < before + mine) {
+            s_b = tid;
+            s_pre = before;
+        }
+        __syncthreads();
+    }
+    int b = s_b;
+    long pre = s_pre;
+
+    uint8_t* ring = smem + warp * C::RING;
+    const uint32_t ring_addr = ptx::smem_u32(ring);
+
+    while (u < u1) {
+        const Span span = span_of<TK, C::ROUND>(p, b);
+        if (span.rounds == 0) {
+            ++b;
             continue;
         }
-        const long row = ((long)page * p.cache.kv_heads + hk) * p.cache.page_size + (i & (p.cache.page_size - 1));
-        float dot = 0.0f;
-        for (int r = 0; r < R; ++r) {
-            const float2 k = read_two<KIND>(p.cache.k, p.cache.k_scale, row, D, 64 * r + 2 * lane);
-            dot += q[r].x * k.x + q[r].y * k.y;
+        const long local = u - pre;
+        const int unit = (int)(local / span.rounds), r0 = (int)(local - (long)unit * span.rounds);
+        const int r1 = (int)min((long)span.rounds, r0 + (u1 - u));
+        const int kv_head = unit / p.group_tiles, in_group = (unit - kv_head * p.group_tiles) * HEADS;
+        const int head0 = kv_head * p.group + in_group, live_heads = min(HEADS, p.group - in_group);
+
+        // ---- the stream of this warp's steps
+        const int* table = p.table + (size_t)b * p.table_stride;
+        const int step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
+        int steps = r1 - r0;
+        if (steps > 0 && (long)step0 + (long)(steps - 1) * C::ROUND >= span.len) --steps;
+        const int my_key = lane & (TK - 1);
+        auto page_of = [&](int s) {  // page of the lane's key of step s; -2 for a masked key
+            const long key = (long)step0 + (long)s * C::ROUND + my_key;
+            return s < steps && key >= span.first && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
+        };
+        int next_page = page_of(0);
+        auto issue = [&](int s) {
+            if (s < steps) {
+                const int key = step0 + s * C::ROUND + my_key;
+                int row = -1;  // the lane's key's row; -1: zero-filled
+                if (next_page >= 0 && next_page < p.cache.num_pages)
+                    row = (next_page * p.cache.kv_heads + kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
+                else if (next_page != -2)
+                    decode::report(p.err, kErrPageRange);
+                next_page = page_of(s + 1);
+                const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE;
+                constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
+#pragma unroll
+                for (int i = 0; i < TK / PER; ++i) {
+                    const int r = i * PER + lane / LR, c = lane % LR;
+                    const int from = __shfl_sync(0xffffffffu, row, r);
+                    const size_t at = (size_t)(from < 0 ? 0 : from) * RB + 16 * c;
+                    copy_async<16>(dst + k_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.k) + at, from >= 0);
+                    copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.v) + at, from >= 0);
+                }
+                if constexpr (SB > 0) {
+                    const size_t at = (size_t)(row < 0 ? 0 : row) * SB;
+                    const uint32_t to = dst + 2 * TK * RB + my_key * SB;
+                    if (TK == 32 || lane < 16) copy_async<SB>(to, static_cast<const uint8_t*>(p.cache.k_scale) + at, row >= 0);
+                    if (TK == 32 || lane >= 16)
+                        copy_async<SB>(to + TK * SB, static_cast<const uint8_t*>(p.cache.v_scale) + at, row >= 0);
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+
+        // ---- queries: column g of head tile nt, element 4 EK (j / (EK/4)) + EK t + 4 (j % (EK/4)) of k-step j
+        uint32_t qf[NT][MT][2];
+        float f0[NT], f1[NT];  // score factors of heads 2t, 2t + 1
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int n = 8 * nt + g;
+            const uint16_t* row = p.q + (size_t)b * p.q_sb + (size_t)(head0 + (n < live_heads ? n : 0)) * p.q_sh;
+            uint2 w[MT];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const int d = 4 * C::EK * (j / (C::EK / 4)) + C::EK * t + 4 * (j % (C::EK / 4));
+                w[j] = n < live_heads ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+            }
+            float factor = p.scale2;
+            if constexpr (kBf16) {
+#pragma unroll
+                for (int j = 0; j < MT; ++j) qf[nt][j][0] = w[j].x, qf[nt][j][1] = w[j].y;
+            } else {
+                uint32_t top = 0;  // largest magnitude's bits
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    top = max(top, max((w[j].x & 0x7FFFu) << 16, w[j].x & 0x7FFF0000u));
+                    top = max(top, max((w[j].y & 0x7FFFu) << 16, w[j].y & 0x7FFF0000u));
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int k = min(max(141 - (int)(top >> 23), -126), 126);
+                const float up = __int_as_float((127 + k) << 23);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    qf[nt][j][0] = pack_f16(decode::bf16_lo(w[j].x) * up, decode::bf16_hi(w[j].x) * up);
+                    qf[nt][j][1] = pack_f16(decode::bf16_lo(w[j].y) * up, decode::bf16_hi(w[j].y) * up);
+                }
+                factor *= __int_as_float((127 - k) << 23);
+                if (KIND == kKvNvfp4) factor *= 256.0f;  // of the shifted scales
+            }
+            f0[nt] = __shfl_sync(0xffffffffu, factor, 8 * t);
+            f1[nt] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
         }
-        const float s = decode::group_sum<32>(dot) * p.scale;
-        const float top = fmaxf(m, s);
-        const float keep = m == -INFINITY ? 0.0f : __expf(m - top), w = top == -INFINITY ? 0.0f : __expf(s - top);
-        for (int r = 0; r < R; ++r) {
-            const float2 v = read_two<KIND>(p.cache.v, p.cache.v_scale, row, D, 64 * r + 2 * lane);
-            acc[r].x = acc[r].x * keep + w * v.x;
-            acc[r].y = acc[r].y * keep + w * v.y;
+
+        float acc[NT][MT][4];
+        float ref0[NT], ref1[NT], l0[NT], l1[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            ref0[nt] = ref1[nt] = kNoScore;
+            l0[nt] = l1[nt] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[nt][m][i] = 0.0f;
         }
-        l = l * keep + w;
-        m = top;
+
+        for (int s = 0; s < steps; ++s) {
+            copy_wait<C::STAGES - 2>();
+            __syncwarp();
+            issue(s + C::STAGES - 1);
+            const uint8_t* sk = ring + (s % C::STAGES) * C::STAGE;
+            const uint8_t* sv = sk + TK * RB;
+            const uint8_t* ss = sv + TK * RB;
+            const int key0 = step0 + s * C::ROUND;
+
+            // ---- scores
+            float sc[NT][KT][4];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[nt][kt][i] = 0.0f;
+                const int ra = 16 * kt + g, rb = ra + 8;
+                if constexpr (kBf16) {
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<true>(sc[nt][kt], a.x, c.x, a.y, c.y, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+                            mma<true>(sc[nt][kt], a.z, c.z, a.w, c.w, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+                        }
+                    }
+                } else if constexpr (KIND == kKvFp8) {
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) {
+                        const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+                        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t a0 = decode::e4m3x2_to_f16x2((uint16_t)aw[q]), a2 = decode::e4m3x2_to_f16x2((uint16_t)(aw[q] >> 16));
+                            const uint32_t a1 = decode::e4m3x2_to_f16x2((uint16_t)cw[q]), a3 = decode::e4m3x2_to_f16x2((uint16_t)(cw[q] >> 16));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], a0, a1, a2, a3, qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
+                        }
+                    }
+                } else {
+                    constexpr int WORDS = C::EK / 8, PIECES = D / (4 * C::EK);
+#pragma unroll
+                    for (int i = 0; i < PIECES; ++i) {
+                        uint32_t aw[WORDS], cw[WORDS];
+                        if constexpr (WORDS == 2) {
+                            const uint2 a = lds64(sk + k_offset<RB>(ra, 0) + 8 * t), c = lds64(sk + k_offset<RB>(rb, 0) + 8 * t);
+                            aw[0] = a.x, aw[1] = a.y, cw[0] = c.x, cw[1] = c.y;
+                        } else {
+                            const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+                            aw[0] = a.x, aw[1] = a.y, aw[2] = a.z, aw[3] = a.w, cw[0] = c.x, cw[1] = c.y, cw[2] = c.z, cw[3] = c.w;
+                        }
+#pragma unroll
+                        for (int q = 0; q < WORDS; ++q) {
+                            const int block = (C::EK / 16) * (4 * i + t) + q / 2;
+                            const uint32_t s_a = ue4m3_shifted(ss[ra * SB + block]), s_c = ue4m3_shifted(ss[rb * SB + block]);
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const uint32_t a0 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(aw[q], 2 * half)), s_a);
+                                const uint32_t a2 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(aw[q], 2 * half + 1)), s_a);
+                                const uint32_t a1 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(cw[q], 2 * half)), s_c);
+                                const uint32_t a3 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(cw[q], 2 * half + 1)), s_c);
+                                const int j = (C::EK / 4) * i + 2 * q + half;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], a0, a1, a2, a3, qf[nt][j][0], qf[nt][j][1]);
+                            }
+                        }
+                    }
+                }
+            }
+
+            // ---- in base 2, masked; the row scales of fp8
+            float va[KT], vb[KT], la[KT], lb[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const int ra = 16 * kt + g, rb = ra + 8;
+                float ka = 1.0f, kb = 1.0f;
+                if constexpr (KIND == kKvFp8) {
+                    const float* fs = reinterpret_cast<const float*>(ss);
+                    ka = fs[ra], kb = fs[rb], va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
+                    la[kt] = fmaxf(__log2f(va[kt]), -80.0f), lb[kt] = fmaxf(__log2f(vb[kt]), -80.0f);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    sc[nt][kt][0] *= f0[nt] * ka, sc[nt][kt][1] *= f1[nt] * ka;
+                    sc[nt][kt][2] *= f0[nt] * kb, sc[nt][kt][3] *= f1[nt] * kb;
+                }
+            }
+            if (key0 < span.first || key0 + TK > span.len) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int ka = key0 + 16 * kt + g, kb = ka + 8;
+                    const bool oa = ka >= span.first && ka < span.len, ob = kb >= span.first && kb < span.len;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (!oa) sc[nt][kt][0] = sc[nt][kt][1] = -INFINITY;
+                        if (!ob) sc[nt][kt][2] = sc[nt][kt][3] = -INFINITY;
+                    }
+                }
+            }
+            bool over = false;
+            float t0[NT], t1[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                t0[nt] = t1[nt] = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
+                    t0[nt] = fmaxf(t0[nt], fmaxf(sc[nt][kt][0] + xa, sc[nt][kt][2] + xb));
+                    t1[nt] = fmaxf(t1[nt], fmaxf(sc[nt][kt][1] + xa, sc[nt][kt][3] + xb));
+                }
+                over |= t0[nt] > ref0[nt] + kHeadroom || t1[nt] > ref1[nt] + kHeadroom;
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        t0[nt] = fmaxf(t0[nt], __shfl_xor_sync(0xffffffffu, t0[nt], o));
+                        t1[nt] = fmaxf(t1[nt], __shfl_xor_sync(0xffffffffu, t1[nt], o));
+                    }
+                    const float n0 = fmaxf(ref0[nt], t0[nt] - kBelowMax), n1 = fmaxf(ref1[nt], t1[nt] - kBelowMax);
+                    const float c0 = exp2_approx(ref0[nt] - n0), c1 = exp2_approx(ref1[nt] - n1);
+                    ref0[nt] = n0, ref1[nt] = n1;
+                    l0[nt] *= c0, l1[nt] *= c1;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        acc[nt][m][0] *= c0, acc[nt][m][1] *= c1;
+                        acc[nt][m][2] *= c0, acc[nt][m][3] *= c1;
+                    }
+                }
+            }
+
+            // ---- weights as P^T fragments
+            uint32_t pf[NT][KT][2], pl[NT][KT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[nt][kt][i] - (i & 1 ? ref1[nt] : ref0[nt]));
+                    l0[nt] += w[0] + w[2];
+                    l1[nt] += w[1] + w[3];
+                    if constexpr (KIND == kKvFp8) {
+                        // a masked key's zero-filled scale keeps its weight zero
+                        w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
+                    }
+                    if constexpr (kBf16) {
+                        const uint32_t hi0 = decode::pack_bf16(w[0], w[1]), hi1 = decode::pack_bf16(w[2], w[3]);
+                        pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
+                        pl[nt][kt][0] = transpose8x8(decode::pack_bf16(w[0] - decode::bf16_lo(hi0), w[1] - decode::bf16_hi(hi0)));
+                        pl[nt][kt][1] = transpose8x8(decode::pack_bf16(w[2] - decode::bf16_lo(hi1), w[3] - decode::bf16_hi(hi1)));
+                    } else {
+                        pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
+                        pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
+                    }
+                }
+
+            // ---- values: the lane's keys are 2t, 2t + 1, 2t + 8, 2t + 9 of each 16, its elements run g of each row
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const int r = 16 * kt + 2 * t;
+                constexpr int WORDS = C::EV * RB / D / 4, PIECES = D / (8 * C::EV);  // words of a run, runs of a row
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    uint32_t v[4][WORDS];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int row = r + (x & 1) + 8 * (x >> 1);
+                        if constexpr (WORDS == 4) {
+                            const uint4 w = lds128(sv + v_offset<RB>(row, 8 * i + g));
+                            v[x][0] = w.x, v[x][1] = w.y, v[x][2] = w.z, v[x][3] = w.w;
+                        } else if constexpr (WORDS == 2) {
+                            const uint2 w = lds64(sv + v_offset<RB>(row, g >> 1) + 8 * (g & 1));
+                            v[x][0] = w.x, v[x][1] = w.y;
+                        } else {
+                            v[x][0] = lds32(sv + v_offset<RB>(row, g >> 2) + 4 * (g & 3));
+                        }
+                    }
+                    constexpr int PAIRS = C::EV / 2;  // m-tiles of a run
+#pragma unroll
+                    for (int e = 0; e < PAIRS; ++e) {
+                        uint32_t h[4];  // elements 2e, 2e + 1 of the four keys
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if constexpr (kBf16) {
+                                h[x] = v[x][e];
+                            } else if constexpr (KIND == kKvFp8) {
+                                h[x] = decode::e4m3x2_to_f16x2((uint16_t)(v[x][e / 2] >> (16 * (e & 1))));
+                            } else {
+                                const int row = r + (x & 1) + 8 * (x >> 1);
+                                const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + e / 8;
+                                h[x] = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(v[x][e / 4], e & 3)),
+                                                 ue4m3_shifted(ss[TK * SB + row * SB + block]));
+                            }
+                        }
+                        const uint32_t a0 = __byte_perm(h[0], h[1], 0x5410), a1 = __byte_perm(h[0], h[1], 0x7632);
+                        const uint32_t a2 = __byte_perm(h[2], h[3], 0x5410), a3 = __byte_perm(h[2], h[3], 0x7632);
+                        const int m = i * PAIRS + e;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<kBf16>(acc[nt][m], a0, a1, a2, a3, pf[nt][kt][0], pf[nt][kt][1]);
+                            if constexpr (kBf16) mma<true>(acc[nt][m], a0, a1, a2, a3, pl[nt][kt][0], pl[nt][kt][1]);
+                        }
+                    }
+                }
+            }
+        }
+        copy_wait<0>();
+
+        // ---- the warps' results, joined in shared memory (over the idle rings)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], o);
+                l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], o);
+            }
+            if (g == 0) {
+                s_m[warp][8 * nt + 2 * t] = ref0[nt], s_m[warp][8 * nt + 2 * t + 1] = ref1[nt];
+                s_l[warp][8 * nt + 2 * t] = l0[nt], s_l[warp][8 * nt + 2 * t + 1] = l1[nt];
+            }
+        }
+        __syncthreads();
+        float* merge = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int h0 = 8 * nt + 2 * t;
+            float m0 = kNoScore, m1 = kNoScore;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m0 = fmaxf(m0, s_m[w][h0]), m1 = fmaxf(m1, s_m[w][h0 + 1]);
+            const float c0 = exp2_approx(ref0[nt] - m0), c1 = exp2_approx(ref1[nt] - m1);
+            float* to = merge + (warp * HEADS + h0) * C::LD;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int e = 2 * m, d = 8 * C::EV * (e / C::EV) + C::EV * g + e % C::EV;
+                *reinterpret_cast<float2*>(to + d) = make_float2(acc[nt][m][0] * c0, acc[nt][m][2] * c0);
+                *reinterpret_cast<float2*>(to + C::LD + d) = make_float2(acc[nt][m][1] * c1, acc[nt][m][3] * c1);
+            }
+        }
+        __syncthreads();
+
+        const bool whole = r0 == 0 && r1 == span.rounds;
+        const float unit_scale = KIND == kKvNvfp4 ? 256.0f : 1.0f;  // of the shifted value scales
+        const int slot = 2 * blockIdx.x + (r0 == 0 ? 1 : 0);
+        for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
+            const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
+            float m = kNoScore, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][h]);
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float4 x = *reinterpret_cast<const float4*>(merge + (w * HEADS + h) * C::LD + d);
+                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+                l += s_l[w][h] * exp2_approx(s_m[w][h] - m);
+            }
+            if (whole) {
+                const Finish f = finish(p, head0 + h, m, l, unit_scale);
+                *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.q_heads + head0 + h) * D + d) =
+                    make_uint2(decode::pack_bf16(sum.x * f.factor, sum.y * f.factor), decode::pack_bf16(sum.z * f.factor, sum.w * f.factor));
+                if (p.lse && d == 0) p.lse[(size_t)b * p.q_heads + head0 + h] = f.lse;
+            } else {
+                __stcg(reinterpret_cast<float4*>(p.part_acc + ((size_t)slot * HEADS + h) * D + d), sum);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * HEADS + h) * 2), make_float2(m, l));
+            }
+        }
+        if (!whole) {
+            // The CTAs that hold this unit's rounds: the first one's counter counts them.
+            const long from = pre + (long)unit * span.rounds, to = from + span.rounds - 1;
+            const int first_cta = (int)(((from + 1) * ctas - 1) / total), last_cta = (int)(((to + 1) * ctas - 1) / total);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(p.counters + first_cta, 1u) == (uint32_t)(last_cta - first_cta);
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
+                    const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
+                    float m = kNoScore, l = 0.0f;
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int c = first_cta; c <= last_cta; ++c) {
+                        const size_t at = (size_t)(2 * c + (c == first_cta ? 1 : 0)) * HEADS + h;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_acc + at * D + d));
+                        const float top = fmaxf(m, ml.x), old = exp2_approx(m - top), add = exp2_approx(ml.x - top);
+                        sum.x = sum.x * old + x.x * add, sum.y = sum.y * old + x.y * add;
+                        sum.z = sum.z * old + x.z * add, sum.w = sum.w * old + x.w * add;
+                        l = l * old + ml.y * add;
+                        m = top;
+                    }
+                    const Finish f = finish(p, head0 + h, m, l, unit_scale);
+                    *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.q_heads + head0 + h) * D + d) = make_uint2(
+                        decode::pack_bf16(sum.x * f.factor, sum.y * f.factor), decode::pack_bf16(sum.z * f.factor, sum.w * f.factor));
+                    if (p.lse && d == 0) p.lse[(size_t)b * p.q_heads + head0 + h] = f.lse;
+                }
+                if (tid == 0) p.counters[first_cta] = 0u;  // as it was found
+            }
+        }
+        __syncthreads();  // the merge area is the rings again
+        u += r1 - r0;
+        if (u == pre + (long)span.rounds * units) {
+            pre = u;
+            ++b;
+        }
     }
-    if (p.sinks) {
-        const float sink = p.sinks[h], top = fmaxf(m, sink);
-        const float keep = m == -INFINITY ? 0.0f : __expf(m - top);
-        for (int r = 0; r < R; ++r) acc[r].x *= keep, acc[r].y *= keep;
-        l = l * keep + (top == -INFINITY ? 0.0f : __expf(sink - top));
-        m = top;
+}
+
+constexpr int kMaxDevices = 64;
+
+int sm_count() {
+    static int counts[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
+    if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -1;
+    return counts[dev];
+}
+
+// Workspace: counters, then the parts' (maximum, sum) and accumulators.
+struct Layout {
+    long slots, ml, acc, bytes;
+};
+Layout layout_of(int sms, int heads, int d) {
+    Layout w;
+    const long ctas = (long)sms * kMaxCtasPerSm;
+    w.slots = 2 * ctas;
+    w.ml = (ctas * 4 + 255) / 256 * 256;
+    w.acc = w.ml + w.slots * heads * 8;
+    w.bytes = w.acc + w.slots * heads * d * 4;
+    return w;
+}
+
+int unit_heads(int group) { return group <= 8 ? 8 : 16; }
+
+template <int KIND, int D, int NT>
+cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
+    using C = Cfg<KIND, D, NT>;
+    static std::mutex mu;
+    static int resident[kMaxDevices];  // CTAs that fit on the device at once
+    auto* kernel = decode_attention_kernel<KIND, D, NT>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const int sms = sm_count();
+    if (sms <= 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!resident[dev]) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+            int per = 0;
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, C::SMEM);
+            if (e != cudaSuccess) return e;
+            resident[dev] = sms * std::max(1, std::min(per, kMaxCtasPerSm));
+        }
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    for (int r = 0; r < R; ++r)
-        *reinterpret_cast<uint32_t*>(p.out + ((size_t)b * p.q_heads + h) * D + 64 * r + 2 * lane) =
-            decode::pack_bf16(acc[r].x * inv, acc[r].y * inv);
-    if (p.lse && lane == 0) p.lse[(size_t)b * p.q_heads + h] = m == -INFINITY ? -INFINITY : m + logf(l);
+    p.group_tiles = (p.group + C::HEADS - 1) / C::HEADS;
+    const Layout w = layout_of(sms, C::HEADS, D);
+    p.counters = reinterpret_cast<uint32_t*>(workspace);
+    p.part_ml = reinterpret_cast<float*>(workspace + w.ml);
+    p.part_acc = reinterpret_cast<float*>(workspace + w.acc);
+    // No more CTAs than the page table has rounds for (and one for each empty sequence's row).
+    const long keys = (long)p.table_width << p.page_shift;
+    const long most = (long)p.batch * std::max(1l, (keys + C::ROUND - 1) / C::ROUND * p.cache.kv_heads * p.group_tiles);
+    kernel<<<(unsigned)std::min<long>(resident[dev], most), kThreads, C::SMEM, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <int KIND, int D>
+cudaError_t launch_heads(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
+    return unit_heads(p.group) == 8 ? launch<KIND, D, 1>(p, workspace, st) : launch<KIND, D, 2>(p, workspace, st);
 }
 
 template <int KIND>
-cudaError_t launch(const AttentionParams& p, cudaStream_t st) {
-    const unsigned blocks = (unsigned)(((long)p.batch * p.q_heads + 3) / 4);
-    if (p.cache.head_dim == 64) decode_attention_kernel<KIND, 64><<<blocks, 128, 0, st>>>(p);
-    else if (p.cache.head_dim == 128) decode_attention_kernel<KIND, 128><<<blocks, 128, 0, st>>>(p);
-    else decode_attention_kernel<KIND, 256><<<blocks, 128, 0, st>>>(p);
-    return cudaGetLastError();
+cudaError_t launch_dim(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
+    return p.cache.head_dim == 64    ? launch_heads<KIND, 64>(p, workspace, st)
+           : p.cache.head_dim == 128 ? launch_heads<KIND, 128>(p, workspace, st)
+                                     : launch_heads<KIND, 256>(p, workspace, st);
 }
 
 }  // namespace
@@ -131,8 +795,17 @@ cudaError_t launch(const AttentionParams& p, cudaStream_t st) {
 using namespace fp4b;
 
 FP4B_EXPORT long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int head_dim) {
-    if (q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) return -1;
-    return 16;
+    if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0) {
+        set_last_error("fp4b_decode_attention_workspace: bad head counts");
+        return -1;
+    }
+    const int sms = sm_count();
+    if (sms <= 0) {
+        cudaGetLastError();
+        set_last_error("fp4b_decode_attention_workspace: no device");
+        return -1;
+    }
+    return layout_of(sms, unit_heads(q_heads / kv_heads), head_dim).bytes;
 }
 
 FP4B_EXPORT int fp4b_decode_attention(const void* q, long q_sb, long q_sh, int batch, int q_heads,
@@ -145,7 +818,7 @@ FP4B_EXPORT int fp4b_decode_attention(const void* q, long q_sb, long q_sh, int b
         why = "query heads must be a multiple of the cache's heads";
     if (!why && batch > 0 && (!q || !out || !seq_lens || (table_width > 0 && !page_table))) why = "null tensor";
     if (!why && (table_width < 0 || table_stride < table_width)) why = "bad page table";
-    if (!why && (long)table_width * cache->page_size > 0x7fffffffL) why = "more than 2^31 keys in one sequence";
+    if (!why && (long)table_width * cache->page_size > 0x7fff0000L) why = "more than 2^31 keys in one sequence";
     if (!why && (long)batch * q_heads > 0x7fffffffL) why = "more than 2^31 output rows";
     if (!why && (window < 0 || !std::isfinite(scale))) why = "window must not be negative, scale finite";
     if (!why && ((reinterpret_cast<uintptr_t>(q) & 7) || q_sb % 4 || q_sh % 4 || (reinterpret_cast<uintptr_t>(out) & 15)))
@@ -159,13 +832,18 @@ FP4B_EXPORT int fp4b_decode_attention(const void* q, long q_sb, long q_sh, int b
         return -1;
     }
     if (batch == 0) return 0;
-    AttentionParams p{static_cast<const uint16_t*>(q), q_sb, q_sh, batch, q_heads, q_heads / cache->kv_heads, *cache, 0,
-                      page_table, table_stride, table_width, seq_lens, scale, window, sinks,
-                      static_cast<uint16_t*>(out), lse, device_error_word()};
+    AttentionParams p{};
+    p.q = static_cast<const uint16_t*>(q), p.q_sb = q_sb, p.q_sh = q_sh;
+    p.batch = batch, p.q_heads = q_heads, p.group = q_heads / cache->kv_heads;
+    p.cache = *cache;
     while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
+    p.table = page_table, p.table_stride = table_stride, p.table_width = table_width;
+    p.lens = seq_lens, p.scale2 = scale * kLog2e, p.window = window, p.sinks = sinks;
+    p.out = static_cast<uint16_t*>(out), p.lse = lse, p.err = device_error_word();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = cache->kind == kKvBf16 ? launch<kKvBf16>(p, st)
-                          : cache->kind == kKvFp8 ? launch<kKvFp8>(p, st)
-                                                  : launch<kKvNvfp4>(p, st);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const cudaError_t e = cache->kind == kKvBf16 ? launch_dim<kKvBf16>(p, ws, st)
+                          : cache->kind == kKvFp8 ? launch_dim<kKvFp8>(p, ws, st)
+                                                  : launch_dim<kKvNvfp4>(p, ws, st);
     return launch_status(e, "fp4b_decode_attention");
 }
