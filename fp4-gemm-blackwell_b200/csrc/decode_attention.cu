@@ -59,6 +59,8 @@
 namespace fp4b {
 namespace {
 
+using namespace decode;
+
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCtasPerSm = 4;
@@ -124,61 +126,6 @@ __device__ __forceinline__ int v_offset(int r, int c) {
     else return r * RB + 16 * (c ^ (((r >> 1) & 3) << 1));
 }
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(live ? BYTES : 0)
-                     : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
-__device__ __forceinline__ uint2 lds64(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
-__device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
-
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-
-// A UE4M3 byte as 2^-8 of its value in both halves: the byte's exponent and
-// mantissa shifted into FP16's (exact, subnormals too).
-__device__ __forceinline__ uint32_t ue4m3_shifted(uint32_t byte) { return byte * 0x00800080u; }
-
-__device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
-
 // First key of a sequence's rounds, its clamped length and first visible key.
 struct Span {
     int start, first, len, rounds;
@@ -189,7 +136,7 @@ __device__ __forceinline__ Span span_of(const AttentionParams& p, int b) {
     const long most = (long)p.table_width << p.page_shift;
     s.len = p.lens[b];
     if (s.len < 0 || s.len > most) {
-        decode::report(p.err, kErrPageRange);
+        report(p.err, kErrPageRange);
         s.len = s.len < 0 ? 0 : (int)most;
     }
     s.first = p.window > 0 && s.len > p.window ? s.len - p.window : 0;
@@ -331,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 if (next_page >= 0 && next_page < p.cache.num_pages)
                     row = (next_page * p.cache.kv_heads + kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
                 else if (next_page != -2)
-                    decode::report(p.err, kErrPageRange);
+                    report(p.err, kErrPageRange);
                 next_page = page_of(s + 1);
                 const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE;
                 constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
@@ -386,8 +333,8 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 const float up = __int_as_float((127 + k) << 23);
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
-                    qf[nt][j][0] = pack_f16(decode::bf16_lo(w[j].x) * up, decode::bf16_hi(w[j].x) * up);
-                    qf[nt][j][1] = pack_f16(decode::bf16_lo(w[j].y) * up, decode::bf16_hi(w[j].y) * up);
+                    qf[nt][j][0] = pack_f16(bf16_lo(w[j].x) * up, bf16_hi(w[j].x) * up);
+                    qf[nt][j][1] = pack_f16(bf16_lo(w[j].y) * up, bf16_hi(w[j].y) * up);
                 }
                 factor *= __int_as_float((127 - k) << 23);
                 if (KIND == kKvNvfp4) factor *= 256.0f;  // of the shifted scales
@@ -443,8 +390,8 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                         const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const uint32_t a0 = decode::e4m3x2_to_f16x2((uint16_t)aw[q]), a2 = decode::e4m3x2_to_f16x2((uint16_t)(aw[q] >> 16));
-                            const uint32_t a1 = decode::e4m3x2_to_f16x2((uint16_t)cw[q]), a3 = decode::e4m3x2_to_f16x2((uint16_t)(cw[q] >> 16));
+                            const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)aw[q]), a2 = e4m3x2_to_f16x2((uint16_t)(aw[q] >> 16));
+                            const uint32_t a1 = e4m3x2_to_f16x2((uint16_t)cw[q]), a3 = e4m3x2_to_f16x2((uint16_t)(cw[q] >> 16));
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], a0, a1, a2, a3, qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
                         }
@@ -467,10 +414,10 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                             const uint32_t s_a = ue4m3_shifted(ss[ra * SB + block]), s_c = ue4m3_shifted(ss[rb * SB + block]);
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
-                                const uint32_t a0 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(aw[q], 2 * half)), s_a);
-                                const uint32_t a2 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(aw[q], 2 * half + 1)), s_a);
-                                const uint32_t a1 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(cw[q], 2 * half)), s_c);
-                                const uint32_t a3 = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(cw[q], 2 * half + 1)), s_c);
+                                const uint32_t a0 = mul_f16x2(e2m1x2_to_f16x2(byte_of(aw[q], 2 * half)), s_a);
+                                const uint32_t a2 = mul_f16x2(e2m1x2_to_f16x2(byte_of(aw[q], 2 * half + 1)), s_a);
+                                const uint32_t a1 = mul_f16x2(e2m1x2_to_f16x2(byte_of(cw[q], 2 * half)), s_c);
+                                const uint32_t a3 = mul_f16x2(e2m1x2_to_f16x2(byte_of(cw[q], 2 * half + 1)), s_c);
                                 const int j = (C::EK / 4) * i + 2 * q + half;
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], a0, a1, a2, a3, qf[nt][j][0], qf[nt][j][1]);
@@ -558,10 +505,10 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                         w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
                     }
                     if constexpr (kBf16) {
-                        const uint32_t hi0 = decode::pack_bf16(w[0], w[1]), hi1 = decode::pack_bf16(w[2], w[3]);
+                        const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
                         pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
-                        pl[nt][kt][0] = transpose8x8(decode::pack_bf16(w[0] - decode::bf16_lo(hi0), w[1] - decode::bf16_hi(hi0)));
-                        pl[nt][kt][1] = transpose8x8(decode::pack_bf16(w[2] - decode::bf16_lo(hi1), w[3] - decode::bf16_hi(hi1)));
+                        pl[nt][kt][0] = transpose8x8(pack_bf16(w[0] - bf16_lo(hi0), w[1] - bf16_hi(hi0)));
+                        pl[nt][kt][1] = transpose8x8(pack_bf16(w[2] - bf16_lo(hi1), w[3] - bf16_hi(hi1)));
                     } else {
                         pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
                         pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
@@ -598,11 +545,11 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                             if constexpr (kBf16) {
                                 h[x] = v[x][e];
                             } else if constexpr (KIND == kKvFp8) {
-                                h[x] = decode::e4m3x2_to_f16x2((uint16_t)(v[x][e / 2] >> (16 * (e & 1))));
+                                h[x] = e4m3x2_to_f16x2((uint16_t)(v[x][e / 2] >> (16 * (e & 1))));
                             } else {
                                 const int row = r + (x & 1) + 8 * (x >> 1);
                                 const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + e / 8;
-                                h[x] = mul_f16x2(decode::e2m1x2_to_f16x2(byte_of(v[x][e / 4], e & 3)),
+                                h[x] = mul_f16x2(e2m1x2_to_f16x2(byte_of(v[x][e / 4], e & 3)),
                                                  ue4m3_shifted(ss[TK * SB + row * SB + block]));
                             }
                         }
@@ -670,7 +617,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             if (whole) {
                 const Finish f = finish(p, head0 + h, m, l, unit_scale);
                 *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.q_heads + head0 + h) * D + d) =
-                    make_uint2(decode::pack_bf16(sum.x * f.factor, sum.y * f.factor), decode::pack_bf16(sum.z * f.factor, sum.w * f.factor));
+                    make_uint2(pack_bf16(sum.x * f.factor, sum.y * f.factor), pack_bf16(sum.z * f.factor, sum.w * f.factor));
                 if (p.lse && d == 0) p.lse[(size_t)b * p.q_heads + head0 + h] = f.lse;
             } else {
                 __stcg(reinterpret_cast<float4*>(p.part_acc + ((size_t)slot * HEADS + h) * D + d), sum);
@@ -703,7 +650,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                     }
                     const Finish f = finish(p, head0 + h, m, l, unit_scale);
                     *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.q_heads + head0 + h) * D + d) = make_uint2(
-                        decode::pack_bf16(sum.x * f.factor, sum.y * f.factor), decode::pack_bf16(sum.z * f.factor, sum.w * f.factor));
+                        pack_bf16(sum.x * f.factor, sum.y * f.factor), pack_bf16(sum.z * f.factor, sum.w * f.factor));
                     if (p.lse && d == 0) p.lse[(size_t)b * p.q_heads + head0 + h] = f.lse;
                 }
                 if (tid == 0) p.counters[first_cta] = 0u;  // as it was found
