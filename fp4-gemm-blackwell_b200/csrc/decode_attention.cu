@@ -265,37 +265,57 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         const int step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
         int steps = r1 - r0;
         if (steps > 0 && (long)step0 + (long)(steps - 1) * C::ROUND >= span.len) --steps;
+        const bool in_page = p.cache.page_size >= TK;  // a step's keys are one run of one page
         const int my_key = lane & (TK - 1);
-        auto page_of = [&](int s) {  // page of the lane's key of step s; -2 for a masked key
-            const long key = (long)step0 + (long)s * C::ROUND + my_key;
-            return s < steps && key >= span.first && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
+        auto page_of = [&](int s) {  // page of the lane's key of step s (of all its keys, if in_page); -2 for a masked key
+            if (s >= steps) return -2;
+            const int key0 = step0 + s * C::ROUND, key = key0 + (in_page ? 0 : my_key);
+            return (in_page || key >= span.first) && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
         };
         int next_page = page_of(0);
         auto issue = [&](int s) {
             if (s < steps) {
-                const int key = step0 + s * C::ROUND + my_key;
-                int row = -1;  // the lane's key's row; -1: zero-filled
-                if (next_page >= 0 && next_page < p.cache.num_pages)
-                    row = (next_page * p.cache.kv_heads + kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
-                else if (next_page != -2)
-                    report(p.err, kErrPageRange);
+                const int key0 = step0 + s * C::ROUND;
+                int page = next_page;
                 next_page = page_of(s + 1);
+                const bool known = page >= 0 && page < p.cache.num_pages;
+                if (!known && page != -2) report(p.err, kErrPageRange);
+                if (!known) page = 0;
+                const int first = in_page ? key0 : key0 + my_key;
+                // the lane's key's row, or the first of the step's
+                const int row = (page * p.cache.kv_heads + kv_head) * p.cache.page_size + (first & (p.cache.page_size - 1));
                 const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE;
                 constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
+                const int sub = lane / LR, c = lane % LR;
+                // rows lo .. hi - 1 of the step are read, the others zero-filled
+                const int lo = known ? span.first - key0 : TK, hi = span.len - key0;
+                if (in_page) {
+                    const size_t at = (size_t)row * RB + 16 * lane;
+                    const uint8_t* k_src = static_cast<const uint8_t*>(p.cache.k) + at;
+                    const uint8_t* v_src = static_cast<const uint8_t*>(p.cache.v) + at;
 #pragma unroll
-                for (int i = 0; i < TK / PER; ++i) {
-                    const int r = i * PER + lane / LR, c = lane % LR;
-                    const int from = __shfl_sync(0xffffffffu, row, r);
-                    const size_t at = (size_t)(from < 0 ? 0 : from) * RB + 16 * c;
-                    copy_async<16>(dst + k_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.k) + at, from >= 0);
-                    copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.v) + at, from >= 0);
+                    for (int i = 0; i < TK / PER; ++i) {
+                        const int r = i * PER + sub;
+                        const bool live = r >= lo && r < hi;
+                        copy_async<16>(dst + k_offset<RB>(r, c), k_src + 512 * i, live);
+                        copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), v_src + 512 * i, live);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < TK / PER; ++i) {
+                        const int r = i * PER + sub;
+                        const size_t at = (size_t)__shfl_sync(0xffffffffu, row, r) * RB + 16 * c;
+                        const bool live = __shfl_sync(0xffffffffu, known, r) && r >= span.first - key0 && r < hi;
+                        copy_async<16>(dst + k_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.k) + at, live);
+                        copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.v) + at, live);
+                    }
                 }
                 if constexpr (SB > 0) {
-                    const size_t at = (size_t)(row < 0 ? 0 : row) * SB;
+                    const size_t at = (size_t)(row + (in_page ? my_key : 0)) * SB;
+                    const bool live = my_key >= lo && my_key < hi;
                     const uint32_t to = dst + 2 * TK * RB + my_key * SB;
-                    if (TK == 32 || lane < 16) copy_async<SB>(to, static_cast<const uint8_t*>(p.cache.k_scale) + at, row >= 0);
-                    if (TK == 32 || lane >= 16)
-                        copy_async<SB>(to + TK * SB, static_cast<const uint8_t*>(p.cache.v_scale) + at, row >= 0);
+                    if (TK == 32 || lane < 16) copy_async<SB>(to, static_cast<const uint8_t*>(p.cache.k_scale) + at, live);
+                    if (TK == 32 || lane >= 16) copy_async<SB>(to + TK * SB, static_cast<const uint8_t*>(p.cache.v_scale) + at, live);
                 }
             }
             copy_commit();
@@ -337,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                     qf[nt][j][1] = pack_f16(bf16_lo(w[j].y) * up, bf16_hi(w[j].y) * up);
                 }
                 factor *= __int_as_float((127 - k) << 23);
-                if (KIND == kKvNvfp4) factor *= 256.0f;  // of the shifted scales
+                if (KIND == kKvNvfp4) factor *= kScaleUnit;
             }
             f0[nt] = __shfl_sync(0xffffffffu, factor, 8 * t);
             f1[nt] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
@@ -390,10 +410,11 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                         const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)aw[q]), a2 = e4m3x2_to_f16x2((uint16_t)(aw[q] >> 16));
-                            const uint32_t a1 = e4m3x2_to_f16x2((uint16_t)cw[q]), a3 = e4m3x2_to_f16x2((uint16_t)(cw[q] >> 16));
+                            uint32_t ha[2], hc[2];
+                            e4m3x4_to_f16(aw[q], ha);
+                            e4m3x4_to_f16(cw[q], hc);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], a0, a1, a2, a3, qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
+                            for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
                         }
                     }
                 } else {
@@ -411,39 +432,48 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 #pragma unroll
                         for (int q = 0; q < WORDS; ++q) {
                             const int block = (C::EK / 16) * (4 * i + t) + q / 2;
-                            const uint32_t s_a = ue4m3_shifted(ss[ra * SB + block]), s_c = ue4m3_shifted(ss[rb * SB + block]);
+                            const uint32_t s_a = ue4m3x2_to_f16(ss[ra * SB + block] * 0x10001u), s_c = ue4m3x2_to_f16(ss[rb * SB + block] * 0x10001u);
+                            uint32_t ha[4], hc[4];
+                            e2m1x8_to_f16(aw[q], ha);
+                            e2m1x8_to_f16(cw[q], hc);
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                const uint32_t a0 = mul_f16x2(e2m1x2_to_f16x2(byte_of(aw[q], 2 * half)), s_a);
-                                const uint32_t a2 = mul_f16x2(e2m1x2_to_f16x2(byte_of(aw[q], 2 * half + 1)), s_a);
-                                const uint32_t a1 = mul_f16x2(e2m1x2_to_f16x2(byte_of(cw[q], 2 * half)), s_c);
-                                const uint32_t a3 = mul_f16x2(e2m1x2_to_f16x2(byte_of(cw[q], 2 * half + 1)), s_c);
-                                const int j = (C::EK / 4) * i + 2 * q + half;
+                            for (int e = 0; e < 4; ++e) ha[e] = mul_f16x2(ha[e], s_a), hc[e] = mul_f16x2(hc[e], s_c);
+                            const int j = (C::EK / 4) * i + 2 * q;
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], a0, a1, a2, a3, qf[nt][j][0], qf[nt][j][1]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][j][0], qf[nt][j][1]);
+                                mma<false>(sc[nt][kt], ha[2], hc[2], ha[3], hc[3], qf[nt][j + 1][0], qf[nt][j + 1][1]);
                             }
                         }
                     }
                 }
             }
 
-            // ---- in base 2, masked; the row scales of fp8
-            float va[KT], vb[KT], la[KT], lb[KT];
+            // ---- x = score in base 2 less the reference; the row scales of fp8
+            float va[KT], vb[KT], la[KT], lb[KT];  // value scales of the keys and their logarithms
+            if constexpr (KIND == kKvFp8) {
+                const float* fs = reinterpret_cast<const float*>(ss);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const int ra = 16 * kt + g, rb = ra + 8;
-                float ka = 1.0f, kb = 1.0f;
-                if constexpr (KIND == kKvFp8) {
-                    const float* fs = reinterpret_cast<const float*>(ss);
-                    ka = fs[ra], kb = fs[rb], va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int ra = 16 * kt + g, rb = ra + 8;
+                    const float ka = fs[ra], kb = fs[rb];
+                    va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
                     la[kt] = fmaxf(__log2f(va[kt]), -80.0f), lb[kt] = fmaxf(__log2f(vb[kt]), -80.0f);
-                }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    sc[nt][kt][0] *= f0[nt] * ka, sc[nt][kt][1] *= f1[nt] * ka;
-                    sc[nt][kt][2] *= f0[nt] * kb, sc[nt][kt][3] *= f1[nt] * kb;
+                    for (int nt = 0; nt < NT; ++nt) {
+                        sc[nt][kt][0] *= ka, sc[nt][kt][1] *= ka;
+                        sc[nt][kt][2] *= kb, sc[nt][kt][3] *= kb;
+                    }
                 }
             }
+            float x[NT][KT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[nt][kt][i] = i & 1 ? fmaf(sc[nt][kt][i], f1[nt], -ref1[nt]) : fmaf(sc[nt][kt][i], f0[nt], -ref0[nt]);
             if (key0 < span.first || key0 + TK > span.len) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
@@ -451,33 +481,38 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                     const bool oa = ka >= span.first && ka < span.len, ob = kb >= span.first && kb < span.len;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        if (!oa) sc[nt][kt][0] = sc[nt][kt][1] = -INFINITY;
-                        if (!ob) sc[nt][kt][2] = sc[nt][kt][3] = -INFINITY;
+                        if (!oa) x[nt][kt][0] = x[nt][kt][1] = -INFINITY;
+                        if (!ob) x[nt][kt][2] = x[nt][kt][3] = -INFINITY;
                     }
                 }
             }
             bool over = false;
-            float t0[NT], t1[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                t0[nt] = t1[nt] = -INFINITY;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
-                    t0[nt] = fmaxf(t0[nt], fmaxf(sc[nt][kt][0] + xa, sc[nt][kt][2] + xb));
-                    t1[nt] = fmaxf(t1[nt], fmaxf(sc[nt][kt][1] + xa, sc[nt][kt][3] + xb));
-                }
-                over |= t0[nt] > ref0[nt] + kHeadroom || t1[nt] > ref1[nt] + kHeadroom;
-            }
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) over |= x[nt][kt][i] > kHeadroom - (KIND != kKvFp8 ? 0.0f : i < 2 ? la[kt] : lb[kt]);
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
+                    // from the scores themselves (the first reference is too far off to go by x)
+                    float full[KT][4], t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            full[kt][i] = x[nt][kt][i] == -INFINITY ? -INFINITY : sc[nt][kt][i] * (i & 1 ? f1[nt] : f0[nt]);
+                        t0 = fmaxf(t0, fmaxf(full[kt][0] + xa, full[kt][2] + xb));
+                        t1 = fmaxf(t1, fmaxf(full[kt][1] + xa, full[kt][3] + xb));
+                    }
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
-                        t0[nt] = fmaxf(t0[nt], __shfl_xor_sync(0xffffffffu, t0[nt], o));
-                        t1[nt] = fmaxf(t1[nt], __shfl_xor_sync(0xffffffffu, t1[nt], o));
+                        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+                        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
                     }
-                    const float n0 = fmaxf(ref0[nt], t0[nt] - kBelowMax), n1 = fmaxf(ref1[nt], t1[nt] - kBelowMax);
+                    const float n0 = fmaxf(ref0[nt], t0 - kBelowMax), n1 = fmaxf(ref1[nt], t1 - kBelowMax);
                     const float c0 = exp2_approx(ref0[nt] - n0), c1 = exp2_approx(ref1[nt] - n1);
                     ref0[nt] = n0, ref1[nt] = n1;
                     l0[nt] *= c0, l1[nt] *= c1;
@@ -485,6 +520,11 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                     for (int m = 0; m < MT; ++m) {
                         acc[nt][m][0] *= c0, acc[nt][m][1] *= c1;
                         acc[nt][m][2] *= c0, acc[nt][m][3] *= c1;
+                    }
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        x[nt][kt][0] = full[kt][0] - n0, x[nt][kt][1] = full[kt][1] - n1;
+                        x[nt][kt][2] = full[kt][2] - n0, x[nt][kt][3] = full[kt][3] - n1;
                     }
                 }
             }
@@ -497,7 +537,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 for (int kt = 0; kt < KT; ++kt) {
                     float w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[nt][kt][i] - (i & 1 ? ref1[nt] : ref0[nt]));
+                    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[nt][kt][i]);
                     l0[nt] += w[0] + w[2];
                     l1[nt] += w[1] + w[3];
                     if constexpr (KIND == kKvFp8) {
@@ -536,30 +576,54 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                             v[x][0] = lds32(sv + v_offset<RB>(row, g >> 2) + 4 * (g & 3));
                         }
                     }
-                    constexpr int PAIRS = C::EV / 2;  // m-tiles of a run
+                    // A operands: [m-tile][keys 2t, 2t + 1 / 2t + 8, 2t + 9][element 2e / 2e + 1 of the run]
+                    constexpr int PAIRS = C::EV / 2;
+                    uint32_t h[PAIRS][2][2];
 #pragma unroll
-                    for (int e = 0; e < PAIRS; ++e) {
-                        uint32_t h[4];  // elements 2e, 2e + 1 of the four keys
+                    for (int y = 0; y < 2; ++y) {
+                        if constexpr (kBf16) {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if constexpr (kBf16) {
-                                h[x] = v[x][e];
-                            } else if constexpr (KIND == kKvFp8) {
-                                h[x] = e4m3x2_to_f16x2((uint16_t)(v[x][e / 2] >> (16 * (e & 1))));
-                            } else {
-                                const int row = r + (x & 1) + 8 * (x >> 1);
-                                const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + e / 8;
-                                h[x] = mul_f16x2(e2m1x2_to_f16x2(byte_of(v[x][e / 4], e & 3)),
-                                                 ue4m3_shifted(ss[TK * SB + row * SB + block]));
+                            for (int e = 0; e < PAIRS; ++e) {
+                                h[e][y][0] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x5410);
+                                h[e][y][1] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x7632);
+                            }
+                        } else if constexpr (KIND == kKvFp8) {
+                            // the two keys' bytes side by side, then decoded
+#pragma unroll
+                            for (int q = 0; q < WORDS; ++q) {
+                                uint32_t lo[2], hi[2];
+                                e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x5140), lo);
+                                e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x7362), hi);
+                                h[2 * q][y][0] = lo[0], h[2 * q][y][1] = lo[1];
+                                h[2 * q + 1][y][0] = hi[0], h[2 * q + 1][y][1] = hi[1];
+                            }
+                        } else {
+                            // the two keys' codes side by side in each byte, then decoded
+                            const uint8_t* s_row = ss + TK * SB + (r + 8 * y) * SB;
+#pragma unroll
+                            for (int q = 0; q < WORDS; ++q) {
+                                const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + q / 2;
+                                const uint32_t s_v = ue4m3x2_to_f16(s_row[block] + 0x10000u * s_row[SB + block]);
+                                const uint32_t a = v[2 * y][q], c = v[2 * y + 1][q];
+                                uint32_t even[4], odd[4];
+                                e2m1x8_to_f16((a & 0x0F0F0F0Fu) | ((c << 4) & 0xF0F0F0F0u), even);
+                                e2m1x8_to_f16(((a >> 4) & 0x0F0F0F0Fu) | (c & 0xF0F0F0F0u), odd);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    h[4 * q + e][y][0] = mul_f16x2(even[e], s_v);
+                                    h[4 * q + e][y][1] = mul_f16x2(odd[e], s_v);
+                                }
                             }
                         }
-                        const uint32_t a0 = __byte_perm(h[0], h[1], 0x5410), a1 = __byte_perm(h[0], h[1], 0x7632);
-                        const uint32_t a2 = __byte_perm(h[2], h[3], 0x5410), a3 = __byte_perm(h[2], h[3], 0x7632);
+                    }
+#pragma unroll
+                    for (int e = 0; e < PAIRS; ++e) {
                         const int m = i * PAIRS + e;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma<kBf16>(acc[nt][m], a0, a1, a2, a3, pf[nt][kt][0], pf[nt][kt][1]);
-                            if constexpr (kBf16) mma<true>(acc[nt][m], a0, a1, a2, a3, pl[nt][kt][0], pl[nt][kt][1]);
+                            mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pf[nt][kt][0], pf[nt][kt][1]);
+                            if constexpr (kBf16)
+                                mma<true>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
                         }
                     }
                 }
@@ -600,7 +664,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         __syncthreads();
 
         const bool whole = r0 == 0 && r1 == span.rounds;
-        const float unit_scale = KIND == kKvNvfp4 ? 256.0f : 1.0f;  // of the shifted value scales
+        const float unit_scale = KIND == kKvNvfp4 ? kScaleUnit : 1.0f;
         const int slot = 2 * blockIdx.x + (r0 == 0 ? 1 : 0);
         for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
             const int h = i / (D / 4), d = 4 * (i - h * (D / 4));

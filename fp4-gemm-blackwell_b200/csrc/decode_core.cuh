@@ -51,18 +51,31 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// Two E2M1 codes (one byte) -> two fp16 values, exact.
-__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
-    uint32_t r;
-    asm("{\n.reg .b8 b;\ncvt.u8.u32 b, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(r) : "r"(byte));
-    return r;
+// Eight E2M1 codes -> four FP16 pairs, exact; pair i from byte i, the low
+// nibble in the low half.
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&pair)[4]) {
+    asm("{\n"
+        ".reg .b8 b0, b1, b2, b3;\n"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n"
+        "}"
+        : "=r"(pair[0]), "=r"(pair[1]), "=r"(pair[2]), "=r"(pair[3])
+        : "r"(w));
 }
 
-// Two E4M3 codes -> two fp16 values, exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t two) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
-    return r;
+// Four E4M3 codes -> two FP16 pairs, exact.
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t (&pair)[2]) {
+    asm("{\n"
+        ".reg .b16 h0, h1;\n"
+        "mov.b32 {h0, h1}, %2;\n"
+        "cvt.rn.f16x2.e4m3x2 %0, h0;\n"
+        "cvt.rn.f16x2.e4m3x2 %1, h1;\n"
+        "}"
+        : "=r"(pair[0]), "=r"(pair[1])
+        : "r"(w));
 }
 
 __device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) { return __half22float2(*reinterpret_cast<__half2*>(&h)); }
@@ -97,6 +110,14 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(lo) : "f"(a), "f"(b));
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
     return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// Per half: the larger magnitude of two BF16 pairs, NaN if either is; the sign
+// bits of the result mean nothing.
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 
 template <int WIDTH>
@@ -170,11 +191,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// A UE4M3 byte as 2^-8 of its value in both halves: the byte's exponent and
-// mantissa shifted into FP16's (exact, subnormals too).
-__device__ __forceinline__ uint32_t ue4m3_shifted(uint32_t byte) { return byte * 0x00800080u; }
-
-__device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xFFu; }
+// UE4M3 bytes in bits 0-7 and 16-23 as FP16 pair of 2^-8 of their values: the
+// byte's exponent and mantissa moved into FP16's (exact, subnormals too).
+__device__ __forceinline__ uint32_t ue4m3x2_to_f16(uint32_t bytes) { return bytes << 7; }
+constexpr float kScaleUnit = 256.0f;
 
 }  // namespace decode
 

@@ -43,8 +43,6 @@ namespace {
 
 using namespace decode;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 128;                     // elements of K of one step
 constexpr int kStageBytes = 5 * 512;           // a warp's step: four code pieces and the scales, 16 bytes a lane
 constexpr int kStages = 3;
@@ -66,13 +64,15 @@ struct GemvParams {
 // eight lanes of one phase of the reads meet distinct banks.
 __device__ __forceinline__ int x_offset(int row_bytes, int g, int c) { return g * row_bytes + 16 * (c ^ ((c >> 3) & 1) ^ ((g & 1) << 1)); }
 
-template <int NT, int RG>
-__global__ void __launch_bounds__(kThreads) gemv_kernel(const __grid_constant__ GemvParams p) {
+template <int NT, int RG, int W>
+__global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ GemvParams p) {
+    constexpr int kWarps = W, kThreads = 32 * W;
     constexpr int KS = kWarps / RG;                   // slices of K
     constexpr int KC = kChunkBytes / (2 * 8 * NT);    // elements of a chunk
     constexpr int kChunkSteps = KC / kStep;
     constexpr int kRowBytes = 2 * KC;
     constexpr int kPieces = KC / 8 / 32;              // 16-byte pieces of a row's chunk a lane
+    constexpr int kHeld = (8 * NT + kWarps - 1) / kWarps;  // rows of x that a warp converts
     static_assert(kChunkSteps % KS == 0 || KS % kChunkSteps == 0, "slices take whole chunks in turn");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_factor[2][8 * NT];
@@ -106,12 +106,12 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
 
-    // ---- x, chunk by chunk: warp w holds rows w and w + 8 between the global read and the shared write
-    uint4 held[NT][kPieces];
+    // ---- x, chunk by chunk: warp w holds rows w, w + W between the global read and the shared write
+    uint4 held[kHeld][kPieces];
     auto fetch = [&](int c) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int row = warp + 8 * nt;
+        for (int nt = 0; nt < kHeld; ++nt) {
+            const int row = warp + kWarps * nt;
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 held[nt][i] = make_uint4(0u, 0u, 0u, 0u);
@@ -134,17 +134,16 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const __grid_constant__ 
     auto put = [&](int c) {
         uint8_t* to = sx + (c & 1) * kChunkBytes;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int row = warp + 8 * nt;
+        for (int nt = 0; nt < kHeld; ++nt) {
+            const int row = warp + kWarps * nt;
             if (row >= rows) continue;  // such columns are never stored
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const uint32_t w[4] = {held[nt][i].x, held[nt][i].y, held[nt][i].z, held[nt][i].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = max(top, max((w[e] & 0x7FFFu) << 16, w[e] & 0x7FFF0000u));
+                top = max_abs_bf16x2(max_abs_bf16x2(top, held[nt][i].x), held[nt][i].y);
+                top = max_abs_bf16x2(max_abs_bf16x2(top, held[nt][i].z), held[nt][i].w);
             }
-            top = group_umax<32>(top);
+            top = group_umax<32>(max((top << 16) & 0x7FFF0000u, top & 0x7FFF0000u));
             const int up = min(max(141 - (int)(top >> 23), -126), 126);
             const float f = __int_as_float((127 + up) << 23);
 #pragma unroll
@@ -170,6 +169,9 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const __grid_constant__ 
             for (int i = 0; i < 4; ++i) sum[a][nt][i] = 0.0f;
 
     const uint32_t pick0 = t & 1 ? 0x4242u : 0x4040u, pick1 = t & 1 ? 0x4343u : 0x4141u;  // the lane's two scale bytes
+    // x_offset of chunk 4 t + u of the lane's row: the permutation moves u alone
+    const uint8_t* x_lane = sx + g * kRowBytes + 64 * t;
+    const int x_swap = 16 * ((t >> 1) ^ ((g & 1) << 1));
     int i = 0;
     for (int c = 0; c < chunks; ++c) {
         if (c + 1 < chunks) fetch(c + 1);
@@ -191,32 +193,29 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const __grid_constant__ 
             for (int q = 0; q < 4; ++q) {
                 const uint4 v = lds128(st + 512 * q);
                 w[q][0] = v.x, w[q][1] = v.y, w[q][2] = v.z, w[q][3] = v.w;
-                s0[q] = __byte_perm(sw[q], 0u, pick0) << 7;
-                s1[q] = __byte_perm(sw[q], 0u, pick1) << 7;
+                s0[q] = ue4m3x2_to_f16(__byte_perm(sw[q], 0u, pick0));
+                s1[q] = ue4m3x2_to_f16(__byte_perm(sw[q], 0u, pick1));
             }
             issue(i + kStages - 1);
-            const uint8_t* xs = sx + (c & 1) * kChunkBytes + g * kRowBytes;
-            const int c0 = (ks + i * KS - c * kChunkSteps) * 16 + 4 * t;
+            const uint8_t* xs = x_lane + (c & 1) * kChunkBytes + (ks + i * KS - c * kChunkSteps) * 256;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 uint4 xv[NT];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) xv[nt] = lds128(xs + 8 * nt * kRowBytes + x_offset(0, g, c0 + u));
+                for (int nt = 0; nt < NT; ++nt) xv[nt] = lds128(xs + 8 * nt * kRowBytes + ((16 * u) ^ x_swap));
+                uint32_t a[4][4];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t a[4][2];
+                for (int q = 0; q < 4; ++q) {
+                    e2m1x8_to_f16(w[q][u], a[q]);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t s = u < 2 ? s0[q] : s1[q];
-                        a[q][0] = mul_f16x2(e2m1x2_to_f16x2(byte_of(w[q][u], 2 * half)), s);
-                        a[q][1] = mul_f16x2(e2m1x2_to_f16x2(byte_of(w[q][u], 2 * half + 1)), s);
-                    }
+                    for (int e = 0; e < 4; ++e) a[q][e] = mul_f16x2(a[q][e], u < 2 ? s0[q] : s1[q]);
+                }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint32_t b0 = half ? xv[nt].z : xv[nt].x, b1 = half ? xv[nt].w : xv[nt].y;
-                        mma<false>(acc[0][nt], a[0][0], a[1][0], a[0][1], a[1][1], b0, b1);
-                        mma<false>(acc[1][nt], a[2][0], a[3][0], a[2][1], a[3][1], b0, b1);
-                    }
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma<false>(acc[0][nt], a[0][0], a[1][0], a[0][1], a[1][1], xv[nt].x, xv[nt].y);
+                    mma<false>(acc[1][nt], a[2][0], a[3][0], a[2][1], a[3][1], xv[nt].x, xv[nt].y);
+                    mma<false>(acc[0][nt], a[0][2], a[1][2], a[0][3], a[1][3], xv[nt].z, xv[nt].w);
+                    mma<false>(acc[1][nt], a[2][2], a[3][2], a[2][3], a[3][3], xv[nt].z, xv[nt].w);
                 }
             }
         }
@@ -261,11 +260,11 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const __grid_constant__ 
     }
 }
 
-constexpr int kSmem = kWarps * kStages * kStageBytes + 2 * kChunkBytes;
 constexpr int kMaxDevices = 64;
 
-template <int NT, int RG>
+template <int NT, int RG, int W>
 cudaError_t launch(const GemvParams& p, cudaStream_t st) {
+    constexpr int kSmem = W * kStages * kStageBytes + 2 * kChunkBytes;
     static std::mutex mu;
     static bool ready[kMaxDevices];
     int dev = 0;
@@ -275,23 +274,23 @@ cudaError_t launch(const GemvParams& p, cudaStream_t st) {
     {
         std::lock_guard<std::mutex> lk(mu);
         if (!ready[dev]) {
-            e = cudaFuncSetAttribute(gemv_kernel<NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+            e = cudaFuncSetAttribute(gemv_kernel<NT, RG, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
             if (e != cudaSuccess) return e;
             ready[dev] = true;
         }
     }
     const long blocks = ((long)p.n + 127) / 128 * (4 / RG);
     const dim3 grid((unsigned)blocks, (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
-    gemv_kernel<NT, RG><<<grid, kThreads, kSmem, st>>>(p);
+    gemv_kernel<NT, RG, W><<<grid, 32 * W, kSmem, st>>>(p);
     return cudaGetLastError();
 }
 
 template <int NT>
 cudaError_t launch_rows(const GemvParams& p, cudaStream_t st) {
     const long blocks = ((long)p.n + 127) / 128;
-    if (blocks >= 148) return launch<NT, 4>(p, st);
-    if (blocks >= 74) return launch<NT, 2>(p, st);
-    return launch<NT, 1>(p, st);
+    if (blocks >= 120) return launch<NT, 4, 16>(p, st);
+    if (blocks >= 74) return launch<NT, 2, 8>(p, st);
+    return launch<NT, 1, 8>(p, st);
 }
 
 }  // namespace
@@ -313,7 +312,7 @@ FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const
     }
     const bool vec = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     const GemvParams p{static_cast<const uint16_t*>(x), c.fp4, c.sf, static_cast<uint16_t*>(y),
-                       static_cast<const uint16_t*>(bias), ldx, ldy, m, n_out, k_in, c.K, vec, c.w_alpha * 256.0f};
+                       static_cast<const uint16_t*>(bias), ldx, ldy, m, n_out, k_in, c.K, vec, c.w_alpha * kScaleUnit};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launch_status(m <= 8 ? launch_rows<1>(p, st) : launch_rows<2>(p, st), "fp4b_gemv_cached");
 }

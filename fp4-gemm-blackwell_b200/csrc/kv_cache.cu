@@ -308,21 +308,24 @@ __device__ __forceinline__ uint4 read_eight(const void* base, const void* scales
     } else if constexpr (KIND == kKvFp8) {
         const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + (size_t)row * d + e);
         const float s = static_cast<const float*>(scales)[row];
+        uint32_t h[4], lo[2], hi[2];
+        decode::e4m3x4_to_f16(w.x, lo);
+        decode::e4m3x4_to_f16(w.y, hi);
+        h[0] = lo[0], h[1] = lo[1], h[2] = hi[0], h[3] = hi[1];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t two = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
-            const float2 f = decode::f16x2_to_float2(decode::e4m3x2_to_f16x2((uint16_t)two));
-            x[2 * i] = f.x * s;
-            x[2 * i + 1] = f.y * s;
+            const float2 f = decode::f16x2_to_float2(h[i]);
+            x[2 * i] = f.x * s, x[2 * i + 1] = f.y * s;
         }
     } else {
         const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + (size_t)row * (d >> 1) + (e >> 1));
         const float s = decode::ue4m3_float(static_cast<const uint8_t*>(scales)[(size_t)row * (d >> 4) + (e >> 4)]);
+        uint32_t h[4];
+        decode::e2m1x8_to_f16(w, h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = decode::f16x2_to_float2(decode::e2m1x2_to_f16x2((w >> (8 * i)) & 0xFFu));
-            x[2 * i] = f.x * s;
-            x[2 * i + 1] = f.y * s;
+            const float2 f = decode::f16x2_to_float2(h[i]);
+            x[2 * i] = f.x * s, x[2 * i + 1] = f.y * s;
         }
     }
     return make_uint4(decode::pack_bf16(x[0], x[1]), decode::pack_bf16(x[2], x[3]), decode::pack_bf16(x[4], x[5]),
