@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     __shared__ float s_m[kWarps][HEADS], s_l[kWarps][HEADS];
     __shared__ int s_last;
 
+    chain();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int units = p.cache.kv_heads * p.group_tiles;
 
@@ -747,7 +748,7 @@ Layout layout_of(int sms, int heads, int d) {
     Layout w;
     const long ctas = (long)sms * kMaxCtasPerSm;
     w.slots = 2 * ctas;
-    w.ml = (ctas * 4 + 255) / 256 * 256;
+    w.ml = FP4B_DECODE_COUNTER_BYTES;
     w.acc = w.ml + w.slots * heads * 8;
     w.bytes = w.acc + w.slots * heads * d * 4;
     return w;
@@ -765,7 +766,7 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const int sms = sm_count();
-    if (sms <= 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    if (sms <= 0 || sms * kMaxCtasPerSm * 4 > FP4B_DECODE_COUNTER_BYTES || dev >= kMaxDevices) return cudaErrorInvalidDevice;
     {
         std::lock_guard<std::mutex> lk(mu);
         if (!resident[dev]) {
@@ -784,8 +785,7 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     // No more CTAs than the page table has rounds for (and one for each empty sequence's row).
     const long keys = (long)p.table_width << p.page_shift;
     const long most = (long)p.batch * std::max(1l, (keys + C::ROUND - 1) / C::ROUND * p.cache.kv_heads * p.group_tiles);
-    kernel<<<(unsigned)std::min<long>(resident[dev], most), kThreads, C::SMEM, st>>>(p);
-    return cudaGetLastError();
+    return launch_chained(kernel, dim3((unsigned)std::min<long>(resident[dev], most)), kThreads, C::SMEM, st, p);
 }
 
 template <int KIND, int D>
@@ -819,40 +819,42 @@ FP4B_EXPORT long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int 
     return layout_of(sms, unit_heads(q_heads / kv_heads), head_dim).bytes;
 }
 
-FP4B_EXPORT int fp4b_decode_attention(const void* q, long q_sb, long q_sh, int batch, int q_heads,
-                                      const fp4b_kv_cache* cache, const int* page_table, long table_stride,
-                                      int table_width, const int* seq_lens, float scale, int window,
-                                      const float* sinks, void* out, float* lse, void* workspace,
-                                      long workspace_bytes, void* stream) {
+FP4B_EXPORT int fp4b_decode_attention(const fp4b_decode* call, void* stream) {
+    if (!call) {
+        set_last_error("fp4b_decode_attention: null arguments");
+        return -1;
+    }
+    const fp4b_decode& c = *call;
+    const fp4b_kv_cache* cache = c.cache;
     const char* why = kv_cache_check(cache);
-    if (!why && (batch < 0 || q_heads <= 0 || q_heads % cache->kv_heads))
+    if (!why && (c.batch < 0 || c.q_heads <= 0 || c.q_heads % cache->kv_heads))
         why = "query heads must be a multiple of the cache's heads";
-    if (!why && batch > 0 && (!q || !out || !seq_lens || (table_width > 0 && !page_table))) why = "null tensor";
-    if (!why && (table_width < 0 || table_stride < table_width)) why = "bad page table";
-    if (!why && (long)table_width * cache->page_size > 0x7fff0000L) why = "more than 2^31 keys in one sequence";
-    if (!why && (long)batch * q_heads > 0x7fffffffL) why = "more than 2^31 output rows";
-    if (!why && (window < 0 || !std::isfinite(scale))) why = "window must not be negative, scale finite";
-    if (!why && ((reinterpret_cast<uintptr_t>(q) & 7) || q_sb % 4 || q_sh % 4 || (reinterpret_cast<uintptr_t>(out) & 15)))
+    if (!why && c.batch > 0 && (!c.q || !c.out || !c.seq_lens || (c.table_width > 0 && !c.page_table))) why = "null tensor";
+    if (!why && (c.table_width < 0 || c.table_stride < c.table_width)) why = "bad page table";
+    if (!why && (long)c.table_width * cache->page_size > 0x7fff0000L) why = "more than 2^31 keys in one sequence";
+    if (!why && (long)c.batch * c.q_heads > 0x7fffffffL) why = "more than 2^31 output rows";
+    if (!why && (c.window < 0 || !std::isfinite(c.scale))) why = "window must not be negative, scale finite";
+    if (!why && ((reinterpret_cast<uintptr_t>(c.q) & 7) || c.q_sb % 4 || c.q_sh % 4 || (reinterpret_cast<uintptr_t>(c.out) & 15)))
         why = "queries must be 8-byte aligned rows, the output 16-byte aligned";
-    if (!why && batch > 0 &&
-        (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-         workspace_bytes < fp4b_decode_attention_workspace(q_heads, cache->kv_heads, cache->head_dim)))
+    if (!why && c.batch > 0 &&
+        (!c.workspace || (reinterpret_cast<uintptr_t>(c.workspace) & 15) ||
+         c.workspace_bytes < fp4b_decode_attention_workspace(c.q_heads, cache->kv_heads, cache->head_dim)))
         why = "workspace too small or misaligned";
     if (why) {
         set_last_error("fp4b_decode_attention: %s", why);
         return -1;
     }
-    if (batch == 0) return 0;
+    if (c.batch == 0) return 0;
     AttentionParams p{};
-    p.q = static_cast<const uint16_t*>(q), p.q_sb = q_sb, p.q_sh = q_sh;
-    p.batch = batch, p.q_heads = q_heads, p.group = q_heads / cache->kv_heads;
+    p.q = static_cast<const uint16_t*>(c.q), p.q_sb = c.q_sb, p.q_sh = c.q_sh;
+    p.batch = c.batch, p.q_heads = c.q_heads, p.group = c.q_heads / cache->kv_heads;
     p.cache = *cache;
     while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
-    p.table = page_table, p.table_stride = table_stride, p.table_width = table_width;
-    p.lens = seq_lens, p.scale2 = scale * kLog2e, p.window = window, p.sinks = sinks;
-    p.out = static_cast<uint16_t*>(out), p.lse = lse, p.err = device_error_word();
+    p.table = c.page_table, p.table_stride = c.table_stride, p.table_width = c.table_width;
+    p.lens = c.seq_lens, p.scale2 = c.scale * kLog2e, p.window = c.window, p.sinks = c.sinks;
+    p.out = static_cast<uint16_t*>(c.out), p.lse = c.lse, p.err = device_error_word();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    uint8_t* ws = static_cast<uint8_t*>(c.workspace);
     const cudaError_t e = cache->kind == kKvBf16 ? launch_dim<kKvBf16>(p, ws, st)
                           : cache->kind == kKvFp8 ? launch_dim<kKvFp8>(p, ws, st)
                                                   : launch_dim<kKvNvfp4>(p, ws, st);

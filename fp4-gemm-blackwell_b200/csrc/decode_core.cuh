@@ -17,6 +17,7 @@
 
 #include "fp4gemm.h"
 #include "nvfp4_codec.cuh"
+#include "ptx_sm100.cuh"
 
 namespace fp4b {
 
@@ -195,6 +196,31 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // byte's exponent and mantissa moved into FP16's (exact, subnormals too).
 __device__ __forceinline__ uint32_t ue4m3x2_to_f16(uint32_t bytes) { return bytes << 7; }
 constexpr float kScaleUnit = 256.0f;
+
+// Every kernel of the decode side starts with this: it was launched while the
+// kernel before it in the stream may still run, waits here until that one has
+// completed, and lets the next one come the same way.  Nothing in global memory
+// is touched before.  In a chain of such kernels this hides the launch of each
+// behind the one before (about 2 us a kernel on B200).
+__device__ __forceinline__ void chain() {
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+}
+
+template <typename Params>
+cudaError_t launch_chained(void (*kernel)(Params), dim3 grid, int threads, int smem, cudaStream_t stream, const Params& p) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, p);
+}
 
 }  // namespace decode
 

@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ Ge
     static_assert(kChunkSteps % KS == 0 || KS % kChunkSteps == 0, "slices take whole chunks in turn");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_factor[2][8 * NT];
+    chain();
     uint8_t* sx = smem + kWarps * kStages * kStageBytes;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -281,8 +282,7 @@ cudaError_t launch(const GemvParams& p, cudaStream_t st) {
     }
     const long blocks = ((long)p.n + 127) / 128 * (4 / RG);
     const dim3 grid((unsigned)blocks, (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
-    gemv_kernel<NT, RG, W><<<grid, 32 * W, kSmem, st>>>(p);
-    return cudaGetLastError();
+    return launch_chained(gemv_kernel<NT, RG, W>, grid, 32 * W, kSmem, st, p);
 }
 
 template <int NT>

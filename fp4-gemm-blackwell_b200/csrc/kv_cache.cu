@@ -16,8 +16,9 @@
 // two elements of a rotated pair meet in one lane (when all of the row is
 // rotated, or in pairs), a half's 16-element blocks are four lanes each, and
 // the loads of a row are two runs of 8 bytes a lane.  A warp stays with one
-// token and walks its heads, so the table row and the norm weights are read
-// once a token.
+// token and walks several of its heads, kBatch rounds of 32 / L heads in
+// flight at a time; the table row is read once and held.  With few tokens each
+// warp has one round, so that a single token's heads still spread over the GPU.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -34,6 +35,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kBatch = 4;
 
 struct RowsParams {
     const uint16_t *q, *k, *v;  // BF16 rows, null where absent
@@ -49,7 +51,8 @@ struct RowsParams {
     uint16_t *q_out, *k_out;  // BF16 [tokens, heads, d]
     fp4b_kv_cache cache;      // keys and values go here unless KIND is kKvNone
     int page_shift;
-    int rounds;  // head groups of 32 / L heads that one warp walks
+    int rounds;  // rounds of 32 / L heads that one warp walks
+    int walks;   // warps a token: ceil(heads / (rounds * 32 / L))
     int* err;
 };
 
@@ -61,12 +64,19 @@ __device__ __forceinline__ void unpack4(uint2 w, float (&x)[4]) {
 }
 
 // Rotates the lane's two chunks.  c, s: the table's factors for the lane's
-// elements (a: first chunk, b: second).
-template <int L>
+// elements (a: first chunk, b: second; with FULL, the whole row in halves, b's
+// are a's).
+template <int L, bool FULL>
 __device__ __forceinline__ void rotate(const RowsParams& p, float (&a)[4], float (&b)[4], const float (&ca)[4],
                                        const float (&sa)[4], const float (&cb)[4], const float (&sb)[4], int l) {
-    const int half = p.rot >> 1;
-    if (p.pairs) {
+    if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = a[i], y = b[i];
+            a[i] = x * ca[i] - y * sa[i];
+            b[i] = y * ca[i] + x * sa[i];
+        }
+    } else if (p.pairs) {
         // Pair (2i, 2i + 1) lies in one lane; ca[2i] = ca[2i + 1].
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
@@ -77,23 +87,16 @@ __device__ __forceinline__ void rotate(const RowsParams& p, float (&a)[4], float
             b[i] = u * cb[i] - v * sb[i];
             b[i + 1] = v * cb[i] + u * sb[i];
         }
-    } else if (p.rot == p.d) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = a[i], y = b[i];
-            a[i] = x * ca[i] - y * sa[i];
-            b[i] = y * ca[i] + x * sa[i];
-        }
     } else {
         // Part of the row is rotated: chunk c's partner is chunk c +- rot / 8,
         // held by another lane.  Chunks 0 .. d/8 - 1 are the lanes' first
         // ones, d/8 .. d/4 - 1 their second ones.
-        const int shift = half >> 2, lanes = p.d >> 3;
+        const int half = p.rot >> 1, shift = half >> 2, lanes = p.d >> 3;
         const int group = (threadIdx.x & 31) & ~(L - 1);
         float pa[4], pb[4];
-        const int ta = l < shift ? l + shift : l - shift;                  // partner of the first chunk
-        const int tb = l + lanes < shift ? l + lanes + shift : l + lanes - shift;  // of the second
-        const int la = group + (ta >= lanes ? ta - lanes : max(ta, 0)), lb = group + (tb >= lanes ? tb - lanes : max(tb, 0));
+        const int ta = l < shift ? l + shift : l - shift;  // partner of the first chunk
+        const int tb = l + lanes - shift;                  // of the second (never in the row's first rot / 8 chunks)
+        const int la = group + (ta >= lanes ? ta - lanes : ta), lb = group + (tb >= lanes ? tb - lanes : tb);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float fa = __shfl_sync(0xffffffffu, a[i], la), sa2 = __shfl_sync(0xffffffffu, b[i], la);
@@ -122,27 +125,25 @@ __device__ __forceinline__ void factors(const RowsParams& p, const float* row, i
     }
 }
 
-// Four values of a block's lane -> its four E2M1 codes; `byte`: the block's
-// scale.  The four lanes of the block call it together.
-__device__ __forceinline__ uint32_t nvfp4_four(const float (&x)[4], uint32_t& byte) {
+// |x|max of a block from its four lanes' values, as the codec takes it: NaN is
+// skipped.  `literal`: the block holds a NaN, an infinity or a huge value.
+__device__ __forceinline__ float block_absmax(const float (&x)[4], bool& literal) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     top = decode::group_umax<4>(top);
+    literal = top >= kFastAbsmaxF32Limit;
     float amax = __uint_as_float(top);
-    const bool literal = top >= kFastAbsmaxF32Limit;
-    if (literal) {  // the codec's absmax skips NaN
-        amax = 0.0f;
-        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    }
     if (__any_sync(0xffffffffu, literal)) {
-        float other = amax;
-        other = fmaxf(other, __shfl_xor_sync(0xffffffffu, other, 2));
-        other = fmaxf(other, __shfl_xor_sync(0xffffffffu, other, 1));
-        if (literal) amax = other;
+        float f = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 2));
+        f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
+        if (literal) amax = f == f ? f : 0.0f;
     }
-    byte = ue4m3_encode(fmaxf(__fdiv_rn(amax, 6.0f), kScaleMin));
-    const float inv = __fdiv_rn(1.0f, ue4m3_decode((uint8_t)byte));
+    return amax;
+}
+
+__device__ __forceinline__ uint32_t block_codes(const float (&x)[4], float inv, bool literal) {
     if (literal) {
         uint32_t codes = 0;
         for (int i = 0; i < 4; ++i) codes |= (uint32_t)e2m1_scan(__fmul_rn(x[i], inv)) << (4 * i);
@@ -178,8 +179,17 @@ __device__ __forceinline__ void store_row(const RowsParams& p, bool value, long 
         *reinterpret_cast<uint32_t*>(out + half + 4 * l) = decode::e4m3x4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv);
         if (l == 0) static_cast<float*>(scales)[row] = __fdiv_rn(amax, kFp8Max);
     } else if constexpr (KIND == kKvNvfp4) {
-        uint32_t sa, sb;
-        const uint32_t ca = nvfp4_four(a, sa), cb = nvfp4_four(b, sb);
+        // The lane's two blocks: even lanes work out the first's scale, odd ones
+        // the second's, and they exchange them.
+        bool lit_a, lit_b;
+        const float max_a = block_absmax(a, lit_a), max_b = block_absmax(b, lit_b);
+        const bool odd = l & 1;
+        const uint32_t byte = ue4m3_encode(fmaxf(__fdiv_rn(odd ? max_b : max_a, 6.0f), kScaleMin));
+        const float inv = __fdiv_rn(1.0f, ue4m3_decode((uint8_t)byte));
+        const uint32_t other_byte = __shfl_xor_sync(0xffffffffu, byte, 1);
+        const float other_inv = __shfl_xor_sync(0xffffffffu, inv, 1);
+        const uint32_t sa = odd ? other_byte : byte, sb = odd ? byte : other_byte;
+        const uint32_t ca = block_codes(a, odd ? other_inv : inv, lit_a), cb = block_codes(b, odd ? inv : other_inv, lit_b);
         if (!live) return;
         uint8_t* out = static_cast<uint8_t*>(base) + (size_t)row * half;
         *reinterpret_cast<uint16_t*>(out + 2 * l) = (uint16_t)ca;
@@ -192,36 +202,40 @@ __device__ __forceinline__ void store_row(const RowsParams& p, bool value, long 
     }
 }
 
-template <int KIND, int L>
+template <int KIND, int L, bool FULL>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kPer = 32 / L;  // heads of a token that a warp holds at once
+    decode::chain();
     const int lane = threadIdx.x & 31, l = lane & (L - 1), sub = lane / L;
     const int heads = p.q_heads + (p.k ? p.kv_heads : 0) + (p.v ? p.kv_heads : 0);
-    const int walks = (heads + kPer * p.rounds - 1) / (kPer * p.rounds);  // warps a token
-    const long unit = (long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const long t = unit / walks;
-    if (t >= p.tokens) return;
-    const int first = (int)(unit - t * walks) * kPer * p.rounds + sub;
+    const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const unsigned token = unit / (unsigned)p.walks;
+    if (token >= (unsigned)p.tokens) return;
+    const long t = token;
+    const int first = (int)(unit - token * p.walks) * kPer * p.rounds;
     const bool inside = l < (p.d >> 3);
     const int half = p.d >> 1;
 
-    // The token's table row, its slot, and the norm weights of the lane's elements.
-    float ca[4], sa[4], cb[4], sb[4];
-    if (p.rope) {
-        const long pos = decode::load_index(p.positions, t, p.pos64);
-        const bool ok = pos >= 0 && pos < p.rope_rows;
-        if (!ok && lane == 0) decode::report(p.err, kErrPositionRange);
-        const float* row = p.rope + (ok ? pos : 0) * p.rot;
+    uint2 wa[kBatch], wb[kBatch];  // the lane's chunks of the next rounds' rows
+    auto fetch = [&](int r0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ca[i] = cb[i] = 1.0f;
-            sa[i] = sb[i] = 0.0f;
-            if (inside && ok) {
-                factors(p, row, 4 * l + i, ca[i], sa[i]);
-                factors(p, row, half + 4 * l + i, cb[i], sb[i]);
+        for (int r = 0; r < kBatch; ++r) {
+            const int h = first + (r0 + r) * kPer + sub;
+            wa[r] = wb[r] = make_uint2(0u, 0u);
+            if (r0 + r < p.rounds && h < heads && inside) {
+                const int hk = h - p.q_heads;
+                const uint16_t* src;
+                if (hk < 0) src = p.q + t * p.q_st + h * p.q_sh;
+                else if (p.k && hk < p.kv_heads) src = p.k + t * p.k_st + hk * p.k_sh;
+                else src = p.v + t * p.v_st + (p.k ? hk - p.kv_heads : hk) * p.v_sh;
+                wa[r] = *reinterpret_cast<const uint2*>(src + 4 * l);
+                wb[r] = *reinterpret_cast<const uint2*>(src + half + 4 * l);
             }
         }
-    }
+    };
+    fetch(0);
+
+    // The token's slot, its table row, and the norm weights of the lane's elements.
     long row0 = -1;  // cache row of head 0
     if constexpr (KIND != kKvNone) {
         const long slot = decode::load_index(p.slots, t, p.slot64);
@@ -233,59 +247,84 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant
                 decode::report(p.err, kErrSlotRange);
         }
     }
-    for (int r = 0; r < p.rounds; ++r) {
-        const int h = first + r * kPer;
-        const bool query = h < p.q_heads;
-        const int hk = h - p.q_heads;
-        const bool key = !query && p.k && hk < p.kv_heads;
-        const int hv = p.k ? hk - p.kv_heads : hk;
-        const bool live = h < heads && inside;
-        const uint16_t* src = query ? p.q + t * p.q_st + h * p.q_sh
-                              : key ? p.k + t * p.k_st + hk * p.k_sh
-                                    : p.v + t * p.v_st + hv * p.v_sh;
-        float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            unpack4(*reinterpret_cast<const uint2*>(src + 4 * l), a);
-            unpack4(*reinterpret_cast<const uint2*>(src + half + 4 * l), b);
-        }
-        const uint16_t* weight = query ? p.q_weight : p.k_weight;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += a[i] * a[i] + b[i] * b[i];
-        sum = decode::group_sum<L>(sum);
-        if ((query || key) && weight && live) {
-            const float inv = rsqrtf(sum / (float)p.d + p.eps);
-            float wa[4], wb[4];
-            unpack4(*reinterpret_cast<const uint2*>(weight + 4 * l), wa);
-            unpack4(*reinterpret_cast<const uint2*>(weight + half + 4 * l), wb);
+    float ca[4], sa[4], cb[4], sb[4];
+    if (p.rope) {
+        const long pos = decode::load_index(p.positions, t, p.pos64);
+        const bool ok = pos >= 0 && pos < p.rope_rows;
+        if (!ok && lane == 0) decode::report(p.err, kErrPositionRange);
+        const float* row = p.rope + (ok ? pos : 0) * p.rot;
+        if constexpr (FULL) {  // rot == d, 16-byte aligned table
+            const float4 c = inside ? *reinterpret_cast<const float4*>(row + 4 * l) : make_float4(1.f, 1.f, 1.f, 1.f);
+            const float4 s = inside ? *reinterpret_cast<const float4*>(row + half + 4 * l) : make_float4(0.f, 0.f, 0.f, 0.f);
+            ca[0] = ok ? c.x : 1.f, ca[1] = ok ? c.y : 1.f, ca[2] = ok ? c.z : 1.f, ca[3] = ok ? c.w : 1.f;
+            sa[0] = ok ? s.x : 0.f, sa[1] = ok ? s.y : 0.f, sa[2] = ok ? s.z : 0.f, sa[3] = ok ? s.w : 0.f;
+        } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                a[i] = a[i] * inv * wa[i];
-                b[i] = b[i] * inv * wb[i];
-            }
-        }
-        if (p.rope) {
-            float ra[4] = {a[0], a[1], a[2], a[3]}, rb[4] = {b[0], b[1], b[2], b[3]};
-            rotate<L>(p, ra, rb, ca, sa, cb, sb, l);
-            if (query || key) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    a[i] = ra[i];
-                    b[i] = rb[i];
+                ca[i] = cb[i] = 1.0f;
+                sa[i] = sb[i] = 0.0f;
+                if (inside && ok) {
+                    factors(p, row, 4 * l + i, ca[i], sa[i]);
+                    factors(p, row, half + 4 * l + i, cb[i], sb[i]);
                 }
             }
         }
-        if (live && (query || (key && KIND == kKvNone))) {
-            uint16_t* out = query ? p.q_out + ((size_t)t * p.q_heads + h) * p.d : p.k_out + ((size_t)t * p.kv_heads + hk) * p.d;
-            *reinterpret_cast<uint2*>(out + 4 * l) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
-            *reinterpret_cast<uint2*>(out + half + 4 * l) =
-                make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
+    }
+
+    for (int r0 = 0; r0 < p.rounds; r0 += kBatch) {
+#pragma unroll
+        for (int r = 0; r < kBatch; ++r) {
+            if (r0 + r >= p.rounds) break;
+            const int h = first + (r0 + r) * kPer + sub;
+            const int hk = h - p.q_heads;
+            const bool query = hk < 0, key = !query && p.k && hk < p.kv_heads;
+            const int hv = p.k ? hk - p.kv_heads : hk;
+            const bool live = h < heads && inside;
+            float a[4], b[4];
+            unpack4(wa[r], a);
+            unpack4(wb[r], b);
+            const uint16_t* weight = query ? p.q_weight : key ? p.k_weight : nullptr;
+            if (__any_sync(0xffffffffu, weight != nullptr)) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += a[i] * a[i] + b[i] * b[i];
+                sum = decode::group_sum<L>(sum);
+                if (weight && inside) {
+                    const float inv = rsqrtf(sum / (float)p.d + p.eps);
+                    float na[4], nb[4];
+                    unpack4(__ldg(reinterpret_cast<const uint2*>(weight + 4 * l)), na);
+                    unpack4(__ldg(reinterpret_cast<const uint2*>(weight + half + 4 * l)), nb);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        a[i] = a[i] * inv * na[i];
+                        b[i] = b[i] * inv * nb[i];
+                    }
+                }
+            }
+            if (p.rope && __any_sync(0xffffffffu, query || key)) {
+                float ra[4] = {a[0], a[1], a[2], a[3]}, rb[4] = {b[0], b[1], b[2], b[3]};
+                rotate<L, FULL>(p, ra, rb, ca, sa, cb, sb, l);
+                if (query || key) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        a[i] = ra[i];
+                        b[i] = rb[i];
+                    }
+                }
+            }
+            if (live && (query || (key && KIND == kKvNone))) {
+                uint16_t* out = query ? p.q_out + ((size_t)t * p.q_heads + h) * p.d : p.k_out + ((size_t)t * p.kv_heads + hk) * p.d;
+                *reinterpret_cast<uint2*>(out + 4 * l) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
+                *reinterpret_cast<uint2*>(out + half + 4 * l) =
+                    make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
+            }
+            if constexpr (KIND != kKvNone) {
+                const bool stored = live && !query && row0 >= 0;
+                if (__any_sync(0xffffffffu, stored))
+                    store_row<KIND, L>(p, !key, row0 + (long)(key ? hk : hv) * p.cache.page_size, stored, l, a, b);
+            }
         }
-        if constexpr (KIND != kKvNone) {
-            const long row = row0 + (long)(key ? hk : hv) * p.cache.page_size;
-            if (__any_sync(0xffffffffu, live && !query))
-                store_row<KIND, L>(p, !key, row, live && !query && row0 >= 0, l, a, b);
-        }
+        if (r0 + kBatch < p.rounds) fetch(r0 + kBatch);
     }
 }
 
@@ -294,7 +333,8 @@ struct ReadParams {
     int page_shift;
     const void* slots;
     int slot64;
-    long rows;  // slots x heads
+    int count;
+    int walks;  // warps a slot
     uint16_t *k, *v;
     int* err;
 };
@@ -302,7 +342,7 @@ struct ReadParams {
 // Eight elements of a row as BF16.
 template <int KIND>
 __device__ __forceinline__ uint4 read_eight(const void* base, const void* scales, long row, int d, int e) {
-    float x[8];
+    [[maybe_unused]] float x[8];
     if constexpr (KIND == kKvBf16) {
         return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + (size_t)row * d + e);
     } else if constexpr (KIND == kKvFp8) {
@@ -328,32 +368,48 @@ __device__ __forceinline__ uint4 read_eight(const void* base, const void* scales
             x[2 * i] = f.x * s, x[2 * i + 1] = f.y * s;
         }
     }
-    return make_uint4(decode::pack_bf16(x[0], x[1]), decode::pack_bf16(x[2], x[3]), decode::pack_bf16(x[4], x[5]),
-                      decode::pack_bf16(x[6], x[7]));
+    if constexpr (KIND != kKvBf16)
+        return make_uint4(decode::pack_bf16(x[0], x[1]), decode::pack_bf16(x[2], x[3]), decode::pack_bf16(x[4], x[5]),
+                          decode::pack_bf16(x[6], x[7]));
 }
 
-// One thread per eight elements of an output row (16 bytes of K and of V).
+// A warp takes up to kBatch * 32 of a slot's pieces of eight elements (16 bytes
+// of K and of V), all its reads ahead of its writes.
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadParams p) {
-    const int d = p.cache.head_dim, per = d >> 3, heads = p.cache.kv_heads;
-    const long total = p.rows * per;
-    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long)gridDim.x * kThreads) {
-        const long r = i / per;
-        const int e = (int)(i - r * per) * 8;
-        const long t = r / heads;
-        const int h = (int)(r - t * heads);
-        const long slot = decode::load_index(p.slots, t, p.slot64);
-        const long page = slot >> p.page_shift;
-        uint4 k = make_uint4(0, 0, 0, 0), v = k;
-        if (slot >= 0 && page < p.cache.num_pages) {
-            const long row = (page * heads + h) * p.cache.page_size + (slot & (p.cache.page_size - 1));
-            k = read_eight<KIND>(p.cache.k, p.cache.k_scale, row, d, e);
-            v = read_eight<KIND>(p.cache.v, p.cache.v_scale, row, d, e);
-        } else if (slot >= 0) {
-            decode::report(p.err, kErrSlotRange);
+    decode::chain();
+    const int lane = threadIdx.x & 31;
+    const int d = p.cache.head_dim, heads = p.cache.kv_heads, per_shift = d == 64 ? 3 : d == 128 ? 4 : 5;
+    const int pieces = heads << per_shift;
+    const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const unsigned slot_at = unit / (unsigned)p.walks;
+    if (slot_at >= (unsigned)p.count) return;
+    const int first = (int)(unit - slot_at * p.walks) * (32 * kBatch) + lane;
+    const long slot = decode::load_index(p.slots, slot_at, p.slot64);
+    const long page = slot >> p.page_shift;
+    const bool ok = slot >= 0 && page < p.cache.num_pages;
+    if (slot >= 0 && !ok && lane == 0) decode::report(p.err, kErrSlotRange);
+    const long row0 = page * heads * p.cache.page_size + (slot & (p.cache.page_size - 1));
+    uint4 k[kBatch], v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int at = first + 32 * i;
+        k[i] = v[i] = make_uint4(0, 0, 0, 0);
+        if (at < pieces && ok) {
+            const int h = at >> per_shift, e = (at - (h << per_shift)) * 8;
+            const long row = row0 + (long)h * p.cache.page_size;
+            k[i] = read_eight<KIND>(p.cache.k, p.cache.k_scale, row, d, e);
+            v[i] = read_eight<KIND>(p.cache.v, p.cache.v_scale, row, d, e);
         }
-        *reinterpret_cast<uint4*>(p.k + (size_t)r * d + e) = k;
-        *reinterpret_cast<uint4*>(p.v + (size_t)r * d + e) = v;
+    }
+    const size_t out = (size_t)slot_at * pieces;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int at = first + 32 * i;
+        if (at < pieces) {
+            reinterpret_cast<uint4*>(p.k)[out + at] = k[i];
+            reinterpret_cast<uint4*>(p.v)[out + at] = v[i];
+        }
     }
 }
 
@@ -365,15 +421,26 @@ int shift_of(int page_size) {
     return s;
 }
 
-template <int KIND>
-cudaError_t launch_rows(const RowsParams& p, cudaStream_t st) {
+template <int KIND, bool FULL>
+cudaError_t launch_rows(RowsParams& p, cudaStream_t st) {
     const int need = p.d >> 3, lanes = need <= 8 ? 8 : need <= 16 ? 16 : 32, per = 32 / lanes;
     const int heads = p.q_heads + (p.k ? p.kv_heads : 0) + (p.v ? p.kv_heads : 0);
-    const long walks = (heads + per * p.rounds - 1) / (per * p.rounds);
-    const long blocks = (walks * p.tokens + kWarps - 1) / kWarps;
-    auto* kernel = lanes == 8 ? kv_rows_kernel<KIND, 8> : lanes == 16 ? kv_rows_kernel<KIND, 16> : kv_rows_kernel<KIND, 32>;
-    kernel<<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    return cudaGetLastError();
+    // As many rounds a warp as leave about 64 warps for each of 148 SMs: more
+    // rounds share one table row and prologue, fewer spread over the GPU.
+    const int all = (heads + per - 1) / per;
+    p.rounds = (int)std::clamp((long)p.tokens * all / (148 * 64), 1l, (long)all);
+    p.walks = (all + p.rounds - 1) / p.rounds;
+    const long blocks = ((long)p.walks * p.tokens + kWarps - 1) / kWarps;
+    auto* kernel = lanes == 8    ? kv_rows_kernel<KIND, 8, FULL>
+                   : lanes == 16 ? kv_rows_kernel<KIND, 16, FULL>
+                                 : kv_rows_kernel<KIND, 32, FULL>;
+    return decode::launch_chained(kernel, dim3((unsigned)blocks), kThreads, 0, st, p);
+}
+
+template <int KIND>
+cudaError_t launch_kind(RowsParams& p, cudaStream_t st) {
+    const bool full = !p.rope || (p.rot == p.d && !p.pairs && aligned(p.rope, 16));
+    return full ? launch_rows<KIND, true>(p, st) : launch_rows<KIND, false>(p, st);
 }
 
 // Checks shared by the two writing entry points; nullptr when all is well.
@@ -411,52 +478,54 @@ const char* kv_cache_check(const fp4b_kv_cache* c) {
 
 using namespace fp4b;
 
-FP4B_EXPORT int fp4b_kv_rows(const void* q, long q_st, long q_sh, const void* k, long k_st, long k_sh, const void* v,
-                             long v_st, long v_sh, int tokens, int q_heads, int kv_heads, int head_dim,
-                             const void* positions, int pos64, const float* rope, int rope_rows, int rot,
-                             int interleaved, const void* q_weight, const void* k_weight, float eps, void* q_out,
-                             void* k_out, const fp4b_kv_cache* cache, const void* slots, int slot64, void* stream) {
+FP4B_EXPORT int fp4b_kv_rows(const fp4b_rows* rows, void* stream) {
+    if (!rows) {
+        set_last_error("fp4b_kv_rows: null arguments");
+        return -1;
+    }
+    const fp4b_rows& r = *rows;
+    const fp4b_kv_cache* cache = r.cache;
     RowsParams p{};
-    p.q = static_cast<const uint16_t*>(q);
-    p.k = static_cast<const uint16_t*>(k);
-    p.v = static_cast<const uint16_t*>(v);
-    p.q_st = q_st, p.q_sh = q_sh, p.k_st = k_st, p.k_sh = k_sh, p.v_st = v_st, p.v_sh = v_sh;
-    p.tokens = tokens, p.q_heads = q ? q_heads : 0, p.kv_heads = kv_heads, p.d = head_dim;
-    p.positions = positions, p.pos64 = pos64, p.rope = rope, p.rope_rows = rope_rows, p.rot = rot, p.pairs = interleaved;
-    p.q_weight = static_cast<const uint16_t*>(q_weight);
-    p.k_weight = static_cast<const uint16_t*>(k_weight);
-    p.eps = eps;
-    p.q_out = static_cast<uint16_t*>(q_out);
-    p.k_out = static_cast<uint16_t*>(k_out);
-    p.slots = slots, p.slot64 = slot64;
+    p.q = static_cast<const uint16_t*>(r.q);
+    p.k = static_cast<const uint16_t*>(r.k);
+    p.v = static_cast<const uint16_t*>(r.v);
+    p.q_st = r.q_st, p.q_sh = r.q_sh, p.k_st = r.k_st, p.k_sh = r.k_sh, p.v_st = r.v_st, p.v_sh = r.v_sh;
+    p.tokens = r.tokens, p.q_heads = r.q ? r.q_heads : 0, p.kv_heads = r.kv_heads, p.d = r.head_dim;
+    p.positions = r.positions, p.pos64 = r.pos64, p.rope = r.rope, p.rope_rows = r.rope_rows, p.rot = r.rot;
+    p.pairs = r.interleaved;
+    p.q_weight = static_cast<const uint16_t*>(r.q_weight);
+    p.k_weight = static_cast<const uint16_t*>(r.k_weight);
+    p.eps = r.eps;
+    p.q_out = static_cast<uint16_t*>(r.q_out);
+    p.k_out = static_cast<uint16_t*>(r.k_out);
+    p.slots = r.slots, p.slot64 = r.slot64;
     const char* why = rows_check(p);
-    if (!why && !q && !k) why = "neither queries nor keys";
-    if (!why && q && (!q_out || !aligned(q_out, 8) || q_heads <= 0)) why = "queries need an 8-byte aligned output";
+    if (!why && !p.q && !p.k) why = "neither queries nor keys";
+    if (!why && p.q && (!p.q_out || !aligned(p.q_out, 8) || p.q_heads <= 0)) why = "queries need an 8-byte aligned output";
     if (!why && cache) {
         why = kv_cache_check(cache);
-        if (!why && (!k || !v || !slots)) why = "a cache takes keys, values and slots";
-        if (!why && (cache->kv_heads != kv_heads || cache->head_dim != head_dim)) why = "the cache has other heads";
+        if (!why && (!p.k || !p.v || !p.slots)) why = "a cache takes keys, values and slots";
+        if (!why && (cache->kv_heads != p.kv_heads || cache->head_dim != p.d)) why = "the cache has other heads";
     } else if (!why) {
-        if (k && (!k_out || !aligned(k_out, 8))) why = "keys need an 8-byte aligned output or a cache";
-        if (v) why = "values need a cache";
+        if (p.k && (!p.k_out || !aligned(p.k_out, 8))) why = "keys need an 8-byte aligned output or a cache";
+        if (p.v) why = "values need a cache";
     }
     if (why) {
         set_last_error("fp4b_kv_rows: %s", why);
         return -1;
     }
-    if (tokens == 0) return 0;
-    p.rounds = 1;
+    if (p.tokens == 0) return 0;
     p.err = device_error_word();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (cache) {
         p.cache = *cache;
         p.page_shift = shift_of(cache->page_size);
-        e = cache->kind == kKvBf16 ? launch_rows<kKvBf16>(p, st)
-            : cache->kind == kKvFp8 ? launch_rows<kKvFp8>(p, st)
-                                    : launch_rows<kKvNvfp4>(p, st);
+        e = cache->kind == kKvBf16 ? launch_kind<kKvBf16>(p, st)
+            : cache->kind == kKvFp8 ? launch_kind<kKvFp8>(p, st)
+                                    : launch_kind<kKvNvfp4>(p, st);
     } else {
-        e = launch_rows<kKvNone>(p, st);
+        e = launch_kind<kKvNone>(p, st);
     }
     return launch_status(e, "fp4b_kv_rows");
 }
@@ -464,6 +533,7 @@ FP4B_EXPORT int fp4b_kv_rows(const void* q, long q_st, long q_sh, const void* k,
 FP4B_EXPORT int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int slot64, long count, void* k_out,
                              void* v_out, void* stream) {
     const char* why = kv_cache_check(cache);
+    if (!why && count > 0x7fffffffL / std::max(1, cache->kv_heads)) why = "more than 2^31 rows in one call";
     if (!why && (count < 0 || (count > 0 && (!slots || !k_out || !v_out)))) why = "null slots or outputs";
     if (!why && (!aligned(k_out, 16) || !aligned(v_out, 16))) why = "outputs must be 16-byte aligned";
     if (why) {
@@ -471,13 +541,13 @@ FP4B_EXPORT int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int 
         return -1;
     }
     if (count == 0) return 0;
-    ReadParams p{*cache, shift_of(cache->page_size), slots, slot64, count * cache->kv_heads,
+    const int pieces = cache->kv_heads * (cache->head_dim / 8);
+    ReadParams p{*cache, shift_of(cache->page_size), slots, slot64, (int)count, (pieces + 32 * kBatch - 1) / (32 * kBatch),
                  static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), device_error_word()};
-    const long threads = p.rows * (cache->head_dim / 8);
-    const unsigned blocks = (unsigned)std::min<long>((threads + kThreads - 1) / kThreads, 1l << 30);
+    const unsigned blocks = (unsigned)((count * p.walks + kWarps - 1) / kWarps);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (cache->kind == kKvBf16) kv_read_kernel<kKvBf16><<<blocks, kThreads, 0, st>>>(p);
-    else if (cache->kind == kKvFp8) kv_read_kernel<kKvFp8><<<blocks, kThreads, 0, st>>>(p);
-    else kv_read_kernel<kKvNvfp4><<<blocks, kThreads, 0, st>>>(p);
-    return launch_status(cudaGetLastError(), "fp4b_kv_read");
+    auto* kernel = cache->kind == kKvBf16 ? kv_read_kernel<kKvBf16>
+                   : cache->kind == kKvFp8 ? kv_read_kernel<kKvFp8>
+                                           : kv_read_kernel<kKvNvfp4>;
+    return launch_status(decode::launch_chained(kernel, dim3(blocks), kThreads, 0, st, p), "fp4b_kv_read");
 }

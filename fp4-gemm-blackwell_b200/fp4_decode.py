@@ -17,6 +17,7 @@ range is left out by the kernel and shows in ``fp4_gemm.device_error()`` (11 slo
 """
 
 import ctypes
+import struct
 
 import torch
 
@@ -34,25 +35,31 @@ class _CacheView(ctypes.Structure):
                 ("page_size", _i), ("head_dim", _i), ("kind", _i)]
 
 
-_bind("fp4b_kv_rows", _i, [_vp, _l, _l, _vp, _l, _l, _vp, _l, _l, _i, _i, _i, _i, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _vp])
+# fp4b_rows and fp4b_decode, as one call packs them (0: NULL).
+_ROWS, _DECODE = struct.Struct("@PllPllPllPPPPPPPPiiiiiiiiif"), struct.Struct("@PllPPlPPPPPliiiif0l")
+
+_bind("fp4b_kv_rows", _i, [ctypes.c_char_p, _vp])
 _bind("fp4b_kv_read", _i, [_vp, _vp, _i, _l, _vp, _vp, _vp])
 _bind("fp4b_decode_attention_workspace", _l, [_i, _i, _i])
-_bind("fp4b_decode_attention", _i, [_vp, _l, _l, _i, _i, _vp, _vp, _l, _i, _vp, _f, _i, _vp, _vp, _vp, _vp, _l, _vp])
+_bind("fp4b_decode_attention", _i, [ctypes.c_char_p, _vp])
 
 _kv_rows, _kv_read, _attention = _lib.fp4b_kv_rows, _lib.fp4b_kv_read, _lib.fp4b_decode_attention
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# A call's host time is what a small decode step costs, so the current device and stream are asked for without the
+# objects that torch.cuda makes of them.
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _call(device, fn, what: str, *args):
     """fn(*args, stream) with `device` current; raises on a failure code."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream(device))
+    index = device.index
+    if index == _current_device():
+        rc = fn(*args, _current_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
+            rc = fn(*args, _current_stream(index))
     if rc != 0:
         raise RuntimeError(f"{what} failed with error code {rc} ({_last_error()})")
 
@@ -88,10 +95,14 @@ def _weight(w, d: int, what: str, device):
     return w if w.data_ptr() & 7 == 0 else w.clone()
 
 
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _rope(rope, d: int, device):
     """(address, rows, rotated size) of a table; zeros for none."""
     if rope is None:
-        return None, 0, 0
+        return 0, 0, 0
     if rope.dim() != 2 or rope.dtype != torch.float32 or rope.device != device or not rope.is_contiguous():
         raise ValueError("rope must be a contiguous fp32 [rows, rot] table on the queries' device (see rope_table)")
     rows, rot = rope.shape
@@ -130,17 +141,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
     if k.shape[0] != t or k.shape[2] != d:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} have other tokens or head sizes")
     table, rows, rot = _rope(rope, d, dev)
-    if table is not None:
+    if table:
         positions = _indices(positions, t, "positions", dev)
-    q_out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=dev)
-    k_out = torch.empty((t, hk, d), dtype=torch.bfloat16, device=dev)
+    q_out, k_out = q.new_empty((t, hq, d)), q.new_empty((t, hk, d))
     if t == 0:
         return q_out, k_out
     q_weight, k_weight = _weight(q_weight, d, "q_weight", dev), _weight(k_weight, d, "k_weight", dev)
-    _call(dev, _kv_rows, "qk_norm_rope", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), None, 0, 0,
-          t, hq, hk, d, positions.data_ptr() if table is not None else None, positions.dtype == torch.int64 if table is not None else 0,
-          table, rows, rot, interleaved, q_weight.data_ptr() if q_weight is not None else None,
-          k_weight.data_ptr() if k_weight is not None else None, eps, q_out.data_ptr(), k_out.data_ptr(), None, None, 0)
+    qs, ks = q.stride(), k.stride()
+    _call(dev, _kv_rows, "qk_norm_rope", _ROWS.pack(
+        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], 0, 0, 0, positions.data_ptr() if table else 0, 0, table,
+        _address(q_weight), _address(k_weight), q_out.data_ptr(), k_out.data_ptr(), 0, t, hq, hk, d, rows, rot, interleaved,
+        table != 0 and positions.dtype == torch.int64, 0, eps))
     return q_out, k_out
 
 
@@ -208,6 +219,7 @@ class PagedKVCache:
         self._view = _CacheView(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if scales else None,
                                 v_scales.data_ptr() if scales else None, n, h, s, d, KV_KINDS[self.dtype])
         self._ref = ctypes.addressof(self._view)
+        self._attention_bytes = {}  # query heads -> bytes of decode_attention's workspace
 
     @property
     def nbytes(self) -> int:
@@ -226,9 +238,10 @@ class PagedKVCache:
         t = k.shape[0]
         slots = _indices(slots, t, "slots", self.device)
         if t:
-            _call(self.device, _kv_rows, "append", None, 0, 0, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                  v.stride(1), t, 0, self.kv_heads, self.head_dim, None, 0, None, 0, 0, 0, None, None, 0.0, None, None, self._ref,
-                  slots.data_ptr(), slots.dtype == torch.int64)
+            ks, vs = k.stride(), v.stride()
+            _call(self.device, _kv_rows, "append", _ROWS.pack(
+                0, 0, 0, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], 0, slots.data_ptr(), 0, 0, 0, 0, 0, self._ref, t, 0,
+                self.kv_heads, self.head_dim, 0, 0, 0, 0, slots.dtype == torch.int64, 0.0))
 
     def append_qkv(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                    rope: torch.Tensor, q_weight: torch.Tensor = None, k_weight: torch.Tensor = None, eps: float = 1e-6,
@@ -243,24 +256,26 @@ class PagedKVCache:
             raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} have other tokens or head sizes")
         slots = _indices(slots, t, "slots", dev)
         table, rows, rot = _rope(rope, d, dev)
-        if table is not None:
+        if table:
             positions = _indices(positions, t, "positions", dev)
-        q_out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=dev)
+        q_out = q.new_empty((t, hq, d))
         if t == 0:
             return q_out
         q_weight, k_weight = _weight(q_weight, d, "q_weight", dev), _weight(k_weight, d, "k_weight", dev)
-        _call(dev, _kv_rows, "append_qkv", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-              v.data_ptr(), v.stride(0), v.stride(1), t, hq, self.kv_heads, d, positions.data_ptr() if table is not None else None,
-              positions.dtype == torch.int64 if table is not None else 0, table, rows, rot, interleaved,
-              q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None, eps,
-              q_out.data_ptr(), None, self._ref, slots.data_ptr(), slots.dtype == torch.int64)
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        _call(dev, _kv_rows, "append_qkv", _ROWS.pack(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], positions.data_ptr() if table else 0,
+            slots.data_ptr(), table, _address(q_weight), _address(k_weight), q_out.data_ptr(), 0, self._ref, t, hq, self.kv_heads, d,
+            rows, rot, interleaved, table != 0 and positions.dtype == torch.int64, slots.dtype == torch.int64, eps))
         return q_out
 
     def read(self, slots: torch.Tensor):
         """Keys and values of slots [n] as new BF16 tensors [n, kv_heads, head_dim] each; zeros for a negative slot."""
         n = slots.numel()
         slots = _indices(slots, n, "slots", self.device)
-        k, v = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=torch.bfloat16, device=self.device).unbind(0)
+        shape = (n, self.kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
         if n:
             _call(self.device, _kv_read, "read", self._ref, slots.data_ptr(), slots.dtype == torch.int64, n, k.data_ptr(), v.data_ptr())
         return k, v
@@ -270,17 +285,21 @@ class PagedKVCache:
             self.num_pages, self.page_size, self.kv_heads, self.head_dim, self.dtype, self.nbytes / 2 ** 20)
 
 
-_WORKSPACES = {}  # (device, stream) -> zeroed uint8 tensor that decode_attention leaves zeroed where it has to be
+_WORKSPACES = {}  # (device, stream) -> uint8 tensor whose counters decode_attention leaves zeroed
+_COUNTER_BYTES = 16384  # FP4B_DECODE_COUNTER_BYTES
 
 
-def _workspace(device, stream: int, need: int) -> torch.Tensor:
-    """Workspace of the calls on one stream, which run in order.  A captured graph gets one of its own, zeroed in the
-    graph: it may be replayed on any stream, beside anything."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    ws = _WORKSPACES.get((device, stream))
+def _workspace(device, need: int) -> torch.Tensor:
+    """Workspace of the calls on the current stream, which run in order.  A captured graph gets one of its own, its counters
+    zeroed in the graph: it may be replayed on any stream, beside anything."""
+    if _capturing():
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[:_COUNTER_BYTES].zero_()
+        return ws
+    key = (device.index, _current_stream(device.index))
+    ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < need:
-        ws = _WORKSPACES[(device, stream)] = torch.zeros(need, dtype=torch.uint8, device=device)
+        ws = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=device)
     return ws
 
 
@@ -317,14 +336,17 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         if sinks.numel() != hq or sinks.device != dev:
             raise ValueError(f"sinks must have {hq} elements on {dev}")
         sinks = sinks.to(torch.float32).contiguous()
-    out = torch.empty((b, hq, d), dtype=torch.bfloat16, device=dev)
+    out = q.new_empty((b, hq, d))
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     if b:
-        need = _lib.fp4b_decode_attention_workspace(hq, cache.kv_heads, d)
-        ws = _workspace(dev, _stream(dev), need)
-        width = page_table.shape[1]
-        _call(dev, _attention, "decode_attention", q.data_ptr(), q.stride(0), q.stride(1), b, hq, cache._ref, page_table.data_ptr(),
-              max(page_table.stride(0), width), width, seq_lens.data_ptr(), d ** -0.5 if scale is None else scale, window,
-              sinks.data_ptr() if sinks is not None else None, out.data_ptr(), lse.data_ptr() if return_lse else None,
-              ws.data_ptr(), ws.numel())
+        need = cache._attention_bytes.get(hq)
+        if need is None:
+            with torch.cuda.device(dev):
+                need = cache._attention_bytes[hq] = _lib.fp4b_decode_attention_workspace(hq, cache.kv_heads, d)
+        ws = _workspace(dev, need)
+        qs, width = q.stride(), page_table.shape[1]
+        _call(dev, _attention, "decode_attention", _DECODE.pack(
+            q.data_ptr(), qs[0], qs[1], cache._ref, page_table.data_ptr(), max(page_table.stride(0), width), seq_lens.data_ptr(),
+            _address(sinks), out.data_ptr(), _address(lse), ws.data_ptr(), ws.numel(), b, hq, width, window,
+            d ** -0.5 if scale is None else scale))
     return (out, lse) if return_lse else out

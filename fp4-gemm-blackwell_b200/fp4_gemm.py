@@ -581,19 +581,28 @@ def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
     assert x.is_cuda and cache.device.index in (None, x.device.index), "x must be on the cache's CUDA device"
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
-    x_2d, ldx = _rows_view(x.reshape(-1, k))
-    m = x_2d.shape[0]
-    y = torch.empty(*x.shape[:-1], n, dtype=torch.bfloat16, device=x.device)
+    if x.is_contiguous():
+        x_2d, ldx, m = x, k, x.numel() // k
+    else:
+        x_2d, ldx = _rows_view(x.reshape(-1, k))
+        m = x_2d.shape[0]
+    y = x.new_empty(x.shape[:-1] + (n,))
     bias = cache.bias
     fuse_bias = bias is not None and bias.dtype == torch.bfloat16 and bias.is_cuda
     if m > 0:
+        b_ptr = None
         if fuse_bias:
-            bias = bias.reshape(-1).contiguous()
             if bias.numel() != n:
                 raise ValueError(f"the cache's bias has {bias.numel()} elements, not {n}")
-        with torch.cuda.device(x.device):
-            rc = _lib.fp4b_gemv_cached(x_2d.data_ptr(), m, k, ldx, cache._handle, n, y.data_ptr(), n,
-                                       bias.data_ptr() if fuse_bias else None, _stream_ptr(x.device))
+            bias = bias if bias.is_contiguous() else bias.contiguous()
+            b_ptr = bias.data_ptr()
+        index = x.device.index
+        args = (x_2d.data_ptr(), m, k, ldx, cache._handle, n, y.data_ptr(), n, b_ptr, torch._C._cuda_getCurrentRawStream(index))
+        if index == torch._C._cuda_getDevice():  # without the objects of torch.cuda: the host's time counts here
+            rc = _lib.fp4b_gemv_cached(*args)
+        else:
+            with torch.cuda.device(index):
+                rc = _lib.fp4b_gemv_cached(*args)
         if rc != 0:
             raise RuntimeError(f"fp4_cached_gemv failed with error code {rc} ({_last_error()})")
     return y + bias if bias is not None and not fuse_bias else y

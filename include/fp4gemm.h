@@ -302,11 +302,27 @@ typedef struct fp4b_kv_cache {
  * be NULL, k too without a cache.  *_st, *_sh: token and head strides in
  * elements, multiples of 4; rows 8-byte aligned, elements contiguous; outputs
  * contiguous.  positions and slots are int64 where pos64 / slot64, else int32. */
-int fp4b_kv_rows(const void* q, long q_st, long q_sh, const void* k, long k_st, long k_sh, const void* v, long v_st,
-                 long v_sh, int tokens, int q_heads, int kv_heads, int head_dim, const void* positions, int pos64,
-                 const float* rope, int rope_rows, int rot, int interleaved, const void* q_weight,
-                 const void* k_weight, float eps, void* q_out, void* k_out, const fp4b_kv_cache* cache,
-                 const void* slots, int slot64, void* stream);
+typedef struct fp4b_rows {
+    const void* q;
+    long q_st, q_sh;
+    const void* k;
+    long k_st, k_sh;
+    const void* v;
+    long v_st, v_sh;
+    const void* positions;
+    const void* slots;
+    const float* rope;
+    const void* q_weight;
+    const void* k_weight;
+    void* q_out;
+    void* k_out;
+    const fp4b_kv_cache* cache;
+    int tokens, q_heads, kv_heads, head_dim;
+    int rope_rows, rot, interleaved;
+    int pos64, slot64;
+    float eps;
+} fp4b_rows;
+int fp4b_kv_rows(const fp4b_rows* rows, void* stream);
 
 /* Keys and values of `count` slots as BF16 [count, kv_heads, head_dim] each;
  * zeros for a negative slot. */
@@ -319,17 +335,31 @@ int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int slot64, long
  * row stride table_stride, table_width entries); query head h reads key head
  * h / (q_heads / kv_heads).  sinks: fp32 [q_heads] or NULL, one more logit in
  * each head's softmax that no value belongs to.  A sequence without keys gives
- * zeros.  q: BF16, strides in elements (multiples of 4, rows 8-byte aligned);
- * out BF16 [batch, q_heads, head_dim] contiguous; lse: fp32 [batch, q_heads],
- * the log of the softmax's denominator (-inf where it is empty), or NULL.
+ * zeros; a key whose page is out of range counts as a row of zeros.  q: BF16,
+ * strides in elements (multiples of 4, rows 8-byte aligned); out BF16 [batch,
+ * q_heads, head_dim] contiguous; lse: fp32 [batch, q_heads], the log of the
+ * softmax's denominator (-inf where it is empty), or NULL.
  * workspace: fp4b_decode_attention_workspace bytes of device memory, 16-byte
- * aligned, zeroed before its first use and left zeroed where it has to be;
- * calls that share it must be ordered. */
+ * aligned, the first FP4B_DECODE_COUNTER_BYTES of them zeroed before its first
+ * use (every call leaves them zero); calls that share it must be ordered. */
+enum { FP4B_DECODE_COUNTER_BYTES = 16384 };
+typedef struct fp4b_decode {
+    const void* q;
+    long q_sb, q_sh;
+    const fp4b_kv_cache* cache;
+    const int* page_table;
+    long table_stride;
+    const int* seq_lens;
+    const float* sinks;
+    void* out;
+    float* lse;
+    void* workspace;
+    long workspace_bytes;
+    int batch, q_heads, table_width, window;
+    float scale;
+} fp4b_decode;
 long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int head_dim);
-int fp4b_decode_attention(const void* q, long q_sb, long q_sh, int batch, int q_heads, const fp4b_kv_cache* cache,
-                          const int* page_table, long table_stride, int table_width, const int* seq_lens,
-                          float scale, int window, const float* sinks, void* out, float* lse, void* workspace,
-                          long workspace_bytes, void* stream);
+int fp4b_decode_attention(const fp4b_decode* call, void* stream);
 
 #ifdef __cplusplus
 }
