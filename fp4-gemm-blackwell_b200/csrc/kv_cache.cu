@@ -26,6 +26,7 @@
 
 #include "decode_core.cuh"
 #include "fp4b_internal.h"
+#include "quantize_core.cuh"
 
 #define FP4B_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -51,8 +52,10 @@ struct RowsParams {
     uint16_t *q_out, *k_out;  // BF16 [tokens, heads, d]
     fp4b_kv_cache cache;      // keys and values go here unless KIND is kKvNone
     int page_shift;
-    int rounds;  // rounds of 32 / L heads that one warp walks
-    int walks;   // warps a token: ceil(heads / (rounds * 32 / L))
+    float inv_d;
+    int q_rounds, k_rounds, all_rounds;  // rounds of 32 / L heads: the queries', the keys' and all
+    int rounds;                          // of which one warp walks these many
+    int walks;                           // warps a token
     int* err;
 };
 
@@ -203,37 +206,39 @@ __device__ __forceinline__ void store_row(const RowsParams& p, bool value, long 
 }
 
 template <int KIND, int L, bool FULL>
-__global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kThreads, FULL ? 4 : 1) kv_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kPer = 32 / L;  // heads of a token that a warp holds at once
     decode::chain();
     const int lane = threadIdx.x & 31, l = lane & (L - 1), sub = lane / L;
-    const int heads = p.q_heads + (p.k ? p.kv_heads : 0) + (p.v ? p.kv_heads : 0);
     const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
     const unsigned token = unit / (unsigned)p.walks;
     if (token >= (unsigned)p.tokens) return;
     const long t = token;
-    const int first = (int)(unit - token * p.walks) * kPer * p.rounds;
+    const int begin = (int)(unit - token * p.walks) * p.rounds, end = min(begin + p.rounds, p.all_rounds);
     const bool inside = l < (p.d >> 3);
     const int half = p.d >> 1;
+    const uint16_t* q_row = p.q + t * p.q_st + 4 * l;
+    const uint16_t* k_row = p.k + t * p.k_st + 4 * l;
+    const uint16_t* v_row = p.v + t * p.v_st + 4 * l;
 
+    // A round's heads are all queries, all keys or all values.
     uint2 wa[kBatch], wb[kBatch];  // the lane's chunks of the next rounds' rows
     auto fetch = [&](int r0) {
 #pragma unroll
-        for (int r = 0; r < kBatch; ++r) {
-            const int h = first + (r0 + r) * kPer + sub;
-            wa[r] = wb[r] = make_uint2(0u, 0u);
-            if (r0 + r < p.rounds && h < heads && inside) {
-                const int hk = h - p.q_heads;
-                const uint16_t* src;
-                if (hk < 0) src = p.q + t * p.q_st + h * p.q_sh;
-                else if (p.k && hk < p.kv_heads) src = p.k + t * p.k_st + hk * p.k_sh;
-                else src = p.v + t * p.v_st + (p.k ? hk - p.kv_heads : hk) * p.v_sh;
-                wa[r] = *reinterpret_cast<const uint2*>(src + 4 * l);
-                wb[r] = *reinterpret_cast<const uint2*>(src + half + 4 * l);
+        for (int i = 0; i < kBatch; ++i) {
+            const int r = r0 + i;
+            wa[i] = wb[i] = make_uint2(0u, 0u);
+            if (r >= end) continue;
+            const bool query = r < p.q_rounds, key = !query && r < p.k_rounds;
+            const int h = (r - (query ? 0 : key ? p.q_rounds : p.k_rounds)) * kPer + sub;
+            if (h < (query ? p.q_heads : p.kv_heads) && inside) {
+                const uint16_t* src = query ? q_row + (long)h * p.q_sh : key ? k_row + (long)h * p.k_sh : v_row + (long)h * p.v_sh;
+                wa[i] = *reinterpret_cast<const uint2*>(src);
+                wb[i] = *reinterpret_cast<const uint2*>(src + half);
             }
         }
     };
-    fetch(0);
+    fetch(begin);
 
     // The token's slot, its table row, and the norm weights of the lane's elements.
     long row0 = -1;  // cache row of head 0
@@ -271,60 +276,48 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant
         }
     }
 
-    for (int r0 = 0; r0 < p.rounds; r0 += kBatch) {
+    for (int r0 = begin; r0 < end; r0 += kBatch) {
 #pragma unroll
-        for (int r = 0; r < kBatch; ++r) {
-            if (r0 + r >= p.rounds) break;
-            const int h = first + (r0 + r) * kPer + sub;
-            const int hk = h - p.q_heads;
-            const bool query = hk < 0, key = !query && p.k && hk < p.kv_heads;
-            const int hv = p.k ? hk - p.kv_heads : hk;
-            const bool live = h < heads && inside;
+        for (int i = 0; i < kBatch; ++i) {
+            const int r = r0 + i;
+            if (r >= end) break;
+            const bool query = r < p.q_rounds, key = !query && r < p.k_rounds;
+            const int h = (r - (query ? 0 : key ? p.q_rounds : p.k_rounds)) * kPer + sub;
+            const bool live = h < (query ? p.q_heads : p.kv_heads) && inside;
             float a[4], b[4];
-            unpack4(wa[r], a);
-            unpack4(wb[r], b);
-            const uint16_t* weight = query ? p.q_weight : key ? p.k_weight : nullptr;
-            if (__any_sync(0xffffffffu, weight != nullptr)) {
-                float sum = 0.0f;
+            unpack4(wa[i], a);
+            unpack4(wb[i], b);
+            if (query || key) {
+                const uint16_t* weight = query ? p.q_weight : p.k_weight;
+                if (weight) {
+                    float na[4] = {}, nb[4] = {};
+                    if (inside) {
+                        unpack4(__ldg(reinterpret_cast<const uint2*>(weight + 4 * l)), na);
+                        unpack4(__ldg(reinterpret_cast<const uint2*>(weight + half + 4 * l)), nb);
+                    }
+                    float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum += a[i] * a[i] + b[i] * b[i];
-                sum = decode::group_sum<L>(sum);
-                if (weight && inside) {
-                    const float inv = rsqrtf(sum / (float)p.d + p.eps);
-                    float na[4], nb[4];
-                    unpack4(__ldg(reinterpret_cast<const uint2*>(weight + 4 * l)), na);
-                    unpack4(__ldg(reinterpret_cast<const uint2*>(weight + half + 4 * l)), nb);
+                    for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
+                    const float inv = rsqrtf(decode::group_sum<L>(sum) * p.inv_d + p.eps);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        a[i] = a[i] * inv * na[i];
-                        b[i] = b[i] * inv * nb[i];
+                    for (int e = 0; e < 4; ++e) {
+                        a[e] = a[e] * inv * na[e];
+                        b[e] = b[e] * inv * nb[e];
                     }
                 }
+                if (p.rope) rotate<L, FULL>(p, a, b, ca, sa, cb, sb, l);
             }
-            if (p.rope && __any_sync(0xffffffffu, query || key)) {
-                float ra[4] = {a[0], a[1], a[2], a[3]}, rb[4] = {b[0], b[1], b[2], b[3]};
-                rotate<L, FULL>(p, ra, rb, ca, sa, cb, sb, l);
-                if (query || key) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        a[i] = ra[i];
-                        b[i] = rb[i];
-                    }
+            if (query || (key && KIND == kKvNone)) {
+                if (live) {
+                    uint16_t* out = (query ? p.q_out + ((size_t)t * p.q_heads + h) * p.d : p.k_out + ((size_t)t * p.kv_heads + h) * p.d) + 4 * l;
+                    *reinterpret_cast<uint2*>(out) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
+                    *reinterpret_cast<uint2*>(out + half) = make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
                 }
-            }
-            if (live && (query || (key && KIND == kKvNone))) {
-                uint16_t* out = query ? p.q_out + ((size_t)t * p.q_heads + h) * p.d : p.k_out + ((size_t)t * p.kv_heads + hk) * p.d;
-                *reinterpret_cast<uint2*>(out + 4 * l) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
-                *reinterpret_cast<uint2*>(out + half + 4 * l) =
-                    make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
-            }
-            if constexpr (KIND != kKvNone) {
-                const bool stored = live && !query && row0 >= 0;
-                if (__any_sync(0xffffffffu, stored))
-                    store_row<KIND, L>(p, !key, row0 + (long)(key ? hk : hv) * p.cache.page_size, stored, l, a, b);
+            } else if constexpr (KIND != kKvNone) {
+                store_row<KIND, L>(p, !key, row0 + (long)h * p.cache.page_size, live && row0 >= 0, l, a, b);
             }
         }
-        if (r0 + kBatch < p.rounds) fetch(r0 + kBatch);
+        if (r0 + kBatch < end) fetch(r0 + kBatch);
     }
 }
 
@@ -333,8 +326,8 @@ struct ReadParams {
     int page_shift;
     const void* slots;
     int slot64;
-    int count;
-    int walks;  // warps a slot
+    uint32_t total;               // pieces of eight elements
+    uint32_t div_mul, div_shift;  // division by a slot's pieces
     uint16_t *k, *v;
     int* err;
 };
@@ -342,7 +335,6 @@ struct ReadParams {
 // Eight elements of a row as BF16.
 template <int KIND>
 __device__ __forceinline__ uint4 read_eight(const void* base, const void* scales, long row, int d, int e) {
-    [[maybe_unused]] float x[8];
     if constexpr (KIND == kKvBf16) {
         return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + (size_t)row * d + e);
     } else if constexpr (KIND == kKvFp8) {
@@ -352,63 +344,65 @@ __device__ __forceinline__ uint4 read_eight(const void* base, const void* scales
         decode::e4m3x4_to_f16(w.x, lo);
         decode::e4m3x4_to_f16(w.y, hi);
         h[0] = lo[0], h[1] = lo[1], h[2] = hi[0], h[3] = hi[1];
+        uint32_t out[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = decode::f16x2_to_float2(h[i]);
-            x[2 * i] = f.x * s, x[2 * i + 1] = f.y * s;
+            out[i] = decode::pack_bf16(f.x * s, f.y * s);
         }
+        return make_uint4(out[0], out[1], out[2], out[3]);
     } else {
+        // code times scale is exact in FP16 (6 significant bits, 2^-10 to 2880), and in BF16
         const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + (size_t)row * (d >> 1) + (e >> 1));
-        const float s = decode::ue4m3_float(static_cast<const uint8_t*>(scales)[(size_t)row * (d >> 4) + (e >> 4)]);
-        uint32_t h[4];
+        const uint32_t byte = static_cast<const uint8_t*>(scales)[(size_t)row * (d >> 4) + (e >> 4)];
+        const uint32_t s = decode::mul_f16x2(decode::ue4m3x2_to_f16(byte * 0x10001u), 0x5C005C00u);  // times 256
+        uint32_t h[4], out[4];
         decode::e2m1x8_to_f16(w, h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = decode::f16x2_to_float2(h[i]);
-            x[2 * i] = f.x * s, x[2 * i + 1] = f.y * s;
+            const float2 f = decode::f16x2_to_float2(decode::mul_f16x2(h[i], s));
+            out[i] = decode::pack_bf16(f.x, f.y);
         }
+        return make_uint4(out[0], out[1], out[2], out[3]);
     }
-    if constexpr (KIND != kKvBf16)
-        return make_uint4(decode::pack_bf16(x[0], x[1]), decode::pack_bf16(x[2], x[3]), decode::pack_bf16(x[4], x[5]),
-                          decode::pack_bf16(x[6], x[7]));
 }
 
-// A warp takes up to kBatch * 32 of a slot's pieces of eight elements (16 bytes
-// of K and of V), all its reads ahead of its writes.
+// One thread takes kBatch pieces of eight elements (16 bytes of K and of V), 32
+// apart, all its reads ahead of its writes.
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadParams p) {
     decode::chain();
-    const int lane = threadIdx.x & 31;
     const int d = p.cache.head_dim, heads = p.cache.kv_heads, per_shift = d == 64 ? 3 : d == 128 ? 4 : 5;
-    const int pieces = heads << per_shift;
-    const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const unsigned slot_at = unit / (unsigned)p.walks;
-    if (slot_at >= (unsigned)p.count) return;
-    const int first = (int)(unit - slot_at * p.walks) * (32 * kBatch) + lane;
-    const long slot = decode::load_index(p.slots, slot_at, p.slot64);
-    const long page = slot >> p.page_shift;
-    const bool ok = slot >= 0 && page < p.cache.num_pages;
-    if (slot >= 0 && !ok && lane == 0) decode::report(p.err, kErrSlotRange);
-    const long row0 = page * heads * p.cache.page_size + (slot & (p.cache.page_size - 1));
+    const uint32_t pieces = (uint32_t)heads << per_shift;
+    const uint32_t first = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * (32u * kBatch) + (threadIdx.x & 31);
+    long slot[kBatch];
+    uint32_t in_slot[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const uint32_t at = first + 32 * i, slot_at = (__umulhi(at, p.div_mul) + at) >> p.div_shift;  // at / pieces
+        in_slot[i] = at - slot_at * pieces;
+        slot[i] = at < p.total ? decode::load_index(p.slots, slot_at, p.slot64) : -1;
+    }
     uint4 k[kBatch], v[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-        const int at = first + 32 * i;
         k[i] = v[i] = make_uint4(0, 0, 0, 0);
-        if (at < pieces && ok) {
-            const int h = at >> per_shift, e = (at - (h << per_shift)) * 8;
-            const long row = row0 + (long)h * p.cache.page_size;
+        const long page = slot[i] >> p.page_shift;
+        if (slot[i] >= 0 && page < p.cache.num_pages) {
+            const int h = in_slot[i] >> per_shift, e = (in_slot[i] - (h << per_shift)) * 8;
+            const int row = ((int)page * heads + h) * p.cache.page_size + ((int)slot[i] & (p.cache.page_size - 1));
             k[i] = read_eight<KIND>(p.cache.k, p.cache.k_scale, row, d, e);
             v[i] = read_eight<KIND>(p.cache.v, p.cache.v_scale, row, d, e);
+        } else if (slot[i] >= 0) {
+            decode::report(p.err, kErrSlotRange);
         }
     }
-    const size_t out = (size_t)slot_at * pieces;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-        const int at = first + 32 * i;
-        if (at < pieces) {
-            reinterpret_cast<uint4*>(p.k)[out + at] = k[i];
-            reinterpret_cast<uint4*>(p.v)[out + at] = v[i];
+        const uint32_t at = first + 32 * i;
+        if (at < p.total) {
+            reinterpret_cast<uint4*>(p.k)[at] = k[i];
+            reinterpret_cast<uint4*>(p.v)[at] = v[i];
         }
     }
 }
@@ -424,12 +418,14 @@ int shift_of(int page_size) {
 template <int KIND, bool FULL>
 cudaError_t launch_rows(RowsParams& p, cudaStream_t st) {
     const int need = p.d >> 3, lanes = need <= 8 ? 8 : need <= 16 ? 16 : 32, per = 32 / lanes;
-    const int heads = p.q_heads + (p.k ? p.kv_heads : 0) + (p.v ? p.kv_heads : 0);
+    p.q_rounds = (p.q_heads + per - 1) / per;
+    p.k_rounds = p.q_rounds + (p.k ? (p.kv_heads + per - 1) / per : 0);
+    p.all_rounds = p.k_rounds + (p.v ? (p.kv_heads + per - 1) / per : 0);
+    p.inv_d = 1.0f / (float)p.d;
     // As many rounds a warp as leave about 64 warps for each of 148 SMs: more
     // rounds share one table row and prologue, fewer spread over the GPU.
-    const int all = (heads + per - 1) / per;
-    p.rounds = (int)std::clamp((long)p.tokens * all / (148 * 64), 1l, (long)all);
-    p.walks = (all + p.rounds - 1) / p.rounds;
+    p.rounds = (int)std::clamp((long)p.tokens * p.all_rounds / (148 * 64), 1l, (long)p.all_rounds);
+    p.walks = (p.all_rounds + p.rounds - 1) / p.rounds;
     const long blocks = ((long)p.walks * p.tokens + kWarps - 1) / kWarps;
     auto* kernel = lanes == 8    ? kv_rows_kernel<KIND, 8, FULL>
                    : lanes == 16 ? kv_rows_kernel<KIND, 16, FULL>
@@ -533,7 +529,7 @@ FP4B_EXPORT int fp4b_kv_rows(const fp4b_rows* rows, void* stream) {
 FP4B_EXPORT int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int slot64, long count, void* k_out,
                              void* v_out, void* stream) {
     const char* why = kv_cache_check(cache);
-    if (!why && count > 0x7fffffffL / std::max(1, cache->kv_heads)) why = "more than 2^31 rows in one call";
+    if (!why && cache->kv_heads > 0x7fff0000 / (cache->head_dim / 8)) why = "too many heads";
     if (!why && (count < 0 || (count > 0 && (!slots || !k_out || !v_out)))) why = "null slots or outputs";
     if (!why && (!aligned(k_out, 16) || !aligned(v_out, 16))) why = "outputs must be 16-byte aligned";
     if (why) {
@@ -542,12 +538,26 @@ FP4B_EXPORT int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int 
     }
     if (count == 0) return 0;
     const int pieces = cache->kv_heads * (cache->head_dim / 8);
-    ReadParams p{*cache, shift_of(cache->page_size), slots, slot64, (int)count, (pieces + 32 * kBatch - 1) / (32 * kBatch),
-                 static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), device_error_word()};
-    const unsigned blocks = (unsigned)((count * p.walks + kWarps - 1) / kWarps);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    ReadParams p{};
+    p.cache = *cache;
+    p.page_shift = shift_of(cache->page_size);
+    p.slot64 = slot64;
+    qcore::make_fast_div(pieces, &p.div_mul, &p.div_shift);
+    p.err = device_error_word();
     auto* kernel = cache->kind == kKvBf16 ? kv_read_kernel<kKvBf16>
                    : cache->kind == kKvFp8 ? kv_read_kernel<kKvFp8>
                                            : kv_read_kernel<kKvNvfp4>;
-    return launch_status(decode::launch_chained(kernel, dim3(blocks), kThreads, 0, st, p), "fp4b_kv_read");
+    cudaError_t e = cudaSuccess;
+    // Piece numbers are 31-bit: more slots than that in several launches.
+    const long most = 0x7fff0000L / pieces;
+    for (long at = 0; at < count && e == cudaSuccess; at += most) {
+        const long n = std::min(most, count - at);
+        p.total = (uint32_t)(n * pieces);
+        p.slots = static_cast<const uint8_t*>(slots) + at * (slot64 ? 8 : 4);
+        p.k = static_cast<uint16_t*>(k_out) + at * pieces * 8;
+        p.v = static_cast<uint16_t*>(v_out) + at * pieces * 8;
+        const unsigned blocks = (p.total + kThreads * kBatch - 1) / (kThreads * kBatch);
+        e = decode::launch_chained(kernel, dim3(blocks), kThreads, 0, static_cast<cudaStream_t>(stream), p);
+    }
+    return launch_status(e, "fp4b_kv_read");
 }
