@@ -81,18 +81,17 @@ __device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t (&pair)[2]) {
 
 __device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) { return __half22float2(*reinterpret_cast<__half2*>(&h)); }
 
-// One scaled value -> the fp32 stand-in whose hardware conversion to E2M1
-// (nearest even) equals the codec's rule (ties to the lower magnitude, sign
-// only below zero): the odd-bit float at or one ulp below its magnitude.  v
-// must be finite.
-__device__ __forceinline__ float e2m1_stand_in(float v) {
-    const uint32_t a = __float_as_uint(v) & 0x7FFFFFFFu;
-    const uint32_t m = (a - (a != 0u ? 1u : 0u)) | 1u;
-    return __uint_as_float(m | (v < 0.0f ? 0x80000000u : 0u));
+// x * inv -> the fp32 stand-in whose hardware conversion to E2M1 (nearest even)
+// equals the codec's rule (ties to the lower magnitude, no sign on a zero): the
+// odd-bit float at or one ulp below the product's magnitude.  Adding +0 turns a
+// product of -0 into +0, whose bits count as 1.  The product must be finite.
+__device__ __forceinline__ float e2m1_stand_in(float x, float inv) {
+    const uint32_t b = __float_as_uint(__fmaf_rn(x, inv, 0.0f));
+    return __uint_as_float((max(b, 1u) - 1u) | 1u);
 }
 
-// Four scaled values -> four E2M1 codes, the first in the lowest nibble.
-__device__ __forceinline__ uint32_t e2m1x4(float a, float b, float c, float d) {
+// Four values times inv -> four E2M1 codes, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x4(float a, float b, float c, float d, float inv) {
     uint16_t r;
     asm("{\n"
         ".reg .b8 b0, b1;\n"
@@ -101,7 +100,7 @@ __device__ __forceinline__ uint32_t e2m1x4(float a, float b, float c, float d) {
         "mov.b16 %0, {b0, b1};\n"
         "}"
         : "=h"(r)
-        : "f"(e2m1_stand_in(a)), "f"(e2m1_stand_in(b)), "f"(e2m1_stand_in(c)), "f"(e2m1_stand_in(d)));
+        : "f"(e2m1_stand_in(a, inv)), "f"(e2m1_stand_in(b, inv)), "f"(e2m1_stand_in(c, inv)), "f"(e2m1_stand_in(d, inv)));
     return r;
 }
 

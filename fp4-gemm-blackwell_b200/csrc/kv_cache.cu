@@ -66,20 +66,12 @@ __device__ __forceinline__ void unpack4(uint2 w, float (&x)[4]) {
     x[3] = decode::bf16_hi(w.y);
 }
 
-// Rotates the lane's two chunks.  c, s: the table's factors for the lane's
-// elements (a: first chunk, b: second; with FULL, the whole row in halves, b's
-// are a's).
-template <int L, bool FULL>
+// Rotates the lane's two chunks, any rotated size and pairing.  c, s: the
+// table's factors for the lane's elements (a: first chunk, b: second).
+template <int L>
 __device__ __forceinline__ void rotate(const RowsParams& p, float (&a)[4], float (&b)[4], const float (&ca)[4],
                                        const float (&sa)[4], const float (&cb)[4], const float (&sb)[4], int l) {
-    if constexpr (FULL) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = a[i], y = b[i];
-            a[i] = x * ca[i] - y * sa[i];
-            b[i] = y * ca[i] + x * sa[i];
-        }
-    } else if (p.pairs) {
+    if (p.pairs) {
         // Pair (2i, 2i + 1) lies in one lane; ca[2i] = ca[2i + 1].
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
@@ -128,85 +120,323 @@ __device__ __forceinline__ void factors(const RowsParams& p, const float* row, i
     }
 }
 
-// |x|max of a block from its four lanes' values, as the codec takes it: NaN is
-// skipped.  `literal`: the block holds a NaN, an infinity or a huge value.
-__device__ __forceinline__ float block_absmax(const float (&x)[4], bool& literal) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    top = decode::group_umax<4>(top);
-    literal = top >= kFastAbsmaxF32Limit;
-    float amax = __uint_as_float(top);
-    if (__any_sync(0xffffffffu, literal)) {
-        float f = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-        f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 2));
-        f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
-        if (literal) amax = f == f ? f : 0.0f;
-    }
-    return amax;
+// The scale byte of a 16-element block, ue4m3(absmax / 6) by the codec's rule
+// (normal numbers rounded half up, subnormals truncated, at least 2^-9, from
+// 256 up the largest), without the division: absmax / 6 rounded to fp32 reaches
+// a boundary t of the rule exactly when absmax >= 6 t, since 6 t is an fp32
+// number and the float below it, a sixth of an ulp of 6 t (2/3 of one of t or
+// more) short of it, stays below when divided.  With absmax = M 2^e, M in [2^23,
+// 2^24): the mantissa's eighths are floor((2 M - 45 2^h) / (3 2^(h + 1))) with h =
+// 19 from M = 1.5 * 2^23 on, else 18.  absmax finite.
+__device__ __forceinline__ uint32_t scale_byte(float absmax) {
+    if (absmax < 0.09375f) return max(((uint32_t)(absmax * 512.0f) * 43u) >> 8, 1u);  // floor(x / 6) of x < 48
+    const uint32_t bits = __float_as_uint(absmax), mant = (bits & 0x7FFFFFu) | 0x800000u;
+    const uint32_t upper = mant >= 0xC00000u ? 1u : 0u;
+    const uint32_t eighths = (((2u * mant - (45u << (18u + upper))) >> (19u + upper)) * 11u) >> 5;  // floor(y / 3) of y < 32
+    const uint32_t exponent = (bits >> 23) - 123u + upper;
+    return exponent >= 15u ? 0x7Fu : exponent * 8u + eighths;
 }
 
-__device__ __forceinline__ uint32_t block_codes(const float (&x)[4], float inv, bool literal) {
-    if (literal) {
-        uint32_t codes = 0;
-        for (int i = 0; i < 4; ++i) codes |= (uint32_t)e2m1_scan(__fmul_rn(x[i], inv)) << (4 * i);
-        return codes;
-    }
-    return decode::e2m1x4(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv), __fmul_rn(x[2], inv), __fmul_rn(x[3], inv));
+// Lane i < 8 holds 1 / (8 + i) and lane 8 + i 1 / i, rounded to nearest: the
+// reciprocals of the scales' mantissas, from which a power of two makes each
+// scale's own exactly.
+__device__ __forceinline__ float mantissa_reciprocal(int lane) { return __frcp_rn((float)(lane < 8 ? 8 + lane : lane & 7)); }
+__device__ __forceinline__ float scale_reciprocal(float table, uint32_t byte) {
+    const uint32_t e = byte >> 3, m = byte & 7u;
+    return __shfl_sync(0xffffffffu, table, e ? m : 8u + m) * __uint_as_float((e ? 137u - e : 136u) << 23);
 }
 
-// Writes one row's lane share into the cache.  All lanes of the warp call it;
-// `live`: the lane has elements and its slot is valid.
+// Largest magnitudes (as fp32 bits; a NaN or an infinity orders above the rest)
+// of the lane's two chunks, over the four lanes of each block (nvfp4) or over
+// the whole row (fp8: both the same).
 template <int KIND, int L>
-__device__ __forceinline__ void store_row(const RowsParams& p, bool value, long row, bool live, int l,
-                                          const float (&a)[4], const float (&b)[4]) {
-    void* base = value ? p.cache.v : p.cache.k;
-    void* scales = value ? p.cache.v_scale : p.cache.k_scale;
-    const int half = p.d >> 1;
+__device__ __forceinline__ void magnitudes(const float (&a)[4], const float (&b)[4], uint32_t& top_a, uint32_t& top_b) {
+    top_a = top_b = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        top_a = max(top_a, __float_as_uint(a[i]) & 0x7FFFFFFFu);
+        top_b = max(top_b, __float_as_uint(b[i]) & 0x7FFFFFFFu);
+    }
+    if constexpr (KIND == kKvNvfp4) {
+        top_a = decode::group_umax<4>(top_a);
+        top_b = decode::group_umax<4>(top_b);
+    } else {
+        top_a = top_b = decode::group_umax<L>(max(top_a, top_b));
+    }
+}
+// The same of BF16 chunks as they were read.
+template <int KIND, int L>
+__device__ __forceinline__ void magnitudes(uint2 a, uint2 b, uint32_t& top_a, uint32_t& top_b) {
+    const uint32_t ma = decode::max_abs_bf16x2(a.x, a.y), mb = decode::max_abs_bf16x2(b.x, b.y);
+    // chunk a's in the low half, b's in the high one
+    uint32_t both = decode::max_abs_bf16x2(__byte_perm(ma, mb, 0x5410), __byte_perm(ma, mb, 0x7632));
+#pragma unroll
+    for (int o = KIND == kKvNvfp4 ? 2 : L / 2; o > 0; o >>= 1) both = decode::max_abs_bf16x2(both, __shfl_xor_sync(0xffffffffu, both, o));
+    top_a = (both << 16) & 0x7FFF0000u;
+    top_b = both & 0x7FFF0000u;
+    if constexpr (KIND != kKvNvfp4) top_a = top_b = max(top_a, top_b);
+}
+
+// A block that holds a NaN, an infinity or a value from 2^30 on: the codec's
+// absmax (NaN is skipped) and its literal scan.  Rare, and so out of line.  The
+// four lanes of the block call it together; byte in bits 16 and up, four codes
+// below.
+__device__ __noinline__ uint32_t literal_block(float x0, float x1, float x2, float x3) {
+    float f = fmaxf(fmaxf(fabsf(x0), fabsf(x1)), fmaxf(fabsf(x2), fabsf(x3)));
+    f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 2));
+    f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
+    const uint32_t byte = ue4m3_encode(fmaxf(__fdiv_rn(f == f ? f : 0.0f, 6.0f), kScaleMin));
+    const float inv = __fdiv_rn(1.0f, ue4m3_decode((uint8_t)byte));
+    return byte << 16 | (uint32_t)e2m1_scan(__fmul_rn(x0, inv)) | (uint32_t)e2m1_scan(__fmul_rn(x1, inv)) << 4 |
+           (uint32_t)e2m1_scan(__fmul_rn(x2, inv)) << 8 | (uint32_t)e2m1_scan(__fmul_rn(x3, inv)) << 12;
+}
+
+// Bytes of a cache row's elements and of its scales.
+template <int KIND>
+__device__ __forceinline__ int row_bytes(int d) { return KIND == kKvBf16 ? 2 * d : KIND == kKvFp8 ? d : d >> 1; }
+template <int KIND>
+__device__ __forceinline__ int scale_bytes(int d) { return KIND == kKvBf16 ? 0 : KIND == kKvFp8 ? 4 : d >> 4; }
+
+// Where lane l's share of a cache row goes: its first chunk (the second is half
+// a row further) and, if it writes one, its scale.
+struct Place {
+    uint8_t* codes;
+    uint8_t* scale;
+};
+template <int KIND>
+__device__ __forceinline__ Place place_of(const RowsParams& p, bool value, long row, int l) {
+    Place at;
+    at.codes = static_cast<uint8_t*>(value ? p.cache.v : p.cache.k) + row * row_bytes<KIND>(p.d) + l * (KIND == kKvBf16 ? 8 : KIND == kKvFp8 ? 4 : 2);
+    at.scale = static_cast<uint8_t*>(value ? p.cache.v_scale : p.cache.k_scale) + row * scale_bytes<KIND>(p.d);
+    // nvfp4: lane 4j writes the scale of the first half's block j, lane 4j + 1 of the second's
+    if (KIND == kKvNvfp4) at.scale += ((l & 1) ? p.d >> 5 : 0) + (l >> 2);
+    return at;
+}
+
+// Writes one row's lane share.  All lanes of the warp call it; `live`: the lane
+// has elements and its slot is valid.  top_a, top_b: see magnitudes; table: see
+// mantissa_reciprocal.
+template <int KIND, int L>
+__device__ __forceinline__ void store_row(const RowsParams& p, Place at, bool live, int l, const float (&a)[4], const float (&b)[4],
+                                          uint32_t top_a, uint32_t top_b, float table) {
+    uint8_t* second = at.codes + (row_bytes<KIND>(p.d) >> 1);
     if constexpr (KIND == kKvBf16) {
         if (!live) return;
-        uint16_t* out = static_cast<uint16_t*>(base) + (size_t)row * p.d;
-        *reinterpret_cast<uint2*>(out + 4 * l) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
-        *reinterpret_cast<uint2*>(out + half + 4 * l) = make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
+        *reinterpret_cast<uint2*>(at.codes) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
+        *reinterpret_cast<uint2*>(second) = make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
     } else if constexpr (KIND == kKvFp8) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(a[i]) & 0x7FFFFFFFu, __float_as_uint(b[i]) & 0x7FFFFFFFu));
-        // Non-negative floats order like their bits; a NaN orders above all
-        // and makes the row's scale, and so the row, NaN.
-        const float amax = __uint_as_float(max(decode::group_umax<L>(top), __float_as_uint(kFp8AbsmaxFloor)));
         if (!live) return;
+        // (a NaN makes the row's scale, and so the row, NaN)
+        const float amax = __uint_as_float(max(top_a, __float_as_uint(kFp8AbsmaxFloor)));
         const float inv = __fdiv_rn(kFp8Max, amax);
-        uint8_t* out = static_cast<uint8_t*>(base) + (size_t)row * p.d;
-        *reinterpret_cast<uint32_t*>(out + 4 * l) = decode::e4m3x4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-        *reinterpret_cast<uint32_t*>(out + half + 4 * l) = decode::e4m3x4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv);
-        if (l == 0) static_cast<float*>(scales)[row] = __fdiv_rn(amax, kFp8Max);
+        *reinterpret_cast<uint32_t*>(at.codes) = decode::e4m3x4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+        *reinterpret_cast<uint32_t*>(second) = decode::e4m3x4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv);
+        if (l == 0) *reinterpret_cast<float*>(at.scale) = __fdiv_rn(amax, kFp8Max);
     } else if constexpr (KIND == kKvNvfp4) {
         // The lane's two blocks: even lanes work out the first's scale, odd ones
-        // the second's, and they exchange them.
-        bool lit_a, lit_b;
-        const float max_a = block_absmax(a, lit_a), max_b = block_absmax(b, lit_b);
-        const bool odd = l & 1;
-        const uint32_t byte = ue4m3_encode(fmaxf(__fdiv_rn(odd ? max_b : max_a, 6.0f), kScaleMin));
-        const float inv = __fdiv_rn(1.0f, ue4m3_decode((uint8_t)byte));
-        const uint32_t other_byte = __shfl_xor_sync(0xffffffffu, byte, 1);
-        const float other_inv = __shfl_xor_sync(0xffffffffu, inv, 1);
-        const uint32_t sa = odd ? other_byte : byte, sb = odd ? byte : other_byte;
-        const uint32_t ca = block_codes(a, odd ? other_inv : inv, lit_a), cb = block_codes(b, odd ? inv : other_inv, lit_b);
-        if (!live) return;
-        uint8_t* out = static_cast<uint8_t*>(base) + (size_t)row * half;
-        *reinterpret_cast<uint16_t*>(out + 2 * l) = (uint16_t)ca;
-        *reinterpret_cast<uint16_t*>(out + (half >> 1) + 2 * l) = (uint16_t)cb;
-        if ((l & 3) == 0) {
-            uint8_t* sc = static_cast<uint8_t*>(scales) + (size_t)row * (p.d >> 4);
-            sc[l >> 2] = (uint8_t)sa;
-            sc[(p.d >> 5) + (l >> 2)] = (uint8_t)sb;
+        // the second's, and they exchange their reciprocals.
+        const bool odd = l & 1, lit_a = top_a >= kFastAbsmaxF32Limit, lit_b = top_b >= kFastAbsmaxF32Limit;
+        uint32_t byte = scale_byte(__uint_as_float(min(odd ? top_b : top_a, kFastAbsmaxF32Limit)));
+        const float inv = scale_reciprocal(table, byte), other = __shfl_xor_sync(0xffffffffu, inv, 1);
+        const float inv_a = odd ? other : inv, inv_b = odd ? inv : other;
+        uint32_t ca = decode::e2m1x4(a[0], a[1], a[2], a[3], inv_a), cb = decode::e2m1x4(b[0], b[1], b[2], b[3], inv_b);
+        if (__any_sync(0xffffffffu, lit_a || lit_b)) {
+            const uint32_t la = literal_block(a[0], a[1], a[2], a[3]), lb = literal_block(b[0], b[1], b[2], b[3]);
+            if (lit_a) ca = la & 0xFFFFu;
+            if (lit_b) cb = lb & 0xFFFFu;
+            if (odd ? lit_b : lit_a) byte = (odd ? lb : la) >> 16;
         }
+        if (!live) return;
+        *reinterpret_cast<uint16_t*>(at.codes) = (uint16_t)ca;
+        *reinterpret_cast<uint16_t*>(second) = (uint16_t)cb;
+        if ((l & 2) == 0) *at.scale = (uint8_t)byte;
     }
 }
 
-template <int KIND, int L, bool FULL>
-__global__ void __launch_bounds__(kThreads, FULL ? 4 : 1) kv_rows_kernel(const __grid_constant__ RowsParams p) {
+// Cache row of head 0 of token t's slot; -1 for none.
+__device__ __forceinline__ long slot_row(const RowsParams& p, long t, int lane) {
+    const long slot = decode::load_index(p.slots, t, p.slot64);
+    const long page = slot >> p.page_shift;
+    if (slot < 0) return -1;
+    if (page < p.cache.num_pages) return page * p.kv_heads * p.cache.page_size + (slot & (p.cache.page_size - 1));
+    if (lane == 0) decode::report(p.err, kErrSlotRange);
+    return -1;
+}
+
+__device__ __forceinline__ unsigned long long widen(uint32_t w) {
+    return ((unsigned long long)(w & 0xFFFF0000u) << 32) | (unsigned long long)(w << 16);
+}
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
+    return ((unsigned long long)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// The common forms: rows rotated as a whole in halves, normed or not (ROTATED),
+// or written as they are; values as they are.  Two elements an instruction, and
+// the norm weights multiplied into the table's factors once a token: with w_a,
+// w_b a pair's weights,
+//   out_a = (a (w_a c) - b (w_b s)) / rms,  out_b = (b (w_b c) + a (w_a s)) / rms
+// (55 instructions a round of 32 / L rows where the general kernel below, one
+// element and one check at a time, has 200).
+template <int KIND, int L, bool ROTATED>
+__global__ void __launch_bounds__(kThreads, 4) kv_walk_kernel(const __grid_constant__ RowsParams p) {
+    constexpr int kPer = 32 / L;  // heads of a token that a warp holds at once
+    decode::chain();
+    const int lane = threadIdx.x & 31, l = lane & (L - 1), sub = lane / L;
+    const unsigned unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const unsigned token = unit / (unsigned)p.walks;
+    if (token >= (unsigned)p.tokens) return;
+    const long t = token;
+    const int begin = (int)(unit - token * p.walks) * p.rounds, end = min(begin + p.rounds, p.all_rounds);
+    const bool inside = l < (p.d >> 3);
+    const int half = p.d >> 1;
+    [[maybe_unused]] const float table = mantissa_reciprocal(lane & 15);
+    [[maybe_unused]] const long row0 = KIND != kKvNone ? slot_row(p, t, lane) : -1;
+    [[maybe_unused]] float c[4], s[4];
+    if constexpr (ROTATED) {
+        const long pos = decode::load_index(p.positions, t, p.pos64);
+        const bool ok = pos >= 0 && pos < p.rope_rows;
+        if (!ok && lane == 0) decode::report(p.err, kErrPositionRange);
+        const float* row = p.rope + (ok ? pos : 0) * p.rot + 4 * (inside ? l : 0);
+        const float4 cv = *reinterpret_cast<const float4*>(row), sv = *reinterpret_cast<const float4*>(row + half);
+        c[0] = ok ? cv.x : 1.f, c[1] = ok ? cv.y : 1.f, c[2] = ok ? cv.z : 1.f, c[3] = ok ? cv.w : 1.f;
+        s[0] = ok ? sv.x : 0.f, s[1] = ok ? sv.y : 0.f, s[2] = ok ? sv.z : 0.f, s[3] = ok ? sv.w : 0.f;
+    }
+
+    // Walks rounds [from, to) of one kind of rows, two in flight ahead of the two
+    // at hand: `src` the lane's first chunk of head 0, `put(live, wa, wb)` what
+    // is done with each round's two chunks in turn.
+    auto walk = [&](int from, int to, const uint16_t* src, long stride, int heads, auto&& put) {
+        const uint16_t* at = src + (long)(from * kPer + sub) * stride;
+        const long step = kPer * stride;
+        int h = from * kPer + sub;  // the next head to be read
+        uint2 wa[2], wb[2];
+        auto fetch = [&](int r0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i, at += step, h += kPer) {
+                wa[i] = wb[i] = make_uint2(0u, 0u);
+                if (r0 + i < to && h < heads && inside) {
+                    wa[i] = *reinterpret_cast<const uint2*>(at);
+                    wb[i] = *reinterpret_cast<const uint2*>(at + half);
+                }
+            }
+        };
+        fetch(from);
+        int done = from * kPer + sub;  // the next head to be put
+        for (int r0 = from; r0 < to; r0 += 2) {
+            const uint2 a0 = wa[0], b0 = wb[0], a1 = wa[1], b1 = wb[1];
+            if (r0 + 2 < to) fetch(r0 + 2);
+            put(done < heads && inside, a0, b0);
+            if (r0 + 1 < to) put(done + kPer < heads && inside, a1, b1);
+            done += 2 * kPer;
+        }
+    };
+    auto rotated = [&](int from, int to, const uint16_t* src, long stride, int heads, const uint16_t* weight, auto&& put) {
+        unsigned long long ac[2], bs[2], bc[2], as[2];  // w_a c, -w_b s, w_b c, w_a s
+        {
+            float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
+            if (weight && inside) {
+                unpack4(__ldg(reinterpret_cast<const uint2*>(weight + 4 * l)), wa);
+                unpack4(__ldg(reinterpret_cast<const uint2*>(weight + half + 4 * l)), wb);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                ac[i] = pair_of(wa[2 * i] * c[2 * i], wa[2 * i + 1] * c[2 * i + 1]);
+                bs[i] = pair_of(-wb[2 * i] * s[2 * i], -wb[2 * i + 1] * s[2 * i + 1]);
+                bc[i] = pair_of(wb[2 * i] * c[2 * i], wb[2 * i + 1] * c[2 * i + 1]);
+                as[i] = pair_of(wa[2 * i] * s[2 * i], wa[2 * i + 1] * s[2 * i + 1]);
+            }
+        }
+        walk(from, to, src, stride, heads, [&](bool live, uint2 wa, uint2 wb) {
+            const unsigned long long a0 = widen(wa.x), a1 = widen(wa.y), b0 = widen(wb.x), b1 = widen(wb.y);
+            unsigned long long o[4] = {fma2(b0, bs[0], mul2(a0, ac[0])), fma2(b1, bs[1], mul2(a1, ac[1])),
+                                       fma2(a0, as[0], mul2(b0, bc[0])), fma2(a1, as[1], mul2(b1, bc[1]))};
+            if (weight) {
+                const unsigned long long q = fma2(a0, a0, fma2(a1, a1, fma2(b0, b0, mul2(b1, b1))));
+                const float sum = decode::group_sum<L>(__uint_as_float((uint32_t)q) + __uint_as_float((uint32_t)(q >> 32)));
+                const float inv = rsqrtf(sum * p.inv_d + p.eps);
+                const unsigned long long inv2 = pair_of(inv, inv);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = mul2(o[i], inv2);
+            }
+            float a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[2 * i] = __uint_as_float((uint32_t)o[i]), a[2 * i + 1] = __uint_as_float((uint32_t)(o[i] >> 32));
+                b[2 * i] = __uint_as_float((uint32_t)o[2 + i]), b[2 * i + 1] = __uint_as_float((uint32_t)(o[2 + i] >> 32));
+            }
+            put(live, a, b);
+        });
+    };
+    auto to_rows = [&](uint16_t* out, int from) {  // `out`: the lane's first chunk of head 0
+        out += (size_t)(from * kPer + sub) * p.d;
+        return [&, out](bool live, const float (&a)[4], const float (&b)[4]) mutable {
+            if (live) {
+                *reinterpret_cast<uint2*>(out) = make_uint2(decode::pack_bf16(a[0], a[1]), decode::pack_bf16(a[2], a[3]));
+                *reinterpret_cast<uint2*>(out + half) = make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
+            }
+            out += kPer * p.d;
+        };
+    };
+    [[maybe_unused]] const bool stored = row0 >= 0;
+    [[maybe_unused]] auto first_place = [&](bool value, int from) {
+        return place_of<KIND>(p, value, (stored ? row0 : 0) + (long)(from * kPer + sub) * p.cache.page_size, l);
+    };
+    [[maybe_unused]] const long code_step = (long)kPer * p.cache.page_size * row_bytes<KIND>(p.d);
+    [[maybe_unused]] const long scale_step = (long)kPer * p.cache.page_size * scale_bytes<KIND>(p.d);
+    [[maybe_unused]] auto raw_to_cache = [&](bool value, int from) {
+        Place at = first_place(value, from);
+        return [&, at](bool live, uint2 wa, uint2 wb) mutable {
+            float a[4], b[4];
+            unpack4(wa, a);
+            unpack4(wb, b);
+            uint32_t top_a = 0, top_b = 0;
+            if constexpr (KIND == kKvFp8 || KIND == kKvNvfp4) magnitudes<KIND, L>(wa, wb, top_a, top_b);
+            store_row<KIND, L>(p, at, live && stored, l, a, b, top_a, top_b, table);
+            at.codes += code_step, at.scale += scale_step;
+        };
+    };
+
+    if constexpr (ROTATED) {
+        if (begin < p.q_rounds)
+            rotated(begin, min(end, p.q_rounds), p.q + t * p.q_st + 4 * l, p.q_sh, p.q_heads, p.q_weight,
+                    to_rows(p.q_out + (size_t)t * p.q_heads * p.d + 4 * l, begin));
+    }
+    const int k_begin = max(begin - p.q_rounds, 0), k_end = min(end, p.k_rounds) - p.q_rounds;
+    if (k_begin < k_end) {
+        const uint16_t* src = p.k + t * p.k_st + 4 * l;
+        if constexpr (ROTATED && KIND == kKvNone) {
+            rotated(k_begin, k_end, src, p.k_sh, p.kv_heads, p.k_weight, to_rows(p.k_out + (size_t)t * p.kv_heads * p.d + 4 * l, k_begin));
+        } else if constexpr (ROTATED) {
+            Place at = first_place(false, k_begin);
+            rotated(k_begin, k_end, src, p.k_sh, p.kv_heads, p.k_weight, [&](bool live, const float (&a)[4], const float (&b)[4]) {
+                uint32_t top_a = 0, top_b = 0;
+                if constexpr (KIND == kKvFp8 || KIND == kKvNvfp4) magnitudes<KIND, L>(a, b, top_a, top_b);
+                store_row<KIND, L>(p, at, live && stored, l, a, b, top_a, top_b, table);
+                at.codes += code_step, at.scale += scale_step;
+            });
+        } else {
+            walk(k_begin, k_end, src, p.k_sh, p.kv_heads, raw_to_cache(false, k_begin));
+        }
+    }
+    if constexpr (KIND != kKvNone) {
+        const int v_begin = max(begin - p.k_rounds, 0), v_end = end - p.k_rounds;
+        if (v_begin < v_end) walk(v_begin, v_end, p.v + t * p.v_st + 4 * l, p.v_sh, p.kv_heads, raw_to_cache(true, v_begin));
+    }
+}
+
+// Every other form: parts of rows and pairs rotated, norms without a rotation.
+template <int KIND, int L>
+__global__ void __launch_bounds__(kThreads) kv_rows_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kPer = 32 / L;  // heads of a token that a warp holds at once
     decode::chain();
     const int lane = threadIdx.x & 31, l = lane & (L - 1), sub = lane / L;
@@ -241,37 +471,21 @@ __global__ void __launch_bounds__(kThreads, FULL ? 4 : 1) kv_rows_kernel(const _
     fetch(begin);
 
     // The token's slot, its table row, and the norm weights of the lane's elements.
-    long row0 = -1;  // cache row of head 0
-    if constexpr (KIND != kKvNone) {
-        const long slot = decode::load_index(p.slots, t, p.slot64);
-        const long page = slot >> p.page_shift;
-        if (slot >= 0) {
-            if (page < p.cache.num_pages)
-                row0 = page * p.kv_heads * p.cache.page_size + (slot & (p.cache.page_size - 1));
-            else if (lane == 0)
-                decode::report(p.err, kErrSlotRange);
-        }
-    }
+    [[maybe_unused]] const float table = mantissa_reciprocal(lane & 15);
+    [[maybe_unused]] const long row0 = KIND != kKvNone ? slot_row(p, t, lane) : -1;
     float ca[4], sa[4], cb[4], sb[4];
     if (p.rope) {
         const long pos = decode::load_index(p.positions, t, p.pos64);
         const bool ok = pos >= 0 && pos < p.rope_rows;
         if (!ok && lane == 0) decode::report(p.err, kErrPositionRange);
         const float* row = p.rope + (ok ? pos : 0) * p.rot;
-        if constexpr (FULL) {  // rot == d, 16-byte aligned table
-            const float4 c = inside ? *reinterpret_cast<const float4*>(row + 4 * l) : make_float4(1.f, 1.f, 1.f, 1.f);
-            const float4 s = inside ? *reinterpret_cast<const float4*>(row + half + 4 * l) : make_float4(0.f, 0.f, 0.f, 0.f);
-            ca[0] = ok ? c.x : 1.f, ca[1] = ok ? c.y : 1.f, ca[2] = ok ? c.z : 1.f, ca[3] = ok ? c.w : 1.f;
-            sa[0] = ok ? s.x : 0.f, sa[1] = ok ? s.y : 0.f, sa[2] = ok ? s.z : 0.f, sa[3] = ok ? s.w : 0.f;
-        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                ca[i] = cb[i] = 1.0f;
-                sa[i] = sb[i] = 0.0f;
-                if (inside && ok) {
-                    factors(p, row, 4 * l + i, ca[i], sa[i]);
-                    factors(p, row, half + 4 * l + i, cb[i], sb[i]);
-                }
+        for (int i = 0; i < 4; ++i) {
+            ca[i] = cb[i] = 1.0f;
+            sa[i] = sb[i] = 0.0f;
+            if (inside && ok) {
+                factors(p, row, 4 * l + i, ca[i], sa[i]);
+                factors(p, row, half + 4 * l + i, cb[i], sb[i]);
             }
         }
     }
@@ -305,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, FULL ? 4 : 1) kv_rows_kernel(const _
                         b[e] = b[e] * inv * nb[e];
                     }
                 }
-                if (p.rope) rotate<L, FULL>(p, a, b, ca, sa, cb, sb, l);
+                if (p.rope) rotate<L>(p, a, b, ca, sa, cb, sb, l);
             }
             if (query || (key && KIND == kKvNone)) {
                 if (live) {
@@ -314,7 +528,10 @@ __global__ void __launch_bounds__(kThreads, FULL ? 4 : 1) kv_rows_kernel(const _
                     *reinterpret_cast<uint2*>(out + half) = make_uint2(decode::pack_bf16(b[0], b[1]), decode::pack_bf16(b[2], b[3]));
                 }
             } else if constexpr (KIND != kKvNone) {
-                store_row<KIND, L>(p, !key, row0 + (long)h * p.cache.page_size, live && row0 >= 0, l, a, b);
+                uint32_t top_a = 0, top_b = 0;
+                if constexpr (KIND == kKvFp8 || KIND == kKvNvfp4) magnitudes<KIND, L>(a, b, top_a, top_b);
+                const Place at = place_of<KIND>(p, !key, (row0 < 0 ? 0 : row0) + (long)h * p.cache.page_size, l);
+                store_row<KIND, L>(p, at, live && row0 >= 0, l, a, b, top_a, top_b, table);
             }
         }
         if (r0 + kBatch < end) fetch(r0 + kBatch);
@@ -415,9 +632,10 @@ int shift_of(int page_size) {
     return s;
 }
 
-template <int KIND, bool FULL>
+template <int KIND>
 cudaError_t launch_rows(RowsParams& p, cudaStream_t st) {
     const int need = p.d >> 3, lanes = need <= 8 ? 8 : need <= 16 ? 16 : 32, per = 32 / lanes;
+    const bool rotated = p.rope && p.rot == p.d && !p.pairs && aligned(p.rope, 16);
     p.q_rounds = (p.q_heads + per - 1) / per;
     p.k_rounds = p.q_rounds + (p.k ? (p.kv_heads + per - 1) / per : 0);
     p.all_rounds = p.k_rounds + (p.v ? (p.kv_heads + per - 1) / per : 0);
@@ -426,17 +644,16 @@ cudaError_t launch_rows(RowsParams& p, cudaStream_t st) {
     // rounds share one table row and prologue, fewer spread over the GPU.
     p.rounds = (int)std::clamp((long)p.tokens * p.all_rounds / (148 * 64), 1l, (long)p.all_rounds);
     p.walks = (p.all_rounds + p.rounds - 1) / p.rounds;
+    p.rounds = (p.all_rounds + p.walks - 1) / p.walks;  // the same for all, nearly
     const long blocks = ((long)p.walks * p.tokens + kWarps - 1) / kWarps;
-    auto* kernel = lanes == 8    ? kv_rows_kernel<KIND, 8, FULL>
-                   : lanes == 16 ? kv_rows_kernel<KIND, 16, FULL>
-                                 : kv_rows_kernel<KIND, 32, FULL>;
+    void (*kernel)(RowsParams) =
+        rotated ? (lanes == 8 ? kv_walk_kernel<KIND, 8, true> : lanes == 16 ? kv_walk_kernel<KIND, 16, true> : kv_walk_kernel<KIND, 32, true>)
+                : (lanes == 8 ? kv_rows_kernel<KIND, 8> : lanes == 16 ? kv_rows_kernel<KIND, 16> : kv_rows_kernel<KIND, 32>);
+    if constexpr (KIND != kKvNone) {
+        if (!p.rope && !p.k_weight && !p.q)
+            kernel = lanes == 8 ? kv_walk_kernel<KIND, 8, false> : lanes == 16 ? kv_walk_kernel<KIND, 16, false> : kv_walk_kernel<KIND, 32, false>;
+    }
     return decode::launch_chained(kernel, dim3((unsigned)blocks), kThreads, 0, st, p);
-}
-
-template <int KIND>
-cudaError_t launch_kind(RowsParams& p, cudaStream_t st) {
-    const bool full = !p.rope || (p.rot == p.d && !p.pairs && aligned(p.rope, 16));
-    return full ? launch_rows<KIND, true>(p, st) : launch_rows<KIND, false>(p, st);
 }
 
 // Checks shared by the two writing entry points; nullptr when all is well.
@@ -517,11 +734,11 @@ FP4B_EXPORT int fp4b_kv_rows(const fp4b_rows* rows, void* stream) {
     if (cache) {
         p.cache = *cache;
         p.page_shift = shift_of(cache->page_size);
-        e = cache->kind == kKvBf16 ? launch_kind<kKvBf16>(p, st)
-            : cache->kind == kKvFp8 ? launch_kind<kKvFp8>(p, st)
-                                    : launch_kind<kKvNvfp4>(p, st);
+        e = cache->kind == kKvBf16 ? launch_rows<kKvBf16>(p, st)
+            : cache->kind == kKvFp8 ? launch_rows<kKvFp8>(p, st)
+                                    : launch_rows<kKvNvfp4>(p, st);
     } else {
-        e = launch_kind<kKvNone>(p, st);
+        e = launch_rows<kKvNone>(p, st);
     }
     return launch_status(e, "fp4b_kv_rows");
 }

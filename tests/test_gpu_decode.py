@@ -318,6 +318,21 @@ def test_nvfp4_extreme_blocks_equal_the_quantizer(dec, cuda):
     assert torch.equal(cache.v_scales.cpu()[slots // 8, :, slots % 8], scales)
 
 
+def test_nvfp4_scale_of_every_absmax(dec, cuda):
+    # one block for each positive BF16 number, as its absmax: the scale bytes and codes of the weight quantizer
+    amax = torch.arange(1, 0x7F80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    n = -(-len(amax) // 8)
+    x = torch.zeros(n * 8, 16, dtype=torch.bfloat16)
+    x[: len(amax)] = (amax.float().unsqueeze(1) * torch.linspace(-1, 1, 16)).to(torch.bfloat16)
+    x = x.reshape(n, 1, 128)
+    cache = dec.PagedKVCache(-(-n // 64), 64, 1, 128, "nvfp4", device=cuda)
+    slots = torch.arange(n)
+    cache.append(x.to(cuda), x.to(cuda), slots.to(cuda))
+    codes, scales = stored(x, "nvfp4")
+    assert torch.equal(cache.k_scales.cpu()[slots // 64, :, slots % 64], scales)
+    assert torch.equal(cache.v_pages.cpu()[slots // 64, :, slots % 64], codes)
+
+
 def test_fp8_extreme_rows(dec, cuda):
     x = torch.randn(6, 1, 64, generator=torch.Generator().manual_seed(0))
     x[1] *= 2.0 ** -120
