@@ -640,9 +640,9 @@ cudaError_t launch_rows(RowsParams& p, cudaStream_t st) {
     p.k_rounds = p.q_rounds + (p.k ? (p.kv_heads + per - 1) / per : 0);
     p.all_rounds = p.k_rounds + (p.v ? (p.kv_heads + per - 1) / per : 0);
     p.inv_d = 1.0f / (float)p.d;
-    // As many rounds a warp as leave about 64 warps for each of 148 SMs: more
+    // As many rounds a warp as leave about 32 warps for each of 148 SMs: more
     // rounds share one table row and prologue, fewer spread over the GPU.
-    p.rounds = (int)std::clamp((long)p.tokens * p.all_rounds / (148 * 64), 1l, (long)p.all_rounds);
+    p.rounds = (int)std::clamp((long)p.tokens * p.all_rounds / (148 * 32), 1l, (long)p.all_rounds);
     p.walks = (p.all_rounds + p.rounds - 1) / p.rounds;
     p.rounds = (p.all_rounds + p.walks - 1) / p.walks;  // the same for all, nearly
     const long blocks = ((long)p.walks * p.tokens + kWarps - 1) / kWarps;
