@@ -37,9 +37,12 @@
 // keys of one sequence and head unit, one step for each warp; the rounds of the
 // whole batch, in order, are dealt out evenly to the CTAs, each of which finds
 // its share by a prefix sum over the lengths.  Lengths of any unevenness fill
-// the GPU the same.  A share may end inside a sequence: such parts go to the
-// workspace, and the CTA that arrives last at a sequence's counter joins them,
-// in the order of their keys, so that results do not depend on the arrival.
+// the GPU the same.  A share is cut into segments of one head unit each; a unit
+// whose rounds lie in several CTAs has its parts in the workspace, and the CTA
+// that arrives last at its counter joins them, in the order of their keys, so
+// that results do not depend on the arrival.  A CTA has at most two such parts,
+// its first and its last segment, and arrives for both at its end: one fence.
+// The first steps of the next segment are under way while one is finished.
 //
 // A warp streams its steps through a ring of its own in shared memory with
 // cp.async: no barrier in the loop.  Masked keys are zero-filled, not read.
@@ -87,9 +90,13 @@ struct AttentionParams {
     uint16_t* out;
     float* lse;
     int* err;
-    uint32_t* counters;  // [grid], zero before and after
-    float* part_ml;      // [2 * grid][heads of a unit][2]
-    float* part_acc;     // [2 * grid][heads of a unit][D]
+    // Workspace: counters [max_ctas], zero before and after; the parts that go on
+    // in CTA c at c, those that begin in it at max_ctas + c: (maximum, sum)
+    // [2 * max_ctas][heads of a unit][2] and sums [2 * max_ctas][heads][D].
+    int max_ctas;
+    uint32_t* counters;
+    float* part_ml;
+    float* part_acc;
 };
 
 template <int KIND, int D, int NT>
@@ -101,12 +108,14 @@ struct Cfg {
     static constexpr int HEADS = 8 * NT;
     static constexpr int ROUND = kWarps * TK;
     static constexpr int STAGE = 2 * TK * (RB + SB);
-    // About 24 KB of ring a warp where rows are wide, at least 4 stages where they are narrow.
-    static constexpr int STAGES = STAGE >= 16384 ? 3 : STAGE >= 8192 ? 3 : 4;
+    static constexpr int STAGES = STAGE >= 4096 ? 3 : 4;
     static constexpr int RING = STAGES * STAGE;
     static constexpr int LD = D + 8;                // row stride of the merge area
     static constexpr int MERGE = kWarps * HEADS * LD * 4;
-    static constexpr int SMEM = (kWarps * RING > MERGE ? kWarps * RING : MERGE);
+    // Where a third stage would not fit beside it, the merge area lies over the
+    // rings and the next segment's steps start after it was read.
+    static constexpr bool APART = STAGE < 8192;
+    static constexpr int SMEM = APART ? kWarps * RING + MERGE : (kWarps * RING > MERGE ? kWarps * RING : MERGE);
     // Elements of one of a lane's runs in a K row (4 lanes share the row) and in a V row (8 lanes).
     static constexpr int EK = KIND == kKvBf16 ? 8 : KIND == kKvFp8 ? 16 : (D == 64 ? 16 : 32);
     static constexpr int EV = KIND == kKvBf16 ? 8 : KIND == kKvFp8 ? (D == 64 ? 8 : 16) : D / 8;
@@ -133,15 +142,15 @@ struct Span {
 template <int TK, int ROUND>
 __device__ __forceinline__ Span span_of(const AttentionParams& p, int b) {
     Span s;
-    const long most = (long)p.table_width << p.page_shift;
+    const int most = p.table_width << p.page_shift;
     s.len = p.lens[b];
     if (s.len < 0 || s.len > most) {
         report(p.err, kErrPageRange);
-        s.len = s.len < 0 ? 0 : (int)most;
+        s.len = s.len < 0 ? 0 : most;
     }
     s.first = p.window > 0 && s.len > p.window ? s.len - p.window : 0;
     s.start = s.first & ~(TK - 1);
-    s.rounds = (int)(((long)s.len - s.start + ROUND - 1) / ROUND);
+    s.rounds = (s.len - s.start + ROUND - 1) / ROUND;
     return s;
 }
 
@@ -162,118 +171,161 @@ __device__ __forceinline__ Finish finish(const AttentionParams& p, int head, flo
     return Finish{l == 0.0f ? 0.0f : unit * share / l, l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2};
 }
 
+// Four elements of an output row from their sums relative to 2^m; unit: what the
+// sums are to be multiplied by.
+template <int D>
+__device__ __forceinline__ void put_row(const AttentionParams& p, int b, int head, int d, float m, float l, float4 sum, float unit) {
+    const Finish f = finish(p, head, m, l, unit);
+    const size_t row = (size_t)b * p.q_heads + head;
+    *reinterpret_cast<uint2*>(p.out + row * D + d) =
+        make_uint2(pack_bf16(sum.x * f.factor, sum.y * f.factor), pack_bf16(sum.z * f.factor, sum.w * f.factor));
+    if (p.lse && d == 0) p.lse[row] = f.lse;
+}
+
+// A head unit that several CTAs, first to last, have parts of.
+struct Part {
+    int b, head0, heads, first, last;
+};
+
+// Joins a unit's parts in their order: the first one's from the parts that begin
+// in a CTA, the others' from those that go on in one, kAhead of them in flight.
+template <int D, int HEADS>
+__device__ __forceinline__ void join_parts(const AttentionParams& p, const Part& x, float unit) {
+    constexpr int kItems = (HEADS * D / 4 + kThreads - 1) / kThreads;  // quarters of rows a thread
+    constexpr int kAhead = kItems > 4 ? 2 : kItems > 1 ? 4 : 8;
+    const int quarters = x.heads * (D / 4);
+    float m[kItems], l[kItems];
+    float4 sum[kItems];
+    const float2* ml[kItems];
+    const float4* acc[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int j = min((int)threadIdx.x + k * kThreads, quarters - 1);
+        const size_t begin = (size_t)(p.max_ctas + x.first) * HEADS, on = (size_t)(x.first + 1) * HEADS;
+        const float2 one = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + begin + j / (D / 4));
+        sum[k] = __ldcg(reinterpret_cast<const float4*>(p.part_acc + begin * D) + j);
+        m[k] = one.x, l[k] = one.y;
+        ml[k] = reinterpret_cast<const float2*>(p.part_ml) + on + j / (D / 4);
+        acc[k] = reinterpret_cast<const float4*>(p.part_acc + on * D) + j;
+    }
+    for (int left = x.last - x.first; left > 0; left -= kAhead) {
+        float2 a[kItems][kAhead];
+        float4 v[kItems][kAhead];
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                a[k][i] = make_float2(kNoScore, 0.0f);
+                v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < left) {
+                    a[k][i] = __ldcg(ml[k] + i * HEADS);
+                    v[k][i] = __ldcg(acc[k] + i * (HEADS * D / 4));
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            ml[k] += kAhead * HEADS, acc[k] += kAhead * (HEADS * D / 4);
+            float top = m[k];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) top = fmaxf(top, a[k][i].x);
+            const float old = exp2_approx(m[k] - top);
+            sum[k].x *= old, sum[k].y *= old, sum[k].z *= old, sum[k].w *= old, l[k] *= old;
+            m[k] = top;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float add = exp2_approx(a[k][i].x - top);
+                sum[k].x += v[k][i].x * add, sum[k].y += v[k][i].y * add, sum[k].z += v[k][i].z * add, sum[k].w += v[k][i].w * add;
+                l[k] += a[k][i].y * add;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int j = (int)threadIdx.x + k * kThreads, h = j / (D / 4);
+        if (j < quarters) put_row<D>(p, x.b, x.head0 + h, 4 * (j - h * (D / 4)), m[k], l[k], sum[k], unit);
+    }
+}
+
 template <int KIND, int D, int NT>
 __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid_constant__ AttentionParams p) {
     using C = Cfg<KIND, D, NT>;
     constexpr int TK = C::TK, KT = C::KT, RB = C::RB, SB = C::SB, MT = D / 16, HEADS = C::HEADS;
     constexpr bool kBf16 = KIND == kKvBf16;
+    constexpr float kUnit = KIND == kKvNvfp4 ? kScaleUnit : 1.0f;  // of the decoded values
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long s_pre, s_total[kWarps];
-    __shared__ int s_b;
+    __shared__ int s_total[kWarps], s_most[kWarps], s_pre, s_b;
     __shared__ float s_m[kWarps][HEADS], s_l[kWarps][HEADS];
-    __shared__ int s_last;
+    __shared__ Part s_part[2];
+    __shared__ int s_last[2];
 
     chain();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int units = p.cache.kv_heads * p.group_tiles;
 
-    // ---- this CTA's share [u0, u1) of the batch's rounds, and the sequence that it starts in
-    long total = 0, mine = 0, before = 0;
-    for (int base = 0; base < p.batch; base += kThreads) {
+    // ---- the batch's rounds: their number, and the prefix sums of the chunk at hand
+    int total = 0, most = 0, mine = 0, before = 0;
+    auto scan = [&](int base) {
         const int b = base + tid;
-        mine = b < p.batch ? (long)span_of<TK, C::ROUND>(p, b).rounds * units : 0;
-        long scan = mine;
+        const int rounds = b < p.batch ? span_of<TK, C::ROUND>(p, b).rounds : 0;
+        mine = rounds * units;
+        int sum = mine, top = rounds;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long other = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += other;
+            const int other = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += other;
         }
-        if (lane == 31) s_total[warp] = scan;
+        top = __reduce_max_sync(0xffffffffu, top);
         __syncthreads();
-        before = total + scan - mine;
+        if (lane == 31) s_total[warp] = sum, s_most[warp] = top;
+        __syncthreads();
+        before = total + sum - mine;
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) before += s_total[w];
             total += s_total[w];
+            most = max(most, s_most[w]);
         }
+    };
+    for (int base = 0; base < p.batch; base += kThreads) scan(base);
+    // Joining P parts costs about P times 0.06 us, a round about 0.4 us: a CTA
+    // takes at least the rounds that balance the two for the longest sequence.
+    const int least = max(1, (int)sqrtf((float)most * (1.0f / 7.0f)));
+    const int ctas = min((int)gridDim.x, max(total / least, min(total, 1)));
+    if ((int)blockIdx.x < ctas) {
+        // CTA c's share starts at c * each + min(c, extra)
+        const int each = total / ctas, extra = total - each * ctas;
+        int u = (int)blockIdx.x * each + min((int)blockIdx.x, extra);
+        const int u1 = u + each + ((int)blockIdx.x < extra ? 1 : 0);
+        auto owner = [&](int x) {
+            const int cut = extra * (each + 1);
+            return x < cut ? x / (each + 1) : extra + (x - cut) / each;
+        };
+        if (p.batch > kThreads) {  // the sums at hand are the last chunk's: go over them again
+            total = 0;
+            for (int base = 0; base < p.batch && total <= u; base += kThreads) {
+                scan(base);
+                if (before <= u && u < before + mine) s_b = base + tid, s_pre = before;
+            }
+        } else if (before <= u && u < before + mine) {
+            s_b = tid, s_pre = before;
+        }
+        if (tid < 2) s_part[tid].b = -1;
         __syncthreads();
-    }
-    // Sequences without keys: their rows are the sink's alone.
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        if (span_of<TK, C::ROUND>(p, b).rounds > 0) continue;
-        for (int i = tid; i < p.q_heads * (D / 4); i += kThreads)
-            *reinterpret_cast<uint2*>(p.out + (size_t)b * p.q_heads * D + 4 * i) = make_uint2(0u, 0u);
-        if (p.lse)
-            for (int h = tid; h < p.q_heads; h += kThreads)
-                p.lse[(size_t)b * p.q_heads + h] = finish(p, h, kNoScore, 0.0f, 1.0f).lse;
-    }
-    if (total == 0) return;
-    const long ctas = min((long)gridDim.x, total);
-    if ((long)blockIdx.x >= ctas) return;
-    long u = total * blockIdx.x / ctas;
-    const long u1 = total * (blockIdx.x + 1) / ctas;
-    if (p.batch > kThreads) {  // the sums of the last chunk are the ones at hand: go over them again
-        long sum = 0;
-        for (int base = 0; base < p.batch; base += kThreads) {
-            const int b = base + tid;
-            mine = b < p.batch ? (long)span_of<TK, C::ROUND>(p, b).rounds * units : 0;
-            long scan = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long other = __shfl_up_sync(0xffffffffu, scan, o);
-                if (lane >= o) scan += other;
-            }
-            if (lane == 31) s_total[warp] = scan;
-            __syncthreads();
-            before = sum + scan - mine;
-            for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) before += s_total[w];
-                sum += s_total[w];
-            }
-            if (mine > 0 && before <= u && u < before + mine) {
-                s_b = b;
-                s_pre = before;
-            }
-            __syncthreads();
-            if (sum > u) break;
-        }
-    } else {
-        if (mine > 0 && before <= u && u < before + mine) {
-            s_b = tid;
-            s_pre = before;
-        }
-        __syncthreads();
-    }
-    int b = s_b;
-    long pre = s_pre;
+        int b = s_b, pre = s_pre;  // the sequence at hand and the rounds before it
 
-    uint8_t* ring = smem + warp * C::RING;
-    const uint32_t ring_addr = ptx::smem_u32(ring);
-
-    while (u < u1) {
-        const Span span = span_of<TK, C::ROUND>(p, b);
-        if (span.rounds == 0) {
-            ++b;
-            continue;
-        }
-        const long local = u - pre;
-        const int unit = (int)(local / span.rounds), r0 = (int)(local - (long)unit * span.rounds);
-        const int r1 = (int)min((long)span.rounds, r0 + (u1 - u));
-        const int kv_head = unit / p.group_tiles, in_group = (unit - kv_head * p.group_tiles) * HEADS;
-        const int head0 = kv_head * p.group + in_group, live_heads = min(HEADS, p.group - in_group);
-
-        // ---- the stream of this warp's steps
-        const int* table = p.table + (size_t)b * p.table_stride;
-        const int step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
-        int steps = r1 - r0;
-        if (steps > 0 && (long)step0 + (long)(steps - 1) * C::ROUND >= span.len) --steps;
+        uint8_t* ring = smem + warp * C::RING;
+        const uint32_t ring_addr = ptx::smem_u32(ring);
         const bool in_page = p.cache.page_size >= TK;  // a step's keys are one run of one page
         const int my_key = lane & (TK - 1);
+
+        // ---- a segment: rounds [r0, r1) of one head unit, and the stream of this warp's steps of it
+        Span span{};
+        int unit = 0, r0 = 0, r1 = 0, kv_head = 0, step0 = 0, steps = 0, next_page = -2;
+        const int* table = nullptr;
         auto page_of = [&](int s) {  // page of the lane's key of step s (of all its keys, if in_page); -2 for a masked key
             if (s >= steps) return -2;
             const int key0 = step0 + s * C::ROUND, key = key0 + (in_page ? 0 : my_key);
             return (in_page || key >= span.first) && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
         };
-        int next_page = page_of(0);
         auto issue = [&](int s) {
             if (s < steps) {
                 const int key0 = step0 + s * C::ROUND;
@@ -321,411 +373,426 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             }
             copy_commit();
         };
-#pragma unroll
-        for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
-
-        // ---- queries: column g of head tile nt, element 4 EK (j / (EK/4)) + EK t + 4 (j % (EK/4)) of k-step j
-        uint32_t qf[NT][MT][2];
-        float f0[NT], f1[NT];  // score factors of heads 2t, 2t + 1
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int n = 8 * nt + g;
-            const uint16_t* row = p.q + (size_t)b * p.q_sb + (size_t)(head0 + (n < live_heads ? n : 0)) * p.q_sh;
-            uint2 w[MT];
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                const int d = 4 * C::EK * (j / (C::EK / 4)) + C::EK * t + 4 * (j % (C::EK / 4));
-                w[j] = n < live_heads ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+        // Makes the rounds from u on the segment at hand and starts its stream; false at the share's end.
+        auto open = [&]() {
+            if (u >= u1) return false;
+            for (span = span_of<TK, C::ROUND>(p, b); u >= pre + span.rounds * units && b + 1 < p.batch; span = span_of<TK, C::ROUND>(p, b)) {
+                pre += span.rounds * units;
+                ++b;
             }
-            float factor = p.scale2;
-            if constexpr (kBf16) {
+            const int local = u - pre;
+            unit = local / span.rounds;
+            r0 = local - unit * span.rounds;
+            r1 = min(span.rounds, r0 + (u1 - u));
+            kv_head = unit / p.group_tiles;
+            table = p.table + (size_t)b * p.table_stride;
+            step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
+            steps = r1 - r0;
+            if (step0 + (steps - 1) * C::ROUND >= span.len) --steps;
+            next_page = page_of(0);
 #pragma unroll
-                for (int j = 0; j < MT; ++j) qf[nt][j][0] = w[j].x, qf[nt][j][1] = w[j].y;
-            } else {
-                uint32_t top = 0;  // largest magnitude's bits
+            for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+            return true;
+        };
+
+        bool more = open();
+        while (more) {
+            const int in_group = (unit - kv_head * p.group_tiles) * HEADS;
+            const int head0 = kv_head * p.group + in_group, live_heads = min(HEADS, p.group - in_group);
+
+            // ---- queries: column g of head tile nt, element 4 EK (j / (EK/4)) + EK t + 4 (j % (EK/4)) of k-step j
+            uint32_t qf[NT][MT][2];
+            float f0[NT], f1[NT];  // score factors of heads 2t, 2t + 1
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int n = 8 * nt + g;
+                const uint16_t* row = p.q + (size_t)b * p.q_sb + (size_t)(head0 + (n < live_heads ? n : 0)) * p.q_sh;
+                uint2 w[MT];
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
-                    top = max(top, max((w[j].x & 0x7FFFu) << 16, w[j].x & 0x7FFF0000u));
-                    top = max(top, max((w[j].y & 0x7FFFu) << 16, w[j].y & 0x7FFF0000u));
+                    const int d = 4 * C::EK * (j / (C::EK / 4)) + C::EK * t + 4 * (j % (C::EK / 4));
+                    w[j] = n < live_heads ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
                 }
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int k = min(max(141 - (int)(top >> 23), -126), 126);
-                const float up = __int_as_float((127 + k) << 23);
-#pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    qf[nt][j][0] = pack_f16(bf16_lo(w[j].x) * up, bf16_hi(w[j].x) * up);
-                    qf[nt][j][1] = pack_f16(bf16_lo(w[j].y) * up, bf16_hi(w[j].y) * up);
-                }
-                factor *= __int_as_float((127 - k) << 23);
-                if (KIND == kKvNvfp4) factor *= kScaleUnit;
-            }
-            f0[nt] = __shfl_sync(0xffffffffu, factor, 8 * t);
-            f1[nt] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
-        }
-
-        float acc[NT][MT][4];
-        float ref0[NT], ref1[NT], l0[NT], l1[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            ref0[nt] = ref1[nt] = kNoScore;
-            l0[nt] = l1[nt] = 0.0f;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[nt][m][i] = 0.0f;
-        }
-
-        for (int s = 0; s < steps; ++s) {
-            copy_wait<C::STAGES - 2>();
-            __syncwarp();
-            issue(s + C::STAGES - 1);
-            const uint8_t* sk = ring + (s % C::STAGES) * C::STAGE;
-            const uint8_t* sv = sk + TK * RB;
-            const uint8_t* ss = sv + TK * RB;
-            const int key0 = step0 + s * C::ROUND;
-
-            // ---- scores
-            float sc[NT][KT][4];
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[nt][kt][i] = 0.0f;
-                const int ra = 16 * kt + g, rb = ra + 8;
+                float factor = p.scale2;
                 if constexpr (kBf16) {
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma<true>(sc[nt][kt], a.x, c.x, a.y, c.y, qf[nt][2 * i][0], qf[nt][2 * i][1]);
-                            mma<true>(sc[nt][kt], a.z, c.z, a.w, c.w, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
-                        }
-                    }
-                } else if constexpr (KIND == kKvFp8) {
-#pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
-                        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t ha[2], hc[2];
-                            e4m3x4_to_f16(aw[q], ha);
-                            e4m3x4_to_f16(cw[q], hc);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
-                        }
-                    }
+                    for (int j = 0; j < MT; ++j) qf[nt][j][0] = w[j].x, qf[nt][j][1] = w[j].y;
                 } else {
-                    constexpr int WORDS = C::EK / 8, PIECES = D / (4 * C::EK);
+                    uint32_t top = 0;  // largest magnitude's bits
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i) {
-                        uint32_t aw[WORDS], cw[WORDS];
-                        if constexpr (WORDS == 2) {
-                            const uint2 a = lds64(sk + k_offset<RB>(ra, 0) + 8 * t), c = lds64(sk + k_offset<RB>(rb, 0) + 8 * t);
-                            aw[0] = a.x, aw[1] = a.y, cw[0] = c.x, cw[1] = c.y;
-                        } else {
+                    for (int j = 0; j < MT; ++j) {
+                        top = max(top, max((w[j].x & 0x7FFFu) << 16, w[j].x & 0x7FFF0000u));
+                        top = max(top, max((w[j].y & 0x7FFFu) << 16, w[j].y & 0x7FFF0000u));
+                    }
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const int k = min(max(141 - (int)(top >> 23), -126), 126);
+                    const float up = __int_as_float((127 + k) << 23);
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        qf[nt][j][0] = pack_f16(bf16_lo(w[j].x) * up, bf16_hi(w[j].x) * up);
+                        qf[nt][j][1] = pack_f16(bf16_lo(w[j].y) * up, bf16_hi(w[j].y) * up);
+                    }
+                    factor *= __int_as_float((127 - k) << 23);
+                    if (KIND == kKvNvfp4) factor *= kScaleUnit;
+                }
+                f0[nt] = __shfl_sync(0xffffffffu, factor, 8 * t);
+                f1[nt] = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
+            }
+
+            float acc[NT][MT][4];
+            float ref0[NT], ref1[NT], l0[NT], l1[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                ref0[nt] = ref1[nt] = kNoScore;
+                l0[nt] = l1[nt] = 0.0f;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[nt][m][i] = 0.0f;
+            }
+
+            for (int s = 0; s < steps; ++s) {
+                copy_wait<C::STAGES - 2>();
+                __syncwarp();
+                issue(s + C::STAGES - 1);
+                const uint8_t* sk = ring + (s % C::STAGES) * C::STAGE;
+                const uint8_t* sv = sk + TK * RB;
+                const uint8_t* ss = sv + TK * RB;
+                const int key0 = step0 + s * C::ROUND;
+
+                // ---- scores
+                float sc[NT][KT][4];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[nt][kt][i] = 0.0f;
+                    const int ra = 16 * kt + g, rb = ra + 8;
+                    if constexpr (kBf16) {
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
                             const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
-                            aw[0] = a.x, aw[1] = a.y, aw[2] = a.z, aw[3] = a.w, cw[0] = c.x, cw[1] = c.y, cw[2] = c.z, cw[3] = c.w;
-                        }
-#pragma unroll
-                        for (int q = 0; q < WORDS; ++q) {
-                            const int block = (C::EK / 16) * (4 * i + t) + q / 2;
-                            const uint32_t s_a = ue4m3x2_to_f16(ss[ra * SB + block] * 0x10001u), s_c = ue4m3x2_to_f16(ss[rb * SB + block] * 0x10001u);
-                            uint32_t ha[4], hc[4];
-                            e2m1x8_to_f16(aw[q], ha);
-                            e2m1x8_to_f16(cw[q], hc);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) ha[e] = mul_f16x2(ha[e], s_a), hc[e] = mul_f16x2(hc[e], s_c);
-                            const int j = (C::EK / 4) * i + 2 * q;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][j][0], qf[nt][j][1]);
-                                mma<false>(sc[nt][kt], ha[2], hc[2], ha[3], hc[3], qf[nt][j + 1][0], qf[nt][j + 1][1]);
+                                mma<true>(sc[nt][kt], a.x, c.x, a.y, c.y, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+                                mma<true>(sc[nt][kt], a.z, c.z, a.w, c.w, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
                             }
                         }
-                    }
-                }
-            }
-
-            // ---- x = score in base 2 less the reference; the row scales of fp8
-            float va[KT], vb[KT], la[KT], lb[KT];  // value scales of the keys and their logarithms
-            if constexpr (KIND == kKvFp8) {
-                const float* fs = reinterpret_cast<const float*>(ss);
+                    } else if constexpr (KIND == kKvFp8) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int ra = 16 * kt + g, rb = ra + 8;
-                    const float ka = fs[ra], kb = fs[rb];
-                    va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
-                    la[kt] = fmaxf(__log2f(va[kt]), -80.0f), lb[kt] = fmaxf(__log2f(vb[kt]), -80.0f);
+                        for (int i = 0; i < D / 64; ++i) {
+                            const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+                            const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        sc[nt][kt][0] *= ka, sc[nt][kt][1] *= ka;
-                        sc[nt][kt][2] *= kb, sc[nt][kt][3] *= kb;
-                    }
-                }
-            }
-            float x[NT][KT][4];
+                            for (int q = 0; q < 4; ++q) {
+                                uint32_t ha[2], hc[2];
+                                e4m3x4_to_f16(aw[q], ha);
+                                e4m3x4_to_f16(cw[q], hc);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[nt][kt][i] = i & 1 ? fmaf(sc[nt][kt][i], f1[nt], -ref1[nt]) : fmaf(sc[nt][kt][i], f0[nt], -ref0[nt]);
-            if (key0 < span.first || key0 + TK > span.len) {
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int ka = key0 + 16 * kt + g, kb = ka + 8;
-                    const bool oa = ka >= span.first && ka < span.len, ob = kb >= span.first && kb < span.len;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (!oa) x[nt][kt][0] = x[nt][kt][1] = -INFINITY;
-                        if (!ob) x[nt][kt][2] = x[nt][kt][3] = -INFINITY;
-                    }
-                }
-            }
-            bool over = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) over |= x[nt][kt][i] > kHeadroom - (KIND != kKvFp8 ? 0.0f : i < 2 ? la[kt] : lb[kt]);
-            if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    // from the scores themselves (the first reference is too far off to go by x)
-                    float full[KT][4], t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            full[kt][i] = x[nt][kt][i] == -INFINITY ? -INFINITY : sc[nt][kt][i] * (i & 1 ? f1[nt] : f0[nt]);
-                        t0 = fmaxf(t0, fmaxf(full[kt][0] + xa, full[kt][2] + xb));
-                        t1 = fmaxf(t1, fmaxf(full[kt][1] + xa, full[kt][3] + xb));
-                    }
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
-                        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
-                    }
-                    const float n0 = fmaxf(ref0[nt], t0 - kBelowMax), n1 = fmaxf(ref1[nt], t1 - kBelowMax);
-                    const float c0 = exp2_approx(ref0[nt] - n0), c1 = exp2_approx(ref1[nt] - n1);
-                    ref0[nt] = n0, ref1[nt] = n1;
-                    l0[nt] *= c0, l1[nt] *= c1;
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        acc[nt][m][0] *= c0, acc[nt][m][1] *= c1;
-                        acc[nt][m][2] *= c0, acc[nt][m][3] *= c1;
-                    }
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        x[nt][kt][0] = full[kt][0] - n0, x[nt][kt][1] = full[kt][1] - n1;
-                        x[nt][kt][2] = full[kt][2] - n0, x[nt][kt][3] = full[kt][3] - n1;
-                    }
-                }
-            }
-
-            // ---- weights as P^T fragments
-            uint32_t pf[NT][KT][2], pl[NT][KT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[nt][kt][i]);
-                    l0[nt] += w[0] + w[2];
-                    l1[nt] += w[1] + w[3];
-                    if constexpr (KIND == kKvFp8) {
-                        // a masked key's zero-filled scale keeps its weight zero
-                        w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
-                    }
-                    if constexpr (kBf16) {
-                        const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
-                        pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
-                        pl[nt][kt][0] = transpose8x8(pack_bf16(w[0] - bf16_lo(hi0), w[1] - bf16_hi(hi0)));
-                        pl[nt][kt][1] = transpose8x8(pack_bf16(w[2] - bf16_lo(hi1), w[3] - bf16_hi(hi1)));
+                                for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
+                            }
+                        }
                     } else {
-                        pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
-                        pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
-                    }
-                }
-
-            // ---- values: the lane's keys are 2t, 2t + 1, 2t + 8, 2t + 9 of each 16, its elements run g of each row
+                        constexpr int WORDS = C::EK / 8, PIECES = D / (4 * C::EK);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const int r = 16 * kt + 2 * t;
-                constexpr int WORDS = C::EV * RB / D / 4, PIECES = D / (8 * C::EV);  // words of a run, runs of a row
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
-                    uint32_t v[4][WORDS];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int row = r + (x & 1) + 8 * (x >> 1);
-                        if constexpr (WORDS == 4) {
-                            const uint4 w = lds128(sv + v_offset<RB>(row, 8 * i + g));
-                            v[x][0] = w.x, v[x][1] = w.y, v[x][2] = w.z, v[x][3] = w.w;
-                        } else if constexpr (WORDS == 2) {
-                            const uint2 w = lds64(sv + v_offset<RB>(row, g >> 1) + 8 * (g & 1));
-                            v[x][0] = w.x, v[x][1] = w.y;
-                        } else {
-                            v[x][0] = lds32(sv + v_offset<RB>(row, g >> 2) + 4 * (g & 3));
-                        }
-                    }
-                    // A operands: [m-tile][keys 2t, 2t + 1 / 2t + 8, 2t + 9][element 2e / 2e + 1 of the run]
-                    constexpr int PAIRS = C::EV / 2;
-                    uint32_t h[PAIRS][2][2];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        if constexpr (kBf16) {
-#pragma unroll
-                            for (int e = 0; e < PAIRS; ++e) {
-                                h[e][y][0] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x5410);
-                                h[e][y][1] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x7632);
+                        for (int i = 0; i < PIECES; ++i) {
+                            uint32_t aw[WORDS], cw[WORDS];
+                            if constexpr (WORDS == 2) {
+                                const uint2 a = lds64(sk + k_offset<RB>(ra, 0) + 8 * t), c = lds64(sk + k_offset<RB>(rb, 0) + 8 * t);
+                                aw[0] = a.x, aw[1] = a.y, cw[0] = c.x, cw[1] = c.y;
+                            } else {
+                                const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+                                aw[0] = a.x, aw[1] = a.y, aw[2] = a.z, aw[3] = a.w, cw[0] = c.x, cw[1] = c.y, cw[2] = c.z, cw[3] = c.w;
                             }
-                        } else if constexpr (KIND == kKvFp8) {
-                            // the two keys' bytes side by side, then decoded
 #pragma unroll
                             for (int q = 0; q < WORDS; ++q) {
-                                uint32_t lo[2], hi[2];
-                                e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x5140), lo);
-                                e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x7362), hi);
-                                h[2 * q][y][0] = lo[0], h[2 * q][y][1] = lo[1];
-                                h[2 * q + 1][y][0] = hi[0], h[2 * q + 1][y][1] = hi[1];
-                            }
-                        } else {
-                            // the two keys' codes side by side in each byte, then decoded
-                            const uint8_t* s_row = ss + TK * SB + (r + 8 * y) * SB;
+                                const int block = (C::EK / 16) * (4 * i + t) + q / 2;
+                                const uint32_t s_a = ue4m3x2_to_f16(ss[ra * SB + block] * 0x10001u), s_c = ue4m3x2_to_f16(ss[rb * SB + block] * 0x10001u);
+                                uint32_t ha[4], hc[4];
+                                e2m1x8_to_f16(aw[q], ha);
+                                e2m1x8_to_f16(cw[q], hc);
 #pragma unroll
-                            for (int q = 0; q < WORDS; ++q) {
-                                const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + q / 2;
-                                const uint32_t s_v = ue4m3x2_to_f16(s_row[block] + 0x10000u * s_row[SB + block]);
-                                const uint32_t a = v[2 * y][q], c = v[2 * y + 1][q];
-                                uint32_t even[4], odd[4];
-                                e2m1x8_to_f16((a & 0x0F0F0F0Fu) | ((c << 4) & 0xF0F0F0F0u), even);
-                                e2m1x8_to_f16(((a >> 4) & 0x0F0F0F0Fu) | (c & 0xF0F0F0F0u), odd);
+                                for (int e = 0; e < 4; ++e) ha[e] = mul_f16x2(ha[e], s_a), hc[e] = mul_f16x2(hc[e], s_c);
+                                const int j = (C::EK / 4) * i + 2 * q;
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    h[4 * q + e][y][0] = mul_f16x2(even[e], s_v);
-                                    h[4 * q + e][y][1] = mul_f16x2(odd[e], s_v);
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][j][0], qf[nt][j][1]);
+                                    mma<false>(sc[nt][kt], ha[2], hc[2], ha[3], hc[3], qf[nt][j + 1][0], qf[nt][j + 1][1]);
                                 }
                             }
                         }
                     }
+                }
+
+                // ---- x = score in base 2 less the reference; the row scales of fp8
+                float va[KT], vb[KT], la[KT], lb[KT];  // value scales of the keys and their logarithms
+                if constexpr (KIND == kKvFp8) {
+                    const float* fs = reinterpret_cast<const float*>(ss);
 #pragma unroll
-                    for (int e = 0; e < PAIRS; ++e) {
-                        const int m = i * PAIRS + e;
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const int ra = 16 * kt + g, rb = ra + 8;
+                        const float ka = fs[ra], kb = fs[rb];
+                        va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
+                        la[kt] = fmaxf(__log2f(va[kt]), -80.0f), lb[kt] = fmaxf(__log2f(vb[kt]), -80.0f);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pf[nt][kt][0], pf[nt][kt][1]);
-                            if constexpr (kBf16)
-                                mma<true>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
+                            sc[nt][kt][0] *= ka, sc[nt][kt][1] *= ka;
+                            sc[nt][kt][2] *= kb, sc[nt][kt][3] *= kb;
+                        }
+                    }
+                }
+                float x[NT][KT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            x[nt][kt][i] = i & 1 ? fmaf(sc[nt][kt][i], f1[nt], -ref1[nt]) : fmaf(sc[nt][kt][i], f0[nt], -ref0[nt]);
+                if (key0 < span.first || key0 + TK > span.len) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const int ka = key0 + 16 * kt + g, kb = ka + 8;
+                        const bool oa = ka >= span.first && ka < span.len, ob = kb >= span.first && kb < span.len;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (!oa) x[nt][kt][0] = x[nt][kt][1] = -INFINITY;
+                            if (!ob) x[nt][kt][2] = x[nt][kt][3] = -INFINITY;
+                        }
+                    }
+                }
+                bool over = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) over |= x[nt][kt][i] > kHeadroom - (KIND != kKvFp8 ? 0.0f : i < 2 ? la[kt] : lb[kt]);
+                if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        // from the scores themselves (the first reference is too far off to go by x)
+                        float full[KT][4], t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                full[kt][i] = x[nt][kt][i] == -INFINITY ? -INFINITY : sc[nt][kt][i] * (i & 1 ? f1[nt] : f0[nt]);
+                            t0 = fmaxf(t0, fmaxf(full[kt][0] + xa, full[kt][2] + xb));
+                            t1 = fmaxf(t1, fmaxf(full[kt][1] + xa, full[kt][3] + xb));
+                        }
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) {
+                            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+                            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+                        }
+                        const float n0 = fmaxf(ref0[nt], t0 - kBelowMax), n1 = fmaxf(ref1[nt], t1 - kBelowMax);
+                        const float c0 = exp2_approx(ref0[nt] - n0), c1 = exp2_approx(ref1[nt] - n1);
+                        ref0[nt] = n0, ref1[nt] = n1;
+                        l0[nt] *= c0, l1[nt] *= c1;
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            acc[nt][m][0] *= c0, acc[nt][m][1] *= c1;
+                            acc[nt][m][2] *= c0, acc[nt][m][3] *= c1;
+                        }
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            x[nt][kt][0] = full[kt][0] - n0, x[nt][kt][1] = full[kt][1] - n1;
+                            x[nt][kt][2] = full[kt][2] - n0, x[nt][kt][3] = full[kt][3] - n1;
+                        }
+                    }
+                }
+
+                // ---- weights as P^T fragments
+                uint32_t pf[NT][KT][2], pl[NT][KT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[nt][kt][i]);
+                        l0[nt] += w[0] + w[2];
+                        l1[nt] += w[1] + w[3];
+                        if constexpr (KIND == kKvFp8) {
+                            // a masked key's zero-filled scale keeps its weight zero
+                            w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
+                        }
+                        if constexpr (kBf16) {
+                            const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
+                            pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
+                            pl[nt][kt][0] = transpose8x8(pack_bf16(w[0] - bf16_lo(hi0), w[1] - bf16_hi(hi0)));
+                            pl[nt][kt][1] = transpose8x8(pack_bf16(w[2] - bf16_lo(hi1), w[3] - bf16_hi(hi1)));
+                        } else {
+                            pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
+                            pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
+                        }
+                    }
+
+                // ---- values: the lane's keys are 2t, 2t + 1, 2t + 8, 2t + 9 of each 16, its elements run g of each row
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int r = 16 * kt + 2 * t;
+                    constexpr int WORDS = C::EV * RB / D / 4, PIECES = D / (8 * C::EV);  // words of a run, runs of a row
+#pragma unroll
+                    for (int i = 0; i < PIECES; ++i) {
+                        uint32_t v[4][WORDS];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int row = r + (x & 1) + 8 * (x >> 1);
+                            if constexpr (WORDS == 4) {
+                                const uint4 w = lds128(sv + v_offset<RB>(row, 8 * i + g));
+                                v[x][0] = w.x, v[x][1] = w.y, v[x][2] = w.z, v[x][3] = w.w;
+                            } else if constexpr (WORDS == 2) {
+                                const uint2 w = lds64(sv + v_offset<RB>(row, g >> 1) + 8 * (g & 1));
+                                v[x][0] = w.x, v[x][1] = w.y;
+                            } else {
+                                v[x][0] = lds32(sv + v_offset<RB>(row, g >> 2) + 4 * (g & 3));
+                            }
+                        }
+                        // A operands: [m-tile][keys 2t, 2t + 1 / 2t + 8, 2t + 9][element 2e / 2e + 1 of the run]
+                        constexpr int PAIRS = C::EV / 2;
+                        uint32_t h[PAIRS][2][2];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            if constexpr (kBf16) {
+#pragma unroll
+                                for (int e = 0; e < PAIRS; ++e) {
+                                    h[e][y][0] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x5410);
+                                    h[e][y][1] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x7632);
+                                }
+                            } else if constexpr (KIND == kKvFp8) {
+                                // the two keys' bytes side by side, then decoded
+#pragma unroll
+                                for (int q = 0; q < WORDS; ++q) {
+                                    uint32_t lo[2], hi[2];
+                                    e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x5140), lo);
+                                    e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x7362), hi);
+                                    h[2 * q][y][0] = lo[0], h[2 * q][y][1] = lo[1];
+                                    h[2 * q + 1][y][0] = hi[0], h[2 * q + 1][y][1] = hi[1];
+                                }
+                            } else {
+                                // the two keys' codes side by side in each byte, then decoded
+                                const uint8_t* s_row = ss + TK * SB + (r + 8 * y) * SB;
+#pragma unroll
+                                for (int q = 0; q < WORDS; ++q) {
+                                    const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + q / 2;
+                                    const uint32_t s_v = ue4m3x2_to_f16(s_row[block] + 0x10000u * s_row[SB + block]);
+                                    const uint32_t a = v[2 * y][q], c = v[2 * y + 1][q];
+                                    uint32_t even[4], odd[4];
+                                    e2m1x8_to_f16((a & 0x0F0F0F0Fu) | ((c << 4) & 0xF0F0F0F0u), even);
+                                    e2m1x8_to_f16(((a >> 4) & 0x0F0F0F0Fu) | (c & 0xF0F0F0F0u), odd);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        h[4 * q + e][y][0] = mul_f16x2(even[e], s_v);
+                                        h[4 * q + e][y][1] = mul_f16x2(odd[e], s_v);
+                                    }
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < PAIRS; ++e) {
+                            const int m = i * PAIRS + e;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pf[nt][kt][0], pf[nt][kt][1]);
+                                if constexpr (kBf16)
+                                    mma<true>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
+                            }
                         }
                     }
                 }
             }
-        }
-        copy_wait<0>();
-
-        // ---- the warps' results, joined in shared memory (over the idle rings)
+            // ---- the warps' results, joined in shared memory; the next segment's stream starts before
+            const int seg_b = b, seg_first = pre + unit * span.rounds, seg_rounds = span.rounds, seg_r0 = r0, seg_r1 = r1;
+            u += r1 - r0;
+            __syncwarp();
+            if constexpr (C::APART) more = open();
+            float* merge = reinterpret_cast<float*>(smem + (C::APART ? kWarps * C::RING : 0));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], o);
-                l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], o);
-            }
-            if (g == 0) {
-                s_m[warp][8 * nt + 2 * t] = ref0[nt], s_m[warp][8 * nt + 2 * t + 1] = ref1[nt];
-                s_l[warp][8 * nt + 2 * t] = l0[nt], s_l[warp][8 * nt + 2 * t + 1] = l1[nt];
-            }
-        }
-        __syncthreads();
-        float* merge = reinterpret_cast<float*>(smem);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int h0 = 8 * nt + 2 * t;
-            float m0 = kNoScore, m1 = kNoScore;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) m0 = fmaxf(m0, s_m[w][h0]), m1 = fmaxf(m1, s_m[w][h0 + 1]);
-            const float c0 = exp2_approx(ref0[nt] - m0), c1 = exp2_approx(ref1[nt] - m1);
-            float* to = merge + (warp * HEADS + h0) * C::LD;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int e = 2 * m, d = 8 * C::EV * (e / C::EV) + C::EV * g + e % C::EV;
-                *reinterpret_cast<float2*>(to + d) = make_float2(acc[nt][m][0] * c0, acc[nt][m][2] * c0);
-                *reinterpret_cast<float2*>(to + C::LD + d) = make_float2(acc[nt][m][1] * c1, acc[nt][m][3] * c1);
-            }
-        }
-        __syncthreads();
-
-        const bool whole = r0 == 0 && r1 == span.rounds;
-        const float unit_scale = KIND == kKvNvfp4 ? kScaleUnit : 1.0f;
-        const int slot = 2 * blockIdx.x + (r0 == 0 ? 1 : 0);
-        for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
-            const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
-            float m = kNoScore, l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][h]);
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float4 x = *reinterpret_cast<const float4*>(merge + (w * HEADS + h) * C::LD + d);
-                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-                l += s_l[w][h] * exp2_approx(s_m[w][h] - m);
-            }
-            if (whole) {
-                const Finish f = finish(p, head0 + h, m, l, unit_scale);
-                *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.q_heads + head0 + h) * D + d) =
-                    make_uint2(pack_bf16(sum.x * f.factor, sum.y * f.factor), pack_bf16(sum.z * f.factor, sum.w * f.factor));
-                if (p.lse && d == 0) p.lse[(size_t)b * p.q_heads + head0 + h] = f.lse;
-            } else {
-                __stcg(reinterpret_cast<float4*>(p.part_acc + ((size_t)slot * HEADS + h) * D + d), sum);
-                if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * HEADS + h) * 2), make_float2(m, l));
-            }
-        }
-        if (!whole) {
-            // The CTAs that hold this unit's rounds: the first one's counter counts them.
-            const long from = pre + (long)unit * span.rounds, to = from + span.rounds - 1;
-            const int first_cta = (int)(((from + 1) * ctas - 1) / total), last_cta = (int)(((to + 1) * ctas - 1) / total);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.counters + first_cta, 1u) == (uint32_t)(last_cta - first_cta);
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
-                    const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
-                    float m = kNoScore, l = 0.0f;
-                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int c = first_cta; c <= last_cta; ++c) {
-                        const size_t at = (size_t)(2 * c + (c == first_cta ? 1 : 0)) * HEADS + h;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_acc + at * D + d));
-                        const float top = fmaxf(m, ml.x), old = exp2_approx(m - top), add = exp2_approx(ml.x - top);
-                        sum.x = sum.x * old + x.x * add, sum.y = sum.y * old + x.y * add;
-                        sum.z = sum.z * old + x.z * add, sum.w = sum.w * old + x.w * add;
-                        l = l * old + ml.y * add;
-                        m = top;
-                    }
-                    const Finish f = finish(p, head0 + h, m, l, unit_scale);
-                    *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.q_heads + head0 + h) * D + d) = make_uint2(
-                        pack_bf16(sum.x * f.factor, sum.y * f.factor), pack_bf16(sum.z * f.factor, sum.w * f.factor));
-                    if (p.lse && d == 0) p.lse[(size_t)b * p.q_heads + head0 + h] = f.lse;
+                for (int o = 4; o < 32; o <<= 1) {
+                    l0[nt] += __shfl_xor_sync(0xffffffffu, l0[nt], o);
+                    l1[nt] += __shfl_xor_sync(0xffffffffu, l1[nt], o);
                 }
-                if (tid == 0) p.counters[first_cta] = 0u;  // as it was found
+            __syncthreads();  // the merge area (the rings, where it lies over them) is idle
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int h0 = 8 * nt + 2 * t;
+                if (g == 0) {
+                    s_m[warp][h0] = ref0[nt], s_m[warp][h0 + 1] = ref1[nt];
+                    s_l[warp][h0] = l0[nt], s_l[warp][h0 + 1] = l1[nt];
+                }
+                float* to = merge + (warp * HEADS + h0) * C::LD;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const int e = 2 * m, d = 8 * C::EV * (e / C::EV) + C::EV * g + e % C::EV;
+                    *reinterpret_cast<float2*>(to + d) = make_float2(acc[nt][m][0], acc[nt][m][2]);
+                    *reinterpret_cast<float2*>(to + C::LD + d) = make_float2(acc[nt][m][1], acc[nt][m][3]);
+                }
+            }
+            __syncthreads();
+
+            const bool whole = seg_r0 == 0 && seg_r1 == seg_rounds;
+            const int which = seg_r0 == 0 ? 1 : 0, slot = which * p.max_ctas + blockIdx.x;
+            for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
+                const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
+                float m = kNoScore, l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][h]);
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float4 x = *reinterpret_cast<const float4*>(merge + (w * HEADS + h) * C::LD + d);
+                    const float c = exp2_approx(s_m[w][h] - m);
+                    sum.x += x.x * c, sum.y += x.y * c, sum.z += x.z * c, sum.w += x.w * c;
+                    l += s_l[w][h] * c;
+                }
+                if (whole) {
+                    put_row<D>(p, seg_b, head0 + h, d, m, l, sum, kUnit);
+                } else {
+                    __stcg(reinterpret_cast<float4*>(p.part_acc + ((size_t)slot * HEADS + h) * D + d), sum);
+                    if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * HEADS + h) * 2), make_float2(m, l));
+                }
+            }
+            if (!whole && tid == 0)
+                s_part[which] = Part{seg_b, head0, live_heads, owner(seg_first), owner(seg_first + seg_rounds - 1)};
+            if constexpr (!C::APART) {
+                __syncthreads();  // the merge area is the rings again
+                more = open();
             }
         }
-        __syncthreads();  // the merge area is the rings again
-        u += r1 - r0;
-        if (u == pre + (long)span.rounds * units) {
-            pre = u;
-            ++b;
+
+        // ---- the units of which this CTA has a part: counted at their first CTA, joined by the last to arrive
+        __syncthreads();
+        if (s_part[0].b >= 0 || s_part[1].b >= 0) {
+            if (tid < 2) {
+                // The barrier before put all the CTA's parts behind this thread, the
+                // count's release puts them before it, its acquire the others' after.
+                const Part& x = s_part[tid];
+                uint32_t count = 0;
+                if (x.b >= 0)
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(count) : "l"(p.counters + x.first) : "memory");
+                s_last[tid] = x.b >= 0 && count == (uint32_t)(x.last - x.first);
+                if (s_last[tid]) p.counters[x.first] = 0u;  // as it was found
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i)
+                if (s_last[i]) join_parts<D, HEADS>(p, s_part[i], kUnit);
+        }
+    }
+
+    // ---- sequences without keys: zeros, and the sink's share alone
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        if (span_of<TK, C::ROUND>(p, b).rounds > 0) continue;
+        for (int i = tid; i < p.q_heads * (D / 4); i += kThreads) {
+            const int h = i / (D / 4);
+            put_row<D>(p, b, h, 4 * (i - h * (D / 4)), kNoScore, 0.0f, make_float4(0.f, 0.f, 0.f, 0.f), 1.0f);
         }
     }
 }
@@ -779,6 +846,7 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     }
     p.group_tiles = (p.group + C::HEADS - 1) / C::HEADS;
     const Layout w = layout_of(sms, C::HEADS, D);
+    p.max_ctas = sms * kMaxCtasPerSm;
     p.counters = reinterpret_cast<uint32_t*>(workspace);
     p.part_ml = reinterpret_cast<float*>(workspace + w.ml);
     p.part_acc = reinterpret_cast<float*>(workspace + w.acc);
@@ -833,6 +901,8 @@ FP4B_EXPORT int fp4b_decode_attention(const fp4b_decode* call, void* stream) {
     if (!why && (c.table_width < 0 || c.table_stride < c.table_width)) why = "bad page table";
     if (!why && (long)c.table_width * cache->page_size > 0x7fff0000L) why = "more than 2^31 keys in one sequence";
     if (!why && (long)c.batch * c.q_heads > 0x7fffffffL) why = "more than 2^31 output rows";
+    if (!why && (((long)c.table_width * cache->page_size + 63) / 64) * c.q_heads > 0x7fffffffL / std::max(c.batch, 1))
+        why = "more than 2^31 tiles of 64 keys in one call";
     if (!why && (c.window < 0 || !std::isfinite(c.scale))) why = "window must not be negative, scale finite";
     if (!why && ((reinterpret_cast<uintptr_t>(c.q) & 7) || c.q_sb % 4 || c.q_sh % 4 || (reinterpret_cast<uintptr_t>(c.out) & 15)))
         why = "queries must be 8-byte aligned rows, the output 16-byte aligned";
