@@ -43,6 +43,9 @@
 // that results do not depend on the arrival.  A CTA has at most two such parts,
 // its first and its last segment, and arrives for both at its end: one fence.
 // The first steps of the next segment are under way while one is finished.
+// Still a segment costs about as much as kSegmentRounds rounds besides its own
+// (a CTA with four short ones ended 15 us behind the others): shares are even
+// in rounds with these added to each unit.
 //
 // A warp streams its steps through a ring of its own in shared memory with
 // cp.async: no barrier in the loop.  Masked keys are zero-filled, not read.
@@ -67,6 +70,8 @@ using namespace decode;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCtasPerSm = 4;
+constexpr int kSegmentRounds = 3;
+constexpr int kWholeRounds = 12;
 constexpr float kNoScore = -1e30f;    // reference exponent before any key
 constexpr float kHeadroom = 10.0f;    // a score may pass the reference by 2^10 ...
 constexpr float kBelowMax = 4.0f;     // ... which is set 2^4 below the maximum
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     auto scan = [&](int base) {
         const int b = base + tid;
         const int rounds = b < p.batch ? span_of<TK, C::ROUND>(p, b).rounds : 0;
-        mine = rounds * units;
+        mine = rounds > 0 ? (rounds + kSegmentRounds) * units : 0;
         int sum = mine, top = rounds;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -286,9 +291,12 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         }
     };
     for (int base = 0; base < p.batch; base += kThreads) scan(base);
-    // Joining P parts costs about P times 0.06 us, a round about 0.4 us: a CTA
-    // takes at least the rounds that balance the two for the longest sequence.
-    const int least = max(1, (int)sqrtf((float)most * (1.0f / 7.0f)));
+    // A round takes about 0.4 us while the GPU is idle, counting and joining P
+    // parts about 4 us and 0.06 us a part.  So units of up to 12 rounds are not
+    // split at all (each goes whole to the CTA in whose share it starts), and for
+    // longer ones a CTA takes at least the rounds that balance the last two terms.
+    const bool split = most > kWholeRounds;
+    const int least = split ? (int)sqrtf((float)most * (1.0f / 7.0f)) : 1;
     const int ctas = min((int)gridDim.x, max(total / least, min(total, 1)));
     if ((int)blockIdx.x < ctas) {
         // CTA c's share starts at c * each + min(c, extra)
@@ -319,7 +327,8 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 
         // ---- a segment: rounds [r0, r1) of one head unit, and the stream of this warp's steps of it
         Span span{};
-        int unit = 0, r0 = 0, r1 = 0, kv_head = 0, step0 = 0, steps = 0, next_page = -2;
+        int unit = 0, unit_start = 0, r0 = 0, r1 = 0, kv_head = 0, head0 = 0, live_heads = 0, step0 = 0, steps = 0, next_page = -2;
+        uint2 qw[NT][MT];  // the queries as they are read, see below
         const int* table = nullptr;
         auto page_of = [&](int s) {  // page of the lane's key of step s (of all its keys, if in_page); -2 for a masked key
             if (s >= steps) return -2;
@@ -376,15 +385,26 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         // Makes the rounds from u on the segment at hand and starts its stream; false at the share's end.
         auto open = [&]() {
             if (u >= u1) return false;
-            for (span = span_of<TK, C::ROUND>(p, b); u >= pre + span.rounds * units && b + 1 < p.batch; span = span_of<TK, C::ROUND>(p, b)) {
-                pre += span.rounds * units;
-                ++b;
+            for (;;) {
+                span = span_of<TK, C::ROUND>(p, b);
+                const int length = span.rounds > 0 ? span.rounds + kSegmentRounds : 0;  // of a unit
+                if (u < pre + length * units) {
+                    const int local = u - pre;
+                    unit = local / length;
+                    r0 = local - unit * length;
+                    unit_start = pre + unit * length;
+                    if (split ? r0 < span.rounds : r0 == 0) break;
+                    u = unit_start + length;  // no rounds of this unit are this CTA's
+                    if (u >= u1) return false;
+                } else {
+                    pre += length * units;
+                    if (++b >= p.batch) return false;
+                }
             }
-            const int local = u - pre;
-            unit = local / span.rounds;
-            r0 = local - unit * span.rounds;
-            r1 = min(span.rounds, r0 + (u1 - u));
+            r1 = split ? min(span.rounds, r0 + (u1 - u)) : span.rounds;
             kv_head = unit / p.group_tiles;
+            const int in_group = (unit - kv_head * p.group_tiles) * HEADS;
+            head0 = kv_head * p.group + in_group, live_heads = min(HEADS, p.group - in_group);
             table = p.table + (size_t)b * p.table_stride;
             step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
             steps = r1 - r0;
@@ -392,27 +412,27 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             next_page = page_of(0);
 #pragma unroll
             for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int n = 8 * nt + g;
+                const uint16_t* row = p.q + (size_t)b * p.q_sb + (size_t)(head0 + (n < live_heads ? n : 0)) * p.q_sh;
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const int d = 4 * C::EK * (j / (C::EK / 4)) + C::EK * t + 4 * (j % (C::EK / 4));
+                    qw[nt][j] = n < live_heads ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+                }
+            }
             return true;
         };
 
         bool more = open();
         while (more) {
-            const int in_group = (unit - kv_head * p.group_tiles) * HEADS;
-            const int head0 = kv_head * p.group + in_group, live_heads = min(HEADS, p.group - in_group);
-
             // ---- queries: column g of head tile nt, element 4 EK (j / (EK/4)) + EK t + 4 (j % (EK/4)) of k-step j
             uint32_t qf[NT][MT][2];
             float f0[NT], f1[NT];  // score factors of heads 2t, 2t + 1
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const int n = 8 * nt + g;
-                const uint16_t* row = p.q + (size_t)b * p.q_sb + (size_t)(head0 + (n < live_heads ? n : 0)) * p.q_sh;
-                uint2 w[MT];
-#pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    const int d = 4 * C::EK * (j / (C::EK / 4)) + C::EK * t + 4 * (j % (C::EK / 4));
-                    w[j] = n < live_heads ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
-                }
+                const uint2 (&w)[MT] = qw[nt];
                 float factor = p.scale2;
                 if constexpr (kBf16) {
 #pragma unroll
@@ -707,7 +727,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 }
             }
             // ---- the warps' results, joined in shared memory; the next segment's stream starts before
-            const int seg_b = b, seg_first = pre + unit * span.rounds, seg_rounds = span.rounds, seg_r0 = r0, seg_r1 = r1;
+            const int seg_b = b, seg_first = unit_start, seg_rounds = span.rounds, seg_r0 = r0, seg_r1 = r1, seg_head0 = head0, seg_heads = live_heads;
             u += r1 - r0;
             __syncwarp();
             if constexpr (C::APART) more = open();
@@ -739,7 +759,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 
             const bool whole = seg_r0 == 0 && seg_r1 == seg_rounds;
             const int which = seg_r0 == 0 ? 1 : 0, slot = which * p.max_ctas + blockIdx.x;
-            for (int i = tid; i < live_heads * (D / 4); i += kThreads) {
+            for (int i = tid; i < seg_heads * (D / 4); i += kThreads) {
                 const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
                 float m = kNoScore, l = 0.0f;
 #pragma unroll
@@ -753,14 +773,14 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                     l += s_l[w][h] * c;
                 }
                 if (whole) {
-                    put_row<D>(p, seg_b, head0 + h, d, m, l, sum, kUnit);
+                    put_row<D>(p, seg_b, seg_head0 + h, d, m, l, sum, kUnit);
                 } else {
                     __stcg(reinterpret_cast<float4*>(p.part_acc + ((size_t)slot * HEADS + h) * D + d), sum);
                     if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * HEADS + h) * 2), make_float2(m, l));
                 }
             }
             if (!whole && tid == 0)
-                s_part[which] = Part{seg_b, head0, live_heads, owner(seg_first), owner(seg_first + seg_rounds - 1)};
+                s_part[which] = Part{seg_b, seg_head0, seg_heads, owner(seg_first), owner(seg_first + seg_rounds - 1)};
             if constexpr (!C::APART) {
                 __syncthreads();  // the merge area is the rings again
                 more = open();
@@ -901,7 +921,7 @@ FP4B_EXPORT int fp4b_decode_attention(const fp4b_decode* call, void* stream) {
     if (!why && (c.table_width < 0 || c.table_stride < c.table_width)) why = "bad page table";
     if (!why && (long)c.table_width * cache->page_size > 0x7fff0000L) why = "more than 2^31 keys in one sequence";
     if (!why && (long)c.batch * c.q_heads > 0x7fffffffL) why = "more than 2^31 output rows";
-    if (!why && (((long)c.table_width * cache->page_size + 63) / 64) * c.q_heads > 0x7fffffffL / std::max(c.batch, 1))
+    if (!why && (((long)c.table_width * cache->page_size + 63) / 64 + kSegmentRounds) * c.q_heads > 0x7fffffffL / std::max(c.batch, 1))
         why = "more than 2^31 tiles of 64 keys in one call";
     if (!why && (c.window < 0 || !std::isfinite(c.scale))) why = "window must not be negative, scale finite";
     if (!why && ((reinterpret_cast<uintptr_t>(c.q) & 7) || c.q_sb % 4 || c.q_sh % 4 || (reinterpret_cast<uintptr_t>(c.out) & 15)))
