@@ -23,15 +23,16 @@
 // back only what it copied itself: no barrier for the weights.  The order of K
 // inside a step is free; a lane's 32 elements are the ones that it holds.
 //
-// Split.  A CTA's W warps are RG groups of 32 rows times W / RG slices of K (its
-// steps in turn), joined in shared memory: more rows in a CTA read x less
-// often, fewer rows give more CTAs.
-//
-// x.  Few elements of x (up to kWholeBytes in FP16) are converted by every CTA
-// for itself, whole, before its first step.  More of them would cost each CTA
-// more than its weights: a kernel of its own converts them first, into the
-// image of shared memory that the CTAs then copy chunk by chunk; the weights'
-// stream starts while it runs.
+// Split.  Every CTA converts the x that it needs itself, before its first step.
+// Its 8 or 16 warps are RG groups of 32 rows of the weight times slices of K,
+// joined in shared memory.  Where there are too few rows for all SMs, or x does
+// not fit beside the rings, K is cut into slices of CTAs of their own too, whose
+// sums go to the workspace, and a second kernel adds them in their order.
+// Many rows with a large x: a CTA keeps one slice of x and walks groups of rows
+// with it, each warp a group at a time and without a barrier, so that x is
+// converted 148 times at most.  (x by chunks through shared memory instead, all of
+// it for every CTA, took a barrier every two steps and as many bytes of x as of
+// the weight from L2: 53.5 us for 16 x 16384 x 16384, now 44.)
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -52,8 +53,8 @@ using namespace decode;
 constexpr int kStep = 128;                     // elements of K of one step
 constexpr int kStageBytes = 5 * 512;           // a warp's step: four code pieces and the scales, 16 bytes a lane
 constexpr int kStages = 3;
-constexpr int kWholeBytes = 49152;             // of x in FP16 that every CTA converts for itself
-constexpr int kChunkBytes = 32768;             // a chunk of x in FP16
+constexpr int kWalkBytes = 65536;              // of x in FP16 that a CTA keeps that walks rows
+constexpr int kSliceBytes = 49152;             // that any other keeps
 
 struct GemvParams {
     const uint16_t* x;
@@ -65,17 +66,17 @@ struct GemvParams {
     int m, n, k, k_pad;
     int x_vec;  // rows of x are 16-byte aligned
     float alpha;
-    uint8_t* image;  // x in FP16, chunk by chunk as in shared memory, and the rows' factors; null: converted by each CTA
-    float* factors;
+    // Slices of K: their number, their steps (the first `slice_more` have one more),
+    // the row groups' CTAs of each, and the slices' sums [tiles of rows of
+    // x][slices][8 NT][n_pad].
+    int slices, slice_steps, slice_more, ctas;
+    float* sums;
+    int n_pad;
 };
 
 // Chunk c (8 elements) of row g of a chunk of x: where it lies, so that the
 // eight lanes of one phase of the reads meet distinct banks.
 __device__ __forceinline__ int x_offset(int row_bytes, int g, int c) { return g * row_bytes + 16 * (c ^ ((c >> 3) & 1) ^ ((g & 1) << 1)); }
-
-// Elements of a chunk of x with 8 NT rows.
-template <int NT>
-constexpr int chunk_elements() { return kChunkBytes / (16 * NT); }
 
 // Elements k .. k+7 of a row of x, zeros past its end.
 __device__ __forceinline__ uint4 x_eight(const GemvParams& p, const uint16_t* row, int k) {
@@ -101,191 +102,184 @@ __device__ __forceinline__ uint4 eight_to_f16(uint4 v, float f) {
                       pack_f16(bf16_lo(v.z) * f, bf16_hi(v.z) * f), pack_f16(bf16_lo(v.w) * f, bf16_hi(v.w) * f));
 }
 
-// x into its image: a CTA a row.
-template <int NT>
-__global__ void __launch_bounds__(256) gemv_image_kernel(const __grid_constant__ GemvParams p) {
-    constexpr int KC = chunk_elements<NT>();
-    __shared__ uint32_t s_top[8];
-    chain();
-    const int row = blockIdx.x, tile = row / (8 * NT), in_tile = row % (8 * NT);
-    const int chunks = (p.k + KC - 1) / KC;
-    const uint16_t* src = p.x + (size_t)row * p.ldx;
-    uint32_t top = 0;
-    for (int k = 8 * threadIdx.x; k < p.k; k += 8 * 256) top = max_magnitudes(top, x_eight(p, src, k));
-    top = group_umax<32>(max((top << 16) & 0x7FFF0000u, top & 0x7FFF0000u));
-    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+// Elements [k0, k0 + steps * kStep) of `rows` rows of x to shared memory in FP16 (at
+// most kBytes), each row by its own power of two; factor: what undoes it.  All
+// threads of the CTA call it; the reads of all pieces are in flight together.
+template <int kThreads, int kBytes>
+__device__ __forceinline__ void convert_x(const GemvParams& p, int m0, int rows, int k0, int steps, uint8_t* sx, uint32_t* s_top,
+                                          float* factor) {
+    constexpr int kHeld = kBytes / 16 / kThreads;
+    const int per_row = steps * (kStep / 8), pieces = rows * per_row;
+    const float inv = 1.0f / (float)per_row;
+    auto row_of = [&](int piece) { return (int)(((float)piece + 0.5f) * inv); };  // exact: half a piece from a boundary at least
+    if (threadIdx.x < 16) s_top[threadIdx.x] = 0;
+    uint4 v[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int piece = threadIdx.x + i * kThreads, row = row_of(piece), k = k0 + 8 * (piece - row * per_row);
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (piece < pieces && k < p.k) v[i] = x_eight(p, p.x + (size_t)(m0 + row) * p.ldx, k);
+    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, s_top[i]);
-    const int e = scale_exponent(top);
-    const float f = power_of_two(e);
-    if (threadIdx.x == 0) p.factors[row] = power_of_two(-e);
-    uint8_t* image = p.image + (size_t)tile * chunks * kChunkBytes;
-    for (int k = 8 * threadIdx.x; k < chunks * KC; k += 8 * 256)
-        *reinterpret_cast<uint4*>(image + (size_t)(k / KC) * kChunkBytes + x_offset(2 * KC, in_tile, (k % KC) / 8)) =
-            eight_to_f16(k < p.k ? x_eight(p, src, k) : make_uint4(0u, 0u, 0u, 0u), f);
-}
-
-template <int NT, int RG, int W, bool IMAGE>
-__global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ GemvParams p) {
-    constexpr int kThreads = 32 * W;
-    constexpr int KS = W / RG;                        // slices of K
-    constexpr int KC = chunk_elements<NT>();          // elements of a chunk
-    constexpr int kChunkSteps = KC / kStep;
-    static_assert(kChunkSteps % KS == 0, "every warp has the same steps of a whole chunk");
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float s_factor[8 * NT];
-    [[maybe_unused]] __shared__ uint32_t s_top[8 * NT];
-    uint8_t* sx = smem + W * kStages * kStageBytes;
-
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int rg = warp % RG, ks = warp / RG;
-    const int part = blockIdx.x % (4 / RG), block = blockIdx.x / (4 / RG);  // which of the 128 rows' r
-    const int r0 = 8 * (part * RG + rg);                                    // the warp's first r
-    const int m0 = blockIdx.y * 8 * NT, rows = min(8 * NT, p.m - m0);
-    const int steps = p.k_pad / kStep;
-    const int nsb = p.k_pad / 16;
-
-    // ---- the stream of the warp's weights: steps ks, ks + KS, ...
-    const uint8_t* w_src = p.w + ((size_t)(block * 128 + r0 + g) * p.k_pad >> 1) + 16 * t;
-    const size_t w_row32 = (size_t)16 * p.k_pad;  // 32 rows further
-    const uint8_t* s_src = p.sf + (size_t)block * 128 * nsb + (r0 + g) * 16 + (t >> 1) * 512;
-    uint8_t* ring = smem + warp * kStages * kStageBytes + 16 * lane;
-    const uint32_t ring_addr = ptx::smem_u32(ring);
-    const int used = min(steps, (p.k + kStep - 1) / kStep);  // x is zero past p.k
-    const int mine = (used - ks + KS - 1) / KS;
-    auto issue = [&](int i, int slot) {
-        if (i < mine) {
-            const int step = ks + i * KS;
-            const uint32_t dst = ring_addr + slot * kStageBytes;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) copy_async<16>(dst + 512 * q, w_src + q * w_row32 + (size_t)step * (kStep / 2), true);
-            copy_async<16>(dst + 2048, s_src + (size_t)step * 1024, true);
-        }
-        copy_commit();
-    };
-
-    // ---- x, whole or by chunks
-    const int chunks = IMAGE ? (p.k + KC - 1) / KC : 1;
-    const int row_bytes = IMAGE ? 2 * KC : 2 * used * kStep;
-    const uint8_t* image = IMAGE ? p.image + (size_t)blockIdx.y * chunks * kChunkBytes + 16 * tid : nullptr;
-    auto fetch = [&](int c) {
-        const uint32_t dst = ptx::smem_u32(sx) + (c & 1) * kChunkBytes + 16 * tid;
-#pragma unroll
-        for (int i = 0; i < kChunkBytes / (16 * kThreads); ++i)
-            copy_async<16>(dst + i * 16 * kThreads, image + (size_t)c * kChunkBytes + i * 16 * kThreads, true);
-    };
-    if constexpr (IMAGE) {
-        // The image's kernel lets this one start once all that came before it is
-        // complete, the weights among it: only x is waited for.
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) issue(i, i);
-        chain();
-        fetch(0);
-        copy_commit();
-        if (tid < rows) s_factor[tid] = p.factors[m0 + tid];
-        copy_wait<0>();
-    } else {
-        chain();
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) issue(i, i);
-        // A row to kThreads / 2^q threads, 2^q rows or more.
-        const int q = rows > 1 ? 32 - __clz(rows - 1) : 0, team = kThreads >> q, row = tid / team, at = tid % team;
-        const uint16_t* src = p.x + (size_t)(m0 + row) * p.ldx;
-        if (tid < 8 * NT) s_top[tid] = 0;
-        __syncthreads();
-        uint32_t top = 0;
-        if (row < rows) {
-#pragma unroll 4
-            for (int k = 8 * at; k < p.k; k += 8 * team) top = max_magnitudes(top, x_eight(p, src, k));
-        }
+    for (int i = 0; i < kHeld; ++i) {
+        if (i * kThreads >= pieces) break;
+        const int piece = threadIdx.x + i * kThreads, row = row_of(min(piece, pieces - 1));
+        uint32_t top = max_magnitudes(0u, v[i]);
         top = max((top << 16) & 0x7FFF0000u, top & 0x7FFF0000u);
-        top = team >= 32 ? group_umax<32>(top) : group_umax<16>(top);
-        if (row < rows && (at & 15) == 0) atomicMax(&s_top[row], top);
-        __syncthreads();
-        if (row < rows) {
-            const int e = scale_exponent(s_top[row]);
-            const float f = power_of_two(e);
-            if (at == 0) s_factor[row] = power_of_two(-e);
-#pragma unroll 4
-            for (int k = 8 * at; k < used * kStep; k += 8 * team)
-                *reinterpret_cast<uint4*>(sx + x_offset(row_bytes, row, k / 8)) =
-                    eight_to_f16(k < p.k ? x_eight(p, src, k) : make_uint4(0u, 0u, 0u, 0u), f);
+        if (__all_sync(0xffffffffu, row == __shfl_sync(0xffffffffu, row, 0))) {
+            top = __reduce_max_sync(0xffffffffu, top);
+            if ((threadIdx.x & 31) == 0) atomicMax(&s_top[row], top);
+        } else {
+            atomicMax(&s_top[row], top);
         }
     }
     __syncthreads();
+    if (threadIdx.x < rows) factor[threadIdx.x] = power_of_two(-scale_exponent(s_top[threadIdx.x]));
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int piece = threadIdx.x + i * kThreads;
+        if (piece >= pieces) break;
+        const int row = row_of(piece);
+        *reinterpret_cast<uint4*>(sx + x_offset(16 * per_row, row, piece - row * per_row)) =
+            eight_to_f16(v[i], power_of_two(scale_exponent(s_top[row])));
+    }
+    __syncthreads();
+}
 
-    float acc[2][NT][4];
+// A lane's view of the weights of a warp's 32 rows, r0 + g + 32 q of block `block`:
+// where its 16-byte pieces of step 0 lie.
+struct WeightLane {
+    const uint8_t *w, *s;
+    size_t row32;  // 32 rows further
+};
+__device__ __forceinline__ WeightLane weight_lane(const GemvParams& p, int block, int r0, int g, int t) {
+    return WeightLane{p.w + ((size_t)(block * 128 + r0 + g) * p.k_pad >> 1) + 16 * t,
+                      p.sf + (size_t)block * 8 * p.k_pad + (r0 + g) * 16 + (t >> 1) * 512, (size_t)16 * p.k_pad};
+}
+// The lane's copies of one step into its place of a stage.
+__device__ __forceinline__ void copy_step(uint32_t dst, const WeightLane& from, int step) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) copy_async<16>(dst + 512 * q, from.w + q * from.row32 + (size_t)step * (kStep / 2), true);
+    copy_async<16>(dst + 2048, from.s + (size_t)step * 1024, true);
+}
+
+// A lane's view of x in shared memory: chunk 4 t + u of its row in a step lies at
+// base[nt] + 256 step + ((16 u) ^ swap) (x_offset's permutation moves u alone).
+// Lanes whose row does not exist read another one; their columns are never stored.
+template <int NT>
+struct XLane {
+    const uint8_t* base[NT];
+    int swap;
+};
+template <int NT>
+__device__ __forceinline__ XLane<NT> x_lane(const uint8_t* sx, int rows, int row_bytes, int g, int t) {
+    XLane<NT> x;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) x.base[nt] = sx + (8 * nt + g < rows ? 8 * nt + g : rows > 1 ? g & 1 : 0) * row_bytes + 64 * t;
+    x.swap = 16 * ((t >> 1) ^ ((rows > 1 ? g & 1 : 0) << 1));
+    return x;
+}
+
+// The products of one step: the lane's stage (already complete) with x at `step`.
+template <int NT>
+__device__ __forceinline__ void step_products(float (&acc)[2][NT][4], const uint4 (&v)[4], uint4 sc, const XLane<NT>& x, int step, int t) {
+    // the lane's two scale bytes of each of its four rows
+    const uint32_t pick0 = t & 1 ? 0x4242u : 0x4040u, pick1 = t & 1 ? 0x4343u : 0x4141u;
+    const uint32_t sw[4] = {sc.x, sc.y, sc.z, sc.w};
+    uint32_t s0[4], s1[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        s0[q] = ue4m3x2_to_f16(__byte_perm(sw[q], 0u, pick0));
+        s1[q] = ue4m3x2_to_f16(__byte_perm(sw[q], 0u, pick1));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        uint4 xv[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) xv[nt] = lds128(x.base[nt] + 256 * step + ((16 * u) ^ x.swap));
+        uint32_t a[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            e2m1x8_to_f16(u == 0 ? v[q].x : u == 1 ? v[q].y : u == 2 ? v[q].z : v[q].w, a[q]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[q][e] = mul_f16x2(a[q][e], u < 2 ? s0[q] : s1[q]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            mma<false>(acc[0][nt], a[0][0], a[1][0], a[0][1], a[1][1], xv[nt].x, xv[nt].y);
+            mma<false>(acc[1][nt], a[2][0], a[3][0], a[2][1], a[3][1], xv[nt].x, xv[nt].y);
+            mma<false>(acc[0][nt], a[0][2], a[1][2], a[0][3], a[1][3], xv[nt].z, xv[nt].w);
+            mma<false>(acc[1][nt], a[2][2], a[3][2], a[2][3], a[3][3], xv[nt].z, xv[nt].w);
+        }
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void clear(float (&acc)[2][NT][4]) {
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[a][nt][e] = 0.0f;
+}
 
-    const uint32_t pick0 = t & 1 ? 0x4242u : 0x4040u, pick1 = t & 1 ? 0x4343u : 0x4141u;  // the lane's two scale bytes
-    // x_offset of chunk 4 t + u of the lane's row: the permutation moves u alone.
-    // Lanes whose row does not exist read row 0; their columns are never stored.
-    const uint8_t* x_lane[NT];
+// First step and steps of a slice of K.
+__device__ __forceinline__ void slice_steps(const GemvParams& p, int slice, int& first, int& steps) {
+    first = slice * p.slice_steps + min(slice, p.slice_more);
+    steps = p.slice_steps + (slice < p.slice_more ? 1 : 0);
+}
+
+// A CTA's warps are RG row groups times W / RG parts of its slice of K, which take
+// the steps in turn.
+template <int NT, int RG, int W>
+__global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ GemvParams p) {
+    constexpr int kThreads = 32 * W, KS = W / RG, kRows = 32 * RG;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float s_factor[16];
+    __shared__ uint32_t s_top[16];
+    uint8_t* sx = smem + W * kStages * kStageBytes;
+
+    chain();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int rg = warp % RG, ks = warp / RG;
+    const int part = blockIdx.x % (4 / RG), block = blockIdx.x / (4 / RG);  // which of the block's rows r
+    const int m0 = blockIdx.y * 8 * NT, rows = min(8 * NT, p.m - m0);
+    int first, steps;
+    slice_steps(p, blockIdx.z, first, steps);
+    const int mine = (steps - ks + KS - 1) / KS;  // the warp's: ks, ks + KS, ...
+
+    const WeightLane from = weight_lane(p, block, 8 * (part * RG + rg), g, t);
+    uint8_t* ring = smem + warp * kStages * kStageBytes + 16 * lane;
+    const uint32_t ring_addr = ptx::smem_u32(ring);
+    auto issue = [&](int i, int slot) {
+        if (i < mine) copy_step(ring_addr + slot * kStageBytes, from, first + ks + i * KS);
+        copy_commit();
+    };
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) x_lane[nt] = sx + (8 * nt + g < rows ? 8 * nt + g : (g & 1) < rows ? (g & 1) : 0) * row_bytes + 64 * t;
-    const int x_swap = 16 * ((t >> 1) ^ ((rows > 1 ? g & 1 : 0) << 1));
-    int i = 0, slot = 0;
-    for (int c = 0; c < chunks; ++c) {
-        if (IMAGE && c + 1 < chunks) fetch(c + 1);  // completes with the weights' next groups
-        const int end = IMAGE ? min(used, (c + 1) * kChunkSteps) : used;
-        const int x_base = (IMAGE ? (c & 1) * kChunkBytes - c * kChunkSteps * 256 : 0);
-        for (int step = ks + i * KS; step < end; step += KS, ++i) {
-            copy_wait<kStages - 2>();
-            const uint8_t* st = ring + slot * kStageBytes;
-            uint32_t w[4][4], s0[4], s1[4];
-            const uint4 sc = lds128(st + 2048);
-            const uint32_t sw[4] = {sc.x, sc.y, sc.z, sc.w};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint4 v = lds128(st + 512 * q);
-                w[q][0] = v.x, w[q][1] = v.y, w[q][2] = v.z, w[q][3] = v.w;
-                s0[q] = ue4m3x2_to_f16(__byte_perm(sw[q], 0u, pick0));
-                s1[q] = ue4m3x2_to_f16(__byte_perm(sw[q], 0u, pick1));
-            }
-            issue(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
-            slot = slot == kStages - 1 ? 0 : slot + 1;
-            const int at = x_base + step * 256;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                uint4 xv[NT];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) xv[nt] = lds128(x_lane[nt] + at + ((16 * u) ^ x_swap));
-                uint32_t a[4][4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    e2m1x8_to_f16(w[q][u], a[q]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) a[q][e] = mul_f16x2(a[q][e], u < 2 ? s0[q] : s1[q]);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma<false>(acc[0][nt], a[0][0], a[1][0], a[0][1], a[1][1], xv[nt].x, xv[nt].y);
-                    mma<false>(acc[1][nt], a[2][0], a[3][0], a[2][1], a[3][1], xv[nt].x, xv[nt].y);
-                    mma<false>(acc[0][nt], a[0][2], a[1][2], a[0][3], a[1][3], xv[nt].z, xv[nt].w);
-                    mma<false>(acc[1][nt], a[2][2], a[3][2], a[2][3], a[3][3], xv[nt].z, xv[nt].w);
-                }
-            }
-        }
-        if (IMAGE && c + 1 < chunks) {
-            // The next chunk's copies are in the group of this chunk's first step.
-            copy_wait<(kChunkSteps / KS > 1 ? kStages - 2 : 0)>();
-            __syncthreads();
-        }
+    for (int i = 0; i < kStages - 1; ++i) issue(i, i);
+    convert_x<kThreads, kSliceBytes>(p, m0, rows, first * kStep, steps, sx, s_top, s_factor);
+
+    float acc[2][NT][4];
+    clear(acc);
+    const XLane<NT> x = x_lane<NT>(sx, rows, 2 * steps * kStep, g, t);
+    int slot = 0;
+    for (int i = 0; i < mine; ++i) {
+        copy_wait<kStages - 2>();
+        const uint8_t* st = ring + slot * kStageBytes;
+        const uint4 v[4] = {lds128(st), lds128(st + 512), lds128(st + 1024), lds128(st + 1536)}, sc = lds128(st + 2048);
+        issue(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+        slot = slot == kStages - 1 ? 0 : slot + 1;
+        step_products(acc, v, sc, x, ks + i * KS, t);
     }
 
-    // ---- the slices of K joined in their order; row 8 RG q + 8 rg + g of the CTA is weight row
-    // 128 block + 32 q + 8 (part RG + rg) + g
+    // The parts joined in their order; row 8 RG q + 8 rg + g of the CTA is weight row
+    // 128 block + 32 q + 8 (part RG + rg) + g.
     copy_wait<0>();
     __syncthreads();  // the rings are idle
     float* red = reinterpret_cast<float*>(smem);
-    constexpr int kRows = 32 * RG;
-    static_assert(KS * 8 * NT * kRows * 4 <= W * kStages * kStageBytes, "the rings hold the slices' sums");
+    static_assert(KS * 8 * NT * kRows * 4 <= W * kStages * kStageBytes, "the rings hold the parts' sums");
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -303,59 +297,194 @@ __global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ Ge
         float y = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) y += red[(s * 8 * NT + col) * kRows + row];
-        y *= s_factor[col] * p.alpha;
+        y *= s_factor[col];
+        if (p.slices > 1) {
+            p.sums[(((size_t)blockIdx.y * p.slices + blockIdx.z) * 8 * NT + col) * p.n_pad + n] = y;
+            continue;
+        }
+        y *= p.alpha;
         if (p.bias) y += bf16_lo(p.bias[n]);
         p.y[(size_t)(m0 + col) * p.ldy + n] = (uint16_t)(pack_bf16(y, 0.0f) & 0xFFFFu);
     }
 }
 
+// A CTA with one slice of x walks rows: its warps draw row groups (of its share:
+// every p.ctas-th) from a counter, each through a stream of its own that runs on
+// over the groups' ends.
+constexpr int kWalkWarps = 16;
+template <int NT>
+__global__ void __launch_bounds__(32 * kWalkWarps, 1) gemv_walk_kernel(const __grid_constant__ GemvParams p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float s_factor[16];
+    __shared__ uint32_t s_top[16];
+    __shared__ int s_next;
+    uint8_t* sx = smem + kWalkWarps * kStages * kStageBytes;
+
+    chain();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int slice = blockIdx.x % p.slices, cta = blockIdx.x / p.slices;  // the slices of a row run side by side
+    const int m0 = blockIdx.y * 8 * NT, rows = min(8 * NT, p.m - m0);
+    int first, steps;
+    slice_steps(p, slice, first, steps);
+    const int groups = (p.n + 127) / 128 * 4;  // group 4 b + i: rows 8 i + g + 32 q of block b
+    const int share = (groups - cta + p.ctas - 1) / p.ctas;
+
+    uint8_t* ring = smem + warp * kStages * kStageBytes + 16 * lane;
+    const uint32_t ring_addr = ptx::smem_u32(ring);
+    // What is copied: step `ahead` of group `to`.
+    int to = warp, ahead = 0;
+    if (tid == 0) s_next = kWalkWarps;
+    auto lane_of = [&](int i) {
+        const int group = cta + i * p.ctas;
+        return weight_lane(p, group >> 2, 8 * (group & 3), g, t);
+    };
+    WeightLane from = lane_of(min(to, share - 1));
+    int queued = -1;  // the group after the one at hand, once its first step is copied
+    auto issue = [&](int slot) {
+        if (to < share) {
+            copy_step(ring_addr + slot * kStageBytes, from, first + ahead);
+            if (++ahead == steps) {
+                int next = 0;
+                if (lane == 0) next = atomicAdd(&s_next, 1);
+                to = __shfl_sync(0xffffffffu, next, 0);
+                queued = to;
+                ahead = 0;
+                if (to < share) from = lane_of(to);
+            }
+        }
+        copy_commit();
+    };
+    __syncthreads();  // s_next
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    int now = warp;
+    convert_x<32 * kWalkWarps, kWalkBytes>(p, m0, rows, first * kStep, steps, sx, s_top, s_factor);
+
+    const XLane<NT> x = x_lane<NT>(sx, rows, 2 * steps * kStep, g, t);
+    float* sums = p.sums + ((size_t)blockIdx.y * p.slices + slice) * 8 * NT * p.n_pad;
+    int slot = 0;
+    while (now < share) {
+        float acc[2][NT][4];
+        clear(acc);
+        for (int step = 0; step < steps; ++step) {
+            copy_wait<kStages - 2>();
+            const uint8_t* st = ring + slot * kStageBytes;
+            const uint4 v[4] = {lds128(st), lds128(st + 512), lds128(st + 1024), lds128(st + 1536)}, sc = lds128(st + 2048);
+            issue(slot == 0 ? kStages - 1 : slot - 1);
+            slot = slot == kStages - 1 ? 0 : slot + 1;
+            step_products(acc, v, sc, x, step, t);
+        }
+        const int group = cta + now * p.ctas, n0 = (group >> 2) * 128 + 8 * (group & 3) + g;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = 8 * nt + 2 * t + e;
+                if (col < rows) {
+                    float* out = sums + (size_t)col * p.n_pad + n0;
+                    const float f = s_factor[col];
+                    out[0] = acc[0][nt][e] * f, out[32] = acc[0][nt][2 + e] * f;
+                    out[64] = acc[1][nt][e] * f, out[96] = acc[1][nt][2 + e] * f;
+                }
+            }
+        now = queued;
+    }
+    copy_wait<0>();
+}
+
+// The slices' sums added in their order.
+template <int NT>
+__global__ void __launch_bounds__(128) gemv_join_kernel(const __grid_constant__ GemvParams p) {
+    chain();
+    const int n = blockIdx.x * 128 + threadIdx.x, m = blockIdx.y;
+    if (n >= p.n) return;
+    const float* sums = p.sums + ((size_t)(m / (8 * NT)) * p.slices * 8 * NT + m % (8 * NT)) * p.n_pad + n;
+    float y = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < p.slices; ++s) y += __ldcg(sums + (size_t)s * 8 * NT * p.n_pad);
+    y *= p.alpha;
+    if (p.bias) y += bf16_lo(p.bias[n]);
+    p.y[(size_t)m * p.ldy + n] = (uint16_t)(pack_bf16(y, 0.0f) & 0xFFFFu);
+}
+
 constexpr int kMaxDevices = 64;
 
-template <int NT, int RG, int W, bool IMAGE>
-cudaError_t launch(const GemvParams& p, cudaStream_t st) {
-    constexpr int kRing = W * kStages * kStageBytes;
+template <typename Kernel>
+cudaError_t allow_smem(Kernel* kernel, int bytes, bool (&ready)[kMaxDevices]) {
     static std::mutex mu;
-    static bool ready[kMaxDevices];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices) return cudaErrorInvalidDevice;
-    {
-        std::lock_guard<std::mutex> lk(mu);
-        if (!ready[dev]) {
-            e = cudaFuncSetAttribute(gemv_kernel<NT, RG, W, IMAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     kRing + (IMAGE ? 2 * kChunkBytes : kWholeBytes));
-            if (e != cudaSuccess) return e;
-            ready[dev] = true;
-        }
+    std::lock_guard<std::mutex> lk(mu);
+    if (!ready[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        ready[dev] = e == cudaSuccess;
     }
-    if (IMAGE) {
-        e = launch_chained(gemv_image_kernel<NT>, dim3((unsigned)p.m), 256, 0, st, p);
-        if (e != cudaSuccess) return e;
-    }
-    const long blocks = ((long)p.n + 127) / 128 * (4 / RG);
-    const dim3 grid((unsigned)blocks, (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
-    const int x_bytes = IMAGE ? 2 * kChunkBytes : std::min(p.m, 8 * NT) * 2 * ((p.k + kStep - 1) / kStep * kStep);
-    return launch_chained(gemv_kernel<NT, RG, W, IMAGE>, grid, 32 * W, kRing + x_bytes, st, p);
+    return e;
 }
 
 // Rows of x that share a tile's products: 8 or 16.
 int tile_rows(int m) { return m <= 8 ? 8 : 16; }
 
-// Whether every CTA converts x for itself.
-bool x_whole(int m, int k) { return (long)std::min(m, tile_rows(m)) * 2 * ((k + kStep - 1) / kStep * kStep) <= kWholeBytes; }
+// How a call is cut.  Walked or not, 16 rows of x: 16384 x 16384 42.7 us against
+// 62.4 (64 rows a CTA); 10 rows: 1124 x 6282 19.7 us against 11.1.
+struct Cut {
+    bool walk;
+    int rows_per_cta;  // 32 RG
+    int slices, ctas;
+};
+Cut cut_of(int m, int n, int k) {
+    const int all = (k + kStep - 1) / kStep, groups = (n + 127) / 128 * 4, step_bytes = std::min(m, tile_rows(m)) * 2 * kStep;
+    Cut c{};
+    // walked where x is large and every warp of a full GPU finds a group or nearly
+    const int walk_slices = (all * step_bytes + kWalkBytes - 1) / kWalkBytes;
+    if (all * step_bytes > kSliceBytes && groups * walk_slices >= 148 * kWalkWarps * 3 / 4) {
+        c.walk = true;
+        c.slices = (all + kWalkBytes / step_bytes - 1) / (kWalkBytes / step_bytes);
+        c.ctas = std::max(1, std::min(148 / c.slices, groups));
+        return c;
+    }
+    // Slices that fit, of 16 steps or more, and as many as still make one wave of two
+    // CTAs an SM; then 32, 64 or 128 rows of the weight a CTA, as many as leave about
+    // a CTA for each SM (15360 rows x 2880, 5 rows of x: 17.1 / 12.6 / 10.7 us; 2880
+    // rows, one row of x: 4.4 / 5.9 / 8.7 us).
+    const int fit = (all + kSliceBytes / step_bytes - 1) / (kSliceBytes / step_bytes);
+    c.slices = std::max({1, fit, std::min(296 / groups, all / 16)});
+    c.rows_per_cta = groups * c.slices < 296 ? 32 : groups * c.slices < 480 ? 64 : 128;
+    return c;
+}
+static_assert(kWalkBytes / (16 * 2 * kStep) / 2 > kStages, "a walk's stream runs into one further group at most");
 
-template <int NT, bool IMAGE>
-cudaError_t launch_rows(const GemvParams& p, cudaStream_t st) {
-    const long blocks = ((long)p.n + 127) / 128;
-    if (blocks >= 120) return launch<NT, 4, 16, IMAGE>(p, st);
-    if (blocks >= 74) return launch<NT, 2, 8, IMAGE>(p, st);
-    return launch<NT, 1, 8, IMAGE>(p, st);
+int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * 2 * (p.slice_steps + (p.slice_more > 0 ? 1 : 0)) * kStep; }
+
+template <int NT, int RG, int W>
+cudaError_t launch(const GemvParams& p, cudaStream_t st) {
+    constexpr int kRing = W * kStages * kStageBytes;
+    static bool ready[kMaxDevices];
+    if (const cudaError_t e = allow_smem(gemv_kernel<NT, RG, W>, kRing + kSliceBytes, ready)) return e;
+    const long blocks = ((long)p.n + 127) / 128 * (4 / RG);
+    const dim3 grid((unsigned)blocks, (unsigned)((p.m + 8 * NT - 1) / (8 * NT)), (unsigned)p.slices);
+    return launch_chained(gemv_kernel<NT, RG, W>, grid, 32 * W, kRing + x_bytes(p), st, p);
 }
 
 template <int NT>
-cudaError_t launch_x(const GemvParams& p, cudaStream_t st) {
-    return p.image ? launch_rows<NT, true>(p, st) : launch_rows<NT, false>(p, st);
+cudaError_t launch_walk(const GemvParams& p, cudaStream_t st) {
+    constexpr int kRing = kWalkWarps * kStages * kStageBytes;
+    static bool ready[kMaxDevices];
+    if (const cudaError_t e = allow_smem(gemv_walk_kernel<NT>, kRing + kWalkBytes, ready)) return e;
+    const dim3 grid((unsigned)(p.slices * p.ctas), (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
+    return launch_chained(gemv_walk_kernel<NT>, grid, 32 * kWalkWarps, kRing + x_bytes(p), st, p);
+}
+
+template <int NT>
+cudaError_t launch_all(const GemvParams& p, const Cut& c, cudaStream_t st) {
+    const cudaError_t e = c.walk                  ? launch_walk<NT>(p, st)
+                          : c.rows_per_cta == 128 ? launch<NT, 4, 16>(p, st)
+                          : c.rows_per_cta == 64  ? launch<NT, 2, 8>(p, st)
+                                                  : launch<NT, 1, 8>(p, st);
+    if (e != cudaSuccess || (p.slices == 1 && !c.walk)) return e;
+    return launch_chained(gemv_join_kernel<NT>, dim3((p.n + 127) / 128, p.m), 128, 0, st, p);
 }
 
 }  // namespace
@@ -363,14 +492,14 @@ cudaError_t launch_x(const GemvParams& p, cudaStream_t st) {
 
 using namespace fp4b;
 
-FP4B_EXPORT long fp4b_gemv_workspace(int m, int k_in) {
-    if (m <= 0 || k_in <= 0) {
-        set_last_error("fp4b_gemv_workspace: m and k must be positive");
+FP4B_EXPORT long fp4b_gemv_workspace(int m, int k_in, int n_out) {
+    if (m <= 0 || k_in <= 0 || n_out <= 0) {
+        set_last_error("fp4b_gemv_workspace: m, k and n must be positive");
         return -1;
     }
-    if (x_whole(m, k_in)) return 0;
-    const int rows = tile_rows(m), chunk = kChunkBytes / (2 * rows);
-    return (long)((m + rows - 1) / rows) * ((k_in + chunk - 1) / chunk) * kChunkBytes + 4l * m;
+    const Cut c = cut_of(m, n_out, k_in);
+    const long rows = tile_rows(m);
+    return c.slices == 1 && !c.walk ? 0 : (m + rows - 1) / rows * rows * c.slices * ((n_out + 127l) / 128 * 128) * 4;
 }
 
 FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const void* handle, int n_out, void* y,
@@ -380,21 +509,29 @@ FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const
         set_last_error("null or invalid cache handle");
         return -1;
     }
-    if (!x || !y || m <= 0 || m > 8 * 65535 || k_in <= 0 || k_in > c.K || ldx < k_in || n_out <= 0 || n_out > c.N ||
+    if (!x || !y || m <= 0 || m > 65535 || k_in <= 0 || k_in > c.K || ldx < k_in || n_out <= 0 || n_out > c.N ||
         ldy < n_out) {
         set_last_error("fp4b_gemv_cached: bad shape (m=%d k=%d n=%d vs cache %dx%d)", m, k_in, n_out, c.N, c.K);
         return -1;
     }
-    const long need = fp4b_gemv_workspace(m, k_in);
+    const long need = fp4b_gemv_workspace(m, k_in, n_out);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) {
         set_last_error("fp4b_gemv_cached: needs a 16-byte aligned workspace of %ld bytes", need);
         return -1;
     }
-    const bool vec = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    uint8_t* image = need > 0 ? static_cast<uint8_t*>(workspace) : nullptr;
-    const GemvParams p{static_cast<const uint16_t*>(x), c.fp4, c.sf, static_cast<uint16_t*>(y),
-                       static_cast<const uint16_t*>(bias), ldx, ldy, m, n_out, k_in, c.K, vec, c.w_alpha * kScaleUnit, image,
-                       image ? reinterpret_cast<float*>(image + (need - 4l * m)) : nullptr};
+    GemvParams p{};
+    p.x = static_cast<const uint16_t*>(x), p.ldx = ldx;
+    p.w = c.fp4, p.sf = c.sf, p.k_pad = c.K;
+    p.y = static_cast<uint16_t*>(y), p.ldy = ldy;
+    p.bias = static_cast<const uint16_t*>(bias);
+    p.m = m, p.n = n_out, p.k = k_in;
+    p.x_vec = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    p.alpha = c.w_alpha * kScaleUnit;
+    const Cut cut = cut_of(m, n_out, k_in);
+    const int all = (k_in + kStep - 1) / kStep;
+    p.slices = cut.slices, p.slice_steps = all / cut.slices, p.slice_more = all % cut.slices, p.ctas = cut.ctas;
+    p.sums = static_cast<float*>(workspace);
+    p.n_pad = (n_out + 127) / 128 * 128;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return launch_status(tile_rows(m) == 8 ? launch_x<1>(p, st) : launch_x<2>(p, st), "fp4b_gemv_cached");
+    return launch_status(tile_rows(m) == 8 ? launch_all<1>(p, cut, st) : launch_all<2>(p, cut, st), "fp4b_gemv_cached");
 }

@@ -85,7 +85,7 @@ _bind("fp4b_ipc_close", _i, [_vp, ctypes.c_long])
 _bind("fp4b_mma_rate", _i, [_i, _i, _i, _i, _i, ctypes.POINTER(_i), _vp])
 _bind("fp4b_peer_barrier", _i, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_i), _i, _i, ctypes.c_ulonglong, _vp])
 _bind("fp4b_copy2d", _i, [_vp, ctypes.c_long, _vp, ctypes.c_long, ctypes.c_long, ctypes.c_long, _vp])
-_bind("fp4b_gemv_workspace", ctypes.c_long, [_i, _i])
+_bind("fp4b_gemv_workspace", ctypes.c_long, [_i, _i, _i])
 _bind("fp4b_gemv_cached", _i, [_vp, _i, _i, ctypes.c_long, _vp, _i, _vp, ctypes.c_long, _vp, _vp, ctypes.c_long, _vp])
 
 # Query scale factor vector size
@@ -598,7 +598,7 @@ def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
             bias = bias if bias.is_contiguous() else bias.contiguous()
             b_ptr = bias.data_ptr()
         index = x.device.index
-        need = _lib.fp4b_gemv_workspace(m, k)
+        need = _lib.fp4b_gemv_workspace(m, k, n)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         args = (x_2d.data_ptr(), m, k, ldx, cache._handle, n, y.data_ptr(), n, b_ptr, ws.data_ptr() if need else None, need,
                 torch._C._cuda_getCurrentRawStream(index))

@@ -77,6 +77,22 @@ def test_gemv_long_rows(cuda, fp4, m, k):
     gemv_check(cuda, fp4, m, 300, k)
 
 
+@pytest.mark.parametrize("m,n,k", [(16, 7200, 16384), (11, 9700, 15999), (5, 19000, 16000), (17, 7300, 16384)])
+def test_gemv_many_rows_of_a_long_k(cuda, fp4, m, n, k):
+    g = torch.Generator(cuda).manual_seed(m)
+    w = torch.randn(n, k, generator=g, device=cuda, dtype=torch.bfloat16) * 0.02
+    x = torch.randn(m, k, generator=g, device=cuda, dtype=torch.bfloat16)
+    bias = torch.randn(n, generator=g, device=cuda, dtype=torch.bfloat16)
+    cache = fp4.FP4WeightCache(w, bias, global_scale=True)
+    y = fp4.fp4_cached_gemv(x, cache)
+    assert torch.equal(y, fp4.fp4_cached_gemv(x, cache)), "not the same twice"
+    del w
+    wv = weight_values(cache)
+    want, terms = x.double() @ wv.T + bias.double(), x.double().abs() @ wv.abs_().T + bias.double().abs()
+    close(y, want, terms, 64, f"gemv {m}x{n}x{k}")
+    cache.free()
+
+
 def test_gemv_strided_batched_and_cast_rows(cuda, fp4):
     m, n, k = 6, 384, 650
     x, w, _ = W.cached_linear_inputs(m, n, k, seed=3, bias=False)
