@@ -327,57 +327,75 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 
         // ---- a segment: rounds [r0, r1) of one head unit, and the stream of this warp's steps of it
         Span span{};
-        int unit = 0, unit_start = 0, r0 = 0, r1 = 0, kv_head = 0, head0 = 0, live_heads = 0, step0 = 0, steps = 0, next_page = -2;
+        int unit = 0, unit_start = 0, r0 = 0, r1 = 0, kv_head = 0, head0 = 0, live_heads = 0, step0 = 0, steps = 0, next_page = -2, rows = -1;
         uint2 qw[NT][MT];  // the queries as they are read, see below
         const int* table = nullptr;
-        auto page_of = [&](int s) {  // page of the lane's key of step s (of all its keys, if in_page); -2 for a masked key
+        // Where the rows of the steps lie: if in_page, lane i holds the first row (-1: none
+        // to read) of step 32 j + i and the page of step 32 (j + 1) + i is on its way;
+        // otherwise the page of the lane's key of the next step is.
+        auto page_of = [&](int s) {  // -2 for a masked key
             if (s >= steps) return -2;
-            const int key0 = step0 + s * C::ROUND, key = key0 + (in_page ? 0 : my_key);
+            const int key = step0 + s * C::ROUND + (in_page ? 0 : my_key);
             return (in_page || key >= span.first) && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
         };
+        auto row_of = [&](int page, int key) {
+            if (page >= 0 && page < p.cache.num_pages)
+                return (page * p.cache.kv_heads + kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
+            if (page != -2) report(p.err, kErrPageRange);
+            return -1;
+        };
+        constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
+        const int sub = lane / LR, c = lane % LR;
+        const uint8_t* const k_lane = static_cast<const uint8_t*>(p.cache.k) + 16 * (in_page ? lane : c);
+        const uint8_t* const v_lane = static_cast<const uint8_t*>(p.cache.v) + 16 * (in_page ? lane : c);
+        const uint8_t* const ks_lane = static_cast<const uint8_t*>(p.cache.k_scale) + (in_page ? my_key * SB : 0);
+        const uint8_t* const vs_lane = static_cast<const uint8_t*>(p.cache.v_scale) + (in_page ? my_key * SB : 0);
         auto issue = [&](int s) {
             if (s < steps) {
                 const int key0 = step0 + s * C::ROUND;
-                int page = next_page;
-                next_page = page_of(s + 1);
-                const bool known = page >= 0 && page < p.cache.num_pages;
-                if (!known && page != -2) report(p.err, kErrPageRange);
-                if (!known) page = 0;
-                const int first = in_page ? key0 : key0 + my_key;
-                // the lane's key's row, or the first of the step's
-                const int row = (page * p.cache.kv_heads + kv_head) * p.cache.page_size + (first & (p.cache.page_size - 1));
-                const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE;
-                constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
-                const int sub = lane / LR, c = lane % LR;
-                // rows lo .. hi - 1 of the step are read, the others zero-filled
-                const int lo = known ? span.first - key0 : TK, hi = span.len - key0;
+                const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE, scale_dst = dst + 2 * TK * RB + my_key * SB;
+                auto copy_scales = [&](int row, bool live) {
+                    if constexpr (SB > 0) {
+                        if (TK == 32 || lane < 16) copy_async<SB>(scale_dst, ks_lane + (size_t)row * SB, live);
+                        if (TK == 32 || lane >= 16) copy_async<SB>(scale_dst + TK * SB, vs_lane + (size_t)row * SB, live);
+                    }
+                };
                 if (in_page) {
-                    const size_t at = (size_t)row * RB + 16 * lane;
-                    const uint8_t* k_src = static_cast<const uint8_t*>(p.cache.k) + at;
-                    const uint8_t* v_src = static_cast<const uint8_t*>(p.cache.v) + at;
+                    if ((s & 31) == 0) {
+                        rows = row_of(next_page, key0 + lane * C::ROUND);
+                        next_page = page_of(s + 32 + lane);
+                    }
+                    const int row = __shfl_sync(0xffffffffu, rows, s & 31);
+                    // rows lo .. hi - 1 of the step are read, the others zero-filled
+                    const int lo = row >= 0 ? span.first - key0 : TK, hi = span.len - key0, at = max(row, 0);
+                    const uint8_t *k_src = k_lane + (size_t)at * RB, *v_src = v_lane + (size_t)at * RB;
+                    if (lo <= 0 && hi >= TK) {
 #pragma unroll
-                    for (int i = 0; i < TK / PER; ++i) {
-                        const int r = i * PER + sub;
-                        const bool live = r >= lo && r < hi;
-                        copy_async<16>(dst + k_offset<RB>(r, c), k_src + 512 * i, live);
-                        copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), v_src + 512 * i, live);
+                        for (int i = 0; i < TK / PER; ++i) {
+                            copy_async<16>(dst + k_offset<RB>(i * PER + sub, c), k_src + 512 * i, true);
+                            copy_async<16>(dst + TK * RB + v_offset<RB>(i * PER + sub, c), v_src + 512 * i, true);
+                        }
+                        copy_scales(at, true);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < TK / PER; ++i) {
+                            const int r = i * PER + sub;
+                            const bool live = r >= lo && r < hi;
+                            copy_async<16>(dst + k_offset<RB>(r, c), k_src + 512 * i, live);
+                            copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), v_src + 512 * i, live);
+                        }
+                        copy_scales(at, my_key >= lo && my_key < hi);
                     }
                 } else {
+                    const int row = row_of(next_page, key0 + my_key);
+                    next_page = page_of(s + 1);
 #pragma unroll
                     for (int i = 0; i < TK / PER; ++i) {
-                        const int r = i * PER + sub;
-                        const size_t at = (size_t)__shfl_sync(0xffffffffu, row, r) * RB + 16 * c;
-                        const bool live = __shfl_sync(0xffffffffu, known, r) && r >= span.first - key0 && r < hi;
-                        copy_async<16>(dst + k_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.k) + at, live);
-                        copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), static_cast<const uint8_t*>(p.cache.v) + at, live);
+                        const int r = i * PER + sub, from = __shfl_sync(0xffffffffu, row, r), at = max(from, 0);
+                        copy_async<16>(dst + k_offset<RB>(r, c), k_lane + (size_t)at * RB, from >= 0);
+                        copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), v_lane + (size_t)at * RB, from >= 0);
                     }
-                }
-                if constexpr (SB > 0) {
-                    const size_t at = (size_t)(row + (in_page ? my_key : 0)) * SB;
-                    const bool live = my_key >= lo && my_key < hi;
-                    const uint32_t to = dst + 2 * TK * RB + my_key * SB;
-                    if (TK == 32 || lane < 16) copy_async<SB>(to, static_cast<const uint8_t*>(p.cache.k_scale) + at, live);
-                    if (TK == 32 || lane >= 16) copy_async<SB>(to + TK * SB, static_cast<const uint8_t*>(p.cache.v_scale) + at, live);
+                    copy_scales(max(row, 0), row >= 0);
                 }
             }
             copy_commit();
@@ -409,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
             steps = r1 - r0;
             if (step0 + (steps - 1) * C::ROUND >= span.len) --steps;
-            next_page = page_of(0);
+            next_page = page_of(in_page ? lane : 0);
 #pragma unroll
             for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
 #pragma unroll
@@ -555,7 +573,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                         const int ra = 16 * kt + g, rb = ra + 8;
                         const float ka = fs[ra], kb = fs[rb];
                         va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
-                        la[kt] = fmaxf(__log2f(va[kt]), -80.0f), lb[kt] = fmaxf(__log2f(vb[kt]), -80.0f);
+                        la[kt] = fmaxf(log2_approx(va[kt]), -80.0f), lb[kt] = fmaxf(log2_approx(vb[kt]), -80.0f);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             sc[nt][kt][0] *= ka, sc[nt][kt][1] *= ka;
@@ -583,14 +601,15 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                         }
                     }
                 }
-                bool over = false;
+                float most_x = -INFINITY;  // over the headroom anywhere?  (for fp8 with the value scale's share)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) over |= x[nt][kt][i] > kHeadroom - (KIND != kKvFp8 ? 0.0f : i < 2 ? la[kt] : lb[kt]);
-                if (__any_sync(0xffffffffu, over)) {
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const float ta = fmaxf(x[nt][kt][0], x[nt][kt][1]), tb = fmaxf(x[nt][kt][2], x[nt][kt][3]);
+                        most_x = fmaxf(most_x, KIND == kKvFp8 ? fmaxf(ta + la[kt], tb + lb[kt]) : fmaxf(ta, tb));
+                    }
+                if (__any_sync(0xffffffffu, most_x > kHeadroom)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         // from the scores themselves (the first reference is too far off to go by x)
