@@ -587,8 +587,10 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            x[nt][kt][i] = i & 1 ? fmaf(sc[nt][kt][i], f1[nt], -ref1[nt]) : fmaf(sc[nt][kt][i], f0[nt], -ref0[nt]);
+                        for (int i = 0; i < 4; i += 2) {
+                            const unsigned long long both = fma2(pair_of(sc[nt][kt][i], sc[nt][kt][i + 1]), pair_of(f0[nt], f1[nt]), pair_of(-ref0[nt], -ref1[nt]));
+                            x[nt][kt][i] = first_of(both), x[nt][kt][i + 1] = second_of(both);
+                        }
                 if (key0 < span.first || key0 + TK > span.len) {
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt) {
@@ -654,8 +656,8 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                         float w[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[nt][kt][i]);
-                        l0[nt] += w[0] + w[2];
-                        l1[nt] += w[1] + w[3];
+                        const unsigned long long sum = add2(pair_of(l0[nt], l1[nt]), add2(pair_of(w[0], w[1]), pair_of(w[2], w[3])));
+                        l0[nt] = first_of(sum), l1[nt] = second_of(sum);
                         if constexpr (KIND == kKvFp8) {
                             // a masked key's zero-filled scale keeps its weight zero
                             w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];

@@ -263,21 +263,12 @@ __device__ __forceinline__ long slot_row(const RowsParams& p, long t, int lane) 
     return -1;
 }
 
+using decode::fma2;
+using decode::mul2;
+using decode::pair_of;
+
 __device__ __forceinline__ unsigned long long widen(uint32_t w) {
     return ((unsigned long long)(w & 0xFFFF0000u) << 32) | (unsigned long long)(w << 16);
-}
-__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
-    return ((unsigned long long)__float_as_uint(hi) << 32) | __float_as_uint(lo);
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
 }
 
 // The common forms: rows rotated as a whole in halves, normed or not (ROTATED),
