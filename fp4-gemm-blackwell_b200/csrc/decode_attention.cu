@@ -49,6 +49,11 @@
 //
 // A warp streams its steps through a ring of its own in shared memory with
 // cp.async: no barrier in the loop.  Masked keys are zero-filled, not read.
+// What a step costs besides its keys (its pages, addresses, waits, the loop)
+// was 58 of 357 instructions for 32 keys of 32 bytes, where the loop is bound by
+// issue: such steps have 64 keys, worked on in two unrolled parts (3 x 131072
+// keys of nvfp4, D = 64: 58 us by 32 keys and four steps in the ring, 53.7 by
+// 64 and two, 51.6 unrolled).  Pages are looked up for 32 parts at once.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -70,7 +75,7 @@ using namespace decode;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCtasPerSm = 4;
-constexpr int kSegmentRounds = 3;
+constexpr int kSegmentRounds = 3;  // of CK keys a warp, as kWholeRounds
 constexpr int kWholeRounds = 12;
 constexpr float kNoScore = -1e30f;    // reference exponent before any key
 constexpr float kHeadroom = 10.0f;    // a score may pass the reference by 2^10 ...
@@ -108,12 +113,16 @@ template <int KIND, int D, int NT>
 struct Cfg {
     static constexpr int RB = KIND == kKvBf16 ? 2 * D : KIND == kKvFp8 ? D : D / 2;  // bytes of a row
     static constexpr int SB = KIND == kKvBf16 ? 0 : KIND == kKvFp8 ? 4 : D / 16;     // bytes of its scales
-    static constexpr int TK = RB <= 64 ? 32 : 16;   // keys of a step: at least 1 KB of K
-    static constexpr int KT = TK / 16;
+    static constexpr int CK = RB <= 64 ? 32 : 16;   // keys that are worked on at once: at least 1 KB of K
+    static constexpr int KT = CK / 16;
+    static constexpr int PARTS = RB <= 32 ? 2 : 1;  // of them in a step, which is copied at once
+    static constexpr int TK = PARTS * CK;           // keys of a step
+    static constexpr int SEGMENT = (kSegmentRounds + PARTS - 1) / PARTS, WHOLE = kWholeRounds / PARTS;
     static constexpr int HEADS = 8 * NT;
     static constexpr int ROUND = kWarps * TK;
-    static constexpr int STAGE = 2 * TK * (RB + SB);
-    static constexpr int STAGES = STAGE >= 4096 ? 3 : 4;
+    static constexpr int PART = 2 * CK * (RB + SB);
+    static constexpr int STAGE = PARTS * PART;
+    static constexpr int STAGES = PARTS > 1 ? 2 : STAGE >= 4096 ? 3 : 4;
     static constexpr int RING = STAGES * STAGE;
     static constexpr int LD = D + 8;                // row stride of the merge area
     static constexpr int MERGE = kWarps * HEADS * LD * 4;
@@ -254,7 +263,7 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Part&
 template <int KIND, int D, int NT>
 __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid_constant__ AttentionParams p) {
     using C = Cfg<KIND, D, NT>;
-    constexpr int TK = C::TK, KT = C::KT, RB = C::RB, SB = C::SB, MT = D / 16, HEADS = C::HEADS;
+    constexpr int TK = C::TK, CK = C::CK, KT = C::KT, PARTS = C::PARTS, RB = C::RB, SB = C::SB, MT = D / 16, HEADS = C::HEADS;
     constexpr bool kBf16 = KIND == kKvBf16;
     constexpr float kUnit = KIND == kKvNvfp4 ? kScaleUnit : 1.0f;  // of the decoded values
     extern __shared__ __align__(128) uint8_t smem[];
@@ -264,7 +273,8 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     __shared__ int s_last[2];
 
     chain();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    // the shuffle tells the compiler that a warp has one of it: branches on what follows from it are uniform
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int units = p.cache.kv_heads * p.group_tiles;
 
     // ---- the batch's rounds: their number, and the prefix sums of the chunk at hand
@@ -272,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     auto scan = [&](int base) {
         const int b = base + tid;
         const int rounds = b < p.batch ? span_of<TK, C::ROUND>(p, b).rounds : 0;
-        mine = rounds > 0 ? (rounds + kSegmentRounds) * units : 0;
+        mine = rounds > 0 ? (rounds + C::SEGMENT) * units : 0;
         int sum = mine, top = rounds;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -295,8 +305,8 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     // parts about 4 us and 0.06 us a part.  So units of up to 12 rounds are not
     // split at all (each goes whole to the CTA in whose share it starts), and for
     // longer ones a CTA takes at least the rounds that balance the last two terms.
-    const bool split = most > kWholeRounds;
-    const int least = split ? (int)sqrtf((float)most * (1.0f / 7.0f)) : 1;
+    const bool split = most > C::WHOLE;
+    const int least = split ? (int)sqrtf((float)most * (1.0f / (7 * PARTS))) : 1;
     const int ctas = min((int)gridDim.x, max(total / least, min(total, 1)));
     if ((int)blockIdx.x < ctas) {
         // CTA c's share starts at c * each + min(c, extra)
@@ -322,21 +332,27 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 
         uint8_t* ring = smem + warp * C::RING;
         const uint32_t ring_addr = ptx::smem_u32(ring);
-        const bool in_page = p.cache.page_size >= TK;  // a step's keys are one run of one page
-        const int my_key = lane & (TK - 1);
+        const bool in_page = p.cache.page_size >= CK;  // the keys of a step's part are one run of one page
+        const int my_key = lane & (CK - 1);
 
         // ---- a segment: rounds [r0, r1) of one head unit, and the stream of this warp's steps of it
         Span span{};
-        int unit = 0, unit_start = 0, r0 = 0, r1 = 0, kv_head = 0, head0 = 0, live_heads = 0, step0 = 0, steps = 0, next_page = -2, rows = -1;
+        int unit = 0, unit_start = 0, r0 = 0, r1 = 0, kv_head = 0, head0 = 0, live_heads = 0, step0 = 0, steps = 0, rows = -1;
+        int full0 = 0, full1 = 0;  // steps [full0, full1) have all their keys
+        int next_page[PARTS];
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) next_page[h] = -2;
         uint2 qw[NT][MT];  // the queries as they are read, see below
         const int* table = nullptr;
-        // Where the rows of the steps lie: if in_page, lane i holds the first row (-1: none
-        // to read) of step 32 j + i and the page of step 32 (j + 1) + i is on its way;
-        // otherwise the page of the lane's key of the next step is.
-        auto page_of = [&](int s) {  // -2 for a masked key
-            if (s >= steps) return -2;
-            const int key = step0 + s * C::ROUND + (in_page ? 0 : my_key);
-            return (in_page || key >= span.first) && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
+        // Where the rows of the steps' parts lie, part j % PARTS of step j / PARTS being part
+        // j: if in_page, lane i holds the first row (-1: none to read) of part 32 n + i and
+        // the page of part 32 (n + 1) + i is on its way; otherwise the pages of the lane's
+        // keys of the next step are.
+        auto key_of = [&](int j) { return step0 + j / PARTS * C::ROUND + j % PARTS * CK; };
+        auto page_of = [&](int j) {  // -2 for masked keys
+            if (j >= steps * PARTS) return -2;
+            const int key = key_of(j) + (in_page ? 0 : my_key);
+            return key + (in_page ? CK - 1 : 0) >= span.first && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
         };
         auto row_of = [&](int page, int key) {
             if (page >= 0 && page < p.cache.num_pages)
@@ -350,52 +366,72 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         const uint8_t* const v_lane = static_cast<const uint8_t*>(p.cache.v) + 16 * (in_page ? lane : c);
         const uint8_t* const ks_lane = static_cast<const uint8_t*>(p.cache.k_scale) + (in_page ? my_key * SB : 0);
         const uint8_t* const vs_lane = static_cast<const uint8_t*>(p.cache.v_scale) + (in_page ? my_key * SB : 0);
+        auto copy_scales = [&](uint32_t part, int row, bool live) {
+            if constexpr (SB > 0) {
+                const uint32_t to = part + 2 * CK * RB + my_key * SB;
+                if (CK == 32 || lane < 16) copy_async<SB>(to, ks_lane + (size_t)row * SB, live);
+                if (CK == 32 || lane >= 16) copy_async<SB>(to + CK * SB, vs_lane + (size_t)row * SB, live);
+            }
+        };
         auto issue = [&](int s) {
             if (s < steps) {
-                const int key0 = step0 + s * C::ROUND;
-                const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE, scale_dst = dst + 2 * TK * RB + my_key * SB;
-                auto copy_scales = [&](int row, bool live) {
-                    if constexpr (SB > 0) {
-                        if (TK == 32 || lane < 16) copy_async<SB>(scale_dst, ks_lane + (size_t)row * SB, live);
-                        if (TK == 32 || lane >= 16) copy_async<SB>(scale_dst + TK * SB, vs_lane + (size_t)row * SB, live);
-                    }
-                };
+                const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE;
                 if (in_page) {
-                    if ((s & 31) == 0) {
-                        rows = row_of(next_page, key0 + lane * C::ROUND);
-                        next_page = page_of(s + 32 + lane);
+                    if ((s * PARTS & 31) == 0) {
+                        rows = row_of(next_page[0], key_of(s * PARTS + lane));
+                        next_page[0] = page_of(s * PARTS + 32 + lane);
                     }
-                    const int row = __shfl_sync(0xffffffffu, rows, s & 31);
-                    // rows lo .. hi - 1 of the step are read, the others zero-filled
-                    const int lo = row >= 0 ? span.first - key0 : TK, hi = span.len - key0, at = max(row, 0);
-                    const uint8_t *k_src = k_lane + (size_t)at * RB, *v_src = v_lane + (size_t)at * RB;
-                    if (lo <= 0 && hi >= TK) {
+                    int row[PARTS];
+                    bool full = s >= full0 && s < full1;
 #pragma unroll
-                        for (int i = 0; i < TK / PER; ++i) {
-                            copy_async<16>(dst + k_offset<RB>(i * PER + sub, c), k_src + 512 * i, true);
-                            copy_async<16>(dst + TK * RB + v_offset<RB>(i * PER + sub, c), v_src + 512 * i, true);
+                    for (int h = 0; h < PARTS; ++h) {
+                        row[h] = __shfl_sync(0xffffffffu, rows, (s * PARTS + h) & 31);
+                        full = full && row[h] >= 0;
+                    }
+                    if (full) {
+#pragma unroll
+                        for (int h = 0; h < PARTS; ++h) {
+                            const uint32_t part = dst + h * C::PART;
+                            const uint8_t *k_src = k_lane + (size_t)row[h] * RB, *v_src = v_lane + (size_t)row[h] * RB;
+#pragma unroll
+                            for (int i = 0; i < CK / PER; ++i) {
+                                copy_async<16>(part + k_offset<RB>(i * PER + sub, c), k_src + 512 * i, true);
+                                copy_async<16>(part + CK * RB + v_offset<RB>(i * PER + sub, c), v_src + 512 * i, true);
+                            }
+                            copy_scales(part, row[h], true);
                         }
-                        copy_scales(at, true);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < TK / PER; ++i) {
-                            const int r = i * PER + sub;
-                            const bool live = r >= lo && r < hi;
-                            copy_async<16>(dst + k_offset<RB>(r, c), k_src + 512 * i, live);
-                            copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), v_src + 512 * i, live);
+                        for (int h = 0; h < PARTS; ++h) {
+                            // rows lo .. hi - 1 of the part are read, the others zero-filled
+                            const int key0 = step0 + s * C::ROUND + h * CK, at = max(row[h], 0);
+                            const int lo = row[h] >= 0 ? span.first - key0 : CK, hi = span.len - key0;
+                            const uint32_t part = dst + h * C::PART;
+                            const uint8_t *k_src = k_lane + (size_t)at * RB, *v_src = v_lane + (size_t)at * RB;
+#pragma unroll
+                            for (int i = 0; i < CK / PER; ++i) {
+                                const int r = i * PER + sub;
+                                const bool live = r >= lo && r < hi;
+                                copy_async<16>(part + k_offset<RB>(r, c), k_src + 512 * i, live);
+                                copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_src + 512 * i, live);
+                            }
+                            copy_scales(part, at, my_key >= lo && my_key < hi);
                         }
-                        copy_scales(at, my_key >= lo && my_key < hi);
                     }
                 } else {
-                    const int row = row_of(next_page, key0 + my_key);
-                    next_page = page_of(s + 1);
 #pragma unroll
-                    for (int i = 0; i < TK / PER; ++i) {
-                        const int r = i * PER + sub, from = __shfl_sync(0xffffffffu, row, r), at = max(from, 0);
-                        copy_async<16>(dst + k_offset<RB>(r, c), k_lane + (size_t)at * RB, from >= 0);
-                        copy_async<16>(dst + TK * RB + v_offset<RB>(r, c), v_lane + (size_t)at * RB, from >= 0);
+                    for (int h = 0; h < PARTS; ++h) {
+                        const uint32_t part = dst + h * C::PART;
+                        const int row = row_of(next_page[h], key_of(s * PARTS + h) + my_key);
+                        next_page[h] = page_of((s + 1) * PARTS + h);
+#pragma unroll
+                        for (int i = 0; i < CK / PER; ++i) {
+                            const int r = i * PER + sub, from = __shfl_sync(0xffffffffu, row, r), at = max(from, 0);
+                            copy_async<16>(part + k_offset<RB>(r, c), k_lane + (size_t)at * RB, from >= 0);
+                            copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_lane + (size_t)at * RB, from >= 0);
+                        }
+                        copy_scales(part, max(row, 0), row >= 0);
                     }
-                    copy_scales(max(row, 0), row >= 0);
                 }
             }
             copy_commit();
@@ -405,7 +441,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             if (u >= u1) return false;
             for (;;) {
                 span = span_of<TK, C::ROUND>(p, b);
-                const int length = span.rounds > 0 ? span.rounds + kSegmentRounds : 0;  // of a unit
+                const int length = span.rounds > 0 ? span.rounds + C::SEGMENT : 0;  // of a unit
                 if (u < pre + length * units) {
                     const int local = u - pre;
                     unit = local / length;
@@ -427,7 +463,9 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             step0 = span.start + (r0 * kWarps + warp) * TK;  // first key of step 0; steps are ROUND keys apart
             steps = r1 - r0;
             if (step0 + (steps - 1) * C::ROUND >= span.len) --steps;
-            next_page = page_of(in_page ? lane : 0);
+            full0 = step0 < span.first, full1 = span.len - step0 < TK ? 0 : (span.len - step0 - TK) / C::ROUND + 1;
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) next_page[h] = page_of(in_page ? lane : h);
 #pragma unroll
             for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
 #pragma unroll
@@ -479,10 +517,10 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             }
 
             float acc[NT][MT][4];
-            float ref0[NT], ref1[NT], l0[NT], l1[NT];
+            float neg0[NT], neg1[NT], l0[NT], l1[NT];  // the references negated, the sums
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                ref0[nt] = ref1[nt] = kNoScore;
+                neg0[nt] = neg1[nt] = -kNoScore;
                 l0[nt] = l1[nt] = 0.0f;
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
@@ -494,254 +532,257 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 copy_wait<C::STAGES - 2>();
                 __syncwarp();
                 issue(s + C::STAGES - 1);
-                const uint8_t* sk = ring + (s % C::STAGES) * C::STAGE;
-                const uint8_t* sv = sk + TK * RB;
-                const uint8_t* ss = sv + TK * RB;
-                const int key0 = step0 + s * C::ROUND;
+#pragma unroll
+                for (int h = 0; h < PARTS; ++h) {
+                    const uint8_t* sk = ring + (s % C::STAGES) * C::STAGE + h * C::PART;
+                    const uint8_t* sv = sk + CK * RB;
+                    const uint8_t* ss = sv + CK * RB;
 
-                // ---- scores
-                float sc[NT][KT][4];
+                    // ---- scores
+                    float sc[NT][KT][4];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
+                    for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[nt][kt][i] = 0.0f;
-                    const int ra = 16 * kt + g, rb = ra + 8;
-                    if constexpr (kBf16) {
+                            for (int i = 0; i < 4; ++i) sc[nt][kt][i] = 0.0f;
+                        const int ra = 16 * kt + g, rb = ra + 8;
+                        if constexpr (kBf16) {
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
-                            const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                mma<true>(sc[nt][kt], a.x, c.x, a.y, c.y, qf[nt][2 * i][0], qf[nt][2 * i][1]);
-                                mma<true>(sc[nt][kt], a.z, c.z, a.w, c.w, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
-                            }
-                        }
-                    } else if constexpr (KIND == kKvFp8) {
-#pragma unroll
-                        for (int i = 0; i < D / 64; ++i) {
-                            const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
-                            const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                uint32_t ha[2], hc[2];
-                                e4m3x4_to_f16(aw[q], ha);
-                                e4m3x4_to_f16(cw[q], hc);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
-                            }
-                        }
-                    } else {
-                        constexpr int WORDS = C::EK / 8, PIECES = D / (4 * C::EK);
-#pragma unroll
-                        for (int i = 0; i < PIECES; ++i) {
-                            uint32_t aw[WORDS], cw[WORDS];
-                            if constexpr (WORDS == 2) {
-                                const uint2 a = lds64(sk + k_offset<RB>(ra, 0) + 8 * t), c = lds64(sk + k_offset<RB>(rb, 0) + 8 * t);
-                                aw[0] = a.x, aw[1] = a.y, cw[0] = c.x, cw[1] = c.y;
-                            } else {
+                            for (int i = 0; i < D / 32; ++i) {
                                 const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
-                                aw[0] = a.x, aw[1] = a.y, aw[2] = a.z, aw[3] = a.w, cw[0] = c.x, cw[1] = c.y, cw[2] = c.z, cw[3] = c.w;
-                            }
-#pragma unroll
-                            for (int q = 0; q < WORDS; ++q) {
-                                const int block = (C::EK / 16) * (4 * i + t) + q / 2;
-                                const uint32_t s_a = ue4m3x2_to_f16(ss[ra * SB + block] * 0x10001u), s_c = ue4m3x2_to_f16(ss[rb * SB + block] * 0x10001u);
-                                uint32_t ha[4], hc[4];
-                                e2m1x8_to_f16(aw[q], ha);
-                                e2m1x8_to_f16(cw[q], hc);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) ha[e] = mul_f16x2(ha[e], s_a), hc[e] = mul_f16x2(hc[e], s_c);
-                                const int j = (C::EK / 4) * i + 2 * q;
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
-                                    mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][j][0], qf[nt][j][1]);
-                                    mma<false>(sc[nt][kt], ha[2], hc[2], ha[3], hc[3], qf[nt][j + 1][0], qf[nt][j + 1][1]);
+                                    mma<true>(sc[nt][kt], a.x, c.x, a.y, c.y, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+                                    mma<true>(sc[nt][kt], a.z, c.z, a.w, c.w, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
                                 }
                             }
-                        }
-                    }
-                }
-
-                // ---- x = score in base 2 less the reference; the row scales of fp8
-                float va[KT], vb[KT], la[KT], lb[KT];  // value scales of the keys and their logarithms
-                if constexpr (KIND == kKvFp8) {
-                    const float* fs = reinterpret_cast<const float*>(ss);
+                        } else if constexpr (KIND == kKvFp8) {
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        const int ra = 16 * kt + g, rb = ra + 8;
-                        const float ka = fs[ra], kb = fs[rb];
-                        va[kt] = fs[TK + ra], vb[kt] = fs[TK + rb];
-                        la[kt] = fmaxf(log2_approx(va[kt]), -80.0f), lb[kt] = fmaxf(log2_approx(vb[kt]), -80.0f);
+                            for (int i = 0; i < D / 64; ++i) {
+                                const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+                                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            sc[nt][kt][0] *= ka, sc[nt][kt][1] *= ka;
-                            sc[nt][kt][2] *= kb, sc[nt][kt][3] *= kb;
-                        }
-                    }
-                }
-                float x[NT][KT][4];
+                                for (int q = 0; q < 4; ++q) {
+                                    uint32_t ha[2], hc[2];
+                                    e4m3x4_to_f16(aw[q], ha);
+                                    e4m3x4_to_f16(cw[q], hc);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; i += 2) {
-                            const unsigned long long both = fma2(pair_of(sc[nt][kt][i], sc[nt][kt][i + 1]), pair_of(f0[nt], f1[nt]), pair_of(-ref0[nt], -ref1[nt]));
-                            x[nt][kt][i] = first_of(both), x[nt][kt][i + 1] = second_of(both);
-                        }
-                if (key0 < span.first || key0 + TK > span.len) {
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        const int ka = key0 + 16 * kt + g, kb = ka + 8;
-                        const bool oa = ka >= span.first && ka < span.len, ob = kb >= span.first && kb < span.len;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            if (!oa) x[nt][kt][0] = x[nt][kt][1] = -INFINITY;
-                            if (!ob) x[nt][kt][2] = x[nt][kt][3] = -INFINITY;
-                        }
-                    }
-                }
-                float most_x = -INFINITY;  // over the headroom anywhere?  (for fp8 with the value scale's share)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        const float ta = fmaxf(x[nt][kt][0], x[nt][kt][1]), tb = fmaxf(x[nt][kt][2], x[nt][kt][3]);
-                        most_x = fmaxf(most_x, KIND == kKvFp8 ? fmaxf(ta + la[kt], tb + lb[kt]) : fmaxf(ta, tb));
-                    }
-                if (__any_sync(0xffffffffu, most_x > kHeadroom)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        // from the scores themselves (the first reference is too far off to go by x)
-                        float full[KT][4], t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                        for (int kt = 0; kt < KT; ++kt) {
-                            const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                full[kt][i] = x[nt][kt][i] == -INFINITY ? -INFINITY : sc[nt][kt][i] * (i & 1 ? f1[nt] : f0[nt]);
-                            t0 = fmaxf(t0, fmaxf(full[kt][0] + xa, full[kt][2] + xb));
-                            t1 = fmaxf(t1, fmaxf(full[kt][1] + xa, full[kt][3] + xb));
-                        }
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) {
-                            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
-                            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
-                        }
-                        const float n0 = fmaxf(ref0[nt], t0 - kBelowMax), n1 = fmaxf(ref1[nt], t1 - kBelowMax);
-                        const float c0 = exp2_approx(ref0[nt] - n0), c1 = exp2_approx(ref1[nt] - n1);
-                        ref0[nt] = n0, ref1[nt] = n1;
-                        l0[nt] *= c0, l1[nt] *= c1;
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            acc[nt][m][0] *= c0, acc[nt][m][1] *= c1;
-                            acc[nt][m][2] *= c0, acc[nt][m][3] *= c1;
-                        }
-#pragma unroll
-                        for (int kt = 0; kt < KT; ++kt) {
-                            x[nt][kt][0] = full[kt][0] - n0, x[nt][kt][1] = full[kt][1] - n1;
-                            x[nt][kt][2] = full[kt][2] - n0, x[nt][kt][3] = full[kt][3] - n1;
-                        }
-                    }
-                }
-
-                // ---- weights as P^T fragments
-                uint32_t pf[NT][KT][2], pl[NT][KT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        float w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[nt][kt][i]);
-                        const unsigned long long sum = add2(pair_of(l0[nt], l1[nt]), add2(pair_of(w[0], w[1]), pair_of(w[2], w[3])));
-                        l0[nt] = first_of(sum), l1[nt] = second_of(sum);
-                        if constexpr (KIND == kKvFp8) {
-                            // a masked key's zero-filled scale keeps its weight zero
-                            w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
-                        }
-                        if constexpr (kBf16) {
-                            const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
-                            pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
-                            pl[nt][kt][0] = transpose8x8(pack_bf16(w[0] - bf16_lo(hi0), w[1] - bf16_hi(hi0)));
-                            pl[nt][kt][1] = transpose8x8(pack_bf16(w[2] - bf16_lo(hi1), w[3] - bf16_hi(hi1)));
+                                    for (int nt = 0; nt < NT; ++nt) mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][4 * i + q][0], qf[nt][4 * i + q][1]);
+                                }
+                            }
                         } else {
-                            pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
-                            pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
-                        }
-                    }
-
-                // ---- values: the lane's keys are 2t, 2t + 1, 2t + 8, 2t + 9 of each 16, its elements run g of each row
+                            constexpr int WORDS = C::EK / 8, PIECES = D / (4 * C::EK);
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int r = 16 * kt + 2 * t;
-                    constexpr int WORDS = C::EV * RB / D / 4, PIECES = D / (8 * C::EV);  // words of a run, runs of a row
-#pragma unroll
-                    for (int i = 0; i < PIECES; ++i) {
-                        uint32_t v[4][WORDS];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int row = r + (x & 1) + 8 * (x >> 1);
-                            if constexpr (WORDS == 4) {
-                                const uint4 w = lds128(sv + v_offset<RB>(row, 8 * i + g));
-                                v[x][0] = w.x, v[x][1] = w.y, v[x][2] = w.z, v[x][3] = w.w;
-                            } else if constexpr (WORDS == 2) {
-                                const uint2 w = lds64(sv + v_offset<RB>(row, g >> 1) + 8 * (g & 1));
-                                v[x][0] = w.x, v[x][1] = w.y;
-                            } else {
-                                v[x][0] = lds32(sv + v_offset<RB>(row, g >> 2) + 4 * (g & 3));
-                            }
-                        }
-                        // A operands: [m-tile][keys 2t, 2t + 1 / 2t + 8, 2t + 9][element 2e / 2e + 1 of the run]
-                        constexpr int PAIRS = C::EV / 2;
-                        uint32_t h[PAIRS][2][2];
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            if constexpr (kBf16) {
-#pragma unroll
-                                for (int e = 0; e < PAIRS; ++e) {
-                                    h[e][y][0] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x5410);
-                                    h[e][y][1] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x7632);
+                            for (int i = 0; i < PIECES; ++i) {
+                                uint32_t aw[WORDS], cw[WORDS];
+                                if constexpr (WORDS == 2) {
+                                    const uint2 a = lds64(sk + k_offset<RB>(ra, 0) + 8 * t), c = lds64(sk + k_offset<RB>(rb, 0) + 8 * t);
+                                    aw[0] = a.x, aw[1] = a.y, cw[0] = c.x, cw[1] = c.y;
+                                } else {
+                                    const uint4 a = lds128(sk + k_offset<RB>(ra, 4 * i + t)), c = lds128(sk + k_offset<RB>(rb, 4 * i + t));
+                                    aw[0] = a.x, aw[1] = a.y, aw[2] = a.z, aw[3] = a.w, cw[0] = c.x, cw[1] = c.y, cw[2] = c.z, cw[3] = c.w;
                                 }
-                            } else if constexpr (KIND == kKvFp8) {
-                                // the two keys' bytes side by side, then decoded
 #pragma unroll
                                 for (int q = 0; q < WORDS; ++q) {
-                                    uint32_t lo[2], hi[2];
-                                    e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x5140), lo);
-                                    e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x7362), hi);
-                                    h[2 * q][y][0] = lo[0], h[2 * q][y][1] = lo[1];
-                                    h[2 * q + 1][y][0] = hi[0], h[2 * q + 1][y][1] = hi[1];
-                                }
-                            } else {
-                                // the two keys' codes side by side in each byte, then decoded
-                                const uint8_t* s_row = ss + TK * SB + (r + 8 * y) * SB;
+                                    const int block = (C::EK / 16) * (4 * i + t) + q / 2;
+                                    const uint32_t s_a = ue4m3x2_to_f16(ss[ra * SB + block] * 0x10001u), s_c = ue4m3x2_to_f16(ss[rb * SB + block] * 0x10001u);
+                                    uint32_t ha[4], hc[4];
+                                    e2m1x8_to_f16(aw[q], ha);
+                                    e2m1x8_to_f16(cw[q], hc);
 #pragma unroll
-                                for (int q = 0; q < WORDS; ++q) {
-                                    const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + q / 2;
-                                    const uint32_t s_v = ue4m3x2_to_f16(s_row[block] + 0x10000u * s_row[SB + block]);
-                                    const uint32_t a = v[2 * y][q], c = v[2 * y + 1][q];
-                                    uint32_t even[4], odd[4];
-                                    e2m1x8_to_f16((a & 0x0F0F0F0Fu) | ((c << 4) & 0xF0F0F0F0u), even);
-                                    e2m1x8_to_f16(((a >> 4) & 0x0F0F0F0Fu) | (c & 0xF0F0F0F0u), odd);
+                                    for (int e = 0; e < 4; ++e) ha[e] = mul_f16x2(ha[e], s_a), hc[e] = mul_f16x2(hc[e], s_c);
+                                    const int j = (C::EK / 4) * i + 2 * q;
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        h[4 * q + e][y][0] = mul_f16x2(even[e], s_v);
-                                        h[4 * q + e][y][1] = mul_f16x2(odd[e], s_v);
+                                    for (int nt = 0; nt < NT; ++nt) {
+                                        mma<false>(sc[nt][kt], ha[0], hc[0], ha[1], hc[1], qf[nt][j][0], qf[nt][j][1]);
+                                        mma<false>(sc[nt][kt], ha[2], hc[2], ha[3], hc[3], qf[nt][j + 1][0], qf[nt][j + 1][1]);
                                     }
                                 }
                             }
                         }
+                    }
+
+                    // ---- x = score in base 2 less the reference; the row scales of fp8
+                    float va[KT], vb[KT], la[KT], lb[KT];  // value scales of the keys and their logarithms
+                    if constexpr (KIND == kKvFp8) {
+                        const float* fs = reinterpret_cast<const float*>(ss);
 #pragma unroll
-                        for (int e = 0; e < PAIRS; ++e) {
-                            const int m = i * PAIRS + e;
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const int ra = 16 * kt + g, rb = ra + 8;
+                            const float ka = fs[ra], kb = fs[rb];
+                            va[kt] = fs[CK + ra], vb[kt] = fs[CK + rb];
+                            la[kt] = fmaxf(log2_approx(va[kt]), -80.0f), lb[kt] = fmaxf(log2_approx(vb[kt]), -80.0f);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pf[nt][kt][0], pf[nt][kt][1]);
-                                if constexpr (kBf16)
-                                    mma<true>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
+                                sc[nt][kt][0] *= ka, sc[nt][kt][1] *= ka;
+                                sc[nt][kt][2] *= kb, sc[nt][kt][3] *= kb;
+                            }
+                        }
+                    }
+                    float x[NT][KT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                            for (int i = 0; i < 4; i += 2) {
+                                const unsigned long long both = fma2(pair_of(sc[nt][kt][i], sc[nt][kt][i + 1]), pair_of(f0[nt], f1[nt]), pair_of(neg0[nt], neg1[nt]));
+                                x[nt][kt][i] = first_of(both), x[nt][kt][i + 1] = second_of(both);
+                            }
+                    if (s < full0 || s >= full1) {
+                        const int key0 = step0 + s * C::ROUND + h * CK;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const int ka = key0 + 16 * kt + g, kb = ka + 8;
+                            const bool oa = ka >= span.first && ka < span.len, ob = kb >= span.first && kb < span.len;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                if (!oa) x[nt][kt][0] = x[nt][kt][1] = -INFINITY;
+                                if (!ob) x[nt][kt][2] = x[nt][kt][3] = -INFINITY;
+                            }
+                        }
+                    }
+                    float most_x = -INFINITY;  // over the headroom anywhere?  (for fp8 with the value scale's share)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const float ta = fmaxf(x[nt][kt][0], x[nt][kt][1]), tb = fmaxf(x[nt][kt][2], x[nt][kt][3]);
+                            most_x = fmaxf(most_x, KIND == kKvFp8 ? fmaxf(ta + la[kt], tb + lb[kt]) : fmaxf(ta, tb));
+                        }
+                    if (__any_sync(0xffffffffu, most_x > kHeadroom)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            // from the scores themselves (the first reference is too far off to go by x)
+                            float full[KT][4], t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                            for (int kt = 0; kt < KT; ++kt) {
+                                const float xa = KIND == kKvFp8 ? la[kt] : 0.0f, xb = KIND == kKvFp8 ? lb[kt] : 0.0f;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    full[kt][i] = x[nt][kt][i] == -INFINITY ? -INFINITY : sc[nt][kt][i] * (i & 1 ? f1[nt] : f0[nt]);
+                                t0 = fmaxf(t0, fmaxf(full[kt][0] + xa, full[kt][2] + xb));
+                                t1 = fmaxf(t1, fmaxf(full[kt][1] + xa, full[kt][3] + xb));
+                            }
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) {
+                                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+                                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+                            }
+                            const float n0 = fmaxf(-neg0[nt], t0 - kBelowMax), n1 = fmaxf(-neg1[nt], t1 - kBelowMax);
+                            const float c0 = exp2_approx(-neg0[nt] - n0), c1 = exp2_approx(-neg1[nt] - n1);
+                            neg0[nt] = -n0, neg1[nt] = -n1;
+                            l0[nt] *= c0, l1[nt] *= c1;
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                acc[nt][m][0] *= c0, acc[nt][m][1] *= c1;
+                                acc[nt][m][2] *= c0, acc[nt][m][3] *= c1;
+                            }
+#pragma unroll
+                            for (int kt = 0; kt < KT; ++kt) {
+                                x[nt][kt][0] = full[kt][0] - n0, x[nt][kt][1] = full[kt][1] - n1;
+                                x[nt][kt][2] = full[kt][2] - n0, x[nt][kt][3] = full[kt][3] - n1;
+                            }
+                        }
+                    }
+
+                    // ---- weights as P^T fragments
+                    uint32_t pf[NT][KT][2], pl[NT][KT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            float w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[i] = exp2_approx(x[nt][kt][i]);
+                            const unsigned long long sum = add2(pair_of(l0[nt], l1[nt]), add2(pair_of(w[0], w[1]), pair_of(w[2], w[3])));
+                            l0[nt] = first_of(sum), l1[nt] = second_of(sum);
+                            if constexpr (KIND == kKvFp8) {
+                                // a masked key's zero-filled scale keeps its weight zero
+                                w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
+                            }
+                            if constexpr (kBf16) {
+                                const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
+                                pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
+                                pl[nt][kt][0] = transpose8x8(pack_bf16(w[0] - bf16_lo(hi0), w[1] - bf16_hi(hi0)));
+                                pl[nt][kt][1] = transpose8x8(pack_bf16(w[2] - bf16_lo(hi1), w[3] - bf16_hi(hi1)));
+                            } else {
+                                pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
+                                pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
+                            }
+                        }
+
+                    // ---- values: the lane's keys are 2t, 2t + 1, 2t + 8, 2t + 9 of each 16, its elements run g of each row
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const int r = 16 * kt + 2 * t;
+                        constexpr int WORDS = C::EV * RB / D / 4, PIECES = D / (8 * C::EV);  // words of a run, runs of a row
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) {
+                            uint32_t v[4][WORDS];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const int row = r + (x & 1) + 8 * (x >> 1);
+                                if constexpr (WORDS == 4) {
+                                    const uint4 w = lds128(sv + v_offset<RB>(row, 8 * i + g));
+                                    v[x][0] = w.x, v[x][1] = w.y, v[x][2] = w.z, v[x][3] = w.w;
+                                } else if constexpr (WORDS == 2) {
+                                    const uint2 w = lds64(sv + v_offset<RB>(row, g >> 1) + 8 * (g & 1));
+                                    v[x][0] = w.x, v[x][1] = w.y;
+                                } else {
+                                    v[x][0] = lds32(sv + v_offset<RB>(row, g >> 2) + 4 * (g & 3));
+                                }
+                            }
+                            // A operands: [m-tile][keys 2t, 2t + 1 / 2t + 8, 2t + 9][element 2e / 2e + 1 of the run]
+                            constexpr int PAIRS = C::EV / 2;
+                            uint32_t h[PAIRS][2][2];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                if constexpr (kBf16) {
+#pragma unroll
+                                    for (int e = 0; e < PAIRS; ++e) {
+                                        h[e][y][0] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x5410);
+                                        h[e][y][1] = __byte_perm(v[2 * y][e], v[2 * y + 1][e], 0x7632);
+                                    }
+                                } else if constexpr (KIND == kKvFp8) {
+                                    // the two keys' bytes side by side, then decoded
+#pragma unroll
+                                    for (int q = 0; q < WORDS; ++q) {
+                                        uint32_t lo[2], hi[2];
+                                        e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x5140), lo);
+                                        e4m3x4_to_f16(__byte_perm(v[2 * y][q], v[2 * y + 1][q], 0x7362), hi);
+                                        h[2 * q][y][0] = lo[0], h[2 * q][y][1] = lo[1];
+                                        h[2 * q + 1][y][0] = hi[0], h[2 * q + 1][y][1] = hi[1];
+                                    }
+                                } else {
+                                    // the two keys' codes side by side in each byte, then decoded
+                                    const uint8_t* s_row = ss + CK * SB + (r + 8 * y) * SB;
+#pragma unroll
+                                    for (int q = 0; q < WORDS; ++q) {
+                                        const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + q / 2;
+                                        const uint32_t s_v = ue4m3x2_to_f16(s_row[block] + 0x10000u * s_row[SB + block]);
+                                        const uint32_t a = v[2 * y][q], c = v[2 * y + 1][q];
+                                        uint32_t even[4], odd[4];
+                                        e2m1x8_to_f16((a & 0x0F0F0F0Fu) | ((c << 4) & 0xF0F0F0F0u), even);
+                                        e2m1x8_to_f16(((a >> 4) & 0x0F0F0F0Fu) | (c & 0xF0F0F0F0u), odd);
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e) {
+                                            h[4 * q + e][y][0] = mul_f16x2(even[e], s_v);
+                                            h[4 * q + e][y][1] = mul_f16x2(odd[e], s_v);
+                                        }
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < PAIRS; ++e) {
+                                const int m = i * PAIRS + e;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pf[nt][kt][0], pf[nt][kt][1]);
+                                    if constexpr (kBf16)
+                                        mma<true>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
+                                }
                             }
                         }
                     }
@@ -765,7 +806,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             for (int nt = 0; nt < NT; ++nt) {
                 const int h0 = 8 * nt + 2 * t;
                 if (g == 0) {
-                    s_m[warp][h0] = ref0[nt], s_m[warp][h0 + 1] = ref1[nt];
+                    s_m[warp][h0] = -neg0[nt], s_m[warp][h0 + 1] = -neg1[nt];
                     s_l[warp][h0] = l0[nt], s_l[warp][h0 + 1] = l1[nt];
                 }
                 float* to = merge + (warp * HEADS + h0) * C::LD;
