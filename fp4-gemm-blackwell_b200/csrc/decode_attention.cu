@@ -115,7 +115,7 @@ struct Cfg {
     static constexpr int SB = KIND == kKvBf16 ? 0 : KIND == kKvFp8 ? 4 : D / 16;     // bytes of its scales
     static constexpr int CK = RB <= 64 ? 32 : 16;   // keys that are worked on at once: at least 1 KB of K
     static constexpr int KT = CK / 16;
-    static constexpr int PARTS = RB <= 32 ? 2 : 1;  // of them in a step, which is copied at once
+    static constexpr int PARTS = RB <= 64 || KIND == kKvNvfp4 ? 2 : 1;  // of them in a step, which is copied at once
     static constexpr int TK = PARTS * CK;           // keys of a step
     static constexpr int SEGMENT = (kSegmentRounds + PARTS - 1) / PARTS, WHOLE = kWholeRounds / PARTS;
     static constexpr int HEADS = 8 * NT;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     // split at all (each goes whole to the CTA in whose share it starts), and for
     // longer ones a CTA takes at least the rounds that balance the last two terms.
     const bool split = most > C::WHOLE;
-    const int least = split ? (int)sqrtf((float)most * (1.0f / (7 * PARTS))) : 1;
+    const int least = split ? max(1, (int)sqrtf((float)most * (1.0f / (7 * PARTS)))) : 1;
     const int ctas = min((int)gridDim.x, max(total / least, min(total, 1)));
     if ((int)blockIdx.x < ctas) {
         // CTA c's share starts at c * each + min(c, extra)
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 copy_wait<C::STAGES - 2>();
                 __syncwarp();
                 issue(s + C::STAGES - 1);
-#pragma unroll
+#pragma unroll (RB <= 32 ? 2 : 1)
                 for (int h = 0; h < PARTS; ++h) {
                     const uint8_t* sk = ring + (s % C::STAGES) * C::STAGE + h * C::PART;
                     const uint8_t* sv = sk + CK * RB;
