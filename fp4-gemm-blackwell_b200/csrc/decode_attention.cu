@@ -53,7 +53,7 @@
 // was 58 of 357 instructions for 32 keys of 32 bytes, where the loop is bound by
 // issue: such steps have 64 keys, worked on in two unrolled parts (3 x 131072
 // keys of nvfp4, D = 64: 58 us by 32 keys and four steps in the ring, 53.7 by
-// 64 and two, 51.6 unrolled).  Pages are looked up for 32 parts at once.
+// 64 and two, 51.6 unrolled).  Pages are looked up for 32 runs of keys at once.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -76,7 +76,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCtasPerSm = 4;
 constexpr int kSegmentRounds = 3;  // of CK keys a warp, as kWholeRounds
-constexpr int kWholeRounds = 12;
+constexpr int kWholeRounds = 8;
 constexpr float kNoScore = -1e30f;    // reference exponent before any key
 constexpr float kHeadroom = 10.0f;    // a score may pass the reference by 2^10 ...
 constexpr float kBelowMax = 4.0f;     // ... which is set 2^4 below the maximum
@@ -260,7 +260,8 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Part&
     }
 }
 
-template <int KIND, int D, int NT>
+// RUN: a part's keys lie in runs of RUN rows, all CK of them, 16 or one.
+template <int KIND, int D, int NT, int RUN>
 __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid_constant__ AttentionParams p) {
     using C = Cfg<KIND, D, NT>;
     constexpr int TK = C::TK, CK = C::CK, KT = C::KT, PARTS = C::PARTS, RB = C::RB, SB = C::SB, MT = D / 16, HEADS = C::HEADS;
@@ -302,9 +303,11 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
     };
     for (int base = 0; base < p.batch; base += kThreads) scan(base);
     // A round takes about 0.4 us while the GPU is idle, counting and joining P
-    // parts about 4 us and 0.06 us a part.  So units of up to 12 rounds are not
-    // split at all (each goes whole to the CTA in whose share it starts), and for
-    // longer ones a CTA takes at least the rounds that balance the last two terms.
+    // parts about 4 us and 0.06 us a part.  So units of up to 8 rounds (of CK keys a
+    // warp) are not split at all (each goes whole to the CTA in whose share it
+    // starts), and for longer ones a CTA takes at least the rounds that balance the
+    // last two terms.  (5 x 1500 keys of nvfp4, D = 64: 12.4 us whole, 8.5 split;
+    // 33 x 500 of fp8, D = 128: 13.7 whole, 16.7 split.)
     const bool split = most > C::WHOLE;
     const int least = split ? max(1, (int)sqrtf((float)most * (1.0f / (7 * PARTS)))) : 1;
     const int ctas = min((int)gridDim.x, max(total / least, min(total, 1)));
@@ -332,7 +335,6 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 
         uint8_t* ring = smem + warp * C::RING;
         const uint32_t ring_addr = ptx::smem_u32(ring);
-        const bool in_page = p.cache.page_size >= CK;  // the keys of a step's part are one run of one page
         const int my_key = lane & (CK - 1);
 
         // ---- a segment: rounds [r0, r1) of one head unit, and the stream of this warp's steps of it
@@ -344,16 +346,14 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         for (int h = 0; h < PARTS; ++h) next_page[h] = -2;
         uint2 qw[NT][MT];  // the queries as they are read, see below
         const int* table = nullptr;
-        // Where the rows of the steps' parts lie, part j % PARTS of step j / PARTS being part
-        // j: if in_page, lane i holds the first row (-1: none to read) of part 32 n + i and
-        // the page of part 32 (n + 1) + i is on its way; otherwise the pages of the lane's
-        // keys of the next step are.
-        auto key_of = [&](int j) { return step0 + j / PARTS * C::ROUND + j % PARTS * CK; };
-        auto page_of = [&](int j) {  // -2 for masked keys
-            if (j >= steps * PARTS) return -2;
-            const int key = key_of(j) + (in_page ? 0 : my_key);
-            return key + (in_page ? CK - 1 : 0) >= span.first && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
+        // Where the rows of the runs lie: lane i holds the first row (-1: none to read) of
+        // run 32 n + i and the page of run 32 (n + 1) + i is on its way.  Without runs
+        // the pages of the lane's keys of the next step are.
+        constexpr int RUNS = RUN > 1 ? TK / RUN : 1;  // of a step
+        auto page_of = [&](int s, int key) {  // page of step s's key (or run from it on); -2 if masked
+            return s < steps && key + RUN > span.first && key < span.len ? max(table[key >> p.page_shift], -1) : -2;
         };
+        auto run_key = [&](int s) { return step0 + (s + lane / RUNS) * C::ROUND + lane % RUNS * RUN; };
         auto row_of = [&](int page, int key) {
             if (page >= 0 && page < p.cache.num_pages)
                 return (page * p.cache.kv_heads + kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
@@ -362,10 +362,12 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         };
         constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
         const int sub = lane / LR, c = lane % LR;
-        const uint8_t* const k_lane = static_cast<const uint8_t*>(p.cache.k) + 16 * (in_page ? lane : c);
-        const uint8_t* const v_lane = static_cast<const uint8_t*>(p.cache.v) + 16 * (in_page ? lane : c);
-        const uint8_t* const ks_lane = static_cast<const uint8_t*>(p.cache.k_scale) + (in_page ? my_key * SB : 0);
-        const uint8_t* const vs_lane = static_cast<const uint8_t*>(p.cache.v_scale) + (in_page ? my_key * SB : 0);
+        // what a lane adds to its row: an instruction's rows are one run
+        const int lane_at = 16 * (RUN > 1 ? lane : c), scale_at = (my_key & (RUN - 1)) * SB;
+        const uint8_t* const k_lane = static_cast<const uint8_t*>(p.cache.k) + lane_at;
+        const uint8_t* const v_lane = static_cast<const uint8_t*>(p.cache.v) + lane_at;
+        const uint8_t* const ks_lane = static_cast<const uint8_t*>(p.cache.k_scale) + scale_at;
+        const uint8_t* const vs_lane = static_cast<const uint8_t*>(p.cache.v_scale) + scale_at;
         auto copy_scales = [&](uint32_t part, int row, bool live) {
             if constexpr (SB > 0) {
                 const uint32_t to = part + 2 * CK * RB + my_key * SB;
@@ -373,62 +375,66 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                 if (CK == 32 || lane >= 16) copy_async<SB>(to + CK * SB, vs_lane + (size_t)row * SB, live);
             }
         };
+        auto issue_runs = [&](int s, uint32_t dst) {
+            constexpr int PER_PART = RUN > 1 ? CK / RUN : 1;
+            if ((s * RUNS & 31) == 0) {
+                rows = row_of(next_page[0], run_key(s));
+                next_page[0] = page_of(s + 32 / RUNS + lane / RUNS, run_key(s + 32 / RUNS));
+            }
+            int row[RUNS];
+            bool full = s >= full0 && s < full1;
+#pragma unroll
+            for (int n = 0; n < RUNS; ++n) {
+                row[n] = __shfl_sync(0xffffffffu, rows, (s * RUNS + n) & 31);
+                full = full && row[n] >= 0;
+            }
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) {
+                const uint32_t part = dst + h * C::PART;
+                const int key0 = step0 + s * C::ROUND + h * CK;
+                // the lane's key's row, for its scales
+                const int from = PER_PART > 1 && lane >= 16 ? row[h * PER_PART + PER_PART - 1] : row[h * PER_PART];
+                if (full) {
+#pragma unroll
+                    for (int i = 0; i < CK / PER; ++i) {
+                        const int r = i * PER + sub;
+                        const size_t at = (size_t)row[h * PER_PART + i * PER / RUN] * RB + i * PER % RUN * RB;
+                        copy_async<16>(part + k_offset<RB>(r, c), k_lane + at, true);
+                        copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_lane + at, true);
+                    }
+                    copy_scales(part, from, true);
+                } else {
+                    // keys from lo up and below hi are read, the others zero-filled
+                    const int lo = span.first - key0, hi = span.len - key0;
+#pragma unroll
+                    for (int i = 0; i < CK / PER; ++i) {
+                        const int r = i * PER + sub, first = row[h * PER_PART + i * PER / RUN];
+                        const size_t at = (size_t)max(first, 0) * RB + i * PER % RUN * RB;
+                        const bool live = first >= 0 && r >= lo && r < hi;
+                        copy_async<16>(part + k_offset<RB>(r, c), k_lane + at, live);
+                        copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_lane + at, live);
+                    }
+                    copy_scales(part, max(from, 0), from >= 0 && my_key >= lo && my_key < hi);
+                }
+            }
+        };
         auto issue = [&](int s) {
             if (s < steps) {
                 const uint32_t dst = ring_addr + (s % C::STAGES) * C::STAGE;
-                if (in_page) {
-                    if ((s * PARTS & 31) == 0) {
-                        rows = row_of(next_page[0], key_of(s * PARTS + lane));
-                        next_page[0] = page_of(s * PARTS + 32 + lane);
-                    }
-                    int row[PARTS];
-                    bool full = s >= full0 && s < full1;
-#pragma unroll
-                    for (int h = 0; h < PARTS; ++h) {
-                        row[h] = __shfl_sync(0xffffffffu, rows, (s * PARTS + h) & 31);
-                        full = full && row[h] >= 0;
-                    }
-                    if (full) {
-#pragma unroll
-                        for (int h = 0; h < PARTS; ++h) {
-                            const uint32_t part = dst + h * C::PART;
-                            const uint8_t *k_src = k_lane + (size_t)row[h] * RB, *v_src = v_lane + (size_t)row[h] * RB;
-#pragma unroll
-                            for (int i = 0; i < CK / PER; ++i) {
-                                copy_async<16>(part + k_offset<RB>(i * PER + sub, c), k_src + 512 * i, true);
-                                copy_async<16>(part + CK * RB + v_offset<RB>(i * PER + sub, c), v_src + 512 * i, true);
-                            }
-                            copy_scales(part, row[h], true);
-                        }
-                    } else {
-#pragma unroll
-                        for (int h = 0; h < PARTS; ++h) {
-                            // rows lo .. hi - 1 of the part are read, the others zero-filled
-                            const int key0 = step0 + s * C::ROUND + h * CK, at = max(row[h], 0);
-                            const int lo = row[h] >= 0 ? span.first - key0 : CK, hi = span.len - key0;
-                            const uint32_t part = dst + h * C::PART;
-                            const uint8_t *k_src = k_lane + (size_t)at * RB, *v_src = v_lane + (size_t)at * RB;
-#pragma unroll
-                            for (int i = 0; i < CK / PER; ++i) {
-                                const int r = i * PER + sub;
-                                const bool live = r >= lo && r < hi;
-                                copy_async<16>(part + k_offset<RB>(r, c), k_src + 512 * i, live);
-                                copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_src + 512 * i, live);
-                            }
-                            copy_scales(part, at, my_key >= lo && my_key < hi);
-                        }
-                    }
+                if constexpr (RUN > 1) {
+                    issue_runs(s, dst);
                 } else {
 #pragma unroll
                     for (int h = 0; h < PARTS; ++h) {
                         const uint32_t part = dst + h * C::PART;
-                        const int row = row_of(next_page[h], key_of(s * PARTS + h) + my_key);
-                        next_page[h] = page_of((s + 1) * PARTS + h);
+                        const int key = step0 + s * C::ROUND + h * CK + my_key, row = row_of(next_page[h], key);
+                        next_page[h] = page_of(s + 1, key + C::ROUND);
 #pragma unroll
                         for (int i = 0; i < CK / PER; ++i) {
-                            const int r = i * PER + sub, from = __shfl_sync(0xffffffffu, row, r), at = max(from, 0);
-                            copy_async<16>(part + k_offset<RB>(r, c), k_lane + (size_t)at * RB, from >= 0);
-                            copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_lane + (size_t)at * RB, from >= 0);
+                            const int r = i * PER + sub, from = __shfl_sync(0xffffffffu, row, r);
+                            const size_t at = (size_t)max(from, 0) * RB;
+                            copy_async<16>(part + k_offset<RB>(r, c), k_lane + at, from >= 0);
+                            copy_async<16>(part + CK * RB + v_offset<RB>(r, c), v_lane + at, from >= 0);
                         }
                         copy_scales(part, max(row, 0), row >= 0);
                     }
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
             if (step0 + (steps - 1) * C::ROUND >= span.len) --steps;
             full0 = step0 < span.first, full1 = span.len - step0 < TK ? 0 : (span.len - step0 - TK) / C::ROUND + 1;
 #pragma unroll
-            for (int h = 0; h < PARTS; ++h) next_page[h] = page_of(in_page ? lane : h);
+            for (int h = 0; h < PARTS; ++h) next_page[h] = RUN > 1 ? page_of(lane / RUNS, run_key(0)) : page_of(0, step0 + h * CK + my_key);
 #pragma unroll
             for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
 #pragma unroll
@@ -905,12 +911,12 @@ Layout layout_of(int sms, int heads, int d) {
 
 int unit_heads(int group) { return group <= 8 ? 8 : 16; }
 
-template <int KIND, int D, int NT>
+template <int KIND, int D, int NT, int RUN>
 cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     using C = Cfg<KIND, D, NT>;
     static std::mutex mu;
     static int resident[kMaxDevices];  // CTAs that fit on the device at once
-    auto* kernel = decode_attention_kernel<KIND, D, NT>;
+    auto* kernel = decode_attention_kernel<KIND, D, NT, RUN>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -938,9 +944,21 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     return launch_chained(kernel, dim3((unsigned)std::min<long>(resident[dev], most)), kThreads, C::SMEM, st, p);
 }
 
+// Pages of 16 where 32 keys are worked on at once have a form of their own: 3 x
+// 131072 keys of nvfp4, D = 64: 53.1 us against 57 key by key and 51.5 by whole
+// parts (one kernel with all three costs each of them 1.3 us, in registers).
+template <int KIND, int D, int NT>
+cudaError_t launch_run(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
+    constexpr int CK = Cfg<KIND, D, NT>::CK;
+    if (p.cache.page_size >= CK) return launch<KIND, D, NT, CK>(p, workspace, st);
+    if constexpr (CK > 16)
+        if (p.cache.page_size >= 16) return launch<KIND, D, NT, 16>(p, workspace, st);
+    return launch<KIND, D, NT, 1>(p, workspace, st);
+}
+
 template <int KIND, int D>
 cudaError_t launch_heads(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
-    return unit_heads(p.group) == 8 ? launch<KIND, D, 1>(p, workspace, st) : launch<KIND, D, 2>(p, workspace, st);
+    return unit_heads(p.group) == 8 ? launch_run<KIND, D, 1>(p, workspace, st) : launch_run<KIND, D, 2>(p, workspace, st);
 }
 
 template <int KIND>
