@@ -74,9 +74,15 @@ struct GemvParams {
     int n_pad;
 };
 
-// Chunk c (8 elements) of row g of a chunk of x: where it lies, so that the
-// eight lanes of one phase of the reads meet distinct banks.
-__device__ __forceinline__ int x_offset(int row_bytes, int g, int c) { return g * row_bytes + 16 * (c ^ ((c >> 3) & 1) ^ ((g & 1) << 1)); }
+// x in shared memory: 16 bytes more after every 128, and rows 32 bytes more than a
+// multiple of 128, so that the eight lanes of one phase of the reads (two rows, every
+// fourth chunk of 8 elements) meet distinct banks, at constant offsets from a step's
+// start.
+constexpr int kXStep = 2 * kStep + 32;  // bytes of a step of one row
+__host__ __device__ constexpr int x_row_bytes(int steps) { return steps * kXStep + 32 * ((1 - steps) & 3); }
+__device__ __forceinline__ int x_offset(int row_bytes, int g, int c) { return g * row_bytes + 16 * (c + (c >> 3)); }
+// Room for `bytes` of x.
+constexpr int x_room(int bytes) { return bytes / 8 * 9 + 16 * 96; }
 
 // Elements k .. k+7 of a row of x, zeros past its end.
 __device__ __forceinline__ uint4 x_eight(const GemvParams& p, const uint16_t* row, int k) {
@@ -141,7 +147,7 @@ __device__ __forceinline__ void convert_x(const GemvParams& p, int m0, int rows,
         const int piece = threadIdx.x + i * kThreads;
         if (piece >= pieces) break;
         const int row = row_of(piece);
-        *reinterpret_cast<uint4*>(sx + x_offset(16 * per_row, row, piece - row * per_row)) =
+        *reinterpret_cast<uint4*>(sx + x_offset(x_row_bytes(steps), row, piece - row * per_row)) =
             eight_to_f16(v[i], power_of_two(scale_exponent(s_top[row])));
     }
     __syncthreads();
@@ -165,19 +171,17 @@ __device__ __forceinline__ void copy_step(uint32_t dst, const WeightLane& from, 
 }
 
 // A lane's view of x in shared memory: chunk 4 t + u of its row in a step lies at
-// base[nt] + 256 step + ((16 u) ^ swap) (x_offset's permutation moves u alone).
-// Lanes whose row does not exist read another one; their columns are never stored.
+// base[nt] + kXStep step + 16 u.  Lanes whose row does not exist read another one;
+// their columns are never stored.
 template <int NT>
 struct XLane {
     const uint8_t* base[NT];
-    int swap;
 };
 template <int NT>
 __device__ __forceinline__ XLane<NT> x_lane(const uint8_t* sx, int rows, int row_bytes, int g, int t) {
     XLane<NT> x;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) x.base[nt] = sx + (8 * nt + g < rows ? 8 * nt + g : rows > 1 ? g & 1 : 0) * row_bytes + 64 * t;
-    x.swap = 16 * ((t >> 1) ^ ((rows > 1 ? g & 1 : 0) << 1));
+    for (int nt = 0; nt < NT; ++nt) x.base[nt] = sx + (8 * nt + g < rows ? 8 * nt + g : rows > 1 ? g & 1 : 0) * row_bytes + 64 * t + 16 * (t >> 1);
     return x;
 }
 
@@ -197,7 +201,7 @@ __device__ __forceinline__ void step_products(float (&acc)[2][NT][4], const uint
     for (int u = 0; u < 4; ++u) {
         uint4 xv[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) xv[nt] = lds128(x.base[nt] + 256 * step + ((16 * u) ^ x.swap));
+        for (int nt = 0; nt < NT; ++nt) xv[nt] = lds128(x.base[nt] + kXStep * step + 16 * u);
         uint32_t a[4][4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ Ge
 
     float acc[2][NT][4];
     clear(acc);
-    const XLane<NT> x = x_lane<NT>(sx, rows, 2 * steps * kStep, g, t);
+    const XLane<NT> x = x_lane<NT>(sx, rows, x_row_bytes(steps), g, t);
     int slot = 0;
     for (int i = 0; i < mine; ++i) {
         copy_wait<kStages - 2>();
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(32 * kWalkWarps, 1) gemv_walk_kernel(const __g
     int now = warp;
     convert_x<32 * kWalkWarps, kWalkBytes>(p, m0, rows, first * kStep, steps, sx, s_top, s_factor);
 
-    const XLane<NT> x = x_lane<NT>(sx, rows, 2 * steps * kStep, g, t);
+    const XLane<NT> x = x_lane<NT>(sx, rows, x_row_bytes(steps), g, t);
     float* sums = p.sums + ((size_t)blockIdx.y * p.slices + slice) * 8 * NT * p.n_pad;
     int slot = 0;
     while (now < share) {
@@ -456,13 +460,13 @@ Cut cut_of(int m, int n, int k) {
 }
 static_assert(kWalkBytes / (16 * 2 * kStep) / 2 > kStages, "a walk's stream runs into one further group at most");
 
-int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * 2 * (p.slice_steps + (p.slice_more > 0 ? 1 : 0)) * kStep; }
+int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * x_row_bytes(p.slice_steps + (p.slice_more > 0 ? 1 : 0)); }
 
 template <int NT, int RG, int W>
 cudaError_t launch(const GemvParams& p, cudaStream_t st) {
     constexpr int kRing = W * kStages * kStageBytes;
     static bool ready[kMaxDevices];
-    if (const cudaError_t e = allow_smem(gemv_kernel<NT, RG, W>, kRing + kSliceBytes, ready)) return e;
+    if (const cudaError_t e = allow_smem(gemv_kernel<NT, RG, W>, kRing + x_room(kSliceBytes), ready)) return e;
     const long blocks = ((long)p.n + 127) / 128 * (4 / RG);
     const dim3 grid((unsigned)blocks, (unsigned)((p.m + 8 * NT - 1) / (8 * NT)), (unsigned)p.slices);
     return launch_chained(gemv_kernel<NT, RG, W>, grid, 32 * W, kRing + x_bytes(p), st, p);
@@ -472,7 +476,7 @@ template <int NT>
 cudaError_t launch_walk(const GemvParams& p, cudaStream_t st) {
     constexpr int kRing = kWalkWarps * kStages * kStageBytes;
     static bool ready[kMaxDevices];
-    if (const cudaError_t e = allow_smem(gemv_walk_kernel<NT>, kRing + kWalkBytes, ready)) return e;
+    if (const cudaError_t e = allow_smem(gemv_walk_kernel<NT>, kRing + x_room(kWalkBytes), ready)) return e;
     const dim3 grid((unsigned)(p.slices * p.ctas), (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
     return launch_chained(gemv_walk_kernel<NT>, grid, 32 * kWalkWarps, kRing + x_bytes(p), st, p);
 }
