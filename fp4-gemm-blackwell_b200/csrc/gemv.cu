@@ -28,11 +28,11 @@
 // joined in shared memory.  Where there are too few rows for all SMs, or x does
 // not fit beside the rings, K is cut into slices of CTAs of their own too, whose
 // sums go to the workspace, and a second kernel adds them in their order.
-// Many rows with a large x: a CTA keeps one slice of x and walks groups of rows
-// with it, each warp a group at a time and without a barrier, so that x is
-// converted 148 times at most.  (x by chunks through shared memory instead, all of
-// it for every CTA, took a barrier every two steps and as many bytes of x as of
-// the weight from L2: 53.5 us for 16 x 16384 x 16384, now 44.)
+// Large weights: a CTA keeps one slice of x and walks groups of rows with it, each
+// warp a group at a time and without a barrier, so that x is converted 148 times at
+// most.  (x by chunks through shared memory instead, all of it for every CTA, took
+// a barrier every two steps and as many bytes of x as of the weight from L2: 53.5 us
+// for 16 rows of x, 16384 x 16384, now 39.4.)
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -316,6 +316,7 @@ __global__ void __launch_bounds__(32 * W) gemv_kernel(const __grid_constant__ Ge
 // every p.ctas-th) from a counter, each through a stream of its own that runs on
 // over the groups' ends.
 constexpr int kWalkWarps = 16;
+constexpr int kWalkSteps = 5;  // of a slice at least
 template <int NT>
 __global__ void __launch_bounds__(32 * kWalkWarps, 1) gemv_walk_kernel(const __grid_constant__ GemvParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -431,8 +432,7 @@ cudaError_t allow_smem(Kernel* kernel, int bytes, bool (&ready)[kMaxDevices]) {
 // Rows of x that share a tile's products: 8 or 16.
 int tile_rows(int m) { return m <= 8 ? 8 : 16; }
 
-// How a call is cut.  Walked or not, 16 rows of x: 16384 x 16384 42.7 us against
-// 62.4 (64 rows a CTA); 10 rows: 1124 x 6282 19.7 us against 11.1.
+// How a call is cut.
 struct Cut {
     bool walk;
     int rows_per_cta;  // 32 RG
@@ -441,22 +441,23 @@ struct Cut {
 Cut cut_of(int m, int n, int k) {
     const int all = (k + kStep - 1) / kStep, groups = (n + 127) / 128 * 4, step_bytes = std::min(m, tile_rows(m)) * 2 * kStep;
     Cut c{};
-    // walked where x is large and every warp of a full GPU finds a group or nearly
-    const int walk_slices = (all * step_bytes + kWalkBytes - 1) / kWalkBytes;
-    if (all * step_bytes > kSliceBytes && groups * walk_slices >= 148 * kWalkWarps * 3 / 4) {
-        c.walk = true;
-        const int fit = (all + kWalkBytes / step_bytes - 1) / (kWalkBytes / step_bytes);
-        // As many slices as let a CTA's warps end together: the rounds of its groups
-        // times the steps of each, and a third of a step for a slice's sums (16384 x
-        // 16384: 8 slices 42.0 us, 9 40.3, 18 43.9).
-        int least = 0;
-        for (int slices = fit; slices <= std::min(148, 2 * fit) && (slices == fit || all / slices >= 8); ++slices) {
-            const int ctas = std::max(1, std::min(148 / slices, groups)), share = (groups + ctas - 1) / ctas;
-            const int cost = 3 * ((share + kWalkWarps - 1) / kWalkWarps) * ((all + slices - 1) / slices) + slices;
-            if (!least || cost < least) least = cost, c.slices = slices, c.ctas = ctas;
-        }
-        return c;
+    // Walked where slices of a few steps give (nearly) every warp of a full GPU a
+    // group: rows x 28672 x 8192 28.8 us walked and 34.4 not with one row of x, 37.7 and
+    // over 60 with 16; 8 rows, 28672 x 4096 19.4 and 32.7.  Slices of 5 steps do where x
+    // does not fit beside the rings otherwise (16 rows, 15360 x 2880: 13.4 us walked,
+    // 19.2 not), of 8 where it would (5 rows: 11.1 and 9.8).  Of the numbers of slices
+    // the one that lets a CTA's warps end together: the rounds of its groups times the
+    // steps of each, and a third of a step for a slice's sums (16 rows, 16384 x 16384:
+    // 8 slices 42.0 us, 9 39.4, 18 43.9).
+    const int shortest = all * step_bytes > kSliceBytes ? kWalkSteps : 8;
+    const int from = std::max((all * step_bytes + kWalkBytes - 1) / kWalkBytes, (148 * kWalkWarps * 3 / 4 + groups - 1) / groups);
+    int least = 0;
+    for (int slices = from; slices <= std::min(148, 2 * from) && all / slices >= shortest; ++slices) {
+        const int ctas = std::max(1, std::min(148 / slices, groups)), share = (groups + ctas - 1) / ctas;
+        const int cost = 3 * ((share + kWalkWarps - 1) / kWalkWarps) * ((all + slices - 1) / slices) + slices;
+        if (!least || cost < least) least = cost, c.walk = true, c.slices = slices, c.ctas = ctas;
     }
+    if (c.walk) return c;
     // Slices that fit, of 16 steps or more, and as many as still make one wave of two
     // CTAs an SM; then 32, 64 or 128 rows of the weight a CTA, as many as leave about
     // a CTA for each SM (15360 rows x 2880, 5 rows of x: 17.1 / 12.6 / 10.7 us; 2880
@@ -466,7 +467,7 @@ Cut cut_of(int m, int n, int k) {
     c.rows_per_cta = groups * c.slices < 296 ? 32 : groups * c.slices < 480 ? 64 : 128;
     return c;
 }
-static_assert(kWalkBytes / (16 * 2 * kStep) / 2 > kStages, "a walk's stream runs into one further group at most");
+static_assert(kWalkSteps > kStages, "a walk's stream runs into one further group at most");
 
 int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * x_row_bytes(p.slice_steps + (p.slice_more > 0 ? 1 : 0)); }
 
