@@ -93,6 +93,11 @@ def test_gemv_many_rows_of_a_long_k(cuda, fp4, m, n, k):
     cache.free()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 28500, 2050), (5, 28500, 2051), (8, 28416, 2100), (2, 14400, 4200), (16, 15360, 2880), (20, 7000, 6000)])
+def test_gemv_many_rows(cuda, fp4, m, n, k):
+    gemv_check(cuda, fp4, m, n, k, bias=k % 2 == 0)
+
+
 def test_gemv_strided_batched_and_cast_rows(cuda, fp4):
     m, n, k = 6, 384, 650
     x, w, _ = W.cached_linear_inputs(m, n, k, seed=3, bias=False)
@@ -492,6 +497,35 @@ def test_attention_head_layouts(dec, cuda, kind, hq, hk):
 @pytest.mark.parametrize("page", [1, 2, 4, 8, 16, 32, 128, 1024])
 def test_attention_pages(dec, cuda, kind, page):
     attention_check(dec, *attention_case(dec, cuda, kind, 128, 4, 2, page, [3, 333, 0, 1050, 129], seed=page))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("page", [1, 8, 16, 32, 64])
+def test_attention_pages_of_other_heads(dec, cuda, kind, d, page):
+    attention_check(dec, *attention_case(dec, cuda, kind, d, 4, 2, page, [3, 333, 0, 1050, 129], seed=page + d))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [500, 900, 1500, 1793, 2600, 3329])
+def test_attention_of_middle_lengths(dec, cuda, kind, d, n):
+    attention_check(dec, *attention_case(dec, cuda, kind, d, 4, 2, 32, [n, n - 257], seed=n))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [1, 8, 16, 32, 64])
+def test_attention_without_the_pages_before_a_window(dec, cuda, fp4, kind, page):
+    # what lies before a sequence's window may have been given back: its table entries are not read
+    for d in (64, 128):
+        q, cache, table, seq = attention_case(dec, cuda, kind, d, 4, 2, page, [64, 333, 20, 1050, 129], seed=page)
+        for window in (1, 33, 70, 200):
+            want = dec.decode_attention(q, cache, table, seq, window=window)
+            short = table.clone()
+            for i, n in enumerate(seq.tolist()):
+                short[i, : max(0, n - window) // page] = -1
+            assert torch.equal(dec.decode_attention(q, cache, short, seq, window=window), want)
+    assert fp4.device_error() == 0
 
 
 @pytest.mark.parametrize("kind", KINDS)
