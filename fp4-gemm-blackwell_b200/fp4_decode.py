@@ -309,8 +309,8 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     Attention of one new token of each sequence over its keys and values in the cache.
 
     q is [B, Hq, head_dim] BF16, Hq a multiple of the cache's heads (query head h reads key head h // (Hq // kv_heads));
-    page_table [B, W] int32, its first ceil(len / page_size) entries the sequence's pages in order (the others are not
-    read); seq_lens [B] int32, the new token's own key included if it is to be seen.  scale defaults to head_dim ** -0.5;
+    page_table [B, W] int32, its first ceil(len / page_size) entries the sequence's pages in order (the others, and
+    those wholly before the window, are not read); seq_lens [B] int32, the new token's own key included if it is to be seen.  scale defaults to head_dim ** -0.5;
     window > 0 lets a token see its last `window` keys only; sinks [Hq] is one more logit of each head's softmax that no
     value belongs to.  A sequence of length 0 gives zeros.
 

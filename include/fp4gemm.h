@@ -107,7 +107,8 @@ const char* fp4b_last_error(void);
 /* Non-zero if a kernel on the current device gave up on a bounded wait: the
  * first code recorded (GEMM 1 producer, 2 MMA, 3 epilogue, 4 fused-quantize
  * wait; 5 quantizer ring; 7 / 8 the self-test below; 9 fp4b_mma_rate's final
- * wait; 10 fp4b_peer_barrier); clear != 0 resets it.
+ * wait; 10 fp4b_peer_barrier; 11 slot, 12 position, 13 page or length out of
+ * range in a decode-side operator); clear != 0 resets it.
  * Synchronises the device. */
 int fp4b_device_error(int clear);
 
