@@ -78,6 +78,10 @@ def _rows(t: torch.Tensor, what: str, device=None) -> torch.Tensor:
     return t
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _indices(t: torch.Tensor, count: int, what: str, device) -> torch.Tensor:
     if t.dtype not in (torch.int64, torch.int32) or t.device != device or t.numel() != count:
         raise ValueError(f"{what} must be {count} int32 or int64 numbers on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -143,7 +147,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
     table, rows, rot = _rope(rope, d, dev)
     if table:
         positions = _indices(positions, t, "positions", dev)
-    q_out, k_out = q.new_empty((t, hq, d)), q.new_empty((t, hk, d))
+    q_out, k_out = _like(q), _like(k)
     if t == 0:
         return q_out, k_out
     q_weight, k_weight = _weight(q_weight, d, "q_weight", dev), _weight(k_weight, d, "k_weight", dev)
@@ -219,6 +223,7 @@ class PagedKVCache:
         self._view = _CacheView(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if scales else None,
                                 v_scales.data_ptr() if scales else None, n, h, s, d, KV_KINDS[self.dtype])
         self._ref = ctypes.addressof(self._view)
+        self._bf16 = torch.empty(0, dtype=torch.bfloat16, device=self.device)  # what results are made like
         self._attention_bytes = {}  # query heads -> bytes of decode_attention's workspace
 
     @property
@@ -258,7 +263,7 @@ class PagedKVCache:
         table, rows, rot = _rope(rope, d, dev)
         if table:
             positions = _indices(positions, t, "positions", dev)
-        q_out = q.new_empty((t, hq, d))
+        q_out = _like(q)
         if t == 0:
             return q_out
         q_weight, k_weight = _weight(q_weight, d, "q_weight", dev), _weight(k_weight, d, "k_weight", dev)
@@ -273,8 +278,7 @@ class PagedKVCache:
         """Keys and values of slots [n] as new BF16 tensors [n, kv_heads, head_dim] each; zeros for a negative slot."""
         n = slots.numel()
         slots = _indices(slots, n, "slots", self.device)
-        shape = (n, self.kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        k = self._bf16.new_empty(n, self.kv_heads, self.head_dim)
         v = torch.empty_like(k)
         if n:
             _call(self.device, _kv_read, "read", self._ref, slots.data_ptr(), slots.dtype == torch.int64, n, k.data_ptr(), v.data_ptr())
@@ -310,9 +314,9 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
 
     q is [B, Hq, head_dim] BF16, Hq a multiple of the cache's heads (query head h reads key head h // (Hq // kv_heads));
     page_table [B, W] int32, its first ceil(len / page_size) entries the sequence's pages in order (the others, and
-    those wholly before the window, are not read); seq_lens [B] int32, the new token's own key included if it is to be seen.  scale defaults to head_dim ** -0.5;
-    window > 0 lets a token see its last `window` keys only; sinks [Hq] is one more logit of each head's softmax that no
-    value belongs to.  A sequence of length 0 gives zeros.
+    those wholly before the window, are not read); seq_lens [B] int32, the new token's own key included if it is to be
+    seen.  scale defaults to head_dim ** -0.5; window > 0 lets a token see its last `window` keys only; sinks [Hq] is one
+    more logit of each head's softmax that no value belongs to.  A sequence of length 0 gives zeros.
 
     Returns BF16 [B, Hq, head_dim]; with return_lse=True also fp32 [B, Hq], the natural logarithm of the softmax's
     denominator (-inf where there was nothing), by which results over parts of a context can be joined.
@@ -336,7 +340,7 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         if sinks.numel() != hq or sinks.device != dev:
             raise ValueError(f"sinks must have {hq} elements on {dev}")
         sinks = sinks.to(torch.float32).contiguous()
-    out = q.new_empty((b, hq, d))
+    out = _like(q)
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     if b:
         need = cache._attention_bytes.get(hq)

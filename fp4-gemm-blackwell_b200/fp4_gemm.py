@@ -579,7 +579,8 @@ def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
     k, n = cache.K_orig, cache.N_orig
     if x.shape[-1] != k:
         raise ValueError(f"Input K={x.shape[-1]} doesn't match weight K={k}")
-    assert x.is_cuda and cache.device.index in (None, x.device.index), "x must be on the cache's CUDA device"
+    index = x.get_device()  # the host's time counts here: no objects that are not needed
+    assert x.is_cuda and cache.device.index in (None, index), "x must be on the cache's CUDA device"
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
     if x.is_contiguous():
@@ -587,7 +588,7 @@ def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
     else:
         x_2d, ldx = _rows_view(x.reshape(-1, k))
         m = x_2d.shape[0]
-    y = x.new_empty(x.shape[:-1] + (n,))
+    y = x.new_empty(m, n) if x.dim() == 2 else x.new_empty(x.shape[:-1] + (n,))
     bias = cache.bias
     fuse_bias = bias is not None and bias.dtype == torch.bfloat16 and bias.is_cuda
     if m > 0:
@@ -597,12 +598,11 @@ def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
                 raise ValueError(f"the cache's bias has {bias.numel()} elements, not {n}")
             bias = bias if bias.is_contiguous() else bias.contiguous()
             b_ptr = bias.data_ptr()
-        index = x.device.index
         need = _lib.fp4b_gemv_workspace(m, k, n)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         args = (x_2d.data_ptr(), m, k, ldx, cache._handle, n, y.data_ptr(), n, b_ptr, ws.data_ptr() if need else None, need,
                 torch._C._cuda_getCurrentRawStream(index))
-        if index == torch._C._cuda_getDevice():  # without the objects of torch.cuda: the host's time counts here
+        if index == torch._C._cuda_getDevice():
             rc = _lib.fp4b_gemv_cached(*args)
         else:
             with torch.cuda.device(index):
