@@ -23,10 +23,8 @@
 // Measured on B200 (copy bandwidth 6.54 TB/s): norm and rotation of 8192 x 72
 // heads x 64 30.1 us = 5.1 TB/s, bound by instruction issue and by DRAM's mix of
 // reads and writes alike; 4099 tokens x 8 heads x 128 of K and V to nvfp4 and read
-// back 16.4 us = 2.6 TB/s, two short launches; 131072 slots x 8 heads x 64 of
-// nvfp4 read back 70 us = 4.9 TB/s, bound by DRAM writes (4/5 of its bytes).
-// Reading with a grid that stays on the GPU (3 to 100 CTAs an SM, slots read
-// ahead) took 69 to 89 us, in an order of four slots a piece 84.
+// back 14.7 us = 2.9 TB/s, two short launches; 131072 slots x 8 heads x 64 of nvfp4
+// read back 57.3 us = 6.0 TB/s, bound by HBM.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -543,85 +541,84 @@ struct ReadParams {
     int page_shift;
     const void* slots;
     int slot64;
-    uint32_t total;               // pieces of eight elements
+    uint32_t total;               // pieces of sixteen elements
     uint32_t div_mul, div_shift;  // division by a slot's pieces
     uint16_t *k, *v;
     int* err;
 };
 
-// Eight elements of a row as BF16.
+// Sixteen elements of a row as BF16, and their way to 32-byte aligned memory.
+struct Sixteen {
+    uint32_t w[8];
+};
 template <int KIND>
-__device__ __forceinline__ uint4 read_eight(const void* base, const void* scales, long row, int d, int e) {
+__device__ __forceinline__ Sixteen read_sixteen(const void* base, const void* scales, int row, int d, int e) {
+    Sixteen x;
+    const size_t at = (size_t)row * d + e;
     if constexpr (KIND == kKvBf16) {
-        return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + (size_t)row * d + e);
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+        const uint4 a = from[0], b = from[1];
+        x = Sixteen{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
     } else if constexpr (KIND == kKvFp8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + (size_t)row * d + e);
+        const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at);
         const float s = static_cast<const float*>(scales)[row];
-        uint32_t h[4], lo[2], hi[2];
-        decode::e4m3x4_to_f16(w.x, lo);
-        decode::e4m3x4_to_f16(w.y, hi);
-        h[0] = lo[0], h[1] = lo[1], h[2] = hi[0], h[3] = hi[1];
-        uint32_t out[4];
+        const uint32_t word[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = decode::f16x2_to_float2(h[i]);
-            out[i] = decode::pack_bf16(f.x * s, f.y * s);
+            uint32_t h[2];
+            decode::e4m3x4_to_f16(word[i], h);
+            const float2 a = decode::f16x2_to_float2(h[0]), b = decode::f16x2_to_float2(h[1]);
+            x.w[2 * i] = decode::pack_bf16(a.x * s, a.y * s);
+            x.w[2 * i + 1] = decode::pack_bf16(b.x * s, b.y * s);
         }
-        return make_uint4(out[0], out[1], out[2], out[3]);
     } else {
         // code times scale is exact in FP16 (6 significant bits, 2^-10 to 2880), and in BF16
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + (size_t)row * (d >> 1) + (e >> 1));
-        const uint32_t byte = static_cast<const uint8_t*>(scales)[(size_t)row * (d >> 4) + (e >> 4)];
+        const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + (at >> 1));
+        const uint32_t byte = static_cast<const uint8_t*>(scales)[at >> 4];
         const uint32_t s = decode::mul_f16x2(decode::ue4m3x2_to_f16(byte * 0x10001u), 0x5C005C00u);  // times 256
-        uint32_t h[4], out[4];
-        decode::e2m1x8_to_f16(w, h);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = decode::f16x2_to_float2(decode::mul_f16x2(h[i], s));
-            out[i] = decode::pack_bf16(f.x, f.y);
+        for (int half = 0; half < 2; ++half) {
+            uint32_t h[4];
+            decode::e2m1x8_to_f16(half ? c.y : c.x, h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = decode::f16x2_to_float2(decode::mul_f16x2(h[i], s));
+                x.w[4 * half + i] = decode::pack_bf16(f.x, f.y);
+            }
         }
-        return make_uint4(out[0], out[1], out[2], out[3]);
     }
+    return x;
+}
+__device__ __forceinline__ void store_sixteen(uint16_t* to, const Sixteen& x) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(x.w[0]), "r"(x.w[1]), "r"(x.w[2]), "r"(x.w[3]),
+                 "r"(x.w[4]), "r"(x.w[5]), "r"(x.w[6]), "r"(x.w[7])
+                 : "memory");
 }
 
-// One thread takes kBatch pieces of eight elements (16 bytes of K and of V), 32
-// apart, all its reads ahead of its writes.
+// A thread takes one piece of sixteen elements, 32 bytes of K and of V written by one
+// instruction each: 131072 slots x 8 heads x 64 of nvfp4 57.3 us (70.0 with two pieces
+// of eight for one of these, four of them a thread; 61.5 and 66.2 with two and four
+// of sixteen: what counts is many short threads and wide stores).
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadParams p) {
     decode::chain();
-    const int d = p.cache.head_dim, heads = p.cache.kv_heads, per_shift = d == 64 ? 3 : d == 128 ? 4 : 5;
+    const int d = p.cache.head_dim, heads = p.cache.kv_heads, per_shift = d == 64 ? 2 : d == 128 ? 3 : 4;
+    const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
+    if (at >= p.total) return;
     const uint32_t pieces = (uint32_t)heads << per_shift;
-    const uint32_t first = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * (32u * kBatch) + (threadIdx.x & 31);
-    long slot[kBatch];
-    uint32_t in_slot[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-        const uint32_t at = first + 32 * i, slot_at = (__umulhi(at, p.div_mul) + at) >> p.div_shift;  // at / pieces
-        in_slot[i] = at - slot_at * pieces;
-        slot[i] = at < p.total ? decode::load_index(p.slots, slot_at, p.slot64) : -1;
+    const uint32_t slot_at = (__umulhi(at, p.div_mul) + at) >> p.div_shift;  // at / pieces
+    const int in_slot = (int)(at - slot_at * pieces), h = in_slot >> per_shift, e = (in_slot - (h << per_shift)) * 16;
+    const long slot = decode::load_index(p.slots, slot_at, p.slot64), page = slot >> p.page_shift;
+    Sixteen k{}, v{};
+    if (slot >= 0 && page < p.cache.num_pages) {
+        const int row = ((int)page * heads + h) * p.cache.page_size + ((int)slot & (p.cache.page_size - 1));
+        k = read_sixteen<KIND>(p.cache.k, p.cache.k_scale, row, d, e);
+        v = read_sixteen<KIND>(p.cache.v, p.cache.v_scale, row, d, e);
+    } else if (slot >= 0) {
+        decode::report(p.err, kErrSlotRange);
     }
-    uint4 k[kBatch], v[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-        k[i] = v[i] = make_uint4(0, 0, 0, 0);
-        const long page = slot[i] >> p.page_shift;
-        if (slot[i] >= 0 && page < p.cache.num_pages) {
-            const int h = in_slot[i] >> per_shift, e = (in_slot[i] - (h << per_shift)) * 8;
-            const int row = ((int)page * heads + h) * p.cache.page_size + ((int)slot[i] & (p.cache.page_size - 1));
-            k[i] = read_eight<KIND>(p.cache.k, p.cache.k_scale, row, d, e);
-            v[i] = read_eight<KIND>(p.cache.v, p.cache.v_scale, row, d, e);
-        } else if (slot[i] >= 0) {
-            decode::report(p.err, kErrSlotRange);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-        const uint32_t at = first + 32 * i;
-        if (at < p.total) {
-            reinterpret_cast<uint4*>(p.k)[at] = k[i];
-            reinterpret_cast<uint4*>(p.v)[at] = v[i];
-        }
-    }
+    store_sixteen(p.k + (size_t)at * 16, k);
+    store_sixteen(p.v + (size_t)at * 16, v);
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -748,13 +745,13 @@ FP4B_EXPORT int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int 
     const char* why = kv_cache_check(cache);
     if (!why && cache->kv_heads > 0x7fff0000 / (cache->head_dim / 8)) why = "too many heads";
     if (!why && (count < 0 || (count > 0 && (!slots || !k_out || !v_out)))) why = "null slots or outputs";
-    if (!why && (!aligned(k_out, 16) || !aligned(v_out, 16))) why = "outputs must be 16-byte aligned";
+    if (!why && (!aligned(k_out, 32) || !aligned(v_out, 32))) why = "outputs must be 32-byte aligned";
     if (why) {
         set_last_error("fp4b_kv_read: %s", why);
         return -1;
     }
     if (count == 0) return 0;
-    const int pieces = cache->kv_heads * (cache->head_dim / 8);
+    const int pieces = cache->kv_heads * (cache->head_dim / 16);
     ReadParams p{};
     p.cache = *cache;
     p.page_shift = shift_of(cache->page_size);
@@ -771,9 +768,9 @@ FP4B_EXPORT int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int 
         const long n = std::min(most, count - at);
         p.total = (uint32_t)(n * pieces);
         p.slots = static_cast<const uint8_t*>(slots) + at * (slot64 ? 8 : 4);
-        p.k = static_cast<uint16_t*>(k_out) + at * pieces * 8;
-        p.v = static_cast<uint16_t*>(v_out) + at * pieces * 8;
-        const unsigned blocks = (p.total + kThreads * kBatch - 1) / (kThreads * kBatch);
+        p.k = static_cast<uint16_t*>(k_out) + at * pieces * 16;
+        p.v = static_cast<uint16_t*>(v_out) + at * pieces * 16;
+        const unsigned blocks = (p.total + kThreads - 1) / kThreads;
         e = decode::launch_chained(kernel, dim3(blocks), kThreads, 0, static_cast<cudaStream_t>(stream), p);
     }
     return launch_status(e, "fp4b_kv_read");

@@ -328,8 +328,8 @@ typedef struct fp4b_rows {
 } fp4b_rows;
 int fp4b_kv_rows(const fp4b_rows* rows, void* stream);
 
-/* Keys and values of `count` slots as BF16 [count, kv_heads, head_dim] each;
- * zeros for a negative slot. */
+/* Keys and values of `count` slots as BF16 [count, kv_heads, head_dim] each
+ * (32-byte aligned); zeros for a negative slot. */
 int fp4b_kv_read(const fp4b_kv_cache* cache, const void* slots, int slot64, long count, void* k_out, void* v_out,
                  void* stream);
 
