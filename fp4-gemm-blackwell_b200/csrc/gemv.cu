@@ -36,8 +36,8 @@
 //
 // Measured on B200 (copy bandwidth 6.54 TB/s): one row, 28672 x 8192 28.8 us = 4.6
 // TB/s; 16 rows, 16384 x 16384 39.4 us = 3.9 TB/s, where the copies alone take 30
-// and the products alone 31: matrix instructions, shared-memory reads of x and the
-// decoding share four warps a scheduler.  5 rows, 15360 x 2880 9.9 us; one row, 2880 x
+// and the products alone 31: beside mma.sync the decoding's instructions cost a
+// scheduler nearly their own time more.  5 rows, 15360 x 2880 9.9 us; one row, 2880 x
 // 2880 4.5 us, a launch and one chain of waits.
 #include <cuda_runtime.h>
 
