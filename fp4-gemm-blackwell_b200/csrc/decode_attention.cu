@@ -19,13 +19,18 @@
 // element, are byte permutes of two rows' words.  P^T comes from S^T's
 // accumulators by movmatrix.
 //
-// Formats.  bf16 multiplies in BF16, with p split in two BF16 terms (one would
-// round p to 8 bits, as large an error as the output's own rounding).  fp8 and
-// nvfp4 multiply in FP16, which holds their codes exactly (e2m1 * ue4m3 has 6
-// significant bits; the scale enters as 2^-8 of its value, a shift of its
-// byte), q times the power of two that puts its largest element into
-// [2^14, 2^15), and p rounded to 11 bits.  An fp8 row's scale multiplies the
-// score of its key and the weight of its value.
+// Formats.  bf16 multiplies in BF16.  fp8 and nvfp4 multiply in FP16, which
+// holds their codes exactly (e2m1 * ue4m3 has 6 significant bits; the scale
+// enters as 2^-8 of its value, a shift of its byte), and q times the power of
+// two that puts its largest element into [2^14, 2^15).  An fp8 row's scale
+// multiplies the score of its key and the weight of its value.  p enters as two
+// terms, its rounding and what that left: 16 bits in BF16, 22 in FP16 (less
+// below 2^-3, to within 2^-25; the largest weight is 2^4 or more, see below).  One
+// term would be 8 bits in BF16, as large an error as the output's own rounding,
+// and 11 in FP16: outputs would lie 6.5e-4 of their size from those of 32-bit
+// weights, with two they lie 1e-4 or less, and values of either sign that nearly
+// cancel would leave no right digit.  The second term costs nvfp4 13 % (3 x 131072
+// keys, D = 64: 52.0 us without it), fp8 1 % (47.6).
 //
 // Softmax.  In base 2 with a reference exponent per head instead of the exact
 // maximum: it moves (to the maximum less 4) only when a score passes it by
@@ -48,12 +53,12 @@
 // in rounds with these added to each unit.
 //
 // Measured on B200 (copy bandwidth 6.54 TB/s): nvfp4, 3 x 131072 keys x 8 heads x 64
-// under 64 query heads 51.5 us = 4.4 TB/s, bound by instruction issue (314
-// instructions for 32 keys, decoding the codes half of them; 50 us were left of
-// 58.6 with all reads left out); fp8, 33 sequences up to 8000 x 8 x 128 under 32 heads
-// 47.5 us = 5.4 TB/s and bf16, 8 up to 4095 x 16 x 256 under 16 heads 49 us = 5.6 TB/s,
-// bound by HBM behind about 7 us of start, first bytes and joining; one sequence of
-// 77 keys 4.7 us, a launch and a chain of waits.
+// under 64 query heads 58.8 us = 3.9 TB/s, bound by its instructions (24 matrix
+// instructions for 32 keys, 8 cycles of a scheduler each, and beside them the
+// decoding and scaling of the codes, whose cycles come on top); fp8, 33 sequences up
+// to 8000 x 8 x 128 under 32 heads 48.0 us = 5.3 TB/s and bf16, 8 up to 4095 x 16 x 256
+// under 16 heads 49 us = 5.6 TB/s, bound by HBM behind about 7 us of start, first bytes
+// and joining; one sequence of 77 keys 4.7 us, a launch and a chain of waits.
 //
 // A warp streams its steps through a ring of its own in shared memory with
 // cp.async: no barrier in the loop.  Masked keys are zero-filled, not read.
@@ -716,14 +721,18 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
                                 // a masked key's zero-filled scale keeps its weight zero
                                 w[0] *= va[kt], w[1] *= va[kt], w[2] *= vb[kt], w[3] *= vb[kt];
                             }
+                            // (pf: the weights rounded, pl: what that left of them)
                             if constexpr (kBf16) {
                                 const uint32_t hi0 = pack_bf16(w[0], w[1]), hi1 = pack_bf16(w[2], w[3]);
                                 pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
                                 pl[nt][kt][0] = transpose8x8(pack_bf16(w[0] - bf16_lo(hi0), w[1] - bf16_hi(hi0)));
                                 pl[nt][kt][1] = transpose8x8(pack_bf16(w[2] - bf16_lo(hi1), w[3] - bf16_hi(hi1)));
                             } else {
-                                pf[nt][kt][0] = transpose8x8(pack_f16(w[0], w[1]));
-                                pf[nt][kt][1] = transpose8x8(pack_f16(w[2], w[3]));
+                                const uint32_t hi0 = pack_f16(w[0], w[1]), hi1 = pack_f16(w[2], w[3]);
+                                const float2 back0 = f16x2_to_float2(hi0), back1 = f16x2_to_float2(hi1);
+                                pf[nt][kt][0] = transpose8x8(hi0), pf[nt][kt][1] = transpose8x8(hi1);
+                                pl[nt][kt][0] = transpose8x8(pack_f16(w[0] - back0.x, w[1] - back0.y));
+                                pl[nt][kt][1] = transpose8x8(pack_f16(w[2] - back1.x, w[3] - back1.y));
                             }
                         }
 
@@ -794,8 +803,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
                                     mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pf[nt][kt][0], pf[nt][kt][1]);
-                                    if constexpr (kBf16)
-                                        mma<true>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
+                                    mma<kBf16>(acc[nt][m], h[e][0][0], h[e][0][1], h[e][1][0], h[e][1][1], pl[nt][kt][0], pl[nt][kt][1]);
                                 }
                             }
                         }

@@ -316,7 +316,8 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     page_table [B, W] int32, its first ceil(len / page_size) entries the sequence's pages in order (the others, and
     those wholly before the window, are not read); seq_lens [B] int32, the new token's own key included if it is to be
     seen.  scale defaults to head_dim ** -0.5; window > 0 lets a token see its last `window` keys only; sinks [Hq] is one
-    more logit of each head's softmax that no value belongs to.  A sequence of length 0 gives zeros.
+    more logit of each head's softmax that no value belongs to.  A sequence of length 0 gives zeros.  Sums and statistics
+    are fp32; the softmax's weights enter their products with 22 bits over an fp8 or nvfp4 cache, 16 over a BF16 one.
 
     Returns BF16 [B, Hq, head_dim]; with return_lse=True also fp32 [B, Hq], the natural logarithm of the softmax's
     denominator (-inf where there was nothing), by which results over parts of a context can be joined.

@@ -1,0 +1,46 @@
+"""The decode-side operators on a B200 where they can go wrong unseen: slices that just fit, tensors that share or skew their
+memory, weights that nearly cancel.  Against the 64-bit restatements of tests/decode_reference.py, with the tolerances of
+tests/test_gpu_decode.py or ones derived beside the test."""
+import pytest
+import torch
+
+from tests import decode_reference as R
+from tests.test_gpu_decode import KINDS
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dec(cuda):
+    import fp4_decode
+    return fp4_decode
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hk", [(8, 2), (16, 1)])
+def test_attention_of_values_that_nearly_cancel(dec, cuda, kind, d, hq, hk):
+    # Values of +-t in turn under scores within about 2^-6 of each other: the output is a sum of differences of nearly equal
+    # weights, and shows how many bits those hold.  Beside its rounding to BF16 it may be off by 2^-24 of sum(p |v|) for each
+    # of the n terms of the sums in fp32 and 64 times that for the rest: the scores (D * 2^-24 of sum |q k| scale < 2^-4, and
+    # their factors), the exponential (2^-22), the weights (22 bits for fp8 and nvfp4; 16 for bf16, that is 2^-16 more),
+    # value scales, joining and division.
+    lens, page = [2, 16, 34, 60], 16
+    g = torch.Generator().manual_seed(d + hq)
+    n = 64
+    cache = dec.PagedKVCache(len(lens) * n // page, page, hk, d, kind, device=cuda)
+    k = torch.randn(len(lens) * n, hk, d, generator=g)
+    sign = torch.tensor([1.0, -1.0]).repeat(len(lens) * n // 2).reshape(-1, 1, 1)
+    v = sign * (torch.randint(0, 2, (hk, d), generator=g) * 2.0 - 1.0)
+    cache.append(k.to(torch.bfloat16).to(cuda), v.to(torch.bfloat16).to(cuda), torch.arange(len(lens) * n, device=cuda))
+    q = torch.randn(len(lens), hq, d, generator=g).to(torch.bfloat16).to(cuda)
+    table = torch.arange(len(lens) * n // page, dtype=torch.int32, device=cuda).reshape(len(lens), -1)
+    seq = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    scale = 2.0 ** -8 * d ** -0.5
+    out = dec.decode_attention(q, cache, table, seq, scale=scale)
+    rows = [R.cache_values(p, s, kind) for p, s in ((cache.k_pages, cache.k_scales), (cache.v_pages, cache.v_scales))]
+    want, _, mag = R.attention(q, *rows, table, seq, page, scale, 0, None)
+    terms = (seq.double().reshape(-1, 1, 1) + 64) * 2.0 ** -24 + (2.0 ** -16 if kind == "bf16" else 0.0)
+    err = (out.double() - want).abs()
+    bad = err > 2.0 ** -8 * want.abs() + terms * mag
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {(err / mag)[bad].max().item()} of the terms"
