@@ -445,7 +445,12 @@ struct Cut {
     int slices, ctas;
 };
 Cut cut_of(int m, int n, int k) {
-    const int all = (k + kStep - 1) / kStep, groups = (n + 127) / 128 * 4, step_bytes = std::min(m, tile_rows(m)) * 2 * kStep;
+    const int all = (k - 1) / kStep + 1, groups = ((n - 1) / 128 + 1) * 4, step_bytes = std::min(m, tile_rows(m)) * 2 * kStep;
+    // Slices are whole steps and differ by one: the longest fits where there are as many
+    // slices as it takes of the whole steps that fit (by bytes it would not: 9 rows x 113
+    // steps are 4 times 65536 bytes nearly, but one of 4 slices has 29 steps, 66816).
+    const int walk_fit = kWalkBytes / step_bytes, slice_fit = kSliceBytes / step_bytes;
+    auto slices_of = [&](int most_steps) { return (all - 1) / most_steps + 1; };
     Cut c{};
     // Walked where slices of a few steps give (nearly) every warp of a full GPU a
     // group: rows x 28672 x 8192 28.8 us walked and 34.4 not with one row of x, 37.7 and
@@ -455,8 +460,8 @@ Cut cut_of(int m, int n, int k) {
     // the one that lets a CTA's warps end together: the rounds of its groups times the
     // steps of each, and a third of a step for a slice's sums (16 rows, 16384 x 16384:
     // 8 slices 42.0 us, 9 39.4, 18 43.9).
-    const int shortest = all * step_bytes > kSliceBytes ? kWalkSteps : 8;
-    const int from = std::max((all * step_bytes + kWalkBytes - 1) / kWalkBytes, (148 * kWalkWarps * 3 / 4 + groups - 1) / groups);
+    const int shortest = all > slice_fit ? kWalkSteps : 8;
+    const int from = std::max(slices_of(walk_fit), (148 * kWalkWarps * 3 / 4 - 1) / groups + 1);
     int least = 0;
     for (int slices = from; slices <= std::min(148, 2 * from) && all / slices >= shortest; ++slices) {
         const int ctas = std::max(1, std::min(148 / slices, groups)), share = (groups + ctas - 1) / ctas;
@@ -468,19 +473,22 @@ Cut cut_of(int m, int n, int k) {
     // CTAs an SM; then 32, 64 or 128 rows of the weight a CTA, as many as leave about
     // a CTA for each SM (15360 rows x 2880, 5 rows of x: 17.1 / 12.6 / 10.7 us; 2880
     // rows, one row of x: 4.4 / 5.9 / 8.7 us).
-    const int fit = (all + kSliceBytes / step_bytes - 1) / (kSliceBytes / step_bytes);
-    c.slices = std::max({1, fit, std::min(296 / groups, all / 16)});
+    c.slices = std::max(slices_of(slice_fit), std::min(296 / groups, all / 16));
     c.rows_per_cta = groups * c.slices < 296 ? 32 : groups * c.slices < 480 ? 64 : 128;
     return c;
 }
 static_assert(kWalkSteps > kStages, "a walk's stream runs into one further group at most");
 
-int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * x_row_bytes(p.slice_steps + (p.slice_more > 0 ? 1 : 0)); }
+int longest_slice(const GemvParams& p) { return p.slice_steps + (p.slice_more > 0 ? 1 : 0); }
+int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * x_row_bytes(longest_slice(p)); }
+// A slice of `bytes` at most: what convert_x's threads hold and x_room has room for.
+bool slice_fits(const GemvParams& p, int bytes) { return (long)std::min(p.m, tile_rows(p.m)) * longest_slice(p) * 2 * kStep <= bytes; }
 
 template <int NT, int RG, int W>
 cudaError_t launch(const GemvParams& p, cudaStream_t st) {
     constexpr int kRing = W * kStages * kStageBytes;
     static bool ready[kMaxDevices];
+    if (!slice_fits(p, kSliceBytes)) return cudaErrorInvalidConfiguration;
     if (const cudaError_t e = allow_smem(gemv_kernel<NT, RG, W>, kRing + x_room(kSliceBytes), ready)) return e;
     const long blocks = ((long)p.n + 127) / 128 * (4 / RG);
     const dim3 grid((unsigned)blocks, (unsigned)((p.m + 8 * NT - 1) / (8 * NT)), (unsigned)p.slices);
@@ -491,6 +499,7 @@ template <int NT>
 cudaError_t launch_walk(const GemvParams& p, cudaStream_t st) {
     constexpr int kRing = kWalkWarps * kStages * kStageBytes;
     static bool ready[kMaxDevices];
+    if (!slice_fits(p, kWalkBytes)) return cudaErrorInvalidConfiguration;
     if (const cudaError_t e = allow_smem(gemv_walk_kernel<NT>, kRing + x_room(kWalkBytes), ready)) return e;
     const dim3 grid((unsigned)(p.slices * p.ctas), (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
     return launch_chained(gemv_walk_kernel<NT>, grid, 32 * kWalkWarps, kRing + x_bytes(p), st, p);
@@ -547,10 +556,10 @@ FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const
     p.x_vec = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     p.alpha = c.w_alpha * kScaleUnit;
     const Cut cut = cut_of(m, n_out, k_in);
-    const int all = (k_in + kStep - 1) / kStep;
+    const int all = (k_in - 1) / kStep + 1;
     p.slices = cut.slices, p.slice_steps = all / cut.slices, p.slice_more = all % cut.slices, p.ctas = cut.ctas;
     p.sums = static_cast<float*>(workspace);
-    p.n_pad = (n_out + 127) / 128 * 128;
+    p.n_pad = ((n_out - 1) / 128 + 1) * 128;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launch_status(tile_rows(m) == 8 ? launch_all<1>(p, cut, st) : launch_all<2>(p, cut, st), "fp4b_gemv_cached");
 }

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import decode_reference as R
-from tests.test_gpu_decode import KINDS
+from tests.test_gpu_decode import KINDS, close, weight_values
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,20 @@ def test_attention_of_values_that_nearly_cancel(dec, cuda, kind, d, hq, hk):
     err = (out.double() - want).abs()
     bad = err > 2.0 ** -8 * want.abs() + terms * mag
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {(err / mag)[bad].max().item()} of the terms"
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 20480, 32768), (5, 12800, 32768), (6, 19072, 16384), (7, 28672, 9344), (9, 15360, 14464), (9, 16384, 14400),
+                                   (10, 14336, 16384), (12, 12288, 16384), (13, 12416, 12288), (13, 14336, 12288), (14, 10240, 16384),
+                                   (11, 15360, 11904), (25, 12288, 16384)])
+def test_gemv_where_a_slice_only_just_fits(cuda, fp4, m, n, k):
+    # rows whose bytes a step do not divide what a CTA holds of x: the longest slice has to fit, its last row to its end
+    g = torch.Generator(cuda).manual_seed(m + k)
+    w = torch.randn(n, k, generator=g, device=cuda, dtype=torch.bfloat16) * 0.02
+    x = torch.randn(m, k, generator=g, device=cuda, dtype=torch.bfloat16)
+    cache = fp4.FP4WeightCache(w, global_scale=True)
+    del w
+    y = fp4.fp4_cached_gemv(x, cache)
+    assert torch.equal(y, fp4.fp4_cached_gemv(x, cache)), "not the same twice"
+    wv = weight_values(cache)
+    close(y, x.double() @ wv.T, x.double().abs() @ wv.abs_().T, 64, f"gemv {m}x{n}x{k}")
+    cache.free()
