@@ -88,6 +88,15 @@ def _indices(t: torch.Tensor, count: int, what: str, device) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _table(t: torch.Tensor):
+    """(t, distance of its rows) of a page table [B, W] as the kernel goes over it, entry i of row b at b * distance + i: copied
+    where its rows are not of unit stride, are one row for all (expand) or overlap.  A single row's distance is its length."""
+    b, width = t.shape
+    if (width > 1 and t.stride(1) != 1) or (b > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t, t.stride(0) if b > 1 else width
+
+
 def _weight(w, d: int, what: str, device):
     if w is None:
         return None
@@ -333,8 +342,7 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
         raise ValueError(f"seq_lens must be int32 [{b}] on {dev}")
     if window < 0:
         raise ValueError("window must not be negative")
-    if page_table.stride(1) != 1:
-        page_table = page_table.contiguous()
+    page_table, table_stride = _table(page_table)
     if seq_lens.stride(0) != 1:
         seq_lens = seq_lens.contiguous()
     if sinks is not None:
@@ -349,9 +357,9 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
             with torch.cuda.device(dev):
                 need = cache._attention_bytes[hq] = _lib.fp4b_decode_attention_workspace(hq, cache.kv_heads, d)
         ws = _workspace(dev, need)
-        qs, width = q.stride(), page_table.shape[1]
+        qs = q.stride()
         _call(dev, _attention, "decode_attention", _DECODE.pack(
-            q.data_ptr(), qs[0], qs[1], cache._ref, page_table.data_ptr(), max(page_table.stride(0), width), seq_lens.data_ptr(),
-            _address(sinks), out.data_ptr(), _address(lse), ws.data_ptr(), ws.numel(), b, hq, width, window,
+            q.data_ptr(), qs[0], qs[1], cache._ref, page_table.data_ptr(), table_stride, seq_lens.data_ptr(),
+            _address(sinks), out.data_ptr(), _address(lse), ws.data_ptr(), ws.numel(), b, hq, page_table.shape[1], window,
             d ** -0.5 if scale is None else scale))
     return (out, lse) if return_lse else out

@@ -1,6 +1,8 @@
 """Host side of the decode operators where shapes only just fit (no GPU)."""
 import pytest
+import torch
 
+import fp4_decode
 import fp4_gemm
 
 lib = fp4_gemm._lib
@@ -41,3 +43,23 @@ def test_slices_of_a_very_long_row():
     # K * rows passes 32 bits in bytes
     for k in (1 << 26, (1 << 26) + 128, 100_000_000):
         assert -(-(-(-k // STEP)) // slices_of(16, 128, k)) * 16 * STEP * 2 <= HELD
+
+
+def test_page_tables_of_any_strides():
+    # entry i of row b is read at b * distance + i from the table's address
+    base = torch.arange(60, dtype=torch.int32)
+    forms = {"plain": base.view(6, 10), "wide": base.view(6, 10)[:, :7], "part": base.view(6, 10)[1:4, 2:9], "one row": base[:9].view(1, 9),
+             "one row for all": base[:9].view(1, 9).expand(5, 9), "one entry for all": base[:1].view(1, 1).expand(5, 7),
+             "one column": base.view(6, 10)[:, 3:4], "one column for all": base[:1].view(1, 1).expand(5, 1), "turned": base.view(10, 6).t(),
+             "overlapping": base.as_strided((4, 9), (3, 1)), "every other": base.view(6, 10)[:, ::2], "every other row": base.view(6, 10)[::2],
+             "one row of a turned table": base.view(10, 6).t()[2:3], "one row, every third": base[::3].view(1, 20), "far rows": base.as_strided((1, 5), (0, 1)),
+             "no columns": base.view(6, 10)[:, :0], "no rows": base.view(6, 10)[:0]}
+    for name, table in forms.items():
+        got, distance = fp4_decode._table(table)
+        b, width = table.shape
+        assert distance >= width, name
+        flat = got.as_strided((max(0, (b - 1) * distance + width) if b and width else 0,), (1,))
+        for r in range(b):
+            assert flat[r * distance: r * distance + width].tolist() == table[r].tolist(), name
+        if name in ("plain", "wide", "part", "one row", "one column", "every other row"):
+            assert got.data_ptr() == table.data_ptr(), name  # nothing to copy

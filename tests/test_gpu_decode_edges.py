@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import decode_reference as R
-from tests.test_gpu_decode import KINDS, close, weight_values
+from tests.test_gpu_decode import KINDS, attention_case, close, weight_values
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,23 @@ def test_gemv_where_a_slice_only_just_fits(cuda, fp4, m, n, k):
     wv = weight_values(cache)
     close(y, x.double() @ wv.T, x.double().abs() @ wv.abs_().T, 64, f"gemv {m}x{n}x{k}")
     cache.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_over_page_tables_of_any_strides(dec, cuda, fp4, kind):
+    # one prefix for all sequences (rows shared by expand), rows that overlap, a column, a turned table
+    q, cache, _, _ = attention_case(dec, cuda, kind, 64, 8, 2, 16, [300] * 5, seed=3)
+    flat = torch.randperm(cache.num_pages, generator=torch.Generator().manual_seed(1)).to(torch.int32).to(cuda)
+    lens = torch.tensor([100, 3, 0, 112, 57], dtype=torch.int32, device=cuda)
+    forms = [flat[:7].view(1, 7).expand(5, 7), flat[:1].view(1, 1).expand(5, 7), flat.as_strided((5, 7), (3, 1)), flat[:70].view(7, 10)[:, :5].t(),
+             flat[:70].view(5, 14)[:, ::2], flat[:70].view(10, 7)[::2]]
+    for table in forms:
+        want = dec.decode_attention(q, cache, table.clone(memory_format=torch.contiguous_format), lens)
+        assert torch.equal(dec.decode_attention(q, cache, table, lens), want)
+    short = torch.clamp(lens, max=16)
+    for table in (flat[:50].view(5, 10)[:, 4:5], flat[:1].view(1, 1).expand(5, 1)):
+        want = dec.decode_attention(q, cache, table.clone(memory_format=torch.contiguous_format), short)
+        assert torch.equal(dec.decode_attention(q, cache, table, short), want)
+    one = flat[:21].view(7, 3).t()[1:2]
+    assert torch.equal(dec.decode_attention(q[:1], cache, one, lens[:1]), dec.decode_attention(q[:1], cache, one.clone(memory_format=torch.contiguous_format), lens[:1]))
+    assert fp4.device_error() == 0
