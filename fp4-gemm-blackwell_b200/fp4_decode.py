@@ -74,7 +74,8 @@ def _rows(t: torch.Tensor, what: str, device=None) -> torch.Tensor:
         t = t.to(torch.bfloat16)
     st, sh, se = t.stride()
     if se != 1 or (st | sh) & 3 or t.data_ptr() & 7:
-        t = t.contiguous()
+        # a new tensor always: contiguous() keeps one that starts anywhere, and the strides of dimensions of size one
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 

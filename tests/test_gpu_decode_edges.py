@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import decode_reference as R
-from tests.test_gpu_decode import KINDS, attention_case, close, weight_values
+from tests.test_gpu_decode import KINDS, attention_case, close, heads, raw, weight_values
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,36 @@ def test_attention_over_page_tables_of_any_strides(dec, cuda, fp4, kind):
     one = flat[:21].view(7, 3).t()[1:2]
     assert torch.equal(dec.decode_attention(q[:1], cache, one, lens[:1]), dec.decode_attention(q[:1], cache, one.clone(memory_format=torch.contiguous_format), lens[:1]))
     assert fp4.device_error() == 0
+
+
+def skewed(x):
+    """Views of x's values that torch calls contiguous (or nearly) and whose rows start anywhere."""
+    t, h, d = x.shape
+    for at in (1, 2, 3, 5):
+        flat = torch.empty(x.numel() + at, dtype=x.dtype, device=x.device)
+        flat[at:] = x.reshape(-1)
+        yield flat[at:].view(t, h, d)
+    padded = torch.empty(t, h, d + 5, dtype=x.dtype, device=x.device)
+    for at in (0, 4, 5):
+        padded[..., at: at + d] = x
+        yield padded[..., at: at + d]
+
+
+@pytest.mark.parametrize("t,hq", [(1, 1), (1, 4), (3, 1), (5, 2)])
+def test_rows_that_start_anywhere(dec, cuda, t, hq):
+    q, k, v, (wq, wk), pos = (x.contiguous() if isinstance(x, torch.Tensor) else x for x in heads(t, hq, 1, 64, t, cuda))
+    table = dec.rope_table(500, 64, device=cuda)
+    slots = torch.arange(t, device=cuda) + 3
+    want = dec.qk_norm_rope(q, k, pos, table, wq, wk)
+    for kind in KINDS:
+        ref = dec.PagedKVCache(2, 16, 1, 64, kind, device=cuda)
+        ref.append(k, v, slots)
+        pages, lens = torch.zeros(t, 1, dtype=torch.int32, device=cuda), torch.full((t,), 3 + t, dtype=torch.int32, device=cuda)
+        seen = dec.decode_attention(q, ref, pages, lens)
+        for a, b, c in zip(skewed(q), skewed(k), skewed(v)):
+            assert all(torch.equal(x, y) for x, y in zip(dec.qk_norm_rope(a, b, pos, table, wq, wk), want))
+            cache = dec.PagedKVCache(2, 16, 1, 64, kind, device=cuda)
+            cache.append(b, c, slots)
+            assert torch.equal(raw(cache.k_pages), raw(ref.k_pages)) and torch.equal(raw(cache.v_pages), raw(ref.v_pages))
+            assert torch.equal(cache.append_qkv(a, b, c, pos, slots, table, wq, wk), want[0])
+            assert torch.equal(dec.decode_attention(a, ref, pages, lens), seen)
