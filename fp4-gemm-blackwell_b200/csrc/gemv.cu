@@ -479,6 +479,20 @@ Cut cut_of(int m, int n, int k) {
 }
 static_assert(kWalkSteps > kStages, "a walk's stream runs into one further group at most");
 
+int padded_rows(int n) { return ((n - 1) / 128 + 1) * 128; }
+
+// Rows of x of one launch; more than that take several, one after the other, with one
+// workspace.  A grid's second dimension ends at 65535 (the join's are rows), and slices'
+// sums of many rows would be gigabytes that a GPU full of tiles does not need: 256 MB of
+// them, or one tile's.
+constexpr long kMostRows = 65520, kMostSums = 256l << 20;
+int launch_rows(int m, int n, const Cut& c) {
+    const int tile = tile_rows(m);
+    long rows = kMostRows;
+    if (c.slices > 1 || c.walk) rows = std::min(rows, std::max(1l, kMostSums / ((long)c.slices * padded_rows(n) * 4 * tile)) * tile);
+    return (int)std::min<long>(m, rows);
+}
+
 int longest_slice(const GemvParams& p) { return p.slice_steps + (p.slice_more > 0 ? 1 : 0); }
 int x_bytes(const GemvParams& p) { return std::min(p.m, tile_rows(p.m)) * x_row_bytes(longest_slice(p)); }
 // A slice of `bytes` at most: what convert_x's threads hold and x_room has room for.
@@ -526,8 +540,8 @@ FP4B_EXPORT long fp4b_gemv_workspace(int m, int k_in, int n_out) {
         return -1;
     }
     const Cut c = cut_of(m, n_out, k_in);
-    const long rows = tile_rows(m);
-    return c.slices == 1 && !c.walk ? 0 : (m + rows - 1) / rows * rows * c.slices * ((n_out + 127l) / 128 * 128) * 4;
+    const long tile = tile_rows(m);
+    return c.slices == 1 && !c.walk ? 0 : (launch_rows(m, n_out, c) + tile - 1) / tile * tile * c.slices * padded_rows(n_out) * 4;
 }
 
 FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const void* handle, int n_out, void* y,
@@ -537,7 +551,7 @@ FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const
         set_last_error("null or invalid cache handle");
         return -1;
     }
-    if (!x || !y || m <= 0 || m > 65535 || k_in <= 0 || k_in > c.K || ldx < k_in || n_out <= 0 || n_out > c.N ||
+    if (!x || !y || m <= 0 || k_in <= 0 || k_in > c.K || ldx < k_in || n_out <= 0 || n_out > c.N ||
         ldy < n_out) {
         set_last_error("fp4b_gemv_cached: bad shape (m=%d k=%d n=%d vs cache %dx%d)", m, k_in, n_out, c.N, c.K);
         return -1;
@@ -548,18 +562,26 @@ FP4B_EXPORT int fp4b_gemv_cached(const void* x, int m, int k_in, long ldx, const
         return -1;
     }
     GemvParams p{};
-    p.x = static_cast<const uint16_t*>(x), p.ldx = ldx;
+    p.ldx = ldx;
     p.w = c.fp4, p.sf = c.sf, p.k_pad = c.K;
-    p.y = static_cast<uint16_t*>(y), p.ldy = ldy;
+    p.ldy = ldy;
     p.bias = static_cast<const uint16_t*>(bias);
-    p.m = m, p.n = n_out, p.k = k_in;
+    p.n = n_out, p.k = k_in;
     p.x_vec = ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     p.alpha = c.w_alpha * kScaleUnit;
     const Cut cut = cut_of(m, n_out, k_in);
     const int all = (k_in - 1) / kStep + 1;
     p.slices = cut.slices, p.slice_steps = all / cut.slices, p.slice_more = all % cut.slices, p.ctas = cut.ctas;
     p.sums = static_cast<float*>(workspace);
-    p.n_pad = ((n_out - 1) / 128 + 1) * 128;
+    p.n_pad = padded_rows(n_out);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return launch_status(tile_rows(m) == 8 ? launch_all<1>(p, cut, st) : launch_all<2>(p, cut, st), "fp4b_gemv_cached");
+    const int most = launch_rows(m, n_out, cut);
+    cudaError_t e = cudaSuccess;
+    for (long at = 0; at < m && e == cudaSuccess; at += most) {
+        p.m = (int)std::min<long>(most, m - at);
+        p.x = static_cast<const uint16_t*>(x) + at * ldx;
+        p.y = static_cast<uint16_t*>(y) + at * ldy;
+        e = tile_rows(m) == 8 ? launch_all<1>(p, cut, st) : launch_all<2>(p, cut, st);
+    }
+    return launch_status(e, "fp4b_gemv_cached");
 }

@@ -272,8 +272,9 @@ int fp4b_ipc_close(void* ptr, long offset);
  * quantized), W the cached weight and bias [n_out] BF16 or NULL; fp32 sums, one
  * rounding to BF16.  Any m >= 1; made for few rows, where the weight's bytes
  * are the cost.  workspace: fp4b_gemv_workspace bytes of device memory
- * (0 for few elements of x, then NULL), 16-byte aligned, in any state; calls
- * that share it must be ordered. */
+ * (0 for few elements of x, then NULL; 256 MB at most, or what 16 rows take:
+ * more rows go in several launches), 16-byte aligned, in any state; calls that
+ * share it must be ordered. */
 long fp4b_gemv_workspace(int m, int k_in, int n_out);
 int fp4b_gemv_cached(const void* x_bf16, int m, int k_in, long ldx, const void* cache_handle, int n_out,
                      void* y_bf16, long ldy, const void* bias_bf16, void* workspace, long workspace_bytes, void* stream);

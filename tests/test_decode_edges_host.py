@@ -63,3 +63,12 @@ def test_page_tables_of_any_strides():
             assert flat[r * distance: r * distance + width].tolist() == table[r].tolist(), name
         if name in ("plain", "wide", "part", "one row", "one column", "every other row"):
             assert got.data_ptr() == table.data_ptr(), name  # nothing to copy
+
+
+def test_workspace_of_many_rows_is_bounded():
+    for n, k in ((128, 128), (128, 4096), (2880, 2880), (16384, 16384), (160000, 65536)):
+        one = lib.fp4b_gemv_workspace(16, k, n)
+        for m in (17, 40, 1000, 8192, 65535, 65536, 1 << 20, (1 << 31) - 1):
+            need = lib.fp4b_gemv_workspace(m, k, n)
+            assert one <= need <= max(one, 256 << 20), (m, n, k, need)
+            assert one == 0 or need % one == 0  # whole tiles of 16 rows

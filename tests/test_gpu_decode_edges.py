@@ -114,3 +114,19 @@ def test_rows_that_start_anywhere(dec, cuda, t, hq):
             assert torch.equal(raw(cache.k_pages), raw(ref.k_pages)) and torch.equal(raw(cache.v_pages), raw(ref.v_pages))
             assert torch.equal(cache.append_qkv(a, b, c, pos, slots, table, wq, wk), want[0])
             assert torch.equal(dec.decode_attention(a, ref, pages, lens), seen)
+
+
+@pytest.mark.parametrize("m,n,k", [(70000, 200, 256), (70001, 120, 4100), (1000, 16384, 16384), (300, 16384, 2880)])
+def test_gemv_of_more_rows_than_a_launch(cuda, fp4, m, n, k):
+    # a row's result does not depend on the rows beside it (from a tile of 16 on): many at once equal 160 at a time
+    g = torch.Generator(cuda).manual_seed(m)
+    cache = fp4.FP4WeightCache(torch.randn(n, k, generator=g, device=cuda, dtype=torch.bfloat16) * 0.02, global_scale=True)
+    wide = torch.randn(m, k + 8, generator=g, device=cuda, dtype=torch.bfloat16)
+    x = wide[:, :k]
+    y = fp4.fp4_cached_gemv(x, cache)
+    for at in [*range(0, m, max(160, m // 8000 * 800)), m - 16, 65440, 65520]:
+        if 0 <= at < m:
+            part = x[at: at + 160] if m - at >= 16 else x[m - 16:]
+            want = fp4.fp4_cached_gemv(part, cache)
+            assert torch.equal(y[at: at + len(part)], want[-len(y[at: at + len(part)]):]), at
+    cache.free()
