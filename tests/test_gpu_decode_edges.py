@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import decode_reference as R
-from tests.test_gpu_decode import KINDS, attention_case, close, heads, raw, weight_values
+from tests.test_gpu_decode import KINDS, attention_case, close, heads, raw, stored, weight_values
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,48 @@ def test_gemv_of_more_rows_than_a_launch(cuda, fp4, m, n, k):
             want = fp4.fp4_cached_gemv(part, cache)
             assert torch.equal(y[at: at + len(part)], want[-len(y[at: at + len(part)]):]), at
     cache.free()
+
+
+def nvfp4_of_fp32(y):
+    """(codes, scale bytes) of fp32 rows y [..., D] by the codec's definition: the oracle's scale of absmax / 6, then the
+    nearest of the levels of y / scale, the lower one at a midpoint."""
+    from oracle import nvfp4_oracle as O
+    lib = O.lib()
+    b = y.reshape(-1, 16)
+    sixth = b.abs().amax(-1) / torch.full((b.shape[0],), 6.0)
+    bytes_ = torch.tensor([lib.oracle_ue4m3_encode(max(s, 2.0 ** -9)) for s in sixth.tolist()], dtype=torch.uint8)
+    x = b * (torch.ones(b.shape[0]) / torch.tensor([lib.oracle_ue4m3_decode(c) for c in bytes_.tolist()])).unsqueeze(-1)
+    code = torch.bucketize(x.abs(), torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])).to(torch.uint8) | ((x < 0).to(torch.uint8) << 3)
+    code = code.reshape(y.shape)
+    return code[..., 0::2] | (code[..., 1::2] << 4), bytes_.reshape(*y.shape[:-1], -1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("part,interleaved", [(1, False), (2, False), (1, True)])
+def test_append_qkv_stores_fp32_keys_to_the_byte(dec, cuda, kind, d, part, interleaved):
+    # A table of factors c with sines of zero makes each key x * c rounded to fp32, nothing else, and so known to the bit: with
+    # c at, just below and just above every absmax where a scale changes (6 times the midpoints of the scales, the powers of
+    # two of the subnormal ones), and anywhere between.  What the cache holds has to be its format's of that number.
+    g = torch.Generator().manual_seed(d)
+    levels = torch.tensor(R.UE4M3[1:128], dtype=torch.float64)
+    edges = torch.cat((levels, (levels[1:] + levels[:-1]) / 2)) * 6.0
+    edges = edges.float()
+    up, down = torch.full_like(edges, float("inf")), torch.zeros_like(edges)
+    c = torch.cat((edges, torch.nextafter(edges, up), torch.nextafter(edges, down), torch.exp2(torch.rand(300, generator=g) * 46 - 18)))
+    t, h, rot = len(c), 2, d // part
+    table = torch.cat((c.unsqueeze(1).expand(t, rot // 2), torch.zeros(t, rot // 2)), dim=1).contiguous()
+    k = (torch.rand(t, h, d, generator=g) * 2 - 1).to(torch.bfloat16)
+    k[..., torch.arange(0, d, 16) + torch.randint(0, 16, (d // 16,), generator=g)] = 1.0  # each block's largest
+    k[:, 1] = -k[:, 1]
+    y = k.float().clone()
+    y[..., :rot] *= c.reshape(-1, 1, 1)
+    q, v = (torch.randn(t, n, d, generator=g).to(torch.bfloat16) for n in (1, h))
+    cache = dec.PagedKVCache(-(-t // 16), 16, h, d, kind, device=cuda)
+    slots = torch.randperm(cache.num_pages * 16, generator=g)[:t]
+    cache.append_qkv(q.to(cuda), k.to(cuda), v.to(cuda), torch.arange(t, device=cuda), slots.to(cuda), table.to(cuda), interleaved=interleaved)
+    for got, scales, want in ((cache.k_pages, cache.k_scales, nvfp4_of_fp32(y) if kind == "nvfp4" else stored(y, kind)),
+                              (cache.v_pages, cache.v_scales, stored(v, kind))):
+        assert torch.equal(raw(got).cpu()[slots // 16, :, slots % 16], raw(want[0]))
+        if scales is not None:
+            assert torch.equal(scales.cpu()[slots // 16, :, slots % 16], want[1])
