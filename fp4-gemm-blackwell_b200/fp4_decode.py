@@ -21,7 +21,7 @@ import struct
 
 import torch
 
-from fp4_gemm import _bind, _f, _i, _last_error, _lib, _vp
+from fp4_gemm import _bind, _f, _i, _last_error, _lib, _on_cleanup, _vp
 
 _l = ctypes.c_long
 
@@ -315,6 +315,14 @@ def _workspace(device, need: int) -> torch.Tensor:
     if ws is None or ws.numel() < need:
         ws = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=device)
     return ws
+
+
+def _drop_workspaces(index: int) -> None:
+    for key in [key for key in _WORKSPACES if key[0] == index]:
+        del _WORKSPACES[key]  # back to the allocator, which hands it out in the order of its stream
+
+
+_on_cleanup.append(_drop_workspaces)
 
 
 def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_lens: torch.Tensor, scale: float = None,

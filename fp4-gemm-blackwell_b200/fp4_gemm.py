@@ -247,9 +247,15 @@ def prealloc(max_M: int, max_N: int, max_K: int):
         raise RuntimeError(f"fp4_gemm_prealloc failed with code {rc}")
 
 
+_on_cleanup = []  # called with a device index: modules beside this one drop their own scratch of that device
+
+
 def cleanup():
     """Free the scratch buffers the library holds on the current device."""
     _lib.fp4_gemm_cleanup()
+    if torch.cuda.is_initialized():
+        for drop in _on_cleanup:
+            drop(torch.cuda.current_device())
 
 
 class FP4WeightCache:

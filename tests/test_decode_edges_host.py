@@ -72,3 +72,9 @@ def test_workspace_of_many_rows_is_bounded():
             need = lib.fp4b_gemv_workspace(m, k, n)
             assert one <= need <= max(one, 256 << 20), (m, n, k, need)
             assert one == 0 or need % one == 0  # whole tiles of 16 rows
+
+
+def test_cleanup_without_a_gpu():
+    if not torch.cuda.is_initialized():
+        fp4_gemm.cleanup()
+        assert not torch.cuda.is_initialized()

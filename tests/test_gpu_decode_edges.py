@@ -175,3 +175,12 @@ def test_append_qkv_stores_fp32_keys_to_the_byte(dec, cuda, kind, d, part, inter
         assert torch.equal(raw(got).cpu()[slots // 16, :, slots % 16], raw(want[0]))
         if scales is not None:
             assert torch.equal(scales.cpu()[slots // 16, :, slots % 16], want[1])
+
+
+def test_cleanup_frees_the_attention_workspaces(dec, cuda, fp4):
+    case = attention_case(dec, cuda, "nvfp4", 64, 8, 2, 16, [600, 50], seed=6)
+    want = dec.decode_attention(*case)
+    assert any(key[0] == cuda.index for key in dec._WORKSPACES)
+    fp4.cleanup()
+    assert not any(key[0] == cuda.index for key in dec._WORKSPACES)
+    assert torch.equal(dec.decode_attention(*case), want)
