@@ -90,7 +90,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCtasPerSm = 4;
 constexpr int kSegmentRounds = 3;  // of CK keys a warp, as kWholeRounds
 constexpr int kWholeRounds = 8;
-constexpr float kNoScore = -1e30f;    // reference exponent before any key
+constexpr float kNoScore = -3.402823466e38f;  // reference exponent before any key: any finite score passes it
 constexpr float kHeadroom = 10.0f;    // a score may pass the reference by 2^10 ...
 constexpr float kBelowMax = 4.0f;     // ... which is set 2^4 below the maximum
 constexpr float kLog2e = 1.4426950408889634f;

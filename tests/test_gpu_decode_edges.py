@@ -184,3 +184,26 @@ def test_cleanup_frees_the_attention_workspaces(dec, cuda, fp4):
     fp4.cleanup()
     assert not any(key[0] == cuda.index for key in dec._WORKSPACES)
     assert torch.equal(dec.decode_attention(*case), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("factor", [-(2.0 ** 80), -(2.0 ** 100), -(2.0 ** 116), 2.0 ** 116])
+def test_attention_of_scores_of_any_size(dec, cuda, kind, factor):
+    # Scores all of one sign and of any finite size, further apart than fp32 can blur: each head sees its largest alone.
+    n, d = 90, 64
+    cache = dec.PagedKVCache(6, 16, 1, d, kind, device=cuda)
+    g = torch.Generator().manual_seed(3)
+    order = torch.randperm(n, generator=g)
+    k = torch.exp2(order.float() / n * 5).reshape(n, 1, 1).expand(n, 1, d)  # each row its one number, apart by 4 %
+    k = k * torch.where(torch.arange(d) < 16, 1.0, 2.0 ** -6)  # (its first block, in nvfp4 a few of them alike)
+    v = torch.randn(n, 1, d, generator=g)
+    cache.append(k.to(torch.bfloat16).to(cuda), v.to(torch.bfloat16).to(cuda), torch.arange(n, device=cuda))
+    q = torch.full((1, 4, d), factor).to(torch.bfloat16).to(cuda)
+    table, lens = torch.arange(6, dtype=torch.int32, device=cuda).reshape(1, 6), torch.tensor([n], dtype=torch.int32, device=cuda)
+    out, lse = dec.decode_attention(q, cache, table, lens, return_lse=True)
+    keys, values = (R.cache_values(p, s, kind).permute(0, 2, 1, 3).reshape(-1, d)[:n] for p, s in ((cache.k_pages, cache.k_scales), (cache.v_pages, cache.v_scales)))
+    s = keys.sum(-1) * q[0, 0, 0].double() * d ** -0.5
+    top = s == s.max()
+    want = values[top].mean(0)
+    assert torch.isfinite(lse).all() and ((lse.double() - s.max()).abs() <= 2.0 ** -18 * s.abs().max()).all()
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * values[top].abs().mean(0)).all()
