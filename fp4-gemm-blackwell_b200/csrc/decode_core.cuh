@@ -134,9 +134,6 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t v) {
     return v;
 }
 
-// UE4M3 byte -> fp32; the fp16 form is exact too (at most 480, at least 2^-9).
-__device__ __forceinline__ float ue4m3_float(uint32_t byte) { return ue4m3_decode((uint8_t)byte); }
-
 // Index `i` of an int32 or int64 array.
 __device__ __forceinline__ long load_index(const void* p, long i, int is64) {
     return is64 ? (long)static_cast<const int64_t*>(p)[i] : (long)static_cast<const int32_t*>(p)[i];
