@@ -5,8 +5,9 @@
 //   l = sum_i p_i (+ exp(sink_h - m))
 //
 // over the keys i of [max(0, len - window), len).  Every cached byte is read
-// once for all query heads of its key head, so the floor is the cache's bytes
-// over the HBM rate; what has to stay below that is the work per key.
+// once for up to 16 query heads of its key head (again for each further 16), so
+// the floor is the cache's bytes over the HBM rate; what has to stay below that
+// is the work per key.
 //
 // Products.  Both run on mma.sync m16n8k16 with the keys (then the elements of
 // a value) as the 16 rows and up to 8 query heads as the 8 columns:
@@ -30,7 +31,7 @@
 // and 11 in FP16: outputs would lie 6.5e-4 of their size from those of 32-bit
 // weights, with two they lie 1e-4 or less, and values of either sign that nearly
 // cancel would leave no right digit.  The second term costs nvfp4 13 % (3 x 131072
-// keys, D = 64: 52.0 us without it), fp8 1 % (47.6).
+// keys, D = 64: 58.5 us, 52.0 without it), fp8 1 % (47.9, 47.5).
 //
 // Softmax.  In base 2 with a reference exponent per head instead of the exact
 // maximum: it moves (to the maximum less 4) only when a score passes it by
@@ -53,20 +54,21 @@
 // in rounds with these added to each unit.
 //
 // Measured on B200 (copy bandwidth 6.54 TB/s): nvfp4, 3 x 131072 keys x 8 heads x 64
-// under 64 query heads 58.8 us = 3.9 TB/s, bound by its instructions (24 matrix
-// instructions for 32 keys, 8 cycles of a scheduler each, and beside them the
-// decoding and scaling of the codes, whose cycles come on top); fp8, 33 sequences up
-// to 8000 x 8 x 128 under 32 heads 48.0 us = 5.3 TB/s and bf16, 8 up to 4095 x 16 x 256
-// under 16 heads 49 us = 5.6 TB/s, bound by HBM behind about 7 us of start, first bytes
-// and joining; one sequence of 77 keys 4.7 us, a launch and a chain of waits.
+// under 64 query heads 58.5 us = 3.9 TB/s, bound by its instructions: 350 for 32 keys,
+// in 580 cycles of a scheduler.  24 are matrix instructions of 8 cycles each, 128 decode
+// and scale the codes; 60 % of the issue slots are used, as the cycles of matrix
+// instructions and of others nearly add up.  fp8, 33 sequences up to 8000 x 8 x 128 under
+// 32 heads 47.9 us = 5.3 TB/s and bf16, 8 up to 4095 x 16 x 256 under 16 heads 49 us = 5.6
+// TB/s, bound by HBM behind about 7 us of start, first bytes and joining; one sequence of
+// 77 keys 4.7 us, a launch and a chain of waits.
 //
 // A warp streams its steps through a ring of its own in shared memory with
 // cp.async: no barrier in the loop.  Masked keys are zero-filled, not read.
 // What a step costs besides its keys (its pages, addresses, waits, the loop)
-// was 58 of 357 instructions for 32 keys of 32 bytes, where the loop is bound by
-// issue: such steps have 64 keys, worked on in two unrolled parts (3 x 131072
-// keys of nvfp4, D = 64: 58 us by 32 keys and four steps in the ring, 53.7 by
-// 64 and two, 51.6 unrolled).  Pages are looked up for 32 runs of keys at once.
+// was 58 of 357 instructions for 32 keys of 32 bytes, where instructions are the
+// bound: such steps have 64 keys, worked on in two unrolled parts (3 x 131072 keys
+// of nvfp4, D = 64, p in one term: 58 us by 32 keys and four steps in the ring, 53.7
+// by 64 and two, 51.6 unrolled).  Pages are looked up for 32 runs of keys at once.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -961,8 +963,9 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
 }
 
 // Pages of 16 where 32 keys are worked on at once have a form of their own: 3 x
-// 131072 keys of nvfp4, D = 64: 53.1 us against 57 key by key and 51.5 by whole
-// parts (one kernel with all three costs each of them 1.3 us, in registers).
+// 131072 keys of nvfp4, D = 64: 60.1 us, where pages of 64 by whole parts take 58.3 and
+// pages of 8 key by key 63.2 (one kernel with all three cost each of them 1.3 us more,
+// in registers).
 template <int KIND, int D, int NT>
 cudaError_t launch_run(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     constexpr int CK = Cfg<KIND, D, NT>::CK;

@@ -32,13 +32,14 @@
 // warp a group at a time and without a barrier, so that x is converted 148 times at
 // most.  (x by chunks through shared memory instead, all of it for every CTA, took
 // a barrier every two steps and as many bytes of x as of the weight from L2: 53.5 us
-// for 16 rows of x, 16384 x 16384, now 39.4.)
+// for 16 rows of x, 16384 x 16384, now 40.)
 //
-// Measured on B200 (copy bandwidth 6.54 TB/s): one row, 28672 x 8192 28.8 us = 4.6
-// TB/s; 16 rows, 16384 x 16384 39.4 us = 3.9 TB/s, where the copies alone take 30
+// Measured on B200 (copy bandwidth 6.54 TB/s): one row, 28672 x 8192 29.4 us = 4.5
+// TB/s; 16 rows, 16384 x 16384 40.1 us = 3.8 TB/s, where the copies alone take 30
 // and the products alone 31: beside mma.sync the decoding's instructions cost a
-// scheduler nearly their own time more.  5 rows, 15360 x 2880 9.9 us; one row, 2880 x
-// 2880 4.5 us, a launch and one chain of waits.
+// scheduler nearly their own time more.  6 rows, 19072 x 16384 39.1 us; 5 rows, 15360 x
+// 2880 9.9 us, on 120 SMs and with x converted before the weights' third step is asked
+// for; one row, 2880 x 2880 4.5 us, a launch and one chain of waits.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -458,8 +459,8 @@ Cut cut_of(int m, int n, int k) {
     // does not fit beside the rings otherwise (16 rows, 15360 x 2880: 13.4 us walked,
     // 19.2 not), of 8 where it would (5 rows: 11.1 and 9.8).  Of the numbers of slices
     // the one that lets a CTA's warps end together: the rounds of its groups times the
-    // steps of each, and a third of a step for a slice's sums (16 rows, 16384 x 16384:
-    // 8 slices 42.0 us, 9 39.4, 18 43.9).
+    // steps of each, and a third of a step for a slice's sums (16 rows, 16384 x 16384, in
+    // one session: 8 slices 42.0 us, 9 39.4, 18 43.9).
     const int shortest = all > slice_fit ? kWalkSteps : 8;
     const int from = std::max(slices_of(walk_fit), (148 * kWalkWarps * 3 / 4 - 1) / groups + 1);
     int least = 0;

@@ -23,8 +23,11 @@
 // Measured on B200 (copy bandwidth 6.54 TB/s): norm and rotation of 8192 x 72
 // heads x 64 30.1 us = 5.1 TB/s, bound by instruction issue and by DRAM's mix of
 // reads and writes alike; 4099 tokens x 8 heads x 128 of K and V to nvfp4 and read
-// back 14.7 us = 2.9 TB/s, two short launches; 131072 slots x 8 heads x 64 of nvfp4
-// read back 57.3 us = 6.0 TB/s, bound by HBM.
+// back 14.6 us = 3.0 TB/s (9.4 of them the writing), two short launches; 32768 tokens of
+// the same written alone 47.4 us in bf16 = 5.7 TB/s, 45.7 in fp8 = 4.5 and 58.7 in nvfp4 =
+// 2.9 (its codes leave in two-byte, its scales in one-byte stores; what that costs was
+// not measured); 131072 slots x 8 heads x 64 of nvfp4 read back 57.1 us = 6.0 TB/s, bound
+// by HBM.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -284,7 +287,8 @@ __device__ __forceinline__ unsigned long long widen(uint32_t w) {
 //   out_a = (a (w_a c) - b (w_b s)) / rms,  out_b = (b (w_b c) + a (w_a s)) / rms
 // (117 instructions a round of 32 / L rows where the general kernel below, one
 // element and one check at a time, has 200: 8192 tokens x 72 heads x 64 30.1 us
-// against 50.0).
+// against 50.0; what only the latter can do is up to twice as slow: pairs 48.4 us, half
+// of each row rotated 61.8).
 template <int KIND, int L, bool ROTATED>
 __global__ void __launch_bounds__(kThreads, 4) kv_walk_kernel(const __grid_constant__ RowsParams p) {
     constexpr int kPer = 32 / L;  // heads of a token that a warp holds at once

@@ -12,8 +12,9 @@ linear and the output linear when a model answers token by token.
 
 (The linears' own form for few rows is ``fp4_gemm.fp4_cached_gemv``.)  Tensors are BF16 on one CUDA device; work is queued
 on PyTorch's current stream and nothing synchronises, so a decode step can be captured in a CUDA graph.  Inference only,
-like the rest of the library: no gradients.  Slots, positions, page tables and lengths live on the GPU; an index out of
-range is left out by the kernel and shows in ``fp4_gemm.device_error()`` (11 slot, 12 position, 13 page or length).
+like the rest of the library: no gradients.  Slots, positions, page tables and lengths live on the GPU; one out of
+range is never followed and shows in ``fp4_gemm.device_error()``: 11 a slot (nothing written, zeros read), 12 a position (no
+rotation), 13 a page (its keys count as rows of zeros: score 0, value 0) or a length (clamped to the table's pages).
 """
 
 import ctypes

@@ -578,7 +578,8 @@ def fp4_cached_gemv(x: torch.Tensor, cache: FP4WeightCache) -> torch.Tensor:
     synchronises.
 
     For decoding: up to about 16 rows the time is that of reading the weight once.  It takes any number of rows, but
-    reads the weight again for every 16; forward() is the form for many rows (and quantizes the activations).
+    reads the weight again for every 16; forward() is the form for many rows (and quantizes the activations).  For the
+    products each row is scaled by a power of two into FP16: elements below 2^-32 of its largest lose bits.
     """
     if cache._handle is None:
         raise RuntimeError("FP4WeightCache has been freed")

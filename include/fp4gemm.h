@@ -264,8 +264,9 @@ int fp4b_ipc_close(void* ptr, long offset);
  * linear of a decoder layer.  All asynchronous on `stream`; 0 ok, -1 bad
  * arguments, -2 a geometry the kernels cannot take, -4 launch failure.  An
  * index that only the GPU sees (slot, position, page, length) and that is out
- * of range is left out and recorded in the device error word
- * (fp4b_device_error): 11 slot, 12 position, 13 page or length.
+ * of range is never followed (nothing written, zeros read, no rotation, a
+ * length clamped) and recorded in the device error word (fp4b_device_error):
+ * 11 slot, 12 position, 13 page or length.
  * ------------------------------------------------------------------------- */
 
 /* y[m, n_out] = w_alpha * x @ W^T (+ bias) with x [m, k_in] BF16 as it is (not
