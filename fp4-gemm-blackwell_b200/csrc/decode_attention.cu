@@ -29,7 +29,7 @@
 // below 2^-3, to within 2^-25; the largest weight is 2^4 or more, see below).  One
 // term would be 8 bits in BF16, as large an error as the output's own rounding,
 // and 11 in FP16: outputs would lie 6.5e-4 of their size from those of 32-bit
-// weights, with two they lie 1e-4 or less, and values of either sign that nearly
+// weights, with two they lie 1.2e-4 or less, and values of either sign that nearly
 // cancel would leave no right digit.  The second term costs nvfp4 13 % (3 x 131072
 // keys, D = 64: 58.5 us, 52.0 without it), fp8 1 % (47.9, 47.5).
 //

@@ -13,7 +13,7 @@
 // its scale enters as 2^-8 of its value, a shift of its byte.  The activations
 // of one row's chunk of K are multiplied by the power of two that puts their
 // largest into [2^14, 2^15): exact, down to 2^-32 of that largest (below, they
-// lose bits that fp32 sums lose too); the chunk's sums are multiplied back.
+// lose bits, as they do in fp32 sums unless the largest meets a weight of zero); the chunk's sums are multiplied back.
 //
 // Reads.  A warp takes 32 weight rows, the four rows r, r + 32, r + 64, r + 96
 // of eight r: their scales for 64 elements of K are 16 neighbouring bytes of
