@@ -196,6 +196,14 @@ int* device_error_word() {
     return g_err_word[d];
 }
 
+int device_sm_count() {
+    static int counts[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
+    if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -1;
+    return counts[dev];
+}
+
 int read_and_clear_device_error() {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int)) != cudaSuccess) return -1;

@@ -905,14 +905,6 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
 
 constexpr int kMaxDevices = 64;
 
-int sm_count() {
-    static int counts[kMaxDevices];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
-    if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -1;
-    return counts[dev];
-}
-
 // Workspace: counters, then the parts' (maximum, sum) and accumulators.
 struct Layout {
     long slots, ml, acc, bytes;
@@ -938,7 +930,7 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    const int sms = sm_count();
+    const int sms = device_sm_count();
     if (sms <= 0 || sms * kMaxCtasPerSm * 4 > FP4B_DECODE_COUNTER_BYTES || dev >= kMaxDevices) return cudaErrorInvalidDevice;
     {
         std::lock_guard<std::mutex> lk(mu);
@@ -997,7 +989,7 @@ FP4B_EXPORT long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int 
         set_last_error("fp4b_decode_attention_workspace: bad head counts");
         return -1;
     }
-    const int sms = sm_count();
+    const int sms = device_sm_count();
     if (sms <= 0) {
         cudaGetLastError();
         set_last_error("fp4b_decode_attention_workspace: no device");

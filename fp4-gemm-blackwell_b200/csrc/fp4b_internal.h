@@ -93,6 +93,9 @@ struct CacheView {
 // False for a null or foreign handle.
 bool cache_view(const void* handle, CacheView* out);
 
+// SMs of the current device, asked for once; -1 if there is none.
+int device_sm_count();
+
 // Device-side error word written by kernels that gave up on a bounded wait.
 int* device_error_word();
 int read_and_clear_device_error();

@@ -36,15 +36,19 @@ class _CacheView(ctypes.Structure):
                 ("page_size", _i), ("head_dim", _i), ("kind", _i)]
 
 
-# fp4b_rows and fp4b_decode, as one call packs them (0: NULL).
+# The arguments of the C entry points, as one call packs them (0: NULL): fp4b_rows and fp4b_decode,
 _ROWS, _DECODE = struct.Struct("@PllPllPllPPPPPPPPiiiiiiiiif"), struct.Struct("@PllPPlPPPPPliiiif0l")
+_NORM, _SAMPLING = struct.Struct("@PlPlPlPPPPiiiff0l"), struct.Struct("@PlPPPPPPPiiififf0l")  # fp4b_norm, fp4b_sampling
 
 _bind("fp4b_kv_rows", _i, [ctypes.c_char_p, _vp])
 _bind("fp4b_kv_read", _i, [_vp, _vp, _i, _l, _vp, _vp, _vp])
 _bind("fp4b_decode_attention_workspace", _l, [_i, _i, _i])
 _bind("fp4b_decode_attention", _i, [ctypes.c_char_p, _vp])
+_bind("fp4b_block_norm", _i, [ctypes.c_char_p, _vp])
+_bind("fp4b_sample", _i, [ctypes.c_char_p, _vp])
 
 _kv_rows, _kv_read, _attention = _lib.fp4b_kv_rows, _lib.fp4b_kv_read, _lib.fp4b_decode_attention
+_block_norm, _sample = _lib.fp4b_block_norm, _lib.fp4b_sample
 
 
 # A call's host time is what a small decode step costs, so the current device and stream are asked for without the
@@ -373,3 +377,143 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
             _address(sinks), out.data_ptr(), _address(lse), ws.data_ptr(), ws.numel(), b, hq, page_table.shape[1], window,
             d ** -0.5 if scale is None else scale))
     return (out, lse) if return_lse else out
+
+
+def _wide(t: torch.Tensor, what: str, device, dtypes=(torch.bfloat16,)):
+    """(t, row stride) of rows [..., H] as [rows, H] with elements in one run; cast to BF16 where the type is none of `dtypes`."""
+    if t.device != device:
+        raise ValueError(f"{what} must be on {device}, got {t.device}")
+    if t.dtype not in dtypes:
+        t = t.to(torch.bfloat16)
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _vector(t, h: int, what: str, device):
+    """A weight [H] in BF16, its elements in one run."""
+    if t is None:
+        return None
+    if t.numel() != h or t.device != device:
+        raise ValueError(f"{what} must have {h} elements on {device}")
+    if t.dtype != torch.bfloat16:
+        t = t.to(torch.bfloat16)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, post_weight: torch.Tensor = None, gate: torch.Tensor = None,
+               scale: float = 1.0, eps: float = 1e-6):
+    """
+    What lies between two blocks: the norm after a block, its gate, its residual and the norm before the next block, in one pass.
+
+    With x [..., H] the block's output and residual [..., H] what it is added to:
+
+        y = x / sqrt(mean(x^2) + eps) * post_weight     (without post_weight: y = x)
+        r = residual + scale * gate * y                 (without gate: 1)
+        normed = r / sqrt(mean(r^2) + eps) * weight
+
+    x is BF16, residual BF16 or fp32 (a residual stream in 32 bits), gate [H] (each channel's) or of x's shape, the weights
+    [H], all BF16 (other types are cast).  Rows may have any stride.  In fp32 throughout: normed is made from r as it is before
+    its rounding.  x None: normed of the residual alone (before the first block).  H up to 32768.
+
+    Returns new tensors (normed, r): normed BF16, r of residual's type (residual itself where x is None).
+    """
+    dev, h = residual.device, residual.shape[-1] if residual.dim() else 0
+    if not residual.is_cuda:
+        raise ValueError("residual must be on a CUDA device")
+    if not 0 < h <= 32768:
+        raise ValueError(f"rows must have 1 to 32768 elements, got shape {tuple(residual.shape)}")
+    if x is None and (post_weight is not None or gate is not None):
+        raise ValueError("post_weight and gate belong to a block's output: x is None")
+    shape, rows = residual.shape, residual.numel() // h
+    if residual.dtype != torch.float32 and residual.dtype != torch.bfloat16:
+        residual = residual.to(torch.bfloat16)
+    r_rows, r_stride = _wide(residual, "residual", dev, (torch.bfloat16, torch.float32))
+    weight, post_weight = _vector(weight, h, "weight", dev), _vector(post_weight, h, "post_weight", dev)
+    x_stride = gate_stride = 0
+    out = residual
+    if x is not None:
+        if x.shape != shape:
+            raise ValueError(f"x {tuple(x.shape)} and residual {tuple(shape)} have other shapes")
+        x, x_stride = _wide(x, "x", dev)
+        if gate is not None:
+            if gate.dim() == 1 and gate.shape[0] == h:
+                gate = _vector(gate, h, "gate", dev)
+            elif gate.shape == shape:
+                gate, gate_stride = _wide(gate, "gate", dev)
+            else:
+                raise ValueError(f"gate must be [{h}] or {tuple(shape)}, got {tuple(gate.shape)}")
+        out = torch.empty_like(residual, memory_format=torch.contiguous_format)
+    normed = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    if rows:
+        _call(dev, _block_norm, "block_norm", _NORM.pack(
+            _address(x), x_stride, r_rows.data_ptr(), r_stride, _address(gate), gate_stride, weight.data_ptr(), _address(post_weight),
+            normed.data_ptr(), 0 if x is None else out.data_ptr(), rows, h, residual.dtype == torch.float32, scale, eps))
+    return normed, out
+
+
+_LOGITS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # FP4B_LOGITS_*
+
+
+def _setting(v, rows: int, dtype, what: str, device):
+    """(address, number, tensor to keep) of a setting: one number for all rows, or a tensor [rows]."""
+    if not isinstance(v, torch.Tensor):
+        return 0, v, None
+    if v.device != device or v.numel() != rows:
+        raise ValueError(f"{what} must be a number or {rows} numbers on {device}, got {tuple(v.shape)} on {v.device}")
+    if v.dtype != dtype:
+        v = v.to(dtype)
+    if not v.is_contiguous():
+        v = v.contiguous()
+    return v.data_ptr(), 0, v
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_prob: bool = False):
+    """
+    The next token of each row of logits, by temperature, top-k, top-p and min-p, from given uniform numbers.
+
+    logits is [B, V] BF16, FP16 or fp32, rows of any stride; u [B] fp32 in [0, 1) (numbers outside count as the nearest of
+    these).  Each setting is a number or a tensor [B] (top_k int32, the others fp32).  The tokens of a row are taken by logit,
+    largest first, equal ones by index, with w = exp((logit - max) / temperature); -inf (a masked token) and NaN are no
+    candidates.  Kept are
+
+        the first top_k                                        (0 or less: all),
+        of those the ones before which less than top_p of their weights' sum lies   (1 or more: all; the first always),
+        of those the ones with w >= min_p                      (0 or less: all; the first always),
+
+    and the token is the first with which more than u of the kept ones' sum is reached.  A temperature of 0 gives the largest
+    logit's first index.  The sums are exact to 2^-44 and better of the largest weight, so the same call gives the same tokens.
+
+    Returns int64 [B], -1 for a row without candidates; with return_prob=True also fp32 [B], the share of the kept ones' sum
+    that the token has (1 at temperature 0, 0 where there is none).
+    """
+    if logits.dim() != 2 or logits.dtype not in _LOGITS:
+        raise ValueError(f"logits must be [B, V] BF16, FP16 or fp32, got {logits.dtype} {tuple(logits.shape)}")
+    if not logits.is_cuda:
+        raise ValueError("logits must be on a CUDA device")
+    b, v = logits.shape
+    dev = logits.device
+    if v == 0 or v > 1 << 30:
+        raise ValueError(f"the vocabulary must be 1 to 2^30 tokens, got {v}")
+    if u.dtype != torch.float32 or u.device != dev or u.numel() != b:
+        raise ValueError(f"u must be {b} fp32 numbers on {dev}, got {u.dtype} {tuple(u.shape)} on {u.device}")
+    if not u.is_contiguous():
+        u = u.contiguous()
+    if v > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    t_at, t_one, t_keep = _setting(temperature, b, torch.float32, "temperature", dev)
+    k_at, k_one, k_keep = _setting(top_k, b, torch.int32, "top_k", dev)
+    p_at, p_one, p_keep = _setting(top_p, b, torch.float32, "top_p", dev)
+    m_at, m_one, m_keep = _setting(min_p, b, torch.float32, "min_p", dev)
+    if t_at == 0 and not t_one >= 0.0:
+        raise ValueError(f"temperature must not be negative, got {t_one}")
+    tokens = torch.empty(b, dtype=torch.int64, device=dev)
+    probs = torch.empty_like(u) if return_prob else None
+    if b:
+        _call(dev, _sample, "sample", _SAMPLING.pack(
+            logits.data_ptr(), logits.stride(0), u.data_ptr(), t_at, k_at, p_at, m_at, tokens.data_ptr(), _address(probs), b, v,
+            _LOGITS[logits.dtype], t_one, min(max(int(k_one), 0), v), p_one, m_one))
+    return (tokens, probs) if return_prob else tokens

@@ -367,6 +367,65 @@ typedef struct fp4b_decode {
 long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int head_dim);
 int fp4b_decode_attention(const fp4b_decode* call, void* stream);
 
+/* The norms around a block with its gate and residual: of each row
+ *   y = x / sqrt(mean(x^2) + eps) * post_weight     (post_weight NULL: y = x)
+ *   r = residual + scale * gate * y                 (gate NULL: 1)
+ *   normed = r / sqrt(mean(r^2) + eps) * weight
+ * in fp32, normed and r (residual_out) rounded once.  x NULL: r is the
+ * residual, residual_out is not written.  x, gate, weights and normed are BF16,
+ * residual and residual_out BF16 or, with residual_fp32, fp32.  Strides of rows
+ * in elements (gate_stride 0: one gate for all rows); outputs contiguous, not
+ * overlapping the inputs but that residual_out may be the residual itself.
+ * width 1 to 32768. */
+typedef struct fp4b_norm {
+    const void* x;
+    long x_stride;
+    const void* residual;
+    long residual_stride;
+    const void* gate;
+    long gate_stride;
+    const void* weight;
+    const void* post_weight;
+    void* normed;
+    void* residual_out;
+    int rows, width;
+    int residual_fp32;
+    float scale, eps;
+} fp4b_norm;
+int fp4b_block_norm(const fp4b_norm* call, void* stream);
+
+/* Types of logits. */
+enum { FP4B_LOGITS_BF16 = 0, FP4B_LOGITS_FP16 = 1, FP4B_LOGITS_FP32 = 2 };
+
+/* The next token of each row of logits [rows, vocab] (row stride in elements),
+ * from u[row] in [0, 1) (a lower number counts as 0, a NaN too, a larger one as
+ * the largest below 1).  Tokens are taken by logit, largest first, equal ones
+ * by index; -inf and NaN are no candidates.  With w = exp((logit - max) / T),
+ * kept are the first top_k (0 or less: all), of those the ones before which
+ * less than top_p of their weights' sum lies (the first always; top_p >= 1 or
+ * NaN: all) and which have w >= min_p (the first always; NaN: all); tokens[row]
+ * is the first with which more than u of the sum of the kept ones' weights is
+ * reached, probs[row] (NULL: not wanted) its share of that sum.  T = 0, less or
+ * NaN: the first token, with 1.  A row without candidates: -1, with 0.
+ * temperature, top_k, top_p, min_p: arrays [rows], or NULL for the one number
+ * beside. */
+typedef struct fp4b_sampling {
+    const void* logits;
+    long stride;
+    const float* u;
+    const float* temperature;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    long long* tokens;
+    float* probs;
+    int rows, vocab, type;
+    float temperature1;
+    int top_k1;
+    float top_p1, min_p1;
+} fp4b_sampling;
+int fp4b_sample(const fp4b_sampling* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
