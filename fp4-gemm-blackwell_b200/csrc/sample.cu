@@ -1,0 +1,692 @@
+// sample.cu -- the next token of each row of logits, by temperature, top-k,
+// top-p and min-p, from a given uniform number.
+//
+// The tokens of a row are taken in the order of their logits, largest first,
+// equal ones by index (-inf and NaN are no candidates), with the weights
+//   w_i = exp((l_i - max) / T).
+// Kept are: the first k of them; of those, with W their weights' sum, the ones
+// before which less than p * W lies (always the first); and of those the ones
+// with w_i >= min_p.  Each is a prefix of the order, so what is kept is a prefix
+// too, and has a mass; the token is the first whose weights' sum, up to it and
+// with it, is more than u times that mass.  T = 0: the first token.
+//
+// So every question is the same: where in the order does a running count, or a
+// running sum of weights, pass a number.  It is answered without sorting, by a
+// histogram of the logits' leading bits in the order's own direction: a bin has
+// a count and a mass.  Where the leading bits are all the bits (BF16), a bin is
+// one logit: its mass is its count times one weight, no element needs an
+// exponential, and a place in it is a place among equal logits, found by
+// counting.  Where a bin has more bits (FP16, FP32, and the logits nearest to
+// zero), elements add their weights to it, and the bin at hand is split again,
+// 8 bits at a time, until all its logits are one.
+//
+// Bins.  bits 16 up of the logit as FP32: sign, exponent, 7 bits.  The weights
+// that matter lie within 46 of the maximum (e^-46 * 2^32 is below 2^-33, and u
+// is at most 1 - 2^-24), so exponents from the largest of that range down are
+// 16 octaves x 128 bins for each sign; smaller magnitudes are one bin between
+// them, and what lies below the range is in none.
+//
+// Sums.  Which token it is turns on sums over the whole row that lie next to a
+// border, so they are exact: a weight is exp() in FP64, rounded once to a whole
+// multiple of 2^-bits, bits the most that cannot overflow 64 (44 at 2^18
+// tokens), and sums of these do not depend on their order.
+//
+// A row belongs to a cluster of 1 to 8 CTAs, as many as give all rows' CTAs a
+// place on the GPU at once; each counts a slice, then merges its share of the
+// bins over distributed shared memory into the first CTA's, which walks them.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <mutex>
+
+#include "decode_core.cuh"
+#include "fp4b_internal.h"
+
+#define FP4B_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace fp4b {
+namespace {
+
+using namespace decode;
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kOctaves = 16;
+constexpr int kSide = kOctaves * 128;      // bins of a sign
+constexpr int kBins = 2 * kSide + 1;       // the one between them is bin kSide
+constexpr int kPer = (kBins + kThreads - 1) / kThreads;  // bins a thread walks
+constexpr float kReach = 46.0f;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxDevices = 64;
+
+struct SampleParams {
+    const void* logits;
+    long stride;
+    const float* u;
+    const float* temperature;  // null: temperature1, and so on
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    float temperature1, top_p1, min_p1;
+    int top_k1;
+    long long* tokens;
+    float* probs;
+    int vocab, slice;  // slice: elements a CTA, a multiple of 8
+    int bits;          // of a weight behind the point
+};
+
+enum LogitType { kBf16 = FP4B_LOGITS_BF16, kFp16 = FP4B_LOGITS_FP16, kFp32 = FP4B_LOGITS_FP32 };
+
+template <int TYPE>
+struct Traits {
+    using T = uint16_t;
+    static constexpr int PER = 8;                            // elements of 16 bytes
+    static constexpr int FREE = TYPE == kBf16 ? 16 : 13;     // low bits of the FP32 form that are zero
+};
+template <>
+struct Traits<kFp32> {
+    using T = uint32_t;
+    static constexpr int PER = 4;
+    static constexpr int FREE = 0;
+};
+
+// FP32 bits of a logit; what is no candidate (NaN) becomes -inf, -0 becomes +0.
+__device__ __forceinline__ uint32_t tidy(uint32_t b) {
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0xFF800000u;
+    return b == 0x80000000u ? 0u : b;
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t bits_of(typename Traits<TYPE>::T raw) {
+    if constexpr (TYPE == kBf16) return tidy((uint32_t)raw << 16);
+    else if constexpr (TYPE == kFp16) return tidy(__float_as_uint(__half2float(__ushort_as_half(raw))));
+    else return tidy(raw);
+}
+
+// Keys grow with the logits.
+__device__ __forceinline__ uint32_t key_of(uint32_t b) { return b & 0x80000000u ? ~b : b | 0x80000000u; }
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+constexpr uint32_t kMinusInf = 0x007FFFFFu;  // key of -inf
+
+// A run of keys [first, first + 2^size): all the logits of one bin.
+struct Run {
+    uint32_t first;
+    int size;
+    // the logit of a run of one (of BF16's or FP16's: whose other bits are zero)
+    __device__ __forceinline__ float logit() const { return logit_of(first & 0x80000000u ? first : first + ((1u << size) - 1u)); }
+};
+
+struct Row {
+    float max, scale;  // of the weights: 1 / T in FP64
+    double inv;
+    int lo;            // leading bits of the smallest magnitude with a bin of its own
+    double one;        // 2^bits
+    __device__ __forceinline__ u64 weight(float l) const {
+        if (l == max) return (u64)one;
+        return (u64)__double2ll_rn(exp(((double)l - (double)max) * inv) * one);
+    }
+    __device__ __forceinline__ bool keeps(float l, float least) const {
+        return l == max || exp(((double)l - (double)max) * inv) >= (double)least;
+    }
+    // Bin of a candidate's bits, -1 for none.
+    __device__ __forceinline__ int bin(uint32_t b) const {
+        const int i = (int)((b >> 16) & 0x7FFFu) - lo;
+        if (i < 0) return kSide;
+        if (i >= kSide) return b & 0x80000000u ? -1 : 0;
+        return b & 0x80000000u ? kSide + 1 + i : kSide - 1 - i;
+    }
+    __device__ __forceinline__ Run run(int bin) const {
+        if (bin == kSide) {
+            // keys 2^31 - n up to 2^31 + n - 1, n = lo * 2^16
+            const uint32_t n = (uint32_t)lo << 16;
+            return Run{0x80000000u - n, n ? 33 - __clz(n - 1u) : 0};  // 2^size >= 2 n
+        }
+        if (bin < kSide) return Run{0x80000000u + ((uint32_t)(lo + kSide - 1 - bin) << 16), 16};
+        return Run{0x80000000u - ((uint32_t)(lo + bin - kSide) << 16), 16};
+    }
+};
+
+struct Place {  // of a crossing: a bin, and what lies before it
+    int bin;
+    uint32_t before, count;
+    u64 mass_before, mass;
+};
+
+// What the first CTA tells the others to do next.
+struct Command {
+    int what;  // 0: done, 1: split a run, 2: find the token
+    Run run;
+    int cta;
+    uint32_t rank;
+    float prob;
+};
+
+struct Shared {
+    uint32_t hist[kBins];
+    uint32_t sub_count[256];
+    u64 sub_mass[256];
+    float max[kMaxCluster];
+    uint32_t best[kMaxCluster];
+    uint32_t warp_count[kWarps];
+    u64 warp_mass[kWarps];
+    uint32_t least_count;  // candidates with w >= min_p, of the row
+    u64 least_mass;
+    Place place;
+    Command command;
+    int token;
+};
+
+// Sums of the threads before this one (exclusive), over the CTA.
+__device__ __forceinline__ void scan(Shared& s, uint32_t& count, u64& mass) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t c0 = count;
+    const u64 m0 = mass;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t c = __shfl_up_sync(0xffffffffu, count, o);
+        const u64 m = __shfl_up_sync(0xffffffffu, mass, o);
+        if (lane >= o) count += c, mass += m;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp_count[warp] = count, s.warp_mass[warp] = mass;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) count += s.warp_count[w], mass += s.warp_mass[w];
+    count -= c0, mass -= m0;
+}
+
+enum Kind { kByCount, kByMassBefore, kByMassWith };
+
+// The question of one crossing.  kByCount: the last of the first k.
+// kByMassBefore: the last before which less than `target` lies.  kByMassWith:
+// the first with which more than `target` lies.
+struct Question {
+    Kind kind;
+    uint32_t k;
+    double target;
+    // Does it lie in a bin with `count` and `mass`, `before` and `mass_before` before it?
+    __device__ __forceinline__ bool in(uint32_t before, u64 mass_before, uint32_t count, u64 mass) const {
+        if (count == 0) return false;
+        if (kind == kByCount) return before < k && k <= before + count;
+        if (kind == kByMassBefore) {
+            // the last bin before which less than the target lies: its mass reaches it
+            return (double)mass_before < target && (double)(mass_before + mass) >= target;
+        }
+        return (double)mass_before <= target && (double)(mass_before + mass) > target;
+    }
+    // How many of `count` elements of weight w lie up to and with it.
+    __device__ __forceinline__ uint32_t part(uint32_t before, u64 mass_before, uint32_t count, u64 w) const {
+        if (kind == kByCount) return k - before;
+        if (w == 0) return 1;
+        const double d = floor((target - (double)mass_before) / (double)w);
+        uint32_t n = d < 1.0 ? 1u : d >= (double)count ? count : (uint32_t)d;
+        if (kind == kByMassBefore) {
+            while (n < count && (double)(mass_before + (u64)n * w) < target) ++n;
+            while (n > 1 && (double)(mass_before + (u64)(n - 1) * w) >= target) --n;
+        } else {
+            while (n < count && (double)(mass_before + (u64)n * w) <= target) ++n;
+            while (n > 1 && (double)(mass_before + (u64)(n - 1) * w) > target) --n;
+        }
+        return n;
+    }
+};
+
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleParams p) {
+    using T = typename Traits<TYPE>::T;
+    constexpr int PER = Traits<TYPE>::PER, FREE = Traits<TYPE>::FREE;
+    constexpr bool kMasses = FREE < 16;  // bins of more than one logit
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    // the first CTA's: merged bins; with masses every CTA's own
+    u64* const mass = reinterpret_cast<u64*>(dynamic);
+    uint32_t* const count = reinterpret_cast<uint32_t*>(mass + kBins);
+    u64* const my_mass = reinterpret_cast<u64*>(dynamic + kBins * 16);
+    __shared__ Shared s;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
+    const long row = blockIdx.x / ctas;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    chain();
+
+    // ---- this CTA's slice; a warp goes over a run of its own, 16 bytes a lane, in the order of the indices
+    const int first = min(me * p.slice, p.vocab), last = min(first + p.slice, p.vocab);
+    const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
+    // pieces of 16 aligned bytes: piece i holds elements [i * PER - shift, + PER) of the slice
+    const int shift = (int)((reinterpret_cast<uintptr_t>(logits + first) & 15) / sizeof(T));
+    const int pieces = last > first ? (last - first + shift + PER - 1) / PER : 0;
+    const int warp_pieces = ((pieces + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const int piece0 = min(warp * warp_pieces, pieces), piece1 = min(piece0 + warp_pieces, pieces);
+    // The bits of piece i's elements, what lies outside the slice as -inf.
+    auto load = [&](int i, uint32_t (&b)[PER]) {
+        const int at = first + i * PER - shift;
+        if (at >= first && at + PER <= last) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(logits + at));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                if constexpr (PER == 4) b[e] = bits_of<TYPE>(w[e]);
+                else b[e] = bits_of<TYPE>((uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) b[e] = at + e >= first && at + e < last ? bits_of<TYPE>(logits[at + e]) : 0xFF800000u;
+        }
+    };
+
+    // ---- the maximum
+    float most = -INFINITY;
+    for (int i = piece0 + lane; i < piece1; i += 32) {
+        uint32_t b[PER];
+        load(i, b);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) most = fmaxf(most, __uint_as_float(b[e]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int i = tid; i < kBins; i += kThreads) {
+        s.hist[i] = 0;
+        if (kMasses) my_mass[i] = 0;
+        if (!kMasses && i == kSide) my_mass[0] = 0;  // of the bin between
+    }
+    if (tid == 0) s.least_count = 0, s.least_mass = 0, s.token = 0x7fffffff;
+    if (lane == 0) reinterpret_cast<float*>(s.warp_count)[warp] = most;
+    __syncthreads();
+    if (warp == 0) {
+        most = lane < kWarps ? reinterpret_cast<float*>(s.warp_count)[lane] : -INFINITY;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (lane < ctas) cluster.map_shared_rank(s.max, lane)[me] = most;
+    }
+    cluster.sync();
+    most = s.max[0];
+    for (int c = 1; c < ctas; ++c) most = fmaxf(most, s.max[c]);
+    // (no CTA writes its neighbours' s.max again)
+
+    const float t = p.temperature ? p.temperature[row] : p.temperature1;
+    const bool greedy = !(t > 0.0f);
+    if (most == -INFINITY) {  // no candidates
+        if (me == 0 && tid == 0) {
+            p.tokens[row] = -1;
+            if (p.probs) p.probs[row] = 0.0f;
+        }
+        return;
+    }
+    Row r;
+    r.max = most;
+    r.inv = fmax(1.0 / (double)t, 0x1p-1000);  // (an infinite T: all alike)
+    r.one = (double)(1ull << p.bits);
+    {
+        const uint32_t far = __float_as_uint(fmaf(-kReach, t, most)) & 0x7FFFFFFFu, top = __float_as_uint(most) & 0x7FFFFFFFu;
+        const int octave = (int)(max(min(far, 0x7F800000u), top) >> 23);
+        r.lo = max(octave - (kOctaves - 1), 0) << 7;
+    }
+    const float least = p.min_p ? p.min_p[row] : p.min_p1;
+    const bool has_least = least > 0.0f;
+
+    // ---- the token of a run of equal logits: the rank-th of them, in this CTA's slice
+    auto find = [&](Run run, uint32_t rank, float prob) {
+        auto hits = [&](int i, uint32_t& mask) {
+            mask = 0;
+            if (i < piece1) {
+                uint32_t b[PER];
+                load(i, b);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const uint32_t key = key_of(b[e]);
+                    if (key > kMinusInf && key >= run.first && (run.size > 31 || ((key - run.first) >> run.size) == 0)) mask |= 1u << e;
+                }
+            }
+        };
+        uint32_t mine = 0;
+        for (int i = piece0 + lane; i < piece1; i += 32) {
+            uint32_t mask;
+            hits(i, mask);
+            mine += __popc(mask);
+        }
+        const uint32_t all = __reduce_add_sync(0xffffffffu, mine);
+        __syncthreads();
+        if (lane == 0) s.warp_count[warp] = all;
+        __syncthreads();
+        uint32_t before = 0;
+        for (int w = 0; w < warp; ++w) before += s.warp_count[w];
+        if (rank < before || rank >= before + all) return;
+        rank -= before;
+        for (int i = piece0; i < piece1; i += 32) {
+            uint32_t mask;
+            hits(i + lane, mask);
+            const uint32_t here = __popc(mask);
+            uint32_t upto = here;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t other = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += other;
+            }
+            if (rank < upto && rank >= upto - here) {
+                for (uint32_t k = rank - (upto - here); k > 0; --k) mask &= mask - 1;
+                p.tokens[row] = first + (i + lane) * PER - shift + (__ffs(mask) - 1);
+                if (p.probs) p.probs[row] = prob;
+            }
+            const uint32_t tile = __shfl_sync(0xffffffffu, upto, 31);
+            if (rank < tile) return;
+            rank -= tile;
+        }
+    };
+
+    if (greedy) {  // the first of the largest: the least index
+        int at = 0x7fffffff;
+        for (int i = piece0 + lane; i < piece1 && at == 0x7fffffff; i += 32) {
+            uint32_t b[PER];
+            load(i, b);
+#pragma unroll
+            for (int e = PER - 1; e >= 0; --e)
+                if (__uint_as_float(b[e]) == most) at = first + i * PER - shift + e;
+        }
+        at = __reduce_min_sync(0xffffffffu, at);
+        Shared* home = cluster.map_shared_rank(&s, 0);
+        if (lane == 0 && at != 0x7fffffff) atomicMin(&home->token, at);
+        cluster.sync();
+        if (me == 0 && tid == 0) {
+            p.tokens[row] = s.token;
+            if (p.probs) p.probs[row] = 1.0f;
+        }
+        return;
+    }
+
+    // ---- counts (and masses) of the slice's bins
+    uint32_t kept = 0;
+    u64 kept_mass = 0;
+    for (int i = piece0 + lane; i < piece1; i += 32) {
+        uint32_t b[PER];
+        load(i, b);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            if (b[e] == 0xFF800000u) continue;
+            const int bin = r.bin(b[e]);
+            if (bin < 0) continue;
+            atomicAdd(&s.hist[bin], 1u);
+            if (kMasses || bin == kSide) {
+                const float l = __uint_as_float(b[e]);
+                const u64 w = r.weight(l);
+                atomicAdd(&my_mass[kMasses ? bin : 0], w);
+                if (has_least && r.keeps(l, least)) ++kept, kept_mass += w;
+            }
+        }
+    }
+    cluster.sync();
+
+    // ---- this CTA's share of the bins over all slices, into the first CTA's
+    {
+        uint32_t* to_count = cluster.map_shared_rank(count, 0);
+        u64* to_mass = cluster.map_shared_rank(mass, 0);
+        for (int i = me * kThreads + tid; i < kBins; i += ctas * kThreads) {
+            uint32_t n = 0;
+            u64 m = 0;
+            for (int c = 0; c < ctas; ++c) {
+                n += cluster.map_shared_rank(s.hist, c)[i];
+                if (kMasses) m += cluster.map_shared_rank(my_mass, c)[i];
+                else if (i == kSide) m += cluster.map_shared_rank(my_mass, c)[0];
+            }
+            if (!kMasses && i != kSide && n) {
+                const float l = r.run(i).logit();
+                const u64 w = r.weight(l);
+                m = w * n;
+                if (has_least && r.keeps(l, least)) kept += n, kept_mass += m;
+            }
+            to_count[i] = n, to_mass[i] = m;
+        }
+        if (has_least) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                kept += __shfl_xor_sync(0xffffffffu, kept, o);
+                kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
+            }
+            Shared* home = cluster.map_shared_rank(&s, 0);
+            if (lane == 0 && kept) atomicAdd(&home->least_count, kept), atomicAdd(&home->least_mass, kept_mass);
+        }
+    }
+    cluster.sync();
+
+    // ---- the first CTA asks; a run of more than one logit is split by all of them
+    auto split = [&](Run run) {  // all CTAs: counts and masses of the run's 256 parts, ascending
+        for (int i = tid; i < 256; i += kThreads) s.sub_count[i] = 0, s.sub_mass[i] = 0;
+        __syncthreads();
+        const int down = max(run.size - 8, 0);
+        for (int i = piece0 + lane; i < piece1; i += 32) {
+            uint32_t b[PER];
+            load(i, b);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const uint32_t key = key_of(b[e]);
+                if (key <= kMinusInf || key < run.first || (run.size < 32 && ((key - run.first) >> run.size) != 0)) continue;
+                const uint32_t part = (key - run.first) >> down;
+                if (part > 255) continue;
+                if (run.size > 16 && r.bin(b[e]) != kSide) continue;  // (the bin between is less than its power of two)
+                atomicAdd(&s.sub_count[part], 1u);
+                atomicAdd(&s.sub_mass[part], r.weight(__uint_as_float(b[e])));
+            }
+        }
+        cluster.sync();
+    };
+
+    if (me != 0) {
+        for (;;) {
+            cluster.sync();  // a command is there
+            const Command c = s.command;
+            if (c.what == 1) {
+                split(c.run);
+                cluster.sync();  // the parts were read
+            } else {
+                if (c.what == 2 && c.cta == me) find(c.run, c.rank, c.prob);
+                return;
+            }
+        }
+    }
+    auto tell = [&](const Command& c) {
+        if (tid < ctas) cluster.map_shared_rank(&s, tid)->command = c;
+        cluster.sync();
+    };
+
+    struct Answer {
+        uint32_t count;  // up to the place, with it
+        u64 mass;
+        Run run;         // of its logit
+        uint32_t rank;   // among equal ones
+        int bin;         // >= 0: counts are the bins', else the parts'
+        u64 weight;
+        bool found;
+    };
+    auto ask = [&](const Question& q) {
+        // the bin
+        uint32_t n = 0;
+        u64 m = 0;
+        for (int k = 0; k < kPer; ++k) {
+            const int i = tid * kPer + k;
+            if (i < kBins) n += count[i], m += mass[i];
+        }
+        scan(s, n, m);
+        if (tid == 0) s.place.bin = -1;
+        __syncthreads();
+        for (int k = 0; k < kPer; ++k) {
+            const int i = tid * kPer + k;
+            if (i >= kBins) break;
+            if (q.in(n, m, count[i], mass[i])) s.place = Place{i, n, count[i], m, mass[i]};
+            n += count[i], m += mass[i];
+        }
+        __syncthreads();
+        Answer a{};
+        Place x = s.place;
+        a.found = x.bin >= 0;
+        if (!a.found) return a;
+        Run run = r.run(x.bin);
+        int bin = x.bin;
+        while (run.size > FREE) {
+            Command c{};
+            c.what = 1, c.run = run;
+            tell(c);
+            split(run);
+            // parts from the last (the largest logits) down, one a thread
+            const int i = 255 - tid;
+            n = 0, m = 0;
+            if (i >= 0)
+                for (int c = 0; c < ctas; ++c) {
+                    n += cluster.map_shared_rank(s.sub_count, c)[i];
+                    m += cluster.map_shared_rank(s.sub_mass, c)[i];
+                }
+            const uint32_t part_count = n;
+            const u64 part_mass = m;
+            scan(s, n, m);
+            n += x.before, m += x.mass_before;
+            if (i >= 0 && q.in(n, m, part_count, part_mass)) s.place = Place{i, n, part_count, m, part_mass};
+            cluster.sync();
+            x = s.place;
+            const int down = max(run.size - 8, 0);
+            run = Run{run.first + ((uint32_t)x.bin << down), down};
+            bin = -1;
+        }
+        a.weight = r.weight(run.logit());
+        const uint32_t part = q.part(x.before, x.mass_before, x.count, a.weight);
+        a.count = x.before + part, a.mass = x.mass_before + (u64)part * a.weight;
+        a.run = run, a.rank = part - 1, a.bin = bin;
+        s.place = x;  // (the same in every thread) its bin: of the bins or the parts
+        __syncthreads();
+        return a;
+    };
+
+    // ---- what is kept: the sum of its weights
+    u64 total;
+    {
+        uint32_t n = 0;
+        u64 m = 0;
+        for (int k = 0; k < kPer; ++k) {
+            const int i = tid * kPer + k;
+            if (i < kBins) n += count[i], m += mass[i];
+        }
+        scan(s, n, m);
+        if (tid == kThreads - 1) {
+            for (int k = 0; k < kPer; ++k) {
+                const int i = tid * kPer + k;
+                if (i < kBins) n += count[i], m += mass[i];
+            }
+            s.place.before = n, s.place.mass_before = m;
+        }
+        __syncthreads();
+        total = s.place.mass_before;
+        n = s.place.before;
+        __syncthreads();
+        const int k = p.top_k ? p.top_k[row] : p.top_k1;
+        if (k > 0 && (uint32_t)k < n) {
+            const Answer a = ask(Question{kByCount, (uint32_t)k, 0.0});
+            if (a.found) total = a.mass;
+        }
+        const float nucleus = p.top_p ? p.top_p[row] : p.top_p1;
+        u64 smaller = total;
+        if (nucleus < 1.0f) {
+            // (at least the first token: a target of nothing is less than the least weight)
+            const Answer a = ask(Question{kByMassBefore, 0, fmax((double)nucleus * (double)total, 0.5)});
+            if (a.found) smaller = min(smaller, a.mass);
+        }
+        if (has_least) smaller = min(smaller, s.least_mass ? s.least_mass : (u64)r.one);
+        total = smaller;
+    }
+    const float given = p.u[row];
+    const double u = given > 0.0f ? fmin((double)given, 1.0 - 0x1p-24) : 0.0;
+    const Answer a = ask(Question{kByMassWith, 0, u * (double)total});
+    Command c{};
+    c.what = 0;
+    if (a.found) {
+        // which CTA has it: the slices' counts of its logit, in order
+        uint32_t rank = a.rank;
+        for (int i = 0; i < ctas; ++i) {
+            const uint32_t n = a.bin >= 0 ? cluster.map_shared_rank(s.hist, i)[a.bin] : cluster.map_shared_rank(s.sub_count, i)[s.place.bin];
+            if (rank < n) {
+                c = Command{2, a.run, i, rank, (float)((double)a.weight / (double)total)};
+                break;
+            }
+            rank -= n;
+        }
+    }
+    tell(c);
+    if (c.what == 2 && c.cta == 0) find(c.run, c.rank, c.prob);
+}
+
+template <int TYPE>
+cudaError_t launch(SampleParams& p, int rows, cudaStream_t st) {
+    constexpr int kSmem = kBins * 16 + (Traits<TYPE>::FREE < 16 ? kBins * 8 : 16);
+    auto* kernel = sample_kernel<TYPE>;
+    static std::mutex mu;
+    static int resident[kMaxDevices];  // CTAs that fit on the device at once
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const int sms = device_sm_count();
+    if (sms <= 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!resident[dev]) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+            int per = 0;
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, kSmem);
+            if (e != cudaSuccess) return e;
+            resident[dev] = sms * std::max(1, per);
+        }
+    }
+    int ctas = 1;
+    while (ctas < kMaxCluster && (long)rows * ctas * 2 <= resident[dev] && p.vocab / (ctas * 2) >= 2048) ctas *= 2;
+    p.slice = ((p.vocab + ctas - 1) / ctas + 7) / 8 * 8;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)rows * (unsigned)ctas);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSmem;
+    config.stream = st;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = (unsigned)ctas, attributes[0].val.clusterDim.y = 1, attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, kernel, p);
+}
+
+}  // namespace
+}  // namespace fp4b
+
+using namespace fp4b;
+
+FP4B_EXPORT int fp4b_sample(const fp4b_sampling* call, void* stream) {
+    const char* why = nullptr;
+    if (!call) {
+        why = "null arguments";
+    } else {
+        const fp4b_sampling& c = *call;
+        const int size = c.type == FP4B_LOGITS_FP32 ? 4 : 2;
+        if (c.type != FP4B_LOGITS_BF16 && c.type != FP4B_LOGITS_FP16 && c.type != FP4B_LOGITS_FP32) why = "logits must be BF16, FP16 or FP32";
+        else if (c.rows < 0 || c.rows > (1 << 27)) why = "rows must be 0 to 2^27";
+        else if (c.vocab <= 0 || c.vocab > (1 << 30)) why = "the vocabulary must be 1 to 2^30 tokens";
+        else if (c.rows > 0 && (!c.logits || !c.u || !c.tokens)) why = "null tensor";
+        else if (reinterpret_cast<uintptr_t>(c.logits) % size) why = "misaligned logits";
+        else if (!c.temperature && !(c.temperature1 >= 0.0f)) why = "the temperature must not be negative";
+    }
+    if (why) {
+        set_last_error("fp4b_sample: %s", why);
+        return -1;
+    }
+    const fp4b_sampling& c = *call;
+    if (c.rows == 0) return 0;
+    SampleParams p{};
+    p.logits = c.logits, p.stride = c.stride, p.u = c.u;
+    p.temperature = c.temperature, p.top_k = c.top_k, p.top_p = c.top_p, p.min_p = c.min_p;
+    p.temperature1 = c.temperature1, p.top_k1 = c.top_k1, p.top_p1 = c.top_p1, p.min_p1 = c.min_p1;
+    p.tokens = c.tokens, p.probs = c.probs, p.vocab = c.vocab;
+    p.bits = 62;
+    while (p.bits > 0 && ((long long)1 << (62 - p.bits)) < c.vocab) --p.bits;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = c.type == FP4B_LOGITS_BF16   ? launch<kBf16>(p, c.rows, st)
+                          : c.type == FP4B_LOGITS_FP16 ? launch<kFp16>(p, c.rows, st)
+                                                       : launch<kFp32>(p, c.rows, st);
+    return launch_status(e, "fp4b_sample");
+}
