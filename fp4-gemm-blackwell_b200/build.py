@@ -21,8 +21,8 @@ LIB = os.path.join(HERE, "libfp4gemm.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["capi.cu", "quantize.cu", "quantize_units.cu", "gemm_sm100.cu", "noalloc.cu", "selftest.cu", "peak.cu", "peer_barrier.cu",
-           "kv_cache.cu", "decode_attention.cu", "gemv.cu", "block_norm.cu", "sample.cu"]
-HEADERS = ["decode_core.cuh", "fp4b_internal.h", "nvfp4_codec.cuh", "ptx_sm100.cuh", "quantize_core.cuh"]
+           "kv_cache.cu", "decode_attention.cu", "gemv.cu", "shared_attention.cu", "block_norm.cu", "sample.cu"]
+HEADERS = ["decode_attention.cuh", "decode_core.cuh", "fp4b_internal.h", "nvfp4_codec.cuh", "ptx_sm100.cuh", "quantize_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

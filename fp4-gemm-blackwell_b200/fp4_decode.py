@@ -38,17 +38,20 @@ class _CacheView(ctypes.Structure):
 
 # The arguments of the C entry points, as one call packs them (0: NULL): fp4b_rows and fp4b_decode,
 _ROWS, _DECODE = struct.Struct("@PllPllPllPPPPPPPPiiiiiiiiif"), struct.Struct("@PllPPlPPPPPliiiif0l")
+_SHARED = struct.Struct(_DECODE.format.replace("0l", "") + "PlPii0l")  # fp4b_shared: an fp4b_decode, then the prefixes
 _NORM, _SAMPLING = struct.Struct("@PlPlPlPPPPiiiff0l"), struct.Struct("@PlPPPPPPPiiififf0l")  # fp4b_norm, fp4b_sampling
 
 _bind("fp4b_kv_rows", _i, [ctypes.c_char_p, _vp])
 _bind("fp4b_kv_read", _i, [_vp, _vp, _i, _l, _vp, _vp, _vp])
 _bind("fp4b_decode_attention_workspace", _l, [_i, _i, _i])
 _bind("fp4b_decode_attention", _i, [ctypes.c_char_p, _vp])
+_bind("fp4b_shared_attention_workspace", _l, [_i, _i, _i, _i, _i])
+_bind("fp4b_shared_attention", _i, [ctypes.c_char_p, _vp])
 _bind("fp4b_block_norm", _i, [ctypes.c_char_p, _vp])
 _bind("fp4b_sample", _i, [ctypes.c_char_p, _vp])
 
 _kv_rows, _kv_read, _attention = _lib.fp4b_kv_rows, _lib.fp4b_kv_read, _lib.fp4b_decode_attention
-_block_norm, _sample = _lib.fp4b_block_norm, _lib.fp4b_sample
+_shared_attention, _block_norm, _sample = _lib.fp4b_shared_attention, _lib.fp4b_block_norm, _lib.fp4b_sample
 
 
 # A call's host time is what a small decode step costs, so the current device and stream are asked for without the
@@ -330,6 +333,24 @@ def _drop_workspaces(index: int) -> None:
 _on_cleanup.append(_drop_workspaces)
 
 
+def _pages(table, lens, b: int, table_name: str, lens_name: str, device):
+    """(page table, distance of its rows, lengths) of b sequences, as the kernels read them."""
+    if table.dim() != 2 or table.shape[0] != b or table.dtype != torch.int32 or table.device != device:
+        raise ValueError(f"{table_name} must be int32 [{b}, W] on {device}")
+    if lens.dim() != 1 or lens.shape[0] != b or lens.dtype != torch.int32 or lens.device != device:
+        raise ValueError(f"{lens_name} must be int32 [{b}] on {device}")
+    table, stride = _table(table)
+    return table, stride, lens if lens.stride(0) == 1 else lens.contiguous()
+
+
+def _sinks(sinks, hq: int, device):
+    if sinks is None:
+        return None
+    if sinks.numel() != hq or sinks.device != device:
+        raise ValueError(f"sinks must have {hq} elements on {device}")
+    return sinks.to(torch.float32).contiguous()
+
+
 def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_lens: torch.Tensor, scale: float = None,
                      window: int = 0, sinks: torch.Tensor = None, return_lse: bool = False):
     """
@@ -350,19 +371,10 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
     dev = cache.device
     if d != cache.head_dim or hq == 0 or hq % cache.kv_heads:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.kv_heads} heads of {cache.head_dim}")
-    if page_table.dim() != 2 or page_table.shape[0] != b or page_table.dtype != torch.int32 or page_table.device != dev:
-        raise ValueError(f"page_table must be int32 [{b}, W] on {dev}")
-    if seq_lens.dim() != 1 or seq_lens.shape[0] != b or seq_lens.dtype != torch.int32 or seq_lens.device != dev:
-        raise ValueError(f"seq_lens must be int32 [{b}] on {dev}")
+    page_table, table_stride, seq_lens = _pages(page_table, seq_lens, b, "page_table", "seq_lens", dev)
     if window < 0:
         raise ValueError("window must not be negative")
-    page_table, table_stride = _table(page_table)
-    if seq_lens.stride(0) != 1:
-        seq_lens = seq_lens.contiguous()
-    if sinks is not None:
-        if sinks.numel() != hq or sinks.device != dev:
-            raise ValueError(f"sinks must have {hq} elements on {dev}")
-        sinks = sinks.to(torch.float32).contiguous()
+    sinks = _sinks(sinks, hq, dev)
     out = _like(q)
     lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
     if b:
@@ -376,6 +388,45 @@ def decode_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Ten
             q.data_ptr(), qs[0], qs[1], cache._ref, page_table.data_ptr(), table_stride, seq_lens.data_ptr(),
             _address(sinks), out.data_ptr(), _address(lse), ws.data_ptr(), ws.numel(), b, hq, page_table.shape[1], window,
             d ** -0.5 if scale is None else scale))
+    return (out, lse) if return_lse else out
+
+
+def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, prefix_table: torch.Tensor, prefix_lens: torch.Tensor, page_table: torch.Tensor,
+                            seq_lens: torch.Tensor, scale: float = None, sinks: torch.Tensor = None, return_lse: bool = False):
+    """
+    ``decode_attention`` of sequences that share prefixes: one system prompt before all, or several answers to each prompt.
+
+    Each of the G prefixes is read once for all its sequences: prefix_table [G, W0] int32 and prefix_lens [G] int32 hold its
+    pages and length, and sequence b of q's B (a multiple of G) belongs to prefix b // (B // G).  page_table [B, W] and
+    seq_lens [B] are the sequence's own keys behind the prefix, on pages of their own from their first on; either length may
+    be 0.  One softmax goes over both.  q, scale, sinks, the result and its precision as in ``decode_attention`` (no window).
+
+    It pays from a few sequences a prefix on; decode_attention over tables that repeat the prefix's pages gives the same.
+    """
+    q = _rows(q, "q", cache.device)
+    b, hq, d = q.shape
+    dev = cache.device
+    if d != cache.head_dim or hq == 0 or hq % cache.kv_heads:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.kv_heads} heads of {cache.head_dim}")
+    groups = prefix_lens.shape[0] if prefix_lens.dim() == 1 else 0
+    if groups == 0 or b % groups:
+        raise ValueError(f"prefix_lens must be int32 [G] with {b} sequences a multiple of G, got {tuple(prefix_lens.shape)}")
+    prefix_table, prefix_stride, prefix_lens = _pages(prefix_table, prefix_lens, groups, "prefix_table", "prefix_lens", dev)
+    page_table, table_stride, seq_lens = _pages(page_table, seq_lens, b, "page_table", "seq_lens", dev)
+    sinks = _sinks(sinks, hq, dev)
+    out = _like(q)
+    lse = torch.empty((b, hq), dtype=torch.float32, device=dev) if return_lse else None
+    if b:
+        need = cache._attention_bytes.get((groups, b, hq))
+        if need is None:
+            with torch.cuda.device(dev):
+                need = cache._attention_bytes[groups, b, hq] = _lib.fp4b_shared_attention_workspace(groups, b, hq, cache.kv_heads, d)
+        ws = _workspace(dev, need)
+        qs = q.stride()
+        _call(dev, _shared_attention, "shared_prefix_attention", _SHARED.pack(
+            q.data_ptr(), qs[0], qs[1], cache._ref, page_table.data_ptr(), table_stride, seq_lens.data_ptr(),
+            _address(sinks), out.data_ptr(), _address(lse), ws.data_ptr(), ws.numel(), b, hq, page_table.shape[1], 0,
+            d ** -0.5 if scale is None else scale, prefix_table.data_ptr(), prefix_stride, prefix_lens.data_ptr(), groups, prefix_table.shape[1]))
     return (out, lse) if return_lse else out
 
 

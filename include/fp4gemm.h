@@ -367,6 +367,24 @@ typedef struct fp4b_decode {
 long fp4b_decode_attention_workspace(int q_heads, int kv_heads, int head_dim);
 int fp4b_decode_attention(const fp4b_decode* call, void* stream);
 
+/* fp4b_decode_attention of sequences that share prefixes: sequence b sees the
+ * prefix_lens[b / (batch / prefixes)] keys found through that row of
+ * prefix_table (int32, row stride prefix_stride, prefix_width entries), then its
+ * own as own.seq_lens and own.page_table say (own.window has to be 0), in one
+ * softmax.  Every prefix is read once for all its sequences.  own.workspace:
+ * fp4b_shared_attention_workspace bytes, as for fp4b_decode_attention.  A wait
+ * inside the kernel that gives up (after 2 s) is recorded as 14 in the device
+ * error word. */
+typedef struct fp4b_shared {
+    fp4b_decode own;
+    const int* prefix_table;
+    long prefix_stride;
+    const int* prefix_lens;
+    int prefixes, prefix_width;
+} fp4b_shared;
+long fp4b_shared_attention_workspace(int prefixes, int batch, int q_heads, int kv_heads, int head_dim);
+int fp4b_shared_attention(const fp4b_shared* call, void* stream);
+
 /* The norms around a block with its gate and residual: of each row
  *   y = x / sqrt(mean(x^2) + eps) * post_weight     (post_weight NULL: y = x)
  *   r = residual + scale * gate * y                 (gate NULL: 1)

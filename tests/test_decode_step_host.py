@@ -1,5 +1,6 @@
 """Host side of the operators that close a decoding step (no GPU): the argument structs and the C entry points' refusals before
 any device work."""
+import ctypes
 import os
 import struct
 import subprocess
@@ -33,6 +34,45 @@ def test_structs_match_the_header(tmp_path, name):
     subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")])
     got = list(map(int, subprocess.check_output([str(tmp_path / "s")], text=True).split()))
     assert got == [form.size] + [struct.calcsize("@" + codes[:i] + "0" + codes[i]) for i in range(len(codes))]
+
+
+def test_shared_struct_matches_the_header(tmp_path):
+    own = ["q", "q_sb", "q_sh", "cache", "page_table", "table_stride", "seq_lens", "sinks", "out", "lse", "workspace", "workspace_bytes", "batch",
+           "q_heads", "table_width", "window", "scale"]
+    members = [f"own.{m}" for m in own] + ["prefix_table", "prefix_stride", "prefix_lens", "prefixes", "prefix_width"]
+    src = '#include <stddef.h>\n#include <stdio.h>\n#include "fp4gemm.h"\nint main(void) {\nprintf("%zu", sizeof(fp4b_shared));\n'
+    src += "".join(f'printf(" %zu", offsetof(fp4b_shared, {m}));\n' for m in members) + "return 0;\n}\n"
+    (tmp_path / "s.c").write_text(src)
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")])
+    got = list(map(int, subprocess.check_output([str(tmp_path / "s")], text=True).split()))
+    codes = "PllPPlPPPPPliiiifPlPii"
+    assert len(codes) == len(members)
+    assert got == [fp4_decode._SHARED.size] + [struct.calcsize("@" + codes[:i] + "0" + codes[i]) for i in range(len(codes))]
+
+
+def shared_call(cache_fields=(), **other):
+    fields = dict(k=0x10000, v=0x20000, k_scale=None, v_scale=None, num_pages=4, kv_heads=2, page_size=16, head_dim=64, kind=0)
+    cache = fp4_decode._CacheView(**{**fields, **dict(cache_fields)})
+    v = dict(q=0x10000, q_sb=512, q_sh=64, cache=ctypes.addressof(cache), page_table=0x20000, table_stride=4, seq_lens=0x30000, sinks=0, out=0x40000,
+             lse=0, workspace=0x50000, workspace_bytes=1 << 40, batch=4, q_heads=8, table_width=4, window=0, scale=0.125, prefix_table=0x60000,
+             prefix_stride=8, prefix_lens=0x70000, prefixes=2, prefix_width=8)
+    v.update(other)
+    return lib.fp4b_shared_attention(fp4_decode._SHARED.pack(*v.values()), None)
+
+
+def test_bad_shared_attention_calls_are_refused():
+    for other in (dict(batch=-1), dict(q_heads=0), dict(q_heads=7), dict(q=0), dict(out=0), dict(seq_lens=0), dict(page_table=0), dict(table_width=-1),
+                  dict(table_stride=3), dict(window=1), dict(window=-1), dict(scale=float("nan")), dict(q=0x10004), dict(q_sb=511), dict(out=0x40008),
+                  dict(workspace=0), dict(workspace=0x50004), dict(prefixes=0), dict(prefixes=-2), dict(prefixes=3), dict(prefix_lens=0),
+                  dict(prefix_table=0), dict(prefix_width=-1), dict(prefix_stride=7), dict(prefix_width=1 << 28, prefix_stride=1 << 28),
+                  dict(batch=1 << 20, prefixes=1 << 20, prefix_width=1 << 12, prefix_stride=1 << 12), dict(cache=0)):
+        assert shared_call(**other) == -1, other
+        assert "fp4b_shared_attention" in last()
+    for bad in (dict(k=None), dict(page_size=24), dict(head_dim=96), dict(kind=1)):
+        assert shared_call(bad) == -1, bad
+    assert lib.fp4b_shared_attention(None, None) == -1
+    assert shared_call(batch=0) == 0
+    assert lib.fp4b_shared_attention_workspace(1, 4, 7, 2, 64) == -1
 
 
 def norm_call(**other):
