@@ -10,13 +10,18 @@
 //
 // Memory-bound: 2 bytes of x, 2 or 4 of r in and out, 2 of h (and 2 of a gate
 // that differs by row) for about 10 operations an element, so a row is read
-// once and stays in its threads' registers over both means.  A thread has 1, 2,
-// 4 or 8 pieces of 8 elements (16 bytes of BF16), loaded before anything is
-// computed; a row of at most 32 pieces a warp is one warp's, a longer one a
-// CTA's.  Rows that do not start on 16 bytes, or whose width is not a multiple
-// of 8, go by single elements, up to 64 a thread.
+// once and stays in its threads' registers over both means.
+// A row is a CTA's, of as many warps as it takes (up to 16384, or 5120, elements), or
+// (wide rows, and rows so few that they leave SMs idle) a cluster's, which sums
+// over distributed shared memory.  One wave of CTAs goes over the rows; the next
+// row's loads start as soon as this one's registers are free, before its second
+// sum.  A thread has two pieces of 8 elements (16 bytes of BF16), or, where the
+// rows do not start on 16 bytes or the width is not a multiple of 8, four of two or
+// eight single ones.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -29,10 +34,12 @@ namespace fp4b {
 namespace {
 
 using namespace decode;
+namespace cg = cooperative_groups;
 
-constexpr int kMaxThreads = 512;
 constexpr int kMaxWidth = 32768;
-constexpr int kRowsPerCta = 4;  // of one warp each
+constexpr int kMaxCtasPerSm = 32;
+constexpr int kMaxCluster = 8;
+constexpr int kLeastWidth = 2048;  // of a CTA of a cluster that is there to fill the GPU
 
 struct NormParams {
     const uint16_t* x;  // null: no block before
@@ -49,171 +56,270 @@ struct NormParams {
     float scale, eps, inv_width;
 };
 
-// A piece of VEC elements as it is loaded: BF16, or FP32 for a residual.
 template <int VEC>
-struct Piece16 {
-    uint32_t w[VEC > 1 ? VEC / 2 : 1];
-    __device__ __forceinline__ void load(const uint16_t* p) {
-        if constexpr (VEC == 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else {
-            w[0] = *p;
-        }
-    }
-    __device__ __forceinline__ float get(int i) const { return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]); }
-};
-template <int VEC>
-struct Piece32 {
-    float f[VEC];
-    __device__ __forceinline__ void load(const float* p) {
-        if constexpr (VEC == 8) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-        } else {
-            f[0] = *p;
-        }
-    }
-    __device__ __forceinline__ float get(int i) const { return f[i]; }
+struct Shape {
+    static constexpr int ITEMS = VEC == 8 ? 2 : 8 / VEC;    // pieces a thread
+    static constexpr int RESIDENT = VEC == 8 ? 1024 : 1280;  // threads of an SM, by their registers
+    static constexpr int THREADS = VEC == 8 ? 1024 : 640;    // of a CTA at most
 };
 
+typedef unsigned long long pair;  // of fp32 values, see decode_core.cuh
+
+// Loads and stores of what lies below `end`, without a branch: zeros beyond it.
+__device__ __forceinline__ uint4 load_below(const uint4* p, int i, int end) {
+    uint4 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %5, %6;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                 "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"(i), "r"(end) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 load_below(const uint2* p, int i, int end) {
+    uint2 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %3, %4;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.v2.b32 {%0, %1}, [%2];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y) : "l"(p), "r"(i), "r"(end) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t load_below(const uint32_t* p, int i, int end) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
+                 : "=&r"(v) : "l"(p), "r"(i), "r"(end) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t load_below(const uint16_t* p, int i, int end) {
+    uint16_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\tmov.b16 %0, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}"
+                 : "=&h"(v) : "l"(p), "r"(i), "r"(end) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_below(const float* p, int i, int end) {
+    float v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.f32 %0, [%1];\n\t}"
+                 : "=&f"(v) : "l"(p), "r"(i), "r"(end) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_below(uint4* p, uint4 v, int i, int end) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %5, %6;\n\t@p st.global.v4.b32 [%0], {%1, %2, %3, %4};\n\t}"
+                 ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(i), "r"(end) : "memory");
+}
+__device__ __forceinline__ void store_below(uint2* p, uint2 v, int i, int end) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %3, %4;\n\t@p st.global.v2.b32 [%0], {%1, %2};\n\t}"
+                 ::"l"(p), "r"(v.x), "r"(v.y), "r"(i), "r"(end) : "memory");
+}
+__device__ __forceinline__ void store_below(uint32_t* p, uint32_t v, int i, int end) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\t@p st.global.b32 [%0], %1;\n\t}" ::"l"(p), "r"(v), "r"(i), "r"(end) : "memory");
+}
+__device__ __forceinline__ void store_below(uint16_t* p, uint32_t v, int i, int end) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\t@p st.global.b16 [%0], %1;\n\t}" ::"l"(p), "h"((uint16_t)v), "r"(i), "r"(end) : "memory");
+}
+__device__ __forceinline__ void store_below(float* p, float v, int i, int end) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\t@p st.global.f32 [%0], %1;\n\t}" ::"l"(p), "f"(v), "r"(i), "r"(end) : "memory");
+}
+
+// A thread's pieces of a BF16 row or weight, two elements a register.  A warp's
+// pieces are one run; `at` is the thread's first element, the next piece's is the
+// 32nd piece on.
 template <int VEC>
-__device__ __forceinline__ void store16(uint16_t* p, const float (&v)[VEC]) {
-    if constexpr (VEC == 8)
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    else
-        *p = (uint16_t)pack_bf16(v[0], 0.0f);
-}
-template <int VEC>
-__device__ __forceinline__ void store32(float* p, const float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        *p = v[0];
-    }
-}
-
-// Sum over the row's threads (all of them get it).
-__device__ __forceinline__ float row_sum(float v, float* slots) {
-    v = group_sum<32>(v);
-    const int warps = blockDim.x >> 5;
-    if (warps == 1) return v;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) slots[warp] = v;
-    __syncthreads();
-    return group_sum<32>(lane < warps ? slots[lane] : 0.0f);
-}
-
-// VEC elements a piece, ITEMS pieces a thread; R32: the residual is fp32.
-template <int VEC, int ITEMS, bool R32>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const __grid_constant__ NormParams p) {
-    __shared__ float sums[2][32];
-    chain();
-    const long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
-    if (row >= p.rows) return;  // (whole warps: a CTA of several rows has a warp for each)
-    using Res = typename std::conditional<R32, Piece32<VEC>, Piece16<VEC>>::type;
-    using R = typename std::conditional<R32, float, uint16_t>::type;
-    const R* residual = static_cast<const R*>(p.residual) + row * p.residual_stride;
-    const uint16_t* x = p.x + row * p.x_stride;
-    const uint16_t* gate = p.gate + row * p.gate_stride;
-
-    Res res[ITEMS];
-    Piece16<VEC> in[ITEMS];
+struct Pieces {
+    static constexpr int ITEMS = Shape<VEC>::ITEMS, WORDS = VEC * ITEMS / 2;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const uint16_t* p, int at, int width) {
+        p += at;
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int i = (k * (int)blockDim.x + (int)threadIdx.x) * VEC;
-        if (i < p.width) {
-            if (p.x) in[k].load(x + i);
-            res[k].load(residual + i);
-        }
-    }
-    float post = p.scale;  // what y is multiplied by besides the weights
-    if (p.x && p.post_weight) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k)
-            if ((k * (int)blockDim.x + (int)threadIdx.x) * VEC < p.width)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) sum = fmaf(in[k].get(e), in[k].get(e), sum);
-        post *= rsqrtf(fmaf(row_sum(sum, sums[0]), p.inv_width, p.eps));
-    }
-    float r[ITEMS][VEC];
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int i = (k * (int)blockDim.x + (int)threadIdx.x) * VEC;
-        if (i < p.width) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) r[k][e] = res[k].get(e);
-            if (p.x) {
-                float f[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) f[e] = in[k].get(e) * post;
-                if (p.post_weight) {
-                    Piece16<VEC> w;
-                    w.load(p.post_weight + i);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) f[e] *= w.get(e);
-                }
-                if (p.gate) {
-                    Piece16<VEC> w;
-                    w.load(gate + i);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) f[e] *= w.get(e);
-                }
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) r[k][e] += f[e];
-                R* to = static_cast<R*>(p.residual_out) + row * p.width + i;
-                if constexpr (R32) store32<VEC>(to, r[k]);
-                else store16<VEC>(to, r[k]);
+        for (int k = 0; k < ITEMS; ++k) {
+            if constexpr (VEC == 8) {
+                const uint4 v = load_below(reinterpret_cast<const uint4*>(p) + 32 * k, at + 256 * k, width);
+                w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+            } else if constexpr (VEC == 2) {
+                w[k] = load_below(reinterpret_cast<const uint32_t*>(p) + 32 * k, at + 64 * k, width);
+            } else {
+                const uint32_t v = load_below(p + 32 * k, at + 32 * k, width);
+                w[k / 2] = k & 1 ? __byte_perm(w[k / 2], v, 0x5410) : v;
             }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum = fmaf(r[k][e], r[k][e], sum);
         }
     }
-    const float factor = rsqrtf(fmaf(row_sum(sum, sums[1]), p.inv_width, p.eps));
+    __device__ __forceinline__ pair get(int i) const { return pair_of(bf16_lo(w[i]), bf16_hi(w[i])); }
+};
+template <int VEC>
+struct Values {
+    static constexpr int ITEMS = Shape<VEC>::ITEMS, WORDS = VEC * ITEMS / 2;
+    pair v[WORDS];
+    __device__ __forceinline__ void load(const float* p, int at, int width) {
+        p += at;
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int i = (k * (int)blockDim.x + (int)threadIdx.x) * VEC;
-        if (i < p.width) {
-            Piece16<VEC> w;
-            w.load(p.weight + i);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) r[k][e] = r[k][e] * factor * w.get(e);
-            store16<VEC>(p.normed + row * p.width + i, r[k]);
+        for (int k = 0; k < ITEMS; ++k) {
+            if constexpr (VEC == 8) {
+                const uint4 a = load_below(reinterpret_cast<const uint4*>(p) + 64 * k, at + 256 * k, width);
+                const uint4 b = load_below(reinterpret_cast<const uint4*>(p) + 64 * k + 1, at + 256 * k, width);
+                v[4 * k] = words(a.x, a.y), v[4 * k + 1] = words(a.z, a.w), v[4 * k + 2] = words(b.x, b.y), v[4 * k + 3] = words(b.z, b.w);
+            } else if constexpr (VEC == 2) {
+                const uint2 a = load_below(reinterpret_cast<const uint2*>(p) + 32 * k, at + 64 * k, width);
+                v[k] = words(a.x, a.y);
+            } else {
+                const float f = load_below(p + 32 * k, at + 32 * k, width);
+                v[k / 2] = k & 1 ? pair_of(first_of(v[k / 2]), f) : pair_of(f, 0.0f);
+            }
         }
+    }
+    __device__ __forceinline__ void store(uint16_t* p, int at, int width) const {
+        p += at;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            if constexpr (VEC == 8)
+                store_below(reinterpret_cast<uint4*>(p) + 32 * k, make_uint4(pack(4 * k), pack(4 * k + 1), pack(4 * k + 2), pack(4 * k + 3)), at + 256 * k, width);
+            else if constexpr (VEC == 2)
+                store_below(reinterpret_cast<uint32_t*>(p) + 32 * k, pack(k), at + 64 * k, width);
+            else
+                store_below(p + 32 * k, k & 1 ? pack(k / 2) >> 16 : pack(k / 2), at + 32 * k, width);
+        }
+    }
+    __device__ __forceinline__ void store(float* p, int at, int width) const {
+        p += at;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            if constexpr (VEC == 8) {
+                store_below(reinterpret_cast<uint4*>(p) + 64 * k, make_uint4(lo(4 * k), hi(4 * k), lo(4 * k + 1), hi(4 * k + 1)), at + 256 * k, width);
+                store_below(reinterpret_cast<uint4*>(p) + 64 * k + 1, make_uint4(lo(4 * k + 2), hi(4 * k + 2), lo(4 * k + 3), hi(4 * k + 3)), at + 256 * k, width);
+            } else if constexpr (VEC == 2) {
+                store_below(reinterpret_cast<uint2*>(p) + 32 * k, make_uint2(lo(k), hi(k)), at + 64 * k, width);
+            } else {
+                store_below(p + 32 * k, k & 1 ? second_of(v[k / 2]) : first_of(v[k / 2]), at + 32 * k, width);
+            }
+        }
+    }
+    __device__ __forceinline__ pair get(int i) const { return v[i]; }
+    __device__ __forceinline__ uint32_t pack(int i) const { return pack_bf16(first_of(v[i]), second_of(v[i])); }
+    static __device__ __forceinline__ pair words(uint32_t a, uint32_t b) { return ((pair)b << 32) | a; }
+    __device__ __forceinline__ uint32_t lo(int i) const { return (uint32_t)v[i]; }
+    __device__ __forceinline__ uint32_t hi(int i) const { return (uint32_t)(v[i] >> 32); }
+};
+__device__ __forceinline__ pair both(float f) { return pair_of(f, f); }
+
+// Sums over a row's threads, in one order for all of them.  They take two sets
+// of slots in turn: one is written again behind the barrier of the other.
+struct Slots {
+    float warp[2][32], cta[2][kMaxCluster];
+};
+__device__ __forceinline__ float row_sum(float v, Slots& s, int& turn, int ctas) {
+    v = group_sum<32>(v);
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warps > 1) {
+        if (lane == 0) s.warp[turn][warp] = v;
+        __syncthreads();
+        v = group_sum<32>(lane < warps ? s.warp[turn][lane] : 0.0f);
+    }
+    if (ctas > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if ((int)threadIdx.x < ctas) cluster.map_shared_rank(s.cta[turn], threadIdx.x)[cluster.block_rank()] = v;
+        cluster.sync();
+        v = group_sum<kMaxCluster>(lane % kMaxCluster < ctas ? s.cta[turn][lane % kMaxCluster] : 0.0f);
+    }
+    turn ^= 1;
+    return v;
+}
+
+// The arithmetic of a row, in three steps between which its threads meet.
+template <int VEC>
+__device__ __forceinline__ float squares(const Pieces<VEC>& x) {
+    pair sum = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < Pieces<VEC>::WORDS; ++i) sum = fma2(x.get(i), x.get(i), sum);
+    return first_of(sum) + second_of(sum);
+}
+// r, the residual, becomes r'; returns its squares' sum.
+template <int VEC, bool POST, bool GATE>
+__device__ __forceinline__ float block_end(Values<VEC>& r, const Pieces<VEC>& x, const Pieces<VEC>& post_weight, const Pieces<VEC>& gate, float factor) {
+    pair sum = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < Pieces<VEC>::WORDS; ++i) {
+        pair f = both(factor);
+        if constexpr (POST) f = mul2(f, post_weight.get(i));
+        if constexpr (GATE) f = mul2(f, gate.get(i));
+        r.v[i] = fma2(x.get(i), f, r.v[i]);
+        sum = fma2(r.v[i], r.v[i], sum);
+    }
+    return first_of(sum) + second_of(sum);
+}
+template <int VEC>
+__device__ __forceinline__ void norm_begin(Values<VEC>& r, const Pieces<VEC>& weight, float factor) {
+#pragma unroll
+    for (int i = 0; i < Pieces<VEC>::WORDS; ++i) r.v[i] = mul2(mul2(r.v[i], both(factor)), weight.get(i));
+}
+
+template <int VEC, typename R, bool POST, bool GATE>
+__global__ void __launch_bounds__(Shape<VEC>::THREADS, Shape<VEC>::RESIDENT / Shape<VEC>::THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
+    __shared__ Slots slots;
+    chain();
+    const int ctas = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+    const int warp = rank * (int)(blockDim.x >> 5) + (int)(threadIdx.x >> 5);
+    const int at = (warp * 32 * Shape<VEC>::ITEMS + (int)(threadIdx.x & 31)) * VEC;  // the thread's first element
+    const int each = (int)gridDim.x / ctas;  // rows at once
+    int turn = 0;
+    Pieces<VEC> x, gate;
+    typename std::conditional<sizeof(R) == 2, Pieces<VEC>, Values<VEC>>::type residual;
+#pragma unroll
+    for (int i = 0; i < Pieces<VEC>::WORDS; ++i) x.w[i] = 0u;
+    auto load = [&](long row) {
+        if (p.x) x.load(p.x + row * p.x_stride, at, p.width);
+        residual.load(static_cast<const R*>(p.residual) + row * p.residual_stride, at, p.width);
+        if constexpr (GATE) gate.load(p.gate + row * p.gate_stride, at, p.width);
+    };
+    long row = blockIdx.x / ctas;
+    load(row);
+    for (; row < p.rows; row += each) {
+        float factor = p.scale;  // what x is multiplied by besides the weights
+        Pieces<VEC> weight;
+        if constexpr (POST) {
+            weight.load(p.post_weight, at, p.width);
+            factor *= rsqrtf(fmaf(row_sum(squares<VEC>(x), slots, turn, ctas), p.inv_width, p.eps));
+        }
+        Values<VEC> r;
+#pragma unroll
+        for (int i = 0; i < Pieces<VEC>::WORDS; ++i) r.v[i] = residual.get(i);
+        const float sum = block_end<VEC, POST, GATE>(r, x, weight, gate, factor);
+        if (row + each < p.rows) load(row + each);
+        weight.load(p.weight, at, p.width);
+        if (p.x) r.store(static_cast<R*>(p.residual_out) + row * p.width, at, p.width);
+        norm_begin<VEC>(r, weight, rsqrtf(fmaf(row_sum(sum, slots, turn, ctas), p.inv_width, p.eps)));
+        r.store(p.normed + row * p.width, at, p.width);
     }
 }
 
-template <int VEC, int ITEMS, bool R32>
+template <int VEC, typename R, bool POST, bool GATE>
 cudaError_t launch(const NormParams& p, cudaStream_t st) {
-    const int pieces = (p.width + VEC - 1) / VEC;
-    const int threads = ((pieces + ITEMS - 1) / ITEMS + 31) / 32 * 32;
-    const int per = threads == 32 ? kRowsPerCta : 1;
+    using S = Shape<VEC>;
+    const int pieces = (p.width + VEC - 1) / VEC, sms = device_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    int ctas = 1;
+    while (pieces > ctas * S::ITEMS * S::THREADS || (ctas < kMaxCluster && (long)p.rows * ctas * 2 <= sms && p.width >= ctas * 2 * kLeastWidth)) ctas *= 2;
+    const int threads = ((pieces + ctas * S::ITEMS - 1) / (ctas * S::ITEMS) + 31) / 32 * 32;
+    const int resident = std::min(kMaxCtasPerSm, S::RESIDENT / threads);
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)((p.rows + per - 1) / per));
-    config.blockDim = dim3(threads, per);
+    config.gridDim = dim3((unsigned)std::min(p.rows, sms * resident / ctas) * (unsigned)ctas);
+    config.blockDim = dim3(threads);
     config.stream = st;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, block_norm_kernel<VEC, ITEMS, R32>, p);
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = (unsigned)ctas, attributes[1].val.clusterDim.y = 1, attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = ctas > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, block_norm_kernel<VEC, R, POST, GATE>, p);
 }
 
-template <bool R32>
-cudaError_t launch_width(const NormParams& p, bool pieces, cudaStream_t st) {
-    if (pieces) {
-        const int n = p.width / 8;
-        return n <= 2 * kMaxThreads ? launch<8, 2, R32>(p, st) : n <= 4 * kMaxThreads ? launch<8, 4, R32>(p, st) : launch<8, 8, R32>(p, st);
-    }
-    return p.width <= 8 * kMaxThreads ? launch<1, 8, R32>(p, st) : p.width <= 16 * kMaxThreads ? launch<1, 16, R32>(p, st) : launch<1, 64, R32>(p, st);
+template <int VEC, typename R>
+cudaError_t launch_parts(const NormParams& p, cudaStream_t st) {
+    return p.post_weight ? (p.gate ? launch<VEC, R, true, true>(p, st) : launch<VEC, R, true, false>(p, st))
+                         : (p.gate ? launch<VEC, R, false, true>(p, st) : launch<VEC, R, false, false>(p, st));
+}
+template <typename R>
+cudaError_t launch_width(const NormParams& p, int piece, cudaStream_t st) {
+    return piece == 8 ? launch_parts<8, R>(p, st) : piece == 2 ? launch_parts<2, R>(p, st) : launch_parts<1, R>(p, st);
 }
 
 bool whole(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
-bool sixteen(const void* p, long stride, int size) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0; }
+// Are all rows aligned to pieces of `piece` elements?
+bool aligned(const void* p, long stride, int size, int piece) { return whole(p, piece * 2) && stride % piece == 0 && (size == 2 || whole(p, std::min(piece * 4, 16))); }
 
 }  // namespace
 }  // namespace fp4b
@@ -226,7 +332,7 @@ FP4B_EXPORT int fp4b_block_norm(const fp4b_norm* call, void* stream) {
         why = "null arguments";
     } else {
         const fp4b_norm& c = *call;
-        if (c.rows < 0) why = "negative rows";
+        if (c.rows < 0 || c.rows > (1 << 28)) why = "rows must be 0 to 2^28";
         else if (c.width <= 0 || c.width > kMaxWidth) why = "the width must be 1 to 32768";
         else if (c.rows > 0 && (!c.residual || !c.weight || !c.normed || (c.x && !c.residual_out))) why = "null tensor";
         else if (!c.x && (c.post_weight || c.gate)) why = "a gate and a norm after the block need the block's output";
@@ -249,9 +355,12 @@ FP4B_EXPORT int fp4b_block_norm(const fp4b_norm* call, void* stream) {
     p.normed = static_cast<uint16_t*>(c.normed), p.residual_out = c.residual_out;
     p.rows = c.rows, p.width = c.width, p.scale = c.scale, p.eps = c.eps, p.inv_width = 1.0f / (float)c.width;
     const int size = c.residual_fp32 ? 4 : 2;
-    const bool pieces = c.width % 8 == 0 && sixteen(c.x, c.x_stride, 2) && sixteen(c.residual, c.residual_stride, size) &&
-                        sixteen(c.gate, c.gate_stride, 2) && sixteen(c.weight, 0, 2) && sixteen(c.post_weight, 0, 2) &&
-                        sixteen(c.normed, 0, 2) && sixteen(c.residual_out, 0, size);
+    int piece = 8;
+    auto fits = [&](int n) {
+        return c.width % n == 0 && aligned(c.x, c.x_stride, 2, n) && aligned(c.residual, c.residual_stride, size, n) && aligned(c.gate, c.gate_stride, 2, n) &&
+               aligned(c.weight, 0, 2, n) && aligned(c.post_weight, 0, 2, n) && aligned(c.normed, 0, 2, n) && aligned(c.residual_out, 0, size, n);
+    };
+    while (!fits(piece)) piece = piece == 8 ? 2 : 1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return launch_status(c.residual_fp32 ? launch_width<true>(p, pieces, st) : launch_width<false>(p, pieces, st), "fp4b_block_norm");
+    return launch_status(c.residual_fp32 ? launch_width<float>(p, piece, st) : launch_width<uint16_t>(p, piece, st), "fp4b_block_norm");
 }

@@ -202,19 +202,18 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
     };
     // A bounded wait of a whole warp; false when it gave up or another role did.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        bool ok = ptx::mbar_try_wait(bar, parity);
-        if (!ok) {
-            const uint64_t t0 = ptx::global_timer_ns();
-            for (uint32_t i = 1;; ++i) {
-                ok = ptx::mbar_try_wait(bar, parity);
-                if (ok) break;
-                if ((i & 63u) == 0) {
-                    if (*(volatile int*)&s_abort) break;
-                    if (ptx::global_timer_ns() - t0 > ptx::kSpinLimitNs) {
-                        *(volatile int*)&s_abort = 1;
-                        report(p.err, kErrPrefixTimeout);
-                        break;
-                    }
+        bool ok;
+        uint64_t t0 = 0;
+        for (uint32_t i = 1; !(ok = ptx::mbar_try_wait(bar, parity)); ++i) {
+            if ((i & 63u) == 0) {  // (the timer is slow to read)
+                if (*(volatile int*)&s_abort) break;
+                const uint64_t t = ptx::global_timer_ns();
+                if (t0 == 0) {
+                    t0 = t;
+                } else if (t - t0 > ptx::kSpinLimitNs) {
+                    *(volatile int*)&s_abort = 1;
+                    report(p.err, kErrPrefixTimeout);
+                    break;
                 }
             }
         }

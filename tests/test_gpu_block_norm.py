@@ -58,7 +58,7 @@ def inputs(t, h, cuda, kind, seed=0):
     return randn(t, h).bfloat16(), residual, weights, [None, (1 + 0.3 * randn(h)).bfloat16(), torch.sigmoid(randn(t, h)).bfloat16()]
 
 
-WIDTHS = [1, 2, 7, 8, 31, 64, 255, 256, 264, 1000, 1001, 2880, 4096, 4097, 5003, 8192, 8193, 16384, 16392, 20001, 32760, 32767, 32768]
+WIDTHS = [1, 2, 6, 7, 8, 31, 64, 255, 256, 264, 1000, 1001, 2880, 4096, 4097, 5003, 5118, 5120, 5122, 8192, 8193, 16384, 16392, 20001, 32750, 32760, 32767, 32768]
 
 
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
