@@ -83,6 +83,10 @@ cudaError_t gemm_launch_peers(const GemmArgs& g, void* const* peers, int npeers,
 
 
 
+// The CUtensorMap of a byte matrix [rows, row_bytes] that is loaded in boxes of
+// 128 bytes x box_rows with the 128-byte swizzle; false if it cannot be made.
+bool make_byte_map(void* map, const void* base, long rows, long row_bytes, int box_rows);
+
 // Read-only view of a weight-cache handle created by the C ABI.
 struct CacheView {
     const uint8_t* fp4;

@@ -1684,4 +1684,8 @@ cudaError_t gemm_launch(const GemmArgs& g, cudaStream_t stream) {
     }
 }
 
+bool make_byte_map(void* map, const void* base, long rows, long row_bytes, int box_rows) {
+    return make_operand_map(static_cast<CUtensorMap*>(map), base, rows, 2 * row_bytes, box_rows);
+}
+
 }  // namespace fp4b

@@ -10,8 +10,9 @@
 //
 // A CTA, one an SM, takes a share of all tiles of keys (128, or 64 of 256
 // elements): unit by unit (prefix, key head, 128 rows), a tile at a time.
-//   warps 8-11 (4-7)   read pages, decode them to 16 bits, write K and V in the
-//                      128-byte swizzle;
+//   warps 8-11 (4-7)   bring K and V in 16 bits and the 128-byte swizzle, two warps
+//                      each: bf16 by TMA boxes of whole pages, fp8 and nvfp4
+//                      decoded on the way;
 //   warp 12 (8)        issues the products: S of the next tile before O of this;
 //   warps 0-7 (0-3)    two groups of 128 threads, a row a thread, take the tiles
 //                      in turn: each has scores, sums and an O of its own, so
@@ -26,6 +27,8 @@
 //
 // What the parts of a unit found (two for each CTA that has tiles of it) goes to
 // the workspace, with the place and the number of each unit's parts.
+#include <cuda.h>
+
 #include "decode_attention.cuh"
 
 #define FP4B_EXPORT extern "C" __attribute__((visibility("default")))
@@ -54,6 +57,8 @@ struct PrefixParams {
     int2* units;
     float2* ml;
     float* acc;
+    int runs;           // of a tile's rows that are copied as boxes; 0: row by row
+    alignas(64) CUtensorMap k_map, v_map;  // of the pages' rows (bf16)
 };
 
 template <int KIND, int D>
@@ -66,20 +71,21 @@ struct PrefixCfg {
     static constexpr int Q = kTileRows * D * 2;
     static constexpr int PIECE = TK * D * 2;                                         // K or V of a tile in 16 bits
     static constexpr int STAGES = KIND == kKvBf16 ? (D == 64 ? 5 : D == 128 ? 3 : 2) : D == 64 ? 3 : 2;
-    static constexpr int RAW = KIND == kKvBf16 ? 0 : TK * (RB + SB);                 // a piece as it lies in the cache
-    static constexpr int RAWS = KIND == kKvBf16 ? 0 : KIND == kKvFp8 ? (D == 64 ? 8 : D == 128 ? 3 : 2) : D == 64 ? 8 : D == 128 ? 6 : 3;
-    // Pieces on their way.  BF16 is copied in place: with this many the wait for a
-    // free stage is never one for a product that waits for the piece at hand.
-    static constexpr int AHEAD = KIND == kKvBf16 ? 2 * STAGES - 3 : RAWS - 1;
+    // fp8 and nvfp4 come through a ring of half pieces as they lie in the cache: of K,
+    // and of V (with fp8's scales of both).
+    static constexpr int HALF_K = KIND == kKvBf16 ? 0 : TK / 2 * (RB + (KIND == kKvFp8 ? 0 : SB));
+    static constexpr int HALF_V = KIND == kKvBf16 ? 0 : TK / 2 * (RB + (KIND == kKvFp8 ? 2 * SB : SB));
+    static constexpr int HALVES = KIND == kKvFp8 ? (D == 64 ? 6 : D == 128 ? 3 : 2) : D == 64 ? 6 : D == 128 ? 4 : 3;
     static constexpr int SCALES = KIND == kKvFp8 ? 3 * TK * 4 : 0;                   // of a stage: key scales, value scales, their logarithms
-    static constexpr int S_COLUMNS = 2 * TK;
-    static constexpr int OFF_K = Q, OFF_V = OFF_K + STAGES * PIECE, OFF_RAW = OFF_V + STAGES * PIECE;
-    static constexpr int OFF_SCALES = OFF_RAW + RAWS * RAW, OFF_BARS = OFF_SCALES + STAGES * SCALES;
-    static constexpr int OFF_FACTORS = OFF_BARS + (4 * STAGES + 8) * 8, OFF_VARS = OFF_FACTORS + kTileRows * 4;
+    static constexpr int BUFFERS = D == 64 ? 3 : 2;                                  // of S in TMEM
+    static constexpr int S_COLUMNS = BUFFERS * TK;
+    static constexpr int OFF_K = Q, OFF_V = OFF_K + STAGES * PIECE, OFF_RAW_K = OFF_V + STAGES * PIECE, OFF_RAW_V = OFF_RAW_K + HALVES * HALF_K;
+    static constexpr int OFF_SCALES = OFF_RAW_V + HALVES * HALF_V, OFF_BARS = OFF_SCALES + STAGES * SCALES;
+    static constexpr int OFF_FACTORS = OFF_BARS + (4 * STAGES + 2 * BUFFERS + 5 + (KIND == kKvBf16 ? 0 : 4 * HALVES)) * 8, OFF_VARS = OFF_FACTORS + kTileRows * 4;  // (each a multiple of 8)
     static constexpr int SMEM = OFF_VARS + 32;
     static_assert(SMEM <= kSmemMost, "shared memory");
     static_assert(S_COLUMNS + GROUPS * D <= 512, "TMEM");
-    static_assert(OFF_RAW % 1024 == 0 && RAW % 16 == 0 && OFF_SCALES % 16 == 0 && OFF_BARS % 8 == 0, "alignment");
+    static_assert(HALF_K % 32 == 0 && HALF_V % 32 == 0 && OFF_SCALES % 16 == 0 && OFF_BARS % 8 == 0, "alignment");
 };
 
 // The tiles of this CTA, unit by unit: every role goes over them by itself.
@@ -116,7 +122,11 @@ __device__ __forceinline__ bool next_unit(const PrefixParams& p, Walk& w) {
     return true;
 }
 
-__device__ __forceinline__ float at(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 template <int KIND, int D>
 __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attention_kernel(const __grid_constant__ PrefixParams p) {
@@ -132,7 +142,8 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
     int &s_abort = vars[1], &s_total = vars[2], &s_g = vars[3], &s_before = vars[4];
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
     uint64_t *const k_full = bars, *const k_empty = bars + STAGES, *const v_full = bars + 2 * STAGES, *const v_empty = bars + 3 * STAGES;
-    uint64_t *const s_full = bars + 4 * STAGES, *const p_full = s_full + 2, *const q_full = s_full + 4, *const o_done = s_full + 5, *const unit_done = s_full + 6, *const drained = s_full + 7;
+    uint64_t *const s_full = bars + 4 * STAGES, *const p_full = s_full + C::BUFFERS, *const q_full = p_full + C::BUFFERS, *const o_done = q_full + 1;
+    uint64_t *const unit_done = q_full + 3, *const drained = q_full + 4, *const raw_full = q_full + 5;  // (o_done: of each group)
 
     chain();
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -142,11 +153,13 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
     if (tid == 0) {
         s_abort = 0;
         for (int i = 0; i < STAGES; ++i) {
-            ptx::mbar_init(k_full + i, kProducers), ptx::mbar_init(v_full + i, kProducers);
+            ptx::mbar_init(k_full + i, kProducers / 2), ptx::mbar_init(v_full + i, kProducers / 2);
             ptx::mbar_init(k_empty + i, 1), ptx::mbar_init(v_empty + i, 1);
         }
-        for (int i = 0; i < 2; ++i) ptx::mbar_init(s_full + i, 1), ptx::mbar_init(p_full + i, 128);
-        ptx::mbar_init(q_full, GROUPS * 128), ptx::mbar_init(o_done, 1), ptx::mbar_init(unit_done, 1), ptx::mbar_init(drained, 1);
+        for (int i = 0; i < C::BUFFERS; ++i) ptx::mbar_init(s_full + i, 1), ptx::mbar_init(p_full + i, 128);
+        ptx::mbar_init(q_full, GROUPS * 128), ptx::mbar_init(o_done, 1), ptx::mbar_init(o_done + 1, 1), ptx::mbar_init(unit_done, 1), ptx::mbar_init(drained, 1);
+        if (!kBf16)
+            for (int i = 0; i < 4 * C::HALVES; ++i) ptx::mbar_init(raw_full + i, 1);
         ptx::fence_mbar_init();
     }
     if (warp == kMmaWarp) {
@@ -220,6 +233,13 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
         return (bool)__all_sync(0xffffffffu, ok);
     };
 
+    // Rows take more registers than a block has for each thread, the others fewer:
+    // 256 x 184 + 256 x 72 = 512 x 128.
+    if constexpr (GROUPS == 2) {
+        if (warp < kProducerWarp) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    }
+
     if (working && warp < kProducerWarp) {
         // ------------------------------------------------------------ a row a thread: queries, softmax, results
         const int mine = warp >> 2, row = tid & 127;
@@ -230,48 +250,45 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
         while (ok && next_unit<TK>(p, walk)) {
             const int rows = min(kTileRows, p.rows - walk.tile * kTileRows);
             const bool live = (warp & 3) * 32 < rows;
-            if (mine == 0) {
-                // ---- this row of Q, in 16 bits and swizzled; rows that there are not as zeros
-                const int r = walk.tile * kTileRows + row, of = r / p.group;
-                const bool there = row < rows;
-                const uint16_t* from = p.q + (size_t)(walk.g * p.each + (there ? of : 0)) * p.q_sb +
-                                       (size_t)(walk.kv_head * p.group + (there ? r - of * p.group : 0)) * p.q_sh;
-                float up = 1.0f, factor = p.scale2;
-                if constexpr (!kBf16) {
-                    uint32_t top = 0;
-                    for (int d = 0; d < D; d += 4) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(from + d);
-                        top = max(top, max((w.x & 0x7FFFu) << 16, w.x & 0x7FFF0000u));
-                        top = max(top, max((w.y & 0x7FFFu) << 16, w.y & 0x7FFF0000u));
-                    }
-                    const int k = min(max(141 - (int)(top >> 23), -126), 126);
-                    up = __int_as_float((127 + k) << 23);
-                    factor *= __int_as_float((127 - k) << 23);
-                    if (KIND == kKvNvfp4) factor *= kScaleUnit;
-                }
-                s_factor[row] = factor;
-#pragma unroll 4
-                for (int c = 0; c < D / 8; ++c) {
+            {
+                // ---- Q in 16 bits and swizzled, 8 elements a lane; rows that there are not as zeros
+                constexpr int LANES = D / 8, AT_ONCE = GROUPS * 128 / LANES, PASSES = kTileRows / AT_ONCE;
+                const int c = tid % LANES;
+                const uint32_t sign = p.scale2 < 0.0f ? 0x80008000u : 0u;  // goes to the queries
+#pragma unroll 8
+                for (int i = 0; i < PASSES; ++i) {
+                    const int r = i * AT_ONCE + tid / LANES, all = walk.tile * kTileRows + r, of = all / p.group;
                     uint2 a = make_uint2(0u, 0u), b = a;
-                    if (there) a = *reinterpret_cast<const uint2*>(from + 8 * c), b = *reinterpret_cast<const uint2*>(from + 8 * c + 4);
-                    if constexpr (!kBf16) {
-                        a = make_uint2(pack_f16(bf16_lo(a.x) * up, bf16_hi(a.x) * up), pack_f16(bf16_lo(a.y) * up, bf16_hi(a.y) * up));
-                        b = make_uint2(pack_f16(bf16_lo(b.x) * up, bf16_hi(b.x) * up), pack_f16(bf16_lo(b.y) * up, bf16_hi(b.y) * up));
+                    if (r < rows) {
+                        const uint16_t* from = p.q + (size_t)(walk.g * p.each + of) * p.q_sb + (size_t)(walk.kv_head * p.group + all - of * p.group) * p.q_sh + 8 * c;
+                        a = *reinterpret_cast<const uint2*>(from), b = *reinterpret_cast<const uint2*>(from + 4);
                     }
-                    const int at = (c >> 3) * (kTileRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                    *reinterpret_cast<uint4*>(smem + at) = make_uint4(a.x, a.y, b.x, b.y);
+                    float factor = fabsf(p.scale2);
+                    if constexpr (!kBf16) {
+                        auto largest = [](uint32_t w) { return max((w & 0x7FFFu) << 16, w & 0x7FFF0000u); };
+                        const uint32_t top = group_umax<LANES>(max(max(largest(a.x), largest(a.y)), max(largest(b.x), largest(b.y))));
+                        const int k = min(max(141 - (int)(top >> 23), -126), 126);
+                        const float up = __int_as_float((127 + k) << 23);
+                        factor *= __int_as_float((127 - k) << 23);
+                        if (KIND == kKvNvfp4) factor *= kScaleUnit;
+                        auto half = [&](uint32_t w) { return pack_f16(bf16_lo(w) * up, bf16_hi(w) * up); };
+                        a = make_uint2(half(a.x), half(a.y)), b = make_uint2(half(b.x), half(b.y));
+                    }
+                    if (c == 0) s_factor[r] = fmaxf(factor, 0x1p-126f);  // (masked keys' -inf stays one where scale is 0)
+                    const int to = (c >> 3) * (kTileRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(smem + to) = make_uint4(a.x ^ sign, a.y ^ sign, b.x ^ sign, b.y ^ sign);
                 }
                 ptx::fence_proxy_async_smem();
             }
-            ptx::mbar_arrive(q_full);  // (both groups: neither falls a unit behind)
+            ptx::mbar_arrive(q_full);
             ok = wait(q_full, segment & 1);
             const float f = s_factor[row];
             float ref = kNoScore, l = 0.0f;
             bool begun = false;
             for (int j = walk.r0; ok && j < walk.r1; ++j, ++it) {
                 if (GROUPS == 2 && (it & 1) != mine) continue;
-                const int buf = it & 1, stage = it % STAGES;
-                ok = wait(s_full + buf, (it >> 1) & 1);
+                const int buf = it % C::BUFFERS, stage = it % STAGES;
+                ok = wait(s_full + buf, (it / C::BUFFERS) & 1);
                 if (KIND == kKvFp8 && ok) ok = wait(v_full + stage, (it / STAGES) & 1);
                 if (!ok) break;
                 ptx::tc_fence_after();
@@ -279,39 +296,46 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                     const uint32_t s_at = lanes + buf * TK;
                     const float4* const scales = reinterpret_cast<const float4*>(smem + C::OFF_SCALES + stage * C::SCALES);
                     const int seen = walk.valid - j * TK;  // keys of the tile that there are
-                    // ---- the largest score, in base 2 (for fp8 with the value scale's share)
-                    float top = -INFINITY;
-                    auto largest = [&](auto whole) {
+                    float s[TK];
 #pragma unroll
-                        for (int c = 0; c < TK / 32; ++c) {
-                            uint32_t s[32];
-                            ptx::tmem_ld_32x32b_x32(s_at + 32 * c, s);
-                            ptx::tmem_ld_wait();
+                    for (int c = 0; c < TK / 32; ++c) ptx::tmem_ld_32x32b_x32(s_at + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
+                    ptx::tmem_ld_wait();
+                    if constexpr (KIND == kKvFp8) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                float x[4];
-                                [[maybe_unused]] float4 ks, lv;
-                                if constexpr (KIND == kKvFp8) ks = scales[8 * c + i / 4], lv = scales[TK / 2 + 8 * c + i / 4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    x[e] = __uint_as_float(s[i + e]);
-                                    if constexpr (KIND == kKvFp8) x[e] = fmaf(x[e] * at(ks, e), f, at(lv, e));
-                                    else x[e] *= f;
-                                    if (!decltype(whole)::value && 32 * c + i + e >= seen) x[e] = -INFINITY;
-                                }
-                                top = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
-                            }
+                        for (int i = 0; i < TK; i += 4) {
+                            const float4 ks = scales[i / 4];
+                            s[i] *= ks.x, s[i + 1] *= ks.y, s[i + 2] *= ks.z, s[i + 3] *= ks.w;
                         }
-                    };
-                    if (seen >= TK) largest(std::true_type{});
-                    else largest(std::false_type{});
+                    }
+                    if (seen < TK) {
+#pragma unroll
+                        for (int i = 0; i < TK; ++i)
+                            if (i >= seen) s[i] = -INFINITY;
+                    }
+                    // ---- the largest score, in base 2 (for fp8 with the value scale's share); f is not negative
+                    float top = -INFINITY, other = -INFINITY;
+                    const unsigned long long ff = pair_of(f, f);
+                    if constexpr (KIND == kKvFp8) {
+#pragma unroll
+                        for (int i = 0; i < TK; i += 4) {
+                            const float4 lv = scales[TK / 2 + i / 4];
+                            const unsigned long long a = fma2(pair_of(s[i], s[i + 1]), ff, pair_of(lv.x, lv.y)), b = fma2(pair_of(s[i + 2], s[i + 3]), ff, pair_of(lv.z, lv.w));
+                            top = max3(top, first_of(a), second_of(a));
+                            other = max3(other, first_of(b), second_of(b));
+                        }
+                        top = fmaxf(top, other);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < TK; i += 4) top = max3(top, s[i], s[i + 1]), other = max3(other, s[i + 2], s[i + 3]);
+                        top = fmaxf(top, other) * f;
+                    }
                     // ---- the reference moves when a score of the warp's passes it by too much
                     if (__any_sync(0xffffffffu, top > ref + kHeadroom)) {
                         const float to = fmaxf(ref, top - kBelowMax), c = exp2_approx(ref - to);
                         ref = to;
                         l *= c;
                         if (begun) {
-                            if (GROUPS == 1) ok = wait(o_done, (it - 1) & 1);  // (two groups: the scores came after it)
+                            ok = wait(o_done + mine, (it / GROUPS - 1) & 1);  // the group's last product
                             ptx::tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < D; d += 32) {
@@ -325,47 +349,36 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                         }
                     }
                     // ---- weights: 32 scores to 16 columns of their rounding and 16 of what that left
-                    const unsigned long long ff = pair_of(f, f), rr = pair_of(-ref, -ref);
-                    unsigned long long sum = pair_of(0.0f, 0.0f);
-                    auto weigh = [&](auto whole) {
+                    const unsigned long long rr = pair_of(-ref, -ref), less = pair_of(-1.0f, -1.0f);
+                    unsigned long long sum[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll
-                        for (int c = 0; c < TK / 32; ++c) {
-                            uint32_t s[32], w[32];
-                            ptx::tmem_ld_32x32b_x32(s_at + 32 * c, s);
-                            ptx::tmem_ld_wait();
+                    for (int c = 0; c < TK / 32; ++c) {
+                        uint32_t w[32];
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                unsigned long long x = pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                                [[maybe_unused]] float4 ks, vs;
-                                if constexpr (KIND == kKvFp8) {
-                                    ks = scales[8 * c + i / 4], vs = scales[TK / 4 + 8 * c + i / 4];
-                                    x = mul2(x, pair_of(at(ks, i & 2), at(ks, (i & 2) + 1)));
-                                }
-                                x = fma2(x, ff, rr);
-                                float a = exp2_approx(first_of(x)), b = exp2_approx(second_of(x));
-                                if constexpr (!decltype(whole)::value) {
-                                    if (32 * c + i >= seen) a = 0.0f;
-                                    if (32 * c + i + 1 >= seen) b = 0.0f;
-                                }
-                                sum = add2(sum, pair_of(a, b));
-                                if constexpr (KIND == kKvFp8) a *= at(vs, i & 2), b *= at(vs, (i & 2) + 1);
-                                if constexpr (kBf16) {
-                                    const uint32_t hi = pack_bf16(a, b);
-                                    w[i / 2] = hi;
-                                    w[16 + i / 2] = pack_bf16(a - bf16_lo(hi), b - bf16_hi(hi));
-                                } else {
-                                    const uint32_t hi = pack_f16(a, b);
-                                    const float2 back = f16x2_to_float2(hi);
-                                    w[i / 2] = hi;
-                                    w[16 + i / 2] = pack_f16(a - back.x, b - back.y);
-                                }
+                        for (int i = 0; i < 32; i += 2) {
+                            const int k = 32 * c + i;
+                            const unsigned long long x = fma2(pair_of(s[k], s[k + 1]), ff, rr);
+                            unsigned long long e = pair_of(exp2_approx(first_of(x)), exp2_approx(second_of(x)));
+                            sum[i / 2 % 2] = add2(sum[i / 2 % 2], e);
+                            if constexpr (KIND == kKvFp8) {
+                                const float4 vs = scales[TK / 4 + k / 4];
+                                e = mul2(e, i & 2 ? pair_of(vs.z, vs.w) : pair_of(vs.x, vs.y));
                             }
-                            ptx::tmem_st_32x32b_x32(s_at + 32 * c, w);
+                            if constexpr (kBf16) {
+                                w[i / 2] = pack_bf16(first_of(e), second_of(e));
+                                e = fma2(pair_of(bf16_lo(w[i / 2]), bf16_hi(w[i / 2])), less, e);
+                                w[16 + i / 2] = pack_bf16(first_of(e), second_of(e));
+                            } else {
+                                w[i / 2] = pack_f16(first_of(e), second_of(e));
+                                const float2 back = f16x2_to_float2(w[i / 2]);
+                                e = fma2(pair_of(back.x, back.y), less, e);
+                                w[16 + i / 2] = pack_f16(first_of(e), second_of(e));
+                            }
                         }
-                    };
-                    if (seen >= TK) weigh(std::true_type{});
-                    else weigh(std::false_type{});
-                    l += first_of(sum) + second_of(sum);
+                        ptx::tmem_st_32x32b_x32(s_at + 32 * c, w);
+                    }
+                    sum[0] = add2(sum[0], sum[1]);
+                    l += first_of(sum[0]) + second_of(sum[0]);
                     ptx::tmem_st_wait();
                 }
                 begun = true;
@@ -398,132 +411,226 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
         }
     } else if (working && warp < kMmaWarp) {
         // ------------------------------------------------------------ pages to K and V in shared memory
-        const int my = warp - kProducerWarp;
-        constexpr int ROWS = TK / 4;                     // of a tile, a warp
-        constexpr int LR = RB / 16, PER = 32 / LR;       // lanes a row, rows an instruction
-        constexpr int COPIES = ROWS / PER;
+        // Two warps for K, two for V; each warp has half of a tile's rows.
+        const bool value = warp >= kProducerWarp + 2;
+        const int my = warp & 1;
+        constexpr int ROWS = TK / 2;
+        constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
         const int sub = lane / LR, c = lane % LR;
-        uint8_t* const raw = smem + C::OFF_RAW;
-        // pieces: K and V of each tile in turn; `there` is on its way, `here` is decoded
-        Walk there = walk, here = walk;
-        bool more = next_unit<TK>(p, there), ok = true;
-        int tile = there.r0, issued = 0, row = -1, page = -2;
-        auto look = [&]() {  // the page of this lane's key of the tile, on its way; -2 for no key
-            const int key = tile * TK + my * ROWS + lane;
-            page = lane < ROWS && key < there.valid ? max(p.table[(size_t)there.g * p.table_stride + (key >> p.page_shift)], -1) : -2;
+        uint64_t *const full = value ? v_full : k_full, *const empty = value ? v_empty : k_empty;
+        uint8_t* const pieces = smem + (value ? C::OFF_V : C::OFF_K);
+        const uint8_t* const from = static_cast<const uint8_t*>(value ? p.cache.v : p.cache.k);
+        bool ok = true;
+        int t = 0;
+        auto row_of = [&](int page, int key) {  // in the cache; -1: none to read
+            if (page >= 0 && page < p.cache.num_pages)
+                return (page * p.cache.kv_heads + walk.kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
+            if (page != -2) report(p.err, kErrPageRange);
+            return -1;
         };
-        if (more) look();
-        // Starts the copy of piece `issued` (K where even); false at the end of a wait.
-        auto issue = [&]() {
-            if (more) {
-                const bool value = issued & 1;
-                const int t = issued >> 1, stage = t % STAGES;
-                if (!value) {  // the key's row in the cache, -1 for none
-                    const int slot = (tile * TK + my * ROWS + lane) & (p.cache.page_size - 1);
-                    row = -1;
-                    if (page >= 0 && page < p.cache.num_pages) row = (page * p.cache.kv_heads + there.kv_head) * p.cache.page_size + slot;
-                    else if (page != -2) report(p.err, kErrPageRange);
-                }
-                uint32_t to;
-                if constexpr (kBf16) {
-                    if (t >= STAGES && !wait((value ? v_empty : k_empty) + stage, ((t / STAGES) & 1) ^ 1)) return false;
-                    to = ptx::smem_u32(smem + (value ? C::OFF_V : C::OFF_K) + stage * C::PIECE);
-                } else {
-                    to = ptx::smem_u32(raw + issued % C::RAWS * C::RAW);
-                }
-                const uint8_t* const from = static_cast<const uint8_t*>(value ? p.cache.v : p.cache.k);
+        if constexpr (kBf16) {
+            // Whole tiles of whole pages come as boxes that TMA swizzles; others row by row,
+            // each of which is handed on when the next one's copies are under way.
+            int pending = -1;
+            auto hand_on = [&]() {
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(full + pending);
+                pending = -1;
+            };
+            const int run = p.runs > 0 ? TK / p.runs : TK;
+            while (ok && next_unit<TK>(p, walk)) {
+                const int* const table = p.table + (size_t)walk.g * p.table_stride;
+                // the table's entry of this lane's run of a tile, on its way a tile ahead
+                auto look = [&](int j) {
+                    const int key = j * TK + lane * run;
+                    return lane < p.runs && j < walk.r1 && key < walk.valid ? table[key >> p.page_shift] : 0;
+                };
+                int next = look(walk.r0);
+                for (int j = walk.r0; j < walk.r1; ++j, ++t) {
+                    const int stage = t % STAGES, key0 = j * TK, entry = next;
+                    next = look(j + 1);
+                    uint8_t* const to = pieces + stage * C::PIECE;
+                    bool boxes = p.runs > 0 && walk.valid - key0 >= TK;
+                    int first = -1;  // row of this lane's run
+                    if (boxes) {
+                        if (lane < p.runs) first = row_of(max(entry, -1), key0 + lane * run);
+                        boxes = __all_sync(0xffffffffu, lane >= p.runs || first >= 0);
+                    }
+                    if (t >= STAGES && !wait(empty + stage, ((t / STAGES) & 1) ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    if (boxes) {
+                        if (my == 0 && lane == 0) ptx::mbar_arrive_expect_tx(full + stage, C::PIECE);
+                        else ptx::mbar_arrive(full + stage);
+                        __syncwarp();
+                        if (my == 0 && lane < p.runs)
 #pragma unroll
-                for (int i = 0; i < COPIES; ++i) {
-                    const int r = i * PER + sub, at = __shfl_sync(0xffffffffu, row, r);
-                    const uint8_t* src = from + (size_t)max(at, 0) * RB + 16 * c;
-                    if constexpr (kBf16) {
-                        const int tr = my * ROWS + r;
-                        copy_async<16>(to + (c >> 3) * (TK * 128) + tr * 128 + (((c & 7) ^ (tr & 7)) << 4), src, at >= 0);
+                            for (int n = 0; n < D / 64; ++n)
+                                ptx::tma_load_2d(to + n * (TK * 128) + lane * run * 128, value ? &p.v_map : &p.k_map, full + stage, 128 * n, first);
                     } else {
-                        copy_async<16>(to + ((my * COPIES + i) * 32 + lane) * 16, src, at >= 0);
+                        int rows[(ROWS + 31) / 32];
+#pragma unroll
+                        for (int i = 0; i < (ROWS + 31) / 32; ++i) {
+                            const int key = key0 + my * ROWS + 32 * i + lane;
+                            rows[i] = row_of(key < walk.valid ? max(table[key >> p.page_shift], -1) : -2, key);
+                        }
+#pragma unroll 4
+                        for (int i = 0; i < ROWS / PER; ++i) {
+                            const int r = i * PER + sub, at = __shfl_sync(0xffffffffu, i * PER < 32 ? rows[0] : rows[(ROWS + 31) / 32 - 1], r & 31), tr = my * ROWS + r;
+                            copy_async<16>(ptx::smem_u32(to + (c >> 3) * (TK * 128) + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)), from + (size_t)max(at, 0) * RB + 16 * c, at >= 0);
+                        }
+                        copy_commit();
+                        if (pending >= 0) {
+                            copy_wait<1>();
+                            hand_on();
+                        }
+                        pending = stage;
+                        if (p.runs > 0) {  // one among boxes
+                            copy_wait<0>();
+                            hand_on();
+                        }
                     }
                 }
-                if constexpr (SB > 0)
-                    if (lane < ROWS)
-                        copy_async<SB>(to + TK * RB + (my * ROWS + lane) * SB,
-                                       static_cast<const uint8_t*>(value ? p.cache.v_scale : p.cache.k_scale) + (size_t)max(row, 0) * SB, row >= 0);
-                ++issued;
-                if (value) {
-                    if (++tile == there.r1) {
-                        more = next_unit<TK>(p, there);
-                        tile = there.r0;
+            }
+            copy_wait<0>();
+            if (ok && pending >= 0) hand_on();
+            if (!ok)  // (what is under way has to end before shared memory goes)
+                for (int i = max(t - STAGES, 0); i < t; ++i) ptx::mbar_wait(full + i % STAGES, (i / STAGES) & 1);
+        } else {
+            // Half pieces through a ring of the warp's own: bulk copies of whole pages' runs,
+            // or row by row where they are not whole.
+            constexpr int HROWS = ROWS / 2, COPIES = HROWS / PER, AHEAD = C::HALVES - 1;
+            constexpr int GROUP = COPIES < 4 ? COPIES : 4;  // decoded at once
+            const int half_bytes = value ? C::HALF_V : C::HALF_K, warp_bytes = half_bytes / 2;
+            uint8_t* const raw = smem + (value ? C::OFF_RAW_V : C::OFF_RAW_K) + my * warp_bytes;
+            const uint8_t* const scales = static_cast<const uint8_t*>(value ? p.cache.v_scale : p.cache.k_scale);
+            // `walk` is at the tile whose copies start, `here` at the one that is decoded
+            Walk here = walk;
+            bool more = next_unit<TK>(p, walk);
+            int tile = walk.r0, issued = 0, slot = 0, entry = 0;
+            bool there = false;
+            auto key_of = [&]() { return tile * TK + my * ROWS + (issued & 1) * HROWS + lane; };
+            auto look = [&]() {  // the table's entry of this lane's key, on its way (nothing here may wait for it)
+                const int key = key_of();
+                there = lane < HROWS && key < walk.valid;
+                if (there) entry = p.table[(size_t)walk.g * p.table_stride + (key >> p.page_shift)];
+            };
+            if (more) look();
+            uint64_t* const arrived = raw_full + (warp - kProducerWarp) * C::HALVES;
+            uint32_t bulk = 0, parity = 0;  // of the slots: whether bulk copies are under way, their phases
+            const int run = min(p.cache.page_size, HROWS);
+            auto issue = [&]() {
+                if (more) {
+                    const int row = row_of(there ? max(entry, -1) : -2, key_of());
+                    uint8_t* const to = raw + slot * half_bytes;
+                    if (run >= 8 && __all_sync(0xffffffffu, lane >= HROWS || row >= 0)) {
+                        bulk |= 1u << slot;
+                        if (lane == 0) ptx::mbar_arrive_expect_tx(arrived + slot, warp_bytes);
+                        __syncwarp();
+                        if (lane < HROWS && (lane & (run - 1)) == 0) {
+                            ptx::bulk_load(to + lane * RB, from + (size_t)row * RB, run * RB, arrived + slot);
+                            if (KIND != kKvFp8 || value) ptx::bulk_load(to + HROWS * RB + lane * SB, scales + (size_t)row * SB, run * SB, arrived + slot);
+                            if (KIND == kKvFp8 && value)
+                                ptx::bulk_load(to + HROWS * (RB + SB) + lane * SB, static_cast<const uint8_t*>(p.cache.k_scale) + (size_t)row * SB, run * SB, arrived + slot);
+                        }
+                    } else {
+                        bulk &= ~(1u << slot);
+                        const uint32_t at_smem = ptx::smem_u32(to);
+#pragma unroll
+                        for (int i = 0; i < COPIES; ++i) {
+                            const int at = __shfl_sync(0xffffffffu, row, i * PER + sub);
+                            copy_async<16>(at_smem + (i * 32 + lane) * 16, from + (size_t)max(at, 0) * RB + 16 * c, at >= 0);
+                        }
+                        if (lane < HROWS) {
+                            if (KIND != kKvFp8 || value) copy_async<SB>(at_smem + HROWS * RB + lane * SB, scales + (size_t)max(row, 0) * SB, row >= 0);
+                            if (KIND == kKvFp8 && value)
+                                copy_async<SB>(at_smem + HROWS * (RB + SB) + lane * SB, static_cast<const uint8_t*>(p.cache.k_scale) + (size_t)max(row, 0) * SB, row >= 0);
+                        }
+                    }
+                    if (++slot == C::HALVES) slot = 0;
+                    if ((++issued & 1) == 0 && ++tile == walk.r1) {
+                        more = next_unit<TK>(p, walk);
+                        tile = walk.r0;
                     }
                     if (more) look();
                 }
-            }
-            copy_commit();
-            return true;
-        };
-        for (int i = 0; ok && i < C::AHEAD; ++i) ok = issue();
-        int piece = 0;
-        float key_scale = 0.0f;  // of this lane's key (fp8)
-        while (ok && next_unit<TK>(p, here)) {
-            for (int j = 2 * here.r0; ok && j < 2 * here.r1; ++j, ++piece) {
-                const bool value = piece & 1;
-                const int t = piece >> 1, stage = t % STAGES;
-                if constexpr (kBf16) {
-                    copy_wait<C::AHEAD - 1>();
-                } else {
-                    issue();
-                    copy_wait<C::AHEAD>();
-                    __syncwarp();  // the other lanes' copies: a row's scales
-                    if (t >= STAGES) ok = wait((value ? v_empty : k_empty) + stage, ((t / STAGES) & 1) ^ 1);
-                    if (!ok) break;
-                    const uint8_t* const from = raw + piece % C::RAWS * C::RAW;
-                    uint8_t* const to = smem + (value ? C::OFF_V : C::OFF_K) + stage * C::PIECE;
+                copy_commit();
+            };
+            for (int i = 0; i < AHEAD; ++i) issue();
+            int at_slot = 0;
+            while (ok && next_unit<TK>(p, here)) {
+                for (int j = here.r0; ok && j < here.r1; ++j, ++t) {
+                    const int stage = t % STAGES;
+                    uint8_t* const to = pieces + stage * C::PIECE;
 #pragma unroll
-                    for (int i = 0; i < COPIES; ++i) {
-                        const int r = my * ROWS + i * PER + sub;
-                        const uint4 w = lds128(from + ((my * COPIES + i) * 32 + lane) * 16);
-                        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                    for (int half = 0; half < 2; ++half) {
+                        issue();
+                        copy_wait<AHEAD>();
+                        __syncwarp();  // the other lanes' copies: a row's scales
+                        if (bulk >> at_slot & 1) {
+                            ok = wait(arrived + at_slot, parity >> at_slot & 1);
+                            parity ^= 1u << at_slot, bulk &= ~(1u << at_slot);
+                        }
+                        if (ok && half == 0 && t >= STAGES) ok = wait(empty + stage, ((t / STAGES) & 1) ^ 1);
+                        if (!ok) break;
+                        const uint8_t* const in = raw + at_slot * half_bytes;
+                        const int row0 = my * ROWS + half * HROWS;
+#pragma unroll
+                        for (int i0 = 0; i0 < COPIES; i0 += GROUP) {
+                            uint4 w[GROUP];
+                            uint32_t sc[GROUP];
+#pragma unroll
+                            for (int i = 0; i < GROUP; ++i) {
+                                w[i] = lds128(in + ((i0 + i) * 32 + lane) * 16);
+                                if constexpr (KIND == kKvNvfp4) sc[i] = *reinterpret_cast<const uint16_t*>(in + HROWS * RB + ((i0 + i) * PER + sub) * SB + 2 * c);
+                            }
+#pragma unroll
+                            for (int i = 0; i < GROUP; ++i) {
+                                const int r = row0 + (i0 + i) * PER + sub, e = (KIND == kKvFp8 ? 16 : 32) * c;
+                                uint8_t* const line = to + (e >> 6) * (TK * 128) + r * 128;
+                                const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                                auto put = [&](int n, uint4 v) { *reinterpret_cast<uint4*>(line + (((((e & 63) >> 3) + n) ^ (r & 7)) << 4)) = v; };
+                                if constexpr (KIND == kKvFp8) {
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) {
+                                        uint32_t a[2], b[2];
+                                        e4m3x4_to_f16(words[2 * h], a);
+                                        e4m3x4_to_f16(words[2 * h + 1], b);
+                                        put(h, make_uint4(a[0], a[1], b[0], b[1]));
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int h = 0; h < 4; ++h) {
+                                        const uint32_t scale = ue4m3x2_to_f16((h < 2 ? sc[i] & 0xFFu : sc[i] >> 8) * 0x10001u);
+                                        uint32_t a[4];
+                                        e2m1x8_to_f16(words[h], a);
+                                        put(h, make_uint4(mul_f16x2(a[0], scale), mul_f16x2(a[1], scale), mul_f16x2(a[2], scale), mul_f16x2(a[3], scale)));
+                                    }
+                                }
+                            }
+                        }
                         if constexpr (KIND == kKvFp8) {
-                            const int e = 16 * c;
-                            uint8_t* line = to + (e >> 6) * (TK * 128) + r * 128;
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                uint32_t a[2], b[2];
-                                e4m3x4_to_f16(words[2 * h], a);
-                                e4m3x4_to_f16(words[2 * h + 1], b);
-                                *reinterpret_cast<uint4*>(line + (((((e & 63) >> 3) + h) ^ (r & 7)) << 4)) = make_uint4(a[0], a[1], b[0], b[1]);
-                            }
-                        } else {
-                            const int e = 32 * c;
-                            uint8_t* line = to + (e >> 6) * (TK * 128) + r * 128;
-                            const uint32_t sc = *reinterpret_cast<const uint16_t*>(from + TK * RB + r * SB + 2 * c);
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                const uint32_t scale = ue4m3x2_to_f16((h < 2 ? sc & 0xFFu : sc >> 8) * 0x10001u);
-                                uint32_t a[4];
-                                e2m1x8_to_f16(words[h], a);
-                                *reinterpret_cast<uint4*>(line + (((((e & 63) >> 3) + h) ^ (r & 7)) << 4)) =
-                                    make_uint4(mul_f16x2(a[0], scale), mul_f16x2(a[1], scale), mul_f16x2(a[2], scale), mul_f16x2(a[3], scale));
+                            // (with V: the softmax that reads them ends before V's stage is free again)
+                            if (value && lane < HROWS) {
+                                float* const s = reinterpret_cast<float*>(smem + C::OFF_SCALES + stage * C::SCALES) + row0 + lane;
+                                const float scale = *reinterpret_cast<const float*>(in + HROWS * RB + lane * SB);
+                                s[0] = *reinterpret_cast<const float*>(in + HROWS * (RB + SB) + lane * SB);
+                                s[TK] = scale, s[2 * TK] = fmaxf(log2_approx(scale), -80.0f);
                             }
                         }
+                        if (++at_slot == C::HALVES) at_slot = 0;
+                        __syncwarp();  // (the half piece may be copied over)
                     }
-                    if constexpr (KIND == kKvFp8) {
-                        if (lane < ROWS) {
-                            const int r = my * ROWS + lane;
-                            const float scale = *reinterpret_cast<const float*>(from + TK * RB + r * SB);
-                            if (value) {
-                                float* s = reinterpret_cast<float*>(smem + C::OFF_SCALES + stage * C::SCALES);
-                                s[r] = key_scale, s[TK + r] = scale, s[2 * TK + r] = fmaxf(log2_approx(scale), -80.0f);
-                            }
-                            key_scale = scale;
-                        }
-                    }
-                    __syncwarp();  // (the raw piece may be copied over)
+                    if (!ok) break;
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(full + stage);
                 }
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive((value ? v_full : k_full) + stage);
-                if constexpr (kBf16) ok = issue();
             }
+            copy_wait<0>();
+            for (int i = 0; i < C::HALVES; ++i)  // (none are after the last tile)
+                if (bulk >> i & 1) ptx::mbar_wait(arrived + i, parity >> i & 1);
         }
-        copy_wait<0>();
     } else if (working && warp == kMmaWarp) {
         // ------------------------------------------------------------ the products
         constexpr uint32_t s_desc = ptx::idesc_f16(kBf16, false, TK), o_desc = ptx::idesc_f16(kBf16, true, D);
@@ -541,22 +648,23 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                 const uint64_t k = k_at + (uint64_t)((stage * C::PIECE) >> 4);
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
-                    ptx::tc_mma_f16(tmem + (t & 1) * TK, q_at + (uint64_t)(((j >> 2) * kTileRows * 128 + (j & 3) * 32) >> 4),
+                    ptx::tc_mma_f16(tmem + t % C::BUFFERS * TK, q_at + (uint64_t)(((j >> 2) * kTileRows * 128 + (j & 3) * 32) >> 4),
                                     k + (uint64_t)(((j >> 2) * TK * 128 + (j & 3) * 32) >> 4), s_desc, j > 0);
                 ptx::tc_commit(k_empty + stage);
-                ptx::tc_commit(s_full + (t & 1));
+                ptx::tc_commit(s_full + t % C::BUFFERS);
             }
             __syncwarp();
         };
         while (ok && next_unit<TK>(p, walk)) {
             const int n = walk.r1 - walk.r0;
             ok = wait(q_full, segment & 1);
-            if (ok) scores(it);
+            constexpr int kAhead = C::BUFFERS - 1;  // tiles whose scores come before this one's O
+            for (int j = 0; ok && j < min(kAhead, n); ++j) scores(it + j);
             for (int j = 0; ok && j < n; ++j, ++it) {
-                if (j + 1 < n) scores(it + 1);
+                if (j + kAhead < n) scores(it + kAhead);
                 if (!ok) break;
-                const int stage = it % STAGES, buf = it & 1, mine = GROUPS == 2 ? buf : 0;
-                ok = wait(p_full + buf, (it >> 1) & 1) && wait(v_full + stage, (it / STAGES) & 1);
+                const int stage = it % STAGES, buf = it % C::BUFFERS, mine = GROUPS == 2 ? it & 1 : 0;
+                ok = wait(p_full + buf, (it / C::BUFFERS) & 1) && wait(v_full + stage, (it / STAGES) & 1);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 if (ptx::elect_one()) {
@@ -569,7 +677,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                             ptx::tc_mma_f16_ts(o, w + 32 * (k >> 1) + 16 * term + 8 * (k & 1), v + (uint64_t)((k * 2048) >> 4), o_desc,
                                                j >= GROUPS || k > 0 || term > 0);
                     ptx::tc_commit(v_empty + stage);
-                    if (GROUPS == 1) ptx::tc_commit(o_done);
+                    ptx::tc_commit(o_done + mine);
                     if (j + 1 == n) ptx::tc_commit(unit_done);
                 }
                 __syncwarp();
@@ -606,8 +714,16 @@ SharedLayout shared_layout(long own, int sms, int prefixes, int batch, int group
 }
 
 template <int KIND, int D>
-cudaError_t launch_prefix(const PrefixParams& p, int sms, cudaStream_t st) {
+cudaError_t launch_prefix(PrefixParams& p, int sms, cudaStream_t st) {
     using C = PrefixCfg<KIND, D>;
+    // Boxes of the tile's rows in one page, 8 rows (a swizzle's pattern) at least.
+    p.runs = 0;
+    if (KIND == kKvBf16 && p.cache.page_size >= 8) {
+        const int box = std::min(p.cache.page_size, C::TK);
+        const long rows = (long)p.cache.num_pages * p.cache.kv_heads * p.cache.page_size;
+        if (!make_byte_map(&p.k_map, p.cache.k, rows, 2 * D, box) || !make_byte_map(&p.v_map, p.cache.v, rows, 2 * D, box)) return cudaErrorInvalidValue;
+        p.runs = C::TK / box;
+    }
     static std::mutex mu;
     static bool ready[kMaxDevices];
     auto* kernel = prefix_attention_kernel<KIND, D>;
@@ -628,7 +744,7 @@ cudaError_t launch_prefix(const PrefixParams& p, int sms, cudaStream_t st) {
 }
 
 template <int KIND>
-cudaError_t launch_both(const PrefixParams& x, AttentionParams& p, uint8_t* workspace, int sms, cudaStream_t st) {
+cudaError_t launch_both(PrefixParams& x, AttentionParams& p, uint8_t* workspace, int sms, cudaStream_t st) {
     const cudaError_t e = p.cache.head_dim == 64    ? launch_prefix<KIND, 64>(x, sms, st)
                           : p.cache.head_dim == 128 ? launch_prefix<KIND, 128>(x, sms, st)
                                                     : launch_prefix<KIND, 256>(x, sms, st);
