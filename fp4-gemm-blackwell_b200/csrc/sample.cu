@@ -62,6 +62,8 @@ constexpr int kBins = 2 * kSide + 1;       // the one between them is bin kSide
 constexpr int kPer = (kBins + kThreads - 1) / kThreads;  // bins a thread walks
 constexpr float kReach = 46.0f;
 constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;
+constexpr int kList = kThreads;  // candidates of a run that are ranked one by one
 constexpr int kMaxDevices = 64;
 
 struct SampleParams {
@@ -87,12 +89,14 @@ struct Traits {
     using T = uint16_t;
     static constexpr int PER = 8;                            // elements of 16 bytes
     static constexpr int FREE = TYPE == kBf16 ? 16 : 13;     // low bits of the FP32 form that are zero
+    static constexpr uint32_t NONE = TYPE == kBf16 ? 0xFF80u : 0xFC00u;  // -inf
 };
 template <>
 struct Traits<kFp32> {
     using T = uint32_t;
     static constexpr int PER = 4;
     static constexpr int FREE = 0;
+    static constexpr uint32_t NONE = 0xFF800000u;
 };
 
 // FP32 bits of a logit; what is no candidate (NaN) becomes -inf, -0 becomes +0.
@@ -125,13 +129,24 @@ struct Row {
     double inv;
     int lo;            // leading bits of the smallest magnitude with a bin of its own
     double one;        // 2^bits
-    __device__ __forceinline__ u64 weight(float l) const {
-        if (l == max) return (u64)one;
-        return (u64)__double2ll_rn(exp(((double)l - (double)max) * inv) * one);
+    const double* powers;  // 2^(i / 32), i < 32, in shared memory
+    // Weights: of the largest 1.  exp(x) = 2^(n / 32) exp(y), n the nearest whole number
+    // to 32 x / ln 2, |y| <= ln 2 / 64, exp(y) by its series up to y^5 (the next term is
+    // below 3e-15): to within about 1e-14, with a third of the library's instructions.
+    __device__ __forceinline__ double share(float l) const {
+        const double x = l == max ? 0.0 : fmax(((double)l - (double)max) * inv, -700.0);  // (-inf counts as that, whose weight is 0)
+        const double shifted = fma(x, 46.166241308446828384, 6755399441055744.0);  // 32 / ln 2; 1.5 * 2^52 leaves a whole number in the low bits
+        const int n = __double2loint(shifted);
+        const double y = fma(shifted - 6755399441055744.0, -0.021660849392498290195, x);  // ln 2 / 32
+        double e = fma(y, 1.0 / 120.0, 1.0 / 24.0);
+        e = fma(e, y, 1.0 / 6.0);
+        e = fma(e, y, 0.5);
+        e = fma(e, y, 1.0);
+        e = fma(e, y, 1.0) * powers[n & 31];
+        return __hiloint2double(__double2hiint(e) + ((n >> 5) << 20), __double2loint(e));
     }
-    __device__ __forceinline__ bool keeps(float l, float least) const {
-        return l == max || exp(((double)l - (double)max) * inv) >= (double)least;
-    }
+    __device__ __forceinline__ u64 whole(double w) const { return (u64)__double2ll_rn(w * one); }
+    __device__ __forceinline__ u64 weight(float l) const { return whole(share(l)); }
     // Bin of a candidate's bits, -1 for none.
     __device__ __forceinline__ int bin(uint32_t b) const {
         const int i = (int)((b >> 16) & 0x7FFFu) - lo;
@@ -150,15 +165,15 @@ struct Row {
     }
 };
 
-struct Place {  // of a crossing: a bin, and what lies before it
+struct Place {  // of a crossing: a bin or a part of one, and what lies before it
     int bin;
     uint32_t before, count;
-    u64 mass_before, mass;
+    u64 mass_before;
 };
 
 // What the first CTA tells the others to do next.
 struct Command {
-    int what;  // 0: done, 1: split a run, 2: find the token
+    int what;  // 0: done, 1: split a run, 2: find the token, 3: list a run
     Run run;
     int cta;
     uint32_t rank;
@@ -169,12 +184,18 @@ struct Shared {
     uint32_t hist[kBins];
     uint32_t sub_count[256];
     u64 sub_mass[256];
-    float max[kMaxCluster];
-    uint32_t best[kMaxCluster];
+    double powers[32];
+    float max[kMaxCluster], warp_max[kWarps];
+    u64 near_mass;  // of the bin between, where the others have one logit each
     uint32_t warp_count[kWarps];
     u64 warp_mass[kWarps];
     uint32_t least_count;  // candidates with w >= min_p, of the row
     u64 least_mass;
+    u64 list[kList];  // key and what the index lacks of 2^32 - 1: larger ones come first
+    u64 list_weight[kList];
+    uint32_t listed;
+    u64 answer_mass, answer_weight;
+    int answer_token;
     Place place;
     Command command;
     int token;
@@ -234,16 +255,27 @@ struct Question {
     }
 };
 
+// Sums of one bin's or part's entry over the cluster's CTAs, read side by side.
+template <typename T>
+__device__ __forceinline__ T over_cluster(cg::cluster_group& cluster, T* at, int ctas) {
+    T v[kMaxCluster], sum = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) v[c] = c < ctas ? *cluster.map_shared_rank(at, c) : T(0);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) sum += v[c];
+    return sum;
+}
+
 template <int TYPE>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
     using T = typename Traits<TYPE>::T;
     constexpr int PER = Traits<TYPE>::PER, FREE = Traits<TYPE>::FREE;
     constexpr bool kMasses = FREE < 16;  // bins of more than one logit
     extern __shared__ __align__(16) uint8_t dynamic[];
-    // the first CTA's: merged bins; with masses every CTA's own
-    u64* const mass = reinterpret_cast<u64*>(dynamic);
-    uint32_t* const count = reinterpret_cast<uint32_t*>(mass + kBins);
-    u64* const my_mass = reinterpret_cast<u64*>(dynamic + kBins * 16);
+    // With masses: this CTA's [kBins]; in a cluster: what the first CTA has of all of them, masses and counts.
+    u64* const my_mass = reinterpret_cast<u64*>(dynamic);
+    u64* const all_mass = my_mass + (kMasses ? kBins : 0);
+    uint32_t* const all_count = reinterpret_cast<uint32_t*>(all_mass + (kMasses ? kBins : 0));
     __shared__ Shared s;
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
@@ -260,43 +292,74 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     const int pieces = last > first ? (last - first + shift + PER - 1) / PER : 0;
     const int warp_pieces = ((pieces + kWarps - 1) / kWarps + 31) / 32 * 32;
     const int piece0 = min(warp * warp_pieces, pieces), piece1 = min(piece0 + warp_pieces, pieces);
-    // The bits of piece i's elements, what lies outside the slice as -inf.
-    auto load = [&](int i, uint32_t (&b)[PER]) {
+    // Piece i as it lies there, what is outside the slice as -inf.
+    auto load = [&](int i) {
         const int at = first + i * PER - shift;
-        if (at >= first && at + PER <= last) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(logits + at));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (at >= first && at + PER <= last) return __ldg(reinterpret_cast<const uint4*>(logits + at));
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                if constexpr (PER == 4) b[e] = bits_of<TYPE>(w[e]);
-                else b[e] = bits_of<TYPE>((uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]));
+        for (int e = 0; e < PER; ++e) {
+            const uint32_t v = at + e >= first && at + e < last ? (uint32_t)logits[at + e] : Traits<TYPE>::NONE;
+            if constexpr (PER == 4) w[e] = v;
+            else w[e / 2] |= v << (e & 1) * 16;
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto bits = [&](const uint4& v, int e) {  // of its element e, as FP32
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (PER == 4) return bits_of<TYPE>(w[e]);
+        else return bits_of<TYPE>((uint16_t)(e & 1 ? w[e / 2] >> 16 : w[e / 2]));
+    };
+
+    // f of all pieces, kBatch of them on their way at once.
+    auto over_pieces = [&](auto f) {
+        uint4 next[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (piece0 + lane + 32 * k < piece1) next[k] = load(piece0 + lane + 32 * k);
+        for (int i = piece0 + lane; i < piece1; i += 32 * kBatch) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (i + 32 * k >= piece1) break;
+                const uint4 v = next[k];
+                if (i + 32 * (k + kBatch) < piece1) next[k] = load(i + 32 * (k + kBatch));
+                f(v);
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) b[e] = at + e >= first && at + e < last ? bits_of<TYPE>(logits[at + e]) : 0xFF800000u;
         }
     };
 
     // ---- the maximum
     float most = -INFINITY;
-    for (int i = piece0 + lane; i < piece1; i += 32) {
-        uint32_t b[PER];
-        load(i, b);
+    if constexpr (TYPE == kBf16) {
+        __nv_bfloat162 top = __floats2bfloat162_rn(-INFINITY, -INFINITY);
+#pragma unroll 4
+        for (int i = piece0 + lane; i < piece1; i += 32) {
+            const uint4 v = load(i);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < PER; ++e) most = fmaxf(most, __uint_as_float(b[e]));
+            for (int k = 0; k < 4; ++k) top = __hmax2(top, *reinterpret_cast<const __nv_bfloat162*>(&w[k]));  // (not a NaN)
+        }
+        most = fmaxf(__low2float(top), __high2float(top));
+    } else {
+#pragma unroll 4
+        for (int i = piece0 + lane; i < piece1; i += 32) {
+            const uint4 v = load(i);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) most = fmaxf(most, __uint_as_float(bits(v, e)));
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     for (int i = tid; i < kBins; i += kThreads) {
         s.hist[i] = 0;
         if (kMasses) my_mass[i] = 0;
-        if (!kMasses && i == kSide) my_mass[0] = 0;  // of the bin between
     }
-    if (tid == 0) s.least_count = 0, s.least_mass = 0, s.token = 0x7fffffff;
-    if (lane == 0) reinterpret_cast<float*>(s.warp_count)[warp] = most;
+    if (tid == 0) s.near_mass = 0, s.least_count = 0, s.least_mass = 0, s.token = 0x7fffffff;
+    if (lane == 0) s.warp_max[warp] = most;
+    if (tid < 32) s.powers[tid] = exp2((double)tid / 32.0);
     __syncthreads();
     if (warp == 0) {
-        most = lane < kWarps ? reinterpret_cast<float*>(s.warp_count)[lane] : -INFINITY;
+        most = lane < kWarps ? s.warp_max[lane] : -INFINITY;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         if (lane < ctas) cluster.map_shared_rank(s.max, lane)[me] = most;
@@ -304,7 +367,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     cluster.sync();
     most = s.max[0];
     for (int c = 1; c < ctas; ++c) most = fmaxf(most, s.max[c]);
-    // (no CTA writes its neighbours' s.max again)
 
     const float t = p.temperature ? p.temperature[row] : p.temperature1;
     const bool greedy = !(t > 0.0f);
@@ -316,9 +378,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         return;
     }
     Row r;
-    r.max = most;
-    r.inv = fmax(1.0 / (double)t, 0x1p-1000);  // (an infinite T: all alike)
-    r.one = (double)(1ull << p.bits);
+    r.max = most == 0.0f ? 0.0f : most;                // (+0)
+    r.inv = fmax(1.0 / (double)t, 0x1p-1000);          // (an infinite T: all alike)
+    r.one = (double)(1ull << p.bits), r.powers = s.powers;
     {
         const uint32_t far = __float_as_uint(fmaf(-kReach, t, most)) & 0x7FFFFFFFu, top = __float_as_uint(most) & 0x7FFFFFFFu;
         const int octave = (int)(max(min(far, 0x7F800000u), top) >> 23);
@@ -329,24 +391,31 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
 
     // ---- the token of a run of equal logits: the rank-th of them, in this CTA's slice
     auto find = [&](Run run, uint32_t rank, float prob) {
-        auto hits = [&](int i, uint32_t& mask) {
-            mask = 0;
-            if (i < piece1) {
-                uint32_t b[PER];
-                load(i, b);
+        const uint32_t exact = (__float_as_uint(run.logit()) >> 16) * 0x10001u;  // BF16, twice
+        auto hits = [&](int i) {  // of piece i, as bits
+            uint32_t mask = 0;
+            if (i >= piece1) return mask;
+            const uint4 v = load(i);
+            if constexpr (TYPE == kBf16) {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t same = __vcmpeq2(w[k], exact);
+                    if (exact == 0u) same |= __vcmpeq2(w[k], 0x80008000u);
+                    mask |= ((same & 1u) | ((same >> 15) & 2u)) << 2 * k;
+                }
+            } else {
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const uint32_t key = key_of(b[e]);
-                    if (key > kMinusInf && key >= run.first && (run.size > 31 || ((key - run.first) >> run.size) == 0)) mask |= 1u << e;
+                    const uint32_t key = key_of(bits(v, e));
+                    if (key > kMinusInf && key >= run.first && ((key - run.first) >> run.size) == 0) mask |= 1u << e;
                 }
             }
+            return mask;
         };
         uint32_t mine = 0;
-        for (int i = piece0 + lane; i < piece1; i += 32) {
-            uint32_t mask;
-            hits(i, mask);
-            mine += __popc(mask);
-        }
+#pragma unroll 4
+        for (int i = piece0 + lane; i < piece1; i += 32) mine += __popc(hits(i));
         const uint32_t all = __reduce_add_sync(0xffffffffu, mine);
         __syncthreads();
         if (lane == 0) s.warp_count[warp] = all;
@@ -356,8 +425,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         if (rank < before || rank >= before + all) return;
         rank -= before;
         for (int i = piece0; i < piece1; i += 32) {
-            uint32_t mask;
-            hits(i + lane, mask);
+            uint32_t mask = hits(i + lane);
             const uint32_t here = __popc(mask);
             uint32_t upto = here;
 #pragma unroll
@@ -379,11 +447,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     if (greedy) {  // the first of the largest: the least index
         int at = 0x7fffffff;
         for (int i = piece0 + lane; i < piece1 && at == 0x7fffffff; i += 32) {
-            uint32_t b[PER];
-            load(i, b);
+            const uint4 v = load(i);
 #pragma unroll
             for (int e = PER - 1; e >= 0; --e)
-                if (__uint_as_float(b[e]) == most) at = first + i * PER - shift + e;
+                if (__uint_as_float(bits(v, e)) == most) at = first + i * PER - shift + e;
         }
         at = __reduce_min_sync(0xffffffffu, at);
         Shared* home = cluster.map_shared_rank(&s, 0);
@@ -399,74 +466,102 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     // ---- counts (and masses) of the slice's bins
     uint32_t kept = 0;
     u64 kept_mass = 0;
-    for (int i = piece0 + lane; i < piece1; i += 32) {
-        uint32_t b[PER];
-        load(i, b);
+    auto heavy = [&](int bin, float l) {  // of a bin of more than one logit
+        const double w = r.share(l);
+        const u64 m = r.whole(w);
+        atomicAdd(kMasses ? &my_mass[bin] : &s.near_mass, m);
+        if (has_least && w >= (double)least) ++kept, kept_mass += m;
+    };
+    if constexpr (TYPE == kBf16) {
+        // infinities and NaN lie above these
+        const int most_plus = min(kSide, 0x7F81 - r.lo), most_minus = min(kSide, 0x7F80 - r.lo);
+        over_pieces([&](const uint4& v) {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            if (b[e] == 0xFF800000u) continue;
-            const int bin = r.bin(b[e]);
-            if (bin < 0) continue;
-            atomicAdd(&s.hist[bin], 1u);
-            if (kMasses || bin == kSide) {
-                const float l = __uint_as_float(b[e]);
-                const u64 w = r.weight(l);
-                atomicAdd(&my_mass[kMasses ? bin : 0], w);
-                if (has_least && r.keeps(l, least)) ++kept, kept_mass += w;
+            for (int e = 0; e < PER; ++e) {
+                const int h = (int)(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu), k = (h & 0x7FFF) - r.lo;
+                const bool minus = h & 0x8000;
+                if (k >= 0) {
+                    if (k < (minus ? most_minus : most_plus)) atomicAdd(&s.hist[minus ? kSide + 1 + k : kSide - 1 - k], 1u);
+                } else {
+                    atomicAdd(&s.hist[kSide], 1u);
+                    heavy(kSide, __uint_as_float(tidy((uint32_t)h << 16)));
+                }
             }
-        }
+        });
+    } else {
+        over_pieces([&](const uint4& v) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const uint32_t b = bits(v, e);
+                if (b == 0xFF800000u) continue;
+                const int bin = r.bin(b);
+                if (bin < 0) continue;
+                atomicAdd(&s.hist[bin], 1u);
+                heavy(bin, __uint_as_float(b));
+            }
+        });
     }
-    cluster.sync();
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
 
-    // ---- this CTA's share of the bins over all slices, into the first CTA's
-    {
-        uint32_t* to_count = cluster.map_shared_rank(count, 0);
-        u64* to_mass = cluster.map_shared_rank(mass, 0);
+    // ---- in a cluster: this CTA's share of the bins over all slices, into the first CTA's
+    if (ctas > 1) {
+        uint32_t* to_count = cluster.map_shared_rank(all_count, 0);
+        u64* to_mass = cluster.map_shared_rank(all_mass, 0);
         for (int i = me * kThreads + tid; i < kBins; i += ctas * kThreads) {
-            uint32_t n = 0;
-            u64 m = 0;
-            for (int c = 0; c < ctas; ++c) {
-                n += cluster.map_shared_rank(s.hist, c)[i];
-                if (kMasses) m += cluster.map_shared_rank(my_mass, c)[i];
-                else if (i == kSide) m += cluster.map_shared_rank(my_mass, c)[0];
-            }
-            if (!kMasses && i != kSide && n) {
-                const float l = r.run(i).logit();
-                const u64 w = r.weight(l);
-                m = w * n;
-                if (has_least && r.keeps(l, least)) kept += n, kept_mass += m;
-            }
-            to_count[i] = n, to_mass[i] = m;
+            to_count[i] = over_cluster(cluster, &s.hist[i], ctas);
+            if (kMasses) to_mass[i] = over_cluster(cluster, &my_mass[i], ctas);
         }
-        if (has_least) {
+        Shared* home = cluster.map_shared_rank(&s, 0);
+        if (!kMasses && me != 0 && tid == 0 && s.near_mass) atomicAdd(&home->near_mass, s.near_mass);
+        if (me != 0) {
+            if (has_least) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                kept += __shfl_xor_sync(0xffffffffu, kept, o);
-                kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
+                for (int o = 16; o > 0; o >>= 1) {
+                    kept += __shfl_xor_sync(0xffffffffu, kept, o);
+                    kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
+                }
+                if (lane == 0 && kept) atomicAdd(&home->least_count, kept), atomicAdd(&home->least_mass, kept_mass);
             }
-            Shared* home = cluster.map_shared_rank(&s, 0);
-            if (lane == 0 && kept) atomicAdd(&home->least_count, kept), atomicAdd(&home->least_mass, kept_mass);
+            kept = 0, kept_mass = 0;
         }
+        cluster.sync();
     }
-    cluster.sync();
+    const uint32_t* const count = ctas > 1 ? all_count : s.hist;
+    const u64* const mass = ctas > 1 ? all_mass : my_mass;
 
     // ---- the first CTA asks; a run of more than one logit is split by all of them
     auto split = [&](Run run) {  // all CTAs: counts and masses of the run's 256 parts, ascending
         for (int i = tid; i < 256; i += kThreads) s.sub_count[i] = 0, s.sub_mass[i] = 0;
         __syncthreads();
         const int down = max(run.size - 8, 0);
-        for (int i = piece0 + lane; i < piece1; i += 32) {
-            uint32_t b[PER];
-            load(i, b);
+        over_pieces([&](const uint4& v) {
 #pragma unroll
             for (int e = 0; e < PER; ++e) {
-                const uint32_t key = key_of(b[e]);
+                const uint32_t b = bits(v, e), key = key_of(b);
                 if (key <= kMinusInf || key < run.first || (run.size < 32 && ((key - run.first) >> run.size) != 0)) continue;
                 const uint32_t part = (key - run.first) >> down;
                 if (part > 255) continue;
-                if (run.size > 16 && r.bin(b[e]) != kSide) continue;  // (the bin between is less than its power of two)
+                if (run.size > 16 && r.bin(b) != kSide) continue;  // (the bin between is less than its power of two)
                 atomicAdd(&s.sub_count[part], 1u);
-                atomicAdd(&s.sub_mass[part], r.weight(__uint_as_float(b[e])));
+                atomicAdd(&s.sub_mass[part], r.weight(__uint_as_float(b)));
+            }
+        });
+        cluster.sync();
+    };
+
+    auto list = [&](Run run) {  // all CTAs: the run's candidates into the first CTA's list
+        Shared* home = cluster.map_shared_rank(&s, 0);
+        for (int i = piece0 + lane; i < piece1; i += 32) {
+            const uint4 v = load(i);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const uint32_t b = bits(v, e), key = key_of(b);
+                if (key > kMinusInf && key - run.first < (1u << run.size) && (run.size <= 16 || r.bin(b) == kSide)) {
+                    const uint32_t at = atomicAdd(&home->listed, 1u);
+                    if (at < kList) home->list[at] = (u64)key << 32 | (0xFFFFFFFFu - (uint32_t)(first + i * PER - shift + e));
+                }
             }
         }
         cluster.sync();
@@ -476,7 +571,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         for (;;) {
             cluster.sync();  // a command is there
             const Command c = s.command;
-            if (c.what == 1) {
+            if (c.what == 3) {
+                list(c.run);
+            } else if (c.what == 1) {
                 split(c.run);
                 cluster.sync();  // the parts were read
             } else {
@@ -490,132 +587,158 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         cluster.sync();
     };
 
+    // ---- a thread's bins, kPer of them: what lies before them, and in them
+    uint32_t my_before = 0, my_count = 0;
+    u64 my_mass_before = 0, my_total = 0;
+    // (all weights side by side: their exponentials have long chains)
+    u64 bin_mass[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int i = min(tid * kPer + k, kBins - 1);
+        const bool there = tid * kPer + k < kBins;
+        const uint32_t n = there ? count[i] : 0u;
+        if constexpr (kMasses) {
+            bin_mass[k] = there ? mass[i] : 0;
+        } else {
+            const double w = r.share(r.run(i).logit());
+            bin_mass[k] = i == kSide ? (there ? s.near_mass : 0) : r.whole(w) * n;
+            if (has_least && i != kSide && w >= (double)least) kept += n, kept_mass += bin_mass[k];
+        }
+        my_count += n, my_total += bin_mass[k];
+    }
+    my_before = my_count, my_mass_before = my_total;
+    scan(s, my_before, my_mass_before);
+    if (has_least) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            kept += __shfl_xor_sync(0xffffffffu, kept, o);
+            kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
+        }
+        if (lane == 0 && kept) atomicAdd(&s.least_count, kept), atomicAdd(&s.least_mass, kept_mass);
+    }
+    if (tid == kThreads - 1) s.place.before = my_before + my_count, s.place.mass_before = my_mass_before + my_total;
+    __syncthreads();
+    u64 total = s.place.mass_before;
+    const uint32_t candidates = s.place.before;
+    const u64 least_mass = s.least_mass;
+    __syncthreads();
+
     struct Answer {
-        uint32_t count;  // up to the place, with it
-        u64 mass;
-        Run run;         // of its logit
-        uint32_t rank;   // among equal ones
-        int bin;         // >= 0: counts are the bins', else the parts'
+        u64 mass;       // up to the place, with it
+        Run run;        // of its logit
+        uint32_t rank;  // among equal ones
+        int bin;        // >= 0: counts are the bins', else the parts'
         u64 weight;
-        bool found;
+        int token;      // >= 0: it is known
     };
+    // (a question's place is among the candidates)
     auto ask = [&](const Question& q) {
-        // the bin
-        uint32_t n = 0;
-        u64 m = 0;
-        for (int k = 0; k < kPer; ++k) {
-            const int i = tid * kPer + k;
-            if (i < kBins) n += count[i], m += mass[i];
-        }
-        scan(s, n, m);
-        if (tid == 0) s.place.bin = -1;
-        __syncthreads();
-        for (int k = 0; k < kPer; ++k) {
-            const int i = tid * kPer + k;
-            if (i >= kBins) break;
-            if (q.in(n, m, count[i], mass[i])) s.place = Place{i, n, count[i], m, mass[i]};
-            n += count[i], m += mass[i];
+        if (q.in(my_before, my_mass_before, my_count, my_total)) {
+            uint32_t n = my_before;
+            u64 m = my_mass_before;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int i = tid * kPer + k;
+                const uint32_t here = i < kBins ? count[i] : 0;
+                if (q.in(n, m, here, bin_mass[k])) s.place = Place{i, n, here, m};
+                n += here, m += bin_mass[k];
+            }
         }
         __syncthreads();
-        Answer a{};
         Place x = s.place;
-        a.found = x.bin >= 0;
-        if (!a.found) return a;
         Run run = r.run(x.bin);
         int bin = x.bin;
         while (run.size > FREE) {
             Command c{};
             c.what = 1, c.run = run;
+            if (x.count <= kList && run.size <= 24) {
+                // few: each is ranked among all of them
+                c.what = 3;
+                if (tid == 0) s.listed = 0;
+                tell(c);
+                list(run);
+                const int n = (int)min(s.listed, (uint32_t)kList);
+                const u64 mine = tid < n ? s.list[tid] : 0;
+                const u64 w = tid < n ? r.weight(logit_of((uint32_t)(mine >> 32))) : 0;
+                s.list_weight[tid] = w;
+                __syncthreads();
+                if (tid < n) {
+                    uint32_t before = x.before;
+                    u64 m = x.mass_before;
+#pragma unroll 4
+                    for (int j = 0; j < n; ++j)
+                        if (s.list[j] > mine) ++before, m += s.list_weight[j];
+                    if (q.in(before, m, 1, w)) s.answer_mass = m + w, s.answer_weight = w, s.answer_token = (int)(0xFFFFFFFFu - (uint32_t)mine);
+                }
+                __syncthreads();
+                return Answer{s.answer_mass, run, 0, -1, s.answer_weight, s.answer_token};
+            }
             tell(c);
             split(run);
             // parts from the last (the largest logits) down, one a thread
             const int i = 255 - tid;
-            n = 0, m = 0;
-            if (i >= 0)
-                for (int c = 0; c < ctas; ++c) {
-                    n += cluster.map_shared_rank(s.sub_count, c)[i];
-                    m += cluster.map_shared_rank(s.sub_mass, c)[i];
-                }
+            uint32_t n = 0;
+            u64 m = 0;
+            if (i >= 0) n = over_cluster(cluster, &s.sub_count[i], ctas), m = over_cluster(cluster, &s.sub_mass[i], ctas);
             const uint32_t part_count = n;
             const u64 part_mass = m;
             scan(s, n, m);
             n += x.before, m += x.mass_before;
-            if (i >= 0 && q.in(n, m, part_count, part_mass)) s.place = Place{i, n, part_count, m, part_mass};
+            if (i >= 0 && q.in(n, m, part_count, part_mass)) s.place = Place{i, n, part_count, m};
             cluster.sync();
             x = s.place;
             const int down = max(run.size - 8, 0);
             run = Run{run.first + ((uint32_t)x.bin << down), down};
             bin = -1;
         }
+        Answer a;
         a.weight = r.weight(run.logit());
         const uint32_t part = q.part(x.before, x.mass_before, x.count, a.weight);
-        a.count = x.before + part, a.mass = x.mass_before + (u64)part * a.weight;
-        a.run = run, a.rank = part - 1, a.bin = bin;
-        s.place = x;  // (the same in every thread) its bin: of the bins or the parts
+        a.mass = x.mass_before + (u64)part * a.weight;
+        a.run = run, a.rank = part - 1, a.bin = bin, a.token = -1;
         __syncthreads();
         return a;
     };
 
     // ---- what is kept: the sum of its weights
-    u64 total;
     {
-        uint32_t n = 0;
-        u64 m = 0;
-        for (int k = 0; k < kPer; ++k) {
-            const int i = tid * kPer + k;
-            if (i < kBins) n += count[i], m += mass[i];
-        }
-        scan(s, n, m);
-        if (tid == kThreads - 1) {
-            for (int k = 0; k < kPer; ++k) {
-                const int i = tid * kPer + k;
-                if (i < kBins) n += count[i], m += mass[i];
-            }
-            s.place.before = n, s.place.mass_before = m;
-        }
-        __syncthreads();
-        total = s.place.mass_before;
-        n = s.place.before;
-        __syncthreads();
         const int k = p.top_k ? p.top_k[row] : p.top_k1;
-        if (k > 0 && (uint32_t)k < n) {
-            const Answer a = ask(Question{kByCount, (uint32_t)k, 0.0});
-            if (a.found) total = a.mass;
-        }
+        if (k > 0 && (uint32_t)k < candidates) total = ask(Question{kByCount, (uint32_t)k, 0.0}).mass;
         const float nucleus = p.top_p ? p.top_p[row] : p.top_p1;
         u64 smaller = total;
-        if (nucleus < 1.0f) {
-            // (at least the first token: a target of nothing is less than the least weight)
-            const Answer a = ask(Question{kByMassBefore, 0, fmax((double)nucleus * (double)total, 0.5)});
-            if (a.found) smaller = min(smaller, a.mass);
-        }
-        if (has_least) smaller = min(smaller, s.least_mass ? s.least_mass : (u64)r.one);
+        // (at least the first token: a target of nothing is less than the least weight)
+        if (nucleus < 1.0f) smaller = min(smaller, ask(Question{kByMassBefore, 0, fmax((double)nucleus * (double)total, 0.5)}).mass);
+        if (has_least) smaller = min(smaller, least_mass ? least_mass : (u64)r.one);
         total = smaller;
     }
     const float given = p.u[row];
     const double u = given > 0.0f ? fmin((double)given, 1.0 - 0x1p-24) : 0.0;
     const Answer a = ask(Question{kByMassWith, 0, u * (double)total});
     Command c{};
-    c.what = 0;
-    if (a.found) {
-        // which CTA has it: the slices' counts of its logit, in order
-        uint32_t rank = a.rank;
-        for (int i = 0; i < ctas; ++i) {
-            const uint32_t n = a.bin >= 0 ? cluster.map_shared_rank(s.hist, i)[a.bin] : cluster.map_shared_rank(s.sub_count, i)[s.place.bin];
-            if (rank < n) {
-                c = Command{2, a.run, i, rank, (float)((double)a.weight / (double)total)};
-                break;
-            }
-            rank -= n;
+    c.what = 2, c.run = a.run, c.prob = (float)((double)a.weight / (double)total);
+    if (a.token >= 0) {
+        if (tid == 0) {
+            p.tokens[row] = a.token;
+            if (p.probs) p.probs[row] = c.prob;
         }
+        c.what = 0;
+        if (ctas > 1) tell(c);
+        return;
     }
-    tell(c);
-    if (c.what == 2 && c.cta == 0) find(c.run, c.rank, c.prob);
+    // which CTA has it: the slices' counts of its logit, in order
+    c.rank = a.rank;
+    for (; c.cta < ctas - 1; ++c.cta) {
+        const uint32_t n = a.bin >= 0 ? cluster.map_shared_rank(s.hist, c.cta)[a.bin] : cluster.map_shared_rank(s.sub_count, c.cta)[s.place.bin];
+        if (c.rank < n) break;
+        c.rank -= n;
+    }
+    if (ctas > 1) tell(c);
+    if (c.cta == 0) find(c.run, c.rank, c.prob);
 }
 
 template <int TYPE>
 cudaError_t launch(SampleParams& p, int rows, cudaStream_t st) {
-    constexpr int kSmem = kBins * 16 + (Traits<TYPE>::FREE < 16 ? kBins * 8 : 16);
+    constexpr int kOne = Traits<TYPE>::FREE < 16 ? kBins * 8 : 0, kMore = kOne + kBins * 4;  // of a CTA, of one in a cluster
     auto* kernel = sample_kernel<TYPE>;
     static std::mutex mu;
     static int resident[kMaxDevices];  // CTAs that fit on the device at once
@@ -627,9 +750,9 @@ cudaError_t launch(SampleParams& p, int rows, cudaStream_t st) {
     {
         std::lock_guard<std::mutex> lk(mu);
         if (!resident[dev]) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOne + kMore);
             int per = 0;
-            if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, kSmem);
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, kOne + kMore);
             if (e != cudaSuccess) return e;
             resident[dev] = sms * std::max(1, per);
         }
@@ -640,7 +763,7 @@ cudaError_t launch(SampleParams& p, int rows, cudaStream_t st) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3((unsigned)rows * (unsigned)ctas);
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kSmem;
+    config.dynamicSmemBytes = kOne + (ctas > 1 ? kMore : 0);
     config.stream = st;
     cudaLaunchAttribute attributes[2]{};
     attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -648,7 +771,7 @@ cudaError_t launch(SampleParams& p, int rows, cudaStream_t st) {
     attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attributes;
-    config.numAttrs = 2;
+    config.numAttrs = 2;  // (a cluster of one, too)
     return cudaLaunchKernelEx(&config, kernel, p);
 }
 
