@@ -430,27 +430,27 @@ def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, prefix_table: 
     return (out, lse) if return_lse else out
 
 
-def _wide(t: torch.Tensor, what: str, device, dtypes=(torch.bfloat16,)):
-    """(t, row stride) of rows [..., H] as [rows, H] with elements in one run; cast to BF16 where the type is none of `dtypes`."""
-    if t.device != device:
-        raise ValueError(f"{what} must be on {device}, got {t.device}")
-    if t.dtype not in dtypes:
+def _wide(t: torch.Tensor, what: str, index: int):
+    """(t, row stride) of BF16 rows [..., H] as [rows, H] with elements in one run (cast or copied only if they are not)."""
+    if t.get_device() != index:
+        raise ValueError(f"{what} must be on cuda:{index}, got {t.device}")
+    if t.dtype is not torch.bfloat16:
         t = t.to(torch.bfloat16)
-    if t.is_contiguous():
-        return t, t.shape[-1]
+    return (t, t.shape[-1]) if t.is_contiguous() else _strided(t)
+
+
+def _strided(t: torch.Tensor):
     t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    if t.shape[1] > 1 and t.stride(1) != 1:
         t = t.contiguous()
     return t, t.stride(0)
 
 
-def _vector(t, h: int, what: str, device):
+def _vector(t, h: int, what: str, index: int):
     """A weight [H] in BF16, its elements in one run."""
-    if t is None:
-        return None
-    if t.numel() != h or t.device != device:
-        raise ValueError(f"{what} must have {h} elements on {device}")
-    if t.dtype != torch.bfloat16:
+    if t.numel() != h or t.get_device() != index:
+        raise ValueError(f"{what} must have {h} elements on cuda:{index}")
+    if t.dtype is not torch.bfloat16:
         t = t.to(torch.bfloat16)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -472,50 +472,57 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, po
 
     Returns new tensors (normed, r): normed BF16, r of residual's type (residual itself where x is None).
     """
-    dev, h = residual.device, residual.shape[-1] if residual.dim() else 0
-    if not residual.is_cuda:
+    index, shape = residual.get_device(), residual.shape
+    if index < 0:
         raise ValueError("residual must be on a CUDA device")
+    h = shape[-1] if len(shape) else 0
     if not 0 < h <= 32768:
-        raise ValueError(f"rows must have 1 to 32768 elements, got shape {tuple(residual.shape)}")
-    if x is None and (post_weight is not None or gate is not None):
-        raise ValueError("post_weight and gate belong to a block's output: x is None")
-    shape, rows = residual.shape, residual.numel() // h
-    if residual.dtype != torch.float32 and residual.dtype != torch.bfloat16:
+        raise ValueError(f"rows must have 1 to 32768 elements, got shape {tuple(shape)}")
+    fp32 = residual.dtype is torch.float32
+    if not fp32 and residual.dtype is not torch.bfloat16:
         residual = residual.to(torch.bfloat16)
-    r_rows, r_stride = _wide(residual, "residual", dev, (torch.bfloat16, torch.float32))
-    weight, post_weight = _vector(weight, h, "weight", dev), _vector(post_weight, h, "post_weight", dev)
-    x_stride = gate_stride = 0
+    r_rows, r_stride = (residual, h) if residual.is_contiguous() else _strided(residual)
+    weight = _vector(weight, h, "weight", index)
+    normed = weight.new_empty(shape)
     out = residual
+    x_at = x_stride = gate_at = gate_stride = post_at = 0
     if x is not None:
         if x.shape != shape:
             raise ValueError(f"x {tuple(x.shape)} and residual {tuple(shape)} have other shapes")
-        x, x_stride = _wide(x, "x", dev)
+        x, x_stride = _wide(x, "x", index)
+        x_at = x.data_ptr()
+        if post_weight is not None:
+            post_weight = _vector(post_weight, h, "post_weight", index)
+            post_at = post_weight.data_ptr()
         if gate is not None:
             if gate.dim() == 1 and gate.shape[0] == h:
-                gate = _vector(gate, h, "gate", dev)
+                gate = _vector(gate, h, "gate", index)
             elif gate.shape == shape:
-                gate, gate_stride = _wide(gate, "gate", dev)
+                gate, gate_stride = _wide(gate, "gate", index)
             else:
                 raise ValueError(f"gate must be [{h}] or {tuple(shape)}, got {tuple(gate.shape)}")
-        out = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    normed = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+            gate_at = gate.data_ptr()
+        out = residual.new_empty(shape)
+    elif post_weight is not None or gate is not None:
+        raise ValueError("post_weight and gate belong to a block's output: x is None")
+    rows = normed.numel() // h
     if rows:
-        _call(dev, _block_norm, "block_norm", _NORM.pack(
-            _address(x), x_stride, r_rows.data_ptr(), r_stride, _address(gate), gate_stride, weight.data_ptr(), _address(post_weight),
-            normed.data_ptr(), 0 if x is None else out.data_ptr(), rows, h, residual.dtype == torch.float32, scale, eps))
+        _call(normed.device, _block_norm, "block_norm", _NORM.pack(
+            x_at, x_stride, r_rows.data_ptr(), r_stride, gate_at, gate_stride, weight.data_ptr(), post_at, normed.data_ptr(),
+            out.data_ptr() if x_at else 0, rows, h, fp32, scale, eps))
     return normed, out
 
 
 _LOGITS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # FP4B_LOGITS_*
 
 
-def _setting(v, rows: int, dtype, what: str, device):
+def _setting(v, rows: int, dtype, what: str, index: int):
     """(address, number, tensor to keep) of a setting: one number for all rows, or a tensor [rows]."""
     if not isinstance(v, torch.Tensor):
         return 0, v, None
-    if v.device != device or v.numel() != rows:
-        raise ValueError(f"{what} must be a number or {rows} numbers on {device}, got {tuple(v.shape)} on {v.device}")
-    if v.dtype != dtype:
+    if v.get_device() != index or v.numel() != rows:
+        raise ValueError(f"{what} must be a number or {rows} numbers on cuda:{index}, got {tuple(v.shape)} on {v.device}")
+    if v.dtype is not dtype:
         v = v.to(dtype)
     if not v.is_contiguous():
         v = v.contiguous()
@@ -541,30 +548,32 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     Returns int64 [B], -1 for a row without candidates; with return_prob=True also fp32 [B], the share of the kept ones' sum
     that the token has (1 at temperature 0, 0 where there is none).
     """
-    if logits.dim() != 2 or logits.dtype not in _LOGITS:
+    kind = _LOGITS.get(logits.dtype)
+    if kind is None or logits.dim() != 2:
         raise ValueError(f"logits must be [B, V] BF16, FP16 or fp32, got {logits.dtype} {tuple(logits.shape)}")
-    if not logits.is_cuda:
+    index = logits.get_device()
+    if index < 0:
         raise ValueError("logits must be on a CUDA device")
     b, v = logits.shape
-    dev = logits.device
     if v == 0 or v > 1 << 30:
         raise ValueError(f"the vocabulary must be 1 to 2^30 tokens, got {v}")
-    if u.dtype != torch.float32 or u.device != dev or u.numel() != b:
-        raise ValueError(f"u must be {b} fp32 numbers on {dev}, got {u.dtype} {tuple(u.shape)} on {u.device}")
+    if u.dtype is not torch.float32 or u.get_device() != index or u.numel() != b:
+        raise ValueError(f"u must be {b} fp32 numbers on cuda:{index}, got {u.dtype} {tuple(u.shape)} on {u.device}")
     if not u.is_contiguous():
         u = u.contiguous()
-    if v > 1 and logits.stride(1) != 1:
-        logits = logits.contiguous()
-    t_at, t_one, t_keep = _setting(temperature, b, torch.float32, "temperature", dev)
-    k_at, k_one, k_keep = _setting(top_k, b, torch.int32, "top_k", dev)
-    p_at, p_one, p_keep = _setting(top_p, b, torch.float32, "top_p", dev)
-    m_at, m_one, m_keep = _setting(min_p, b, torch.float32, "min_p", dev)
+    stride, step = logits.stride()
+    if step != 1 and v > 1:
+        logits, stride = logits.contiguous(), v
+    t_at, t_one, t_keep = _setting(temperature, b, torch.float32, "temperature", index)
+    k_at, k_one, k_keep = _setting(top_k, b, torch.int32, "top_k", index)
+    p_at, p_one, p_keep = _setting(top_p, b, torch.float32, "top_p", index)
+    m_at, m_one, m_keep = _setting(min_p, b, torch.float32, "min_p", index)
     if t_at == 0 and not t_one >= 0.0:
         raise ValueError(f"temperature must not be negative, got {t_one}")
-    tokens = torch.empty(b, dtype=torch.int64, device=dev)
-    probs = torch.empty_like(u) if return_prob else None
+    tokens = u.new_empty(b, dtype=torch.int64)
+    probs = u.new_empty(b) if return_prob else None
     if b:
-        _call(dev, _sample, "sample", _SAMPLING.pack(
-            logits.data_ptr(), logits.stride(0), u.data_ptr(), t_at, k_at, p_at, m_at, tokens.data_ptr(), _address(probs), b, v,
-            _LOGITS[logits.dtype], t_one, min(max(int(k_one), 0), v), p_one, m_one))
+        _call(tokens.device, _sample, "sample", _SAMPLING.pack(
+            logits.data_ptr(), stride, u.data_ptr(), t_at, k_at, p_at, m_at, tokens.data_ptr(), probs.data_ptr() if return_prob else 0, b, v,
+            kind, t_one, min(max(int(k_one), 0), v), p_one, m_one))
     return (tokens, probs) if return_prob else tokens
