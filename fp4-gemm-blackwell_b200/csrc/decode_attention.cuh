@@ -219,7 +219,7 @@ __device__ __forceinline__ Finish finish(const AttentionParams& p, int head, flo
 // Joins four elements of a row, relative to 2^m, with the parts found over its prefix.
 template <int D>
 __device__ __forceinline__ void join_prefix(const AttentionParams& p, int b, int head, int d, float& m, float& l, float4& sum) {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     const PrefixParts& x = p.prefix;
     const int g = b / x.each, kv_head = head / p.group;
     const int r = (b - g * x.each) * p.group + head - kv_head * p.group;
@@ -947,10 +947,14 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(const __grid
         }
     }
 
-    // ---- sequences without keys: zeros, and the sink's share alone
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    // ---- sequences without keys: zeros, and the sink's share alone (or the prefix's,
+    // whose many parts are joined by as many CTAs as there are)
+    constexpr int PIECES = PREFIX ? kThreads : 1 << 30;  // quarters of rows that a CTA takes of a sequence at once
+    const int quarters = p.q_heads * (D / 4), turns = PREFIX ? (quarters + PIECES - 1) / PIECES : 1;
+    for (int x = blockIdx.x; x < p.batch * turns; x += gridDim.x) {
+        const int b = PREFIX ? x / turns : x, from = PREFIX ? (x - b * turns) * PIECES : 0;
         if (span_of<TK, C::ROUND>(p, b).rounds > 0) continue;
-        for (int i = tid; i < p.q_heads * (D / 4); i += kThreads) {
+        for (int i = from + tid; i < (PREFIX ? min(from + PIECES, quarters) : quarters); i += kThreads) {
             const int h = i / (D / 4);
             put_row<D, PREFIX>(p, b, h, 4 * (i - h * (D / 4)), kNoScore, 0.0f, make_float4(0.f, 0.f, 0.f, 0.f), kUnit);
         }
@@ -1005,7 +1009,8 @@ cudaError_t launch(AttentionParams& p, uint8_t* workspace, cudaStream_t st) {
     // No more CTAs than the page table has rounds for (and one for each empty sequence's row).
     const long keys = (long)p.table_width << p.page_shift;
     const long most = (long)p.batch * std::max(1l, (keys + C::ROUND - 1) / C::ROUND * p.cache.kv_heads * p.group_tiles);
-    return launch_chained(kernel, dim3((unsigned)std::min<long>(resident[dev], most)), kThreads, C::SMEM, st, p);
+    const long rows = PREFIX ? (long)p.batch * ((p.q_heads * (D / 4) + kThreads - 1) / kThreads) : 0;  // that a prefix alone may have
+    return launch_chained(kernel, dim3((unsigned)std::min<long>(resident[dev], std::max(most, rows))), kThreads, C::SMEM, st, p);
 }
 
 // Pages of 16 where 32 keys are worked on at once have a form of their own: 3 x
