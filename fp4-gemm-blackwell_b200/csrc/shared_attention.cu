@@ -10,13 +10,14 @@
 //
 // A CTA, one an SM, takes a share of all tiles of keys (128, or 64 of 256
 // elements): unit by unit (prefix, key head, 128 rows), a tile at a time.
-//   warps 8-11 (4-7)   bring K and V in 16 bits and the 128-byte swizzle, two warps
-//                      each: bf16 by TMA boxes of whole pages, fp8 and nvfp4
-//                      decoded on the way;
-//   warp 12 (8)        issues the products: S of the next tile before O of this;
-//   warps 0-7 (0-3)    two groups of 128 threads, a row a thread, take the tiles
-//                      in turn: each has scores, sums and an O of its own, so
-//                      that neither waits for the other (256 elements: one).
+//   the first 8 (4)    two slots of 128 threads, a row a thread, take the tiles in
+//                      turn: each has scores, sums and an O of its own, so that
+//                      neither waits for the other (256 elements: one);
+//   4 or 8 feeders     bring K and V in 16 bits and the 128-byte swizzle, half of them
+//                      each: bf16 by TMA boxes of whole pages, fp8 and nvfp4 decoded
+//                      on the way (two warps each took 74 us where four take 66:
+//                      32 sequences, 32768 keys x 8 x 64 of nvfp4, 64 heads);
+//   one warp           issues the products: S of the next tiles before O of this.
 // O stays in TMEM over a unit; S (128 columns of fp32) is read twice, for its
 // largest and for the weights, which go back over it as the A operand of the
 // second product.
@@ -38,7 +39,6 @@ namespace {
 
 constexpr int kErrPrefixTimeout = 14;
 constexpr int kTileRows = 128;
-constexpr int kProducers = 128;
 constexpr int kSmemMost = 232448;
 
 struct PrefixParams {
@@ -64,28 +64,33 @@ struct PrefixParams {
 template <int KIND, int D>
 struct PrefixCfg {
     static constexpr int TK = D == 256 ? 64 : 128;                                   // keys of a tile
-    static constexpr int GROUPS = D == 256 ? 1 : 2;
-    static constexpr int THREADS = GROUPS * 128 + kProducers + 128;
+    static constexpr int SLOTS = D == 256 ? 1 : 2;                                   // tiles that are worked on at once
+    // Warps for K, and as many for V: decoding takes time, starting boxes does not.
+    static constexpr int FEEDERS = KIND == kKvBf16 ? 2 : 4;
+    static constexpr int ROW_THREADS = SLOTS * 128, THREADS = ROW_THREADS + 2 * FEEDERS * 32 + 128;
     static constexpr int RB = KIND == kKvBf16 ? 2 * D : KIND == kKvFp8 ? D : D / 2;  // bytes of a row
     static constexpr int SB = KIND == kKvBf16 ? 0 : KIND == kKvFp8 ? 4 : D / 16;     // bytes of its scales
     static constexpr int Q = kTileRows * D * 2;
     static constexpr int PIECE = TK * D * 2;                                         // K or V of a tile in 16 bits
-    static constexpr int STAGES = KIND == kKvBf16 ? (D == 64 ? 5 : D == 128 ? 3 : 2) : D == 64 ? 3 : 2;
-    // fp8 and nvfp4 come through a ring of half pieces as they lie in the cache: of K,
-    // and of V (with fp8's scales of both).
-    static constexpr int HALF_K = KIND == kKvBf16 ? 0 : TK / 2 * (RB + (KIND == kKvFp8 ? 0 : SB));
-    static constexpr int HALF_V = KIND == kKvBf16 ? 0 : TK / 2 * (RB + (KIND == kKvFp8 ? 2 * SB : SB));
-    static constexpr int HALVES = KIND == kKvFp8 ? (D == 64 ? 6 : D == 128 ? 3 : 2) : D == 64 ? 6 : D == 128 ? 4 : 3;
+    static constexpr int K_STAGES = KIND == kKvBf16 ? (D == 64 ? 5 : D == 128 ? 3 : 2) : D == 64 ? 3 : KIND == kKvNvfp4 && D == 128 ? 2 : 1;
+    static constexpr int V_STAGES = KIND == kKvBf16 ? (D == 64 ? 5 : 2) : D == 64 ? 3 : KIND == kKvFp8 && D == 256 ? 1 : 2;
+    // fp8 and nvfp4 come through rings as they lie in the cache, of each producing warp's
+    // own: its rows' codes and scales (with V fp8's scales of both).
+    static constexpr int ROWS = TK / FEEDERS;
+    static constexpr int RAW_K = KIND == kKvBf16 ? 0 : ROWS * (RB + (KIND == kKvFp8 ? 0 : SB));
+    static constexpr int RAW_V = KIND == kKvBf16 ? 0 : ROWS * (RB + (KIND == kKvFp8 ? 2 * SB : SB));
+    static constexpr int RAWS = KIND == kKvBf16 ? 0 : D == 64 ? 4 : KIND == kKvFp8 ? 2 : 3;
     static constexpr int SCALES = KIND == kKvFp8 ? 3 * TK * 4 : 0;                   // of a stage: key scales, value scales, their logarithms
     static constexpr int BUFFERS = D == 64 ? 3 : 2;                                  // of S in TMEM
     static constexpr int S_COLUMNS = BUFFERS * TK;
-    static constexpr int OFF_K = Q, OFF_V = OFF_K + STAGES * PIECE, OFF_RAW_K = OFF_V + STAGES * PIECE, OFF_RAW_V = OFF_RAW_K + HALVES * HALF_K;
-    static constexpr int OFF_SCALES = OFF_RAW_V + HALVES * HALF_V, OFF_BARS = OFF_SCALES + STAGES * SCALES;
-    static constexpr int OFF_FACTORS = OFF_BARS + (4 * STAGES + 2 * BUFFERS + 5 + (KIND == kKvBf16 ? 0 : 4 * HALVES)) * 8, OFF_VARS = OFF_FACTORS + kTileRows * 4;  // (each a multiple of 8)
+    static constexpr int BARS = 2 * K_STAGES + 2 * V_STAGES + 2 * BUFFERS + 5 + 8 * RAWS;
+    static constexpr int OFF_K = Q, OFF_V = OFF_K + K_STAGES * PIECE, OFF_RAW_K = OFF_V + V_STAGES * PIECE, OFF_RAW_V = OFF_RAW_K + 4 * RAWS * RAW_K;
+    static constexpr int OFF_SCALES = OFF_RAW_V + 4 * RAWS * RAW_V, OFF_BARS = OFF_SCALES + V_STAGES * SCALES;
+    static constexpr int OFF_FACTORS = OFF_BARS + BARS * 8, OFF_VARS = OFF_FACTORS + kTileRows * 4;
     static constexpr int SMEM = OFF_VARS + 32;
     static_assert(SMEM <= kSmemMost, "shared memory");
-    static_assert(S_COLUMNS + GROUPS * D <= 512, "TMEM");
-    static_assert(HALF_K % 32 == 0 && HALF_V % 32 == 0 && OFF_SCALES % 16 == 0 && OFF_BARS % 8 == 0, "alignment");
+    static_assert(S_COLUMNS + SLOTS * D <= 512, "TMEM");
+    static_assert(RAW_K % 16 == 0 && RAW_V % 16 == 0 && OFF_SCALES % 16 == 0 && OFF_BARS % 8 == 0, "alignment");
 };
 
 // The tiles of this CTA, unit by unit: every role goes over them by itself.
@@ -131,7 +136,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <int KIND, int D>
 __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attention_kernel(const __grid_constant__ PrefixParams p) {
     using C = PrefixCfg<KIND, D>;
-    constexpr int TK = C::TK, GROUPS = C::GROUPS, STAGES = C::STAGES, RB = C::RB, SB = C::SB;
+    constexpr int TK = C::TK, SLOTS = C::SLOTS, RB = C::RB, SB = C::SB;
     constexpr bool kBf16 = KIND == kKvBf16;
     extern __shared__ __align__(1024) uint8_t tiles_smem[];
     uint8_t* const smem = tiles_smem;
@@ -141,25 +146,22 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
     uint32_t& s_tmem = reinterpret_cast<uint32_t&>(vars[0]);
     int &s_abort = vars[1], &s_total = vars[2], &s_g = vars[3], &s_before = vars[4];
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BARS);
-    uint64_t *const k_full = bars, *const k_empty = bars + STAGES, *const v_full = bars + 2 * STAGES, *const v_empty = bars + 3 * STAGES;
-    uint64_t *const s_full = bars + 4 * STAGES, *const p_full = s_full + C::BUFFERS, *const q_full = p_full + C::BUFFERS, *const o_done = q_full + 1;
-    uint64_t *const unit_done = q_full + 3, *const drained = q_full + 4, *const raw_full = q_full + 5;  // (o_done: of each group)
+    uint64_t *const k_full = bars, *const k_empty = k_full + C::K_STAGES, *const v_full = k_empty + C::K_STAGES, *const v_empty = v_full + C::V_STAGES;
+    uint64_t *const s_full = v_empty + C::V_STAGES, *const p_full = s_full + C::BUFFERS, *const q_full = p_full + C::BUFFERS, *const o_done = q_full + 1;
+    uint64_t *const unit_done = q_full + 3, *const drained = q_full + 4, *const raw_full = q_full + 5;  // (o_done: of each slot)
 
     chain();
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    constexpr int kProducerWarp = GROUPS * 4, kMmaWarp = kProducerWarp + 4;
+    constexpr int kProducerWarp = SLOTS * 4, kMmaWarp = kProducerWarp + 2 * C::FEEDERS;
 
     // ---- set up: barriers, TMEM, this CTA's share
     if (tid == 0) {
         s_abort = 0;
-        for (int i = 0; i < STAGES; ++i) {
-            ptx::mbar_init(k_full + i, kProducers / 2), ptx::mbar_init(v_full + i, kProducers / 2);
-            ptx::mbar_init(k_empty + i, 1), ptx::mbar_init(v_empty + i, 1);
-        }
+        for (int i = 0; i < C::K_STAGES; ++i) ptx::mbar_init(k_full + i, 32 * C::FEEDERS), ptx::mbar_init(k_empty + i, 1);
+        for (int i = 0; i < C::V_STAGES; ++i) ptx::mbar_init(v_full + i, 32 * C::FEEDERS), ptx::mbar_init(v_empty + i, 1);
         for (int i = 0; i < C::BUFFERS; ++i) ptx::mbar_init(s_full + i, 1), ptx::mbar_init(p_full + i, 128);
-        ptx::mbar_init(q_full, GROUPS * 128), ptx::mbar_init(o_done, 1), ptx::mbar_init(o_done + 1, 1), ptx::mbar_init(unit_done, 1), ptx::mbar_init(drained, 1);
-        if (!kBf16)
-            for (int i = 0; i < 4 * C::HALVES; ++i) ptx::mbar_init(raw_full + i, 1);
+        ptx::mbar_init(q_full, C::ROW_THREADS), ptx::mbar_init(o_done, 1), ptx::mbar_init(o_done + 1, 1), ptx::mbar_init(unit_done, 1), ptx::mbar_init(drained, 1);
+        for (int i = 0; i < 8 * C::RAWS; ++i) ptx::mbar_init(raw_full + i, 1);
         ptx::fence_mbar_init();
     }
     if (warp == kMmaWarp) {
@@ -234,28 +236,31 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
     };
 
     // Rows take more registers than a block has for each thread, the others fewer:
-    // 256 x 184 + 256 x 72 = 512 x 128.
-    if constexpr (GROUPS == 2) {
-        if (warp < kProducerWarp) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // 256 x 184 + 256 x 72 = 512 x 128, 256 x 168 + 384 x 48 = 640 x 96.
+    if constexpr (SLOTS == 2) {
+        constexpr int kMore = kBf16 ? 184 : 168, kFewer = kBf16 ? 72 : 48;
+        static_assert(256 * kMore + (C::THREADS - 256) * kFewer == C::THREADS * (65536 / C::THREADS / 8 * 8), "registers");
+        if (warp < kProducerWarp) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMore));
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewer));
     }
 
     if (working && warp < kProducerWarp) {
         // ------------------------------------------------------------ a row a thread: queries, softmax, results
-        const int mine = warp >> 2, row = tid & 127;
+        // Where a wait gives up the tiles are gone through without waiting: every barrier is met.
+        const int mine = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's 32 lanes
         const uint32_t o_at = lanes + C::S_COLUMNS + mine * D;
         int it = 0, segment = 0;
         bool ok = true;
-        while (ok && next_unit<TK>(p, walk)) {
+        while (next_unit<TK>(p, walk)) {
             const int rows = min(kTileRows, p.rows - walk.tile * kTileRows);
             const bool live = (warp & 3) * 32 < rows;
             {
                 // ---- Q in 16 bits and swizzled, 8 elements a lane; rows that there are not as zeros
-                constexpr int LANES = D / 8, AT_ONCE = GROUPS * 128 / LANES, PASSES = kTileRows / AT_ONCE;
+                constexpr int LANES = D / 8, AT_ONCE = C::ROW_THREADS / LANES, PASSES = kTileRows / AT_ONCE;
                 const int c = tid % LANES;
                 const uint32_t sign = p.scale2 < 0.0f ? 0x80008000u : 0u;  // goes to the queries
-#pragma unroll 8
+#pragma unroll 4
                 for (int i = 0; i < PASSES; ++i) {
                     const int r = i * AT_ONCE + tid / LANES, all = walk.tile * kTileRows + r, of = all / p.group;
                     uint2 a = make_uint2(0u, 0u), b = a;
@@ -271,8 +276,8 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                         const float up = __int_as_float((127 + k) << 23);
                         factor *= __int_as_float((127 - k) << 23);
                         if (KIND == kKvNvfp4) factor *= kScaleUnit;
-                        auto half = [&](uint32_t w) { return pack_f16(bf16_lo(w) * up, bf16_hi(w) * up); };
-                        a = make_uint2(half(a.x), half(a.y)), b = make_uint2(half(b.x), half(b.y));
+                        auto half16 = [&](uint32_t w) { return pack_f16(bf16_lo(w) * up, bf16_hi(w) * up); };
+                        a = make_uint2(half16(a.x), half16(a.y)), b = make_uint2(half16(b.x), half16(b.y));
                     }
                     if (c == 0) s_factor[r] = fmaxf(factor, 0x1p-126f);  // (masked keys' -inf stays one where scale is 0)
                     const int to = (c >> 3) * (kTileRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -281,21 +286,20 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                 ptx::fence_proxy_async_smem();
             }
             ptx::mbar_arrive(q_full);
-            ok = wait(q_full, segment & 1);
+            ok = ok && wait(q_full, segment & 1);
             const float f = s_factor[row];
             float ref = kNoScore, l = 0.0f;
             bool begun = false;
-            for (int j = walk.r0; ok && j < walk.r1; ++j, ++it) {
-                if (GROUPS == 2 && (it & 1) != mine) continue;
-                const int buf = it % C::BUFFERS, stage = it % STAGES;
-                ok = wait(s_full + buf, (it / C::BUFFERS) & 1);
-                if (KIND == kKvFp8 && ok) ok = wait(v_full + stage, (it / STAGES) & 1);
-                if (!ok) break;
+            for (int j = walk.r0; j < walk.r1; ++j, ++it) {
+                if (SLOTS == 2 && (it & 1) != mine) continue;
+                const int buf = it % C::BUFFERS, stage = it % C::V_STAGES;
+                ok = ok && wait(s_full + buf, (it / C::BUFFERS) & 1);
+                if (KIND == kKvFp8) ok = ok && wait(v_full + stage, (it / C::V_STAGES) & 1);
                 ptx::tc_fence_after();
+                const uint32_t s_at = lanes + buf * TK;
+                const float4* const scales = reinterpret_cast<const float4*>(smem + C::OFF_SCALES + stage * C::SCALES);
+                const int seen = walk.valid - j * TK;  // keys of the tile that there are
                 if (live) {
-                    const uint32_t s_at = lanes + buf * TK;
-                    const float4* const scales = reinterpret_cast<const float4*>(smem + C::OFF_SCALES + stage * C::SCALES);
-                    const int seen = walk.valid - j * TK;  // keys of the tile that there are
                     float s[TK];
 #pragma unroll
                     for (int c = 0; c < TK / 32; ++c) ptx::tmem_ld_32x32b_x32(s_at + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                         ref = to;
                         l *= c;
                         if (begun) {
-                            ok = wait(o_done + mine, (it / GROUPS - 1) & 1);  // the group's last product
+                            ok = ok && wait(o_done + mine, (it / SLOTS - 1) & 1);  // the slot's last product
                             ptx::tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < D; d += 32) {
@@ -386,12 +390,11 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                 ptx::mbar_arrive(p_full + buf);
             }
             // ---- the unit's part: (reference, sum) and O
-            if (ok) ok = wait(unit_done, segment & 1);
-            if (!ok) break;
+            ok = ok && wait(unit_done, segment & 1);
             ptx::tc_fence_after();
             const int first = owner(walk.u - walk.r1), count = owner(walk.u - walk.r1 + walk.length - 1) - first + 1;
-            const size_t part = ((size_t)walk.unit + blockIdx.x) * GROUPS + mine;
-            if (walk.r0 == 0 && tid == 0) p.units[walk.unit] = make_int2((walk.unit + first) * GROUPS, count * GROUPS);
+            const size_t part = ((size_t)walk.unit + blockIdx.x) * SLOTS + mine;
+            if (walk.r0 == 0 && tid == 0) p.units[walk.unit] = make_int2((walk.unit + first) * SLOTS, count * SLOTS);
             if (live) {
                 const size_t to = part * p.part_rows + row;
                 if (row < rows) p.ml[to] = make_float2(ref, l);
@@ -411,17 +414,18 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
         }
     } else if (working && warp < kMmaWarp) {
         // ------------------------------------------------------------ pages to K and V in shared memory
-        // Two warps for K, two for V; each warp has half of a tile's rows.
-        const bool value = warp >= kProducerWarp + 2;
-        const int my = warp & 1;
-        constexpr int ROWS = TK / 2;
+        // Each warp has its share of a tile's rows.
+        const bool value = warp >= kProducerWarp + C::FEEDERS;
+        const int my = (warp - kProducerWarp) % C::FEEDERS, stages = value ? C::V_STAGES : C::K_STAGES;
+        constexpr int ROWS = C::ROWS;
         constexpr int LR = RB / 16, PER = 32 / LR;  // lanes a row, rows an instruction
         const int sub = lane / LR, c = lane % LR;
         uint64_t *const full = value ? v_full : k_full, *const empty = value ? v_empty : k_empty;
         uint8_t* const pieces = smem + (value ? C::OFF_V : C::OFF_K);
         const uint8_t* const from = static_cast<const uint8_t*>(value ? p.cache.v : p.cache.k);
         bool ok = true;
-        int t = 0;
+        int t = 0, stage = 0;
+        uint32_t round = 0;  // of the stages, its low bit the barriers' phase
         auto row_of = [&](int page, int key) {  // in the cache; -1: none to read
             if (page >= 0 && page < p.cache.num_pages)
                 return (page * p.cache.kv_heads + walk.kv_head) * p.cache.page_size + (key & (p.cache.page_size - 1));
@@ -446,8 +450,8 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                     return lane < p.runs && j < walk.r1 && key < walk.valid ? table[key >> p.page_shift] : 0;
                 };
                 int next = look(walk.r0);
-                for (int j = walk.r0; j < walk.r1; ++j, ++t) {
-                    const int stage = t % STAGES, key0 = j * TK, entry = next;
+                for (int j = walk.r0; j < walk.r1; ++j, ++t, stage = stage + 1 == stages ? (++round, 0) : stage + 1) {
+                    const int key0 = j * TK, entry = next;
                     next = look(j + 1);
                     uint8_t* const to = pieces + stage * C::PIECE;
                     bool boxes = p.runs > 0 && walk.valid - key0 >= TK;
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                         if (lane < p.runs) first = row_of(max(entry, -1), key0 + lane * run);
                         boxes = __all_sync(0xffffffffu, lane >= p.runs || first >= 0);
                     }
-                    if (t >= STAGES && !wait(empty + stage, ((t / STAGES) & 1) ^ 1)) {
+                    if (round > 0 && !wait(empty + stage, (round & 1) ^ 1)) {
                         ok = false;
                         break;
                     }
@@ -469,16 +473,15 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                             for (int n = 0; n < D / 64; ++n)
                                 ptx::tma_load_2d(to + n * (TK * 128) + lane * run * 128, value ? &p.v_map : &p.k_map, full + stage, 128 * n, first);
                     } else {
-                        int rows[(ROWS + 31) / 32];
-#pragma unroll
-                        for (int i = 0; i < (ROWS + 31) / 32; ++i) {
-                            const int key = key0 + my * ROWS + 32 * i + lane;
-                            rows[i] = row_of(key < walk.valid ? max(table[key >> p.page_shift], -1) : -2, key);
-                        }
+#pragma unroll 1
+                        for (int r0 = my * ROWS; r0 < (my + 1) * ROWS; r0 += min(ROWS, 32)) {
+                            const int key = key0 + r0 + lane;
+                            const int mine = row_of(lane < ROWS && key < walk.valid ? max(table[key >> p.page_shift], -1) : -2, key);
 #pragma unroll 4
-                        for (int i = 0; i < ROWS / PER; ++i) {
-                            const int r = i * PER + sub, at = __shfl_sync(0xffffffffu, i * PER < 32 ? rows[0] : rows[(ROWS + 31) / 32 - 1], r & 31), tr = my * ROWS + r;
-                            copy_async<16>(ptx::smem_u32(to + (c >> 3) * (TK * 128) + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)), from + (size_t)max(at, 0) * RB + 16 * c, at >= 0);
+                            for (int i = 0; i < min(ROWS, 32) / PER; ++i) {
+                                const int r = i * PER + sub, at = __shfl_sync(0xffffffffu, mine, r), tr = r0 + r;
+                                copy_async<16>(ptx::smem_u32(to + (c >> 3) * (TK * 128) + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)), from + (size_t)max(at, 0) * RB + 16 * c, at >= 0);
+                            }
                         }
                         copy_commit();
                         if (pending >= 0) {
@@ -496,60 +499,56 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
             copy_wait<0>();
             if (ok && pending >= 0) hand_on();
             if (!ok)  // (what is under way has to end before shared memory goes)
-                for (int i = max(t - STAGES, 0); i < t; ++i) ptx::mbar_wait(full + i % STAGES, (i / STAGES) & 1);
+                for (int i = max(t - stages, 0); i < t; ++i) ptx::mbar_wait(full + i % stages, (i / stages) & 1);
         } else {
-            // Half pieces through a ring of the warp's own: bulk copies of whole pages' runs,
-            // or row by row where they are not whole.
-            constexpr int HROWS = ROWS / 2, COPIES = HROWS / PER, AHEAD = C::HALVES - 1;
+            // Through a ring of the warp's own: bulk copies of whole pages' runs, or row by row
+            // where they are not whole.
+            constexpr int COPIES = ROWS / PER, AHEAD = C::RAWS - 1;
             constexpr int GROUP = COPIES < 4 ? COPIES : 4;  // decoded at once
-            const int half_bytes = value ? C::HALF_V : C::HALF_K, warp_bytes = half_bytes / 2;
-            uint8_t* const raw = smem + (value ? C::OFF_RAW_V : C::OFF_RAW_K) + my * warp_bytes;
+            const int raw_bytes = value ? C::RAW_V : C::RAW_K, run = min(p.cache.page_size, ROWS);
+            uint8_t* const raw = smem + (value ? C::OFF_RAW_V : C::OFF_RAW_K) + my * C::RAWS * raw_bytes;
+            uint64_t* const arrived = raw_full + (warp - kProducerWarp) * C::RAWS;
             const uint8_t* const scales = static_cast<const uint8_t*>(value ? p.cache.v_scale : p.cache.k_scale);
             // `walk` is at the tile whose copies start, `here` at the one that is decoded
             Walk here = walk;
-            bool more = next_unit<TK>(p, walk);
-            int tile = walk.r0, issued = 0, slot = 0, entry = 0;
-            bool there = false;
-            auto key_of = [&]() { return tile * TK + my * ROWS + (issued & 1) * HROWS + lane; };
+            bool more = next_unit<TK>(p, walk), there = false;
+            int tile = walk.r0, slot = 0, entry = 0;
+            uint32_t bulk = 0, parity = 0;  // of the slots: whether bulk copies are under way, their phases
             auto look = [&]() {  // the table's entry of this lane's key, on its way (nothing here may wait for it)
-                const int key = key_of();
-                there = lane < HROWS && key < walk.valid;
+                const int key = tile * TK + my * ROWS + lane;
+                there = lane < ROWS && key < walk.valid;
                 if (there) entry = p.table[(size_t)walk.g * p.table_stride + (key >> p.page_shift)];
             };
             if (more) look();
-            uint64_t* const arrived = raw_full + (warp - kProducerWarp) * C::HALVES;
-            uint32_t bulk = 0, parity = 0;  // of the slots: whether bulk copies are under way, their phases
-            const int run = min(p.cache.page_size, HROWS);
             auto issue = [&]() {
                 if (more) {
-                    const int row = row_of(there ? max(entry, -1) : -2, key_of());
-                    uint8_t* const to = raw + slot * half_bytes;
-                    if (run >= 8 && __all_sync(0xffffffffu, lane >= HROWS || row >= 0)) {
+                    const int row = row_of(there ? max(entry, -1) : -2, tile * TK + my * ROWS + lane);
+                    uint8_t* const to = raw + slot * raw_bytes;
+                    if (run >= 8 && __all_sync(0xffffffffu, lane >= ROWS || row >= 0)) {
                         bulk |= 1u << slot;
-                        if (lane == 0) ptx::mbar_arrive_expect_tx(arrived + slot, warp_bytes);
+                        if (lane == 0) ptx::mbar_arrive_expect_tx(arrived + slot, raw_bytes);
                         __syncwarp();
-                        if (lane < HROWS && (lane & (run - 1)) == 0) {
+                        if (lane < ROWS && (lane & (run - 1)) == 0) {
                             ptx::bulk_load(to + lane * RB, from + (size_t)row * RB, run * RB, arrived + slot);
-                            if (KIND != kKvFp8 || value) ptx::bulk_load(to + HROWS * RB + lane * SB, scales + (size_t)row * SB, run * SB, arrived + slot);
+                            if (KIND != kKvFp8 || value) ptx::bulk_load(to + ROWS * RB + lane * SB, scales + (size_t)row * SB, run * SB, arrived + slot);
                             if (KIND == kKvFp8 && value)
-                                ptx::bulk_load(to + HROWS * (RB + SB) + lane * SB, static_cast<const uint8_t*>(p.cache.k_scale) + (size_t)row * SB, run * SB, arrived + slot);
+                                ptx::bulk_load(to + ROWS * (RB + SB) + lane * SB, static_cast<const uint8_t*>(p.cache.k_scale) + (size_t)row * SB, run * SB, arrived + slot);
                         }
                     } else {
-                        bulk &= ~(1u << slot);
                         const uint32_t at_smem = ptx::smem_u32(to);
 #pragma unroll
                         for (int i = 0; i < COPIES; ++i) {
                             const int at = __shfl_sync(0xffffffffu, row, i * PER + sub);
                             copy_async<16>(at_smem + (i * 32 + lane) * 16, from + (size_t)max(at, 0) * RB + 16 * c, at >= 0);
                         }
-                        if (lane < HROWS) {
-                            if (KIND != kKvFp8 || value) copy_async<SB>(at_smem + HROWS * RB + lane * SB, scales + (size_t)max(row, 0) * SB, row >= 0);
+                        if (lane < ROWS) {
+                            if (KIND != kKvFp8 || value) copy_async<SB>(at_smem + ROWS * RB + lane * SB, scales + (size_t)max(row, 0) * SB, row >= 0);
                             if (KIND == kKvFp8 && value)
-                                copy_async<SB>(at_smem + HROWS * (RB + SB) + lane * SB, static_cast<const uint8_t*>(p.cache.k_scale) + (size_t)max(row, 0) * SB, row >= 0);
+                                copy_async<SB>(at_smem + ROWS * (RB + SB) + lane * SB, static_cast<const uint8_t*>(p.cache.k_scale) + (size_t)max(row, 0) * SB, row >= 0);
                         }
                     }
-                    if (++slot == C::HALVES) slot = 0;
-                    if ((++issued & 1) == 0 && ++tile == walk.r1) {
+                    if (++slot == C::RAWS) slot = 0;
+                    if (++tile == walk.r1) {
                         more = next_unit<TK>(p, walk);
                         tile = walk.r0;
                     }
@@ -560,75 +559,70 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
             for (int i = 0; i < AHEAD; ++i) issue();
             int at_slot = 0;
             while (ok && next_unit<TK>(p, here)) {
-                for (int j = here.r0; ok && j < here.r1; ++j, ++t) {
-                    const int stage = t % STAGES;
-                    uint8_t* const to = pieces + stage * C::PIECE;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        issue();
-                        copy_wait<AHEAD>();
-                        __syncwarp();  // the other lanes' copies: a row's scales
-                        if (bulk >> at_slot & 1) {
-                            ok = wait(arrived + at_slot, parity >> at_slot & 1);
-                            parity ^= 1u << at_slot, bulk &= ~(1u << at_slot);
-                        }
-                        if (ok && half == 0 && t >= STAGES) ok = wait(empty + stage, ((t / STAGES) & 1) ^ 1);
+                for (int j = here.r0; j < here.r1; ++j, stage = stage + 1 == stages ? (++round, 0) : stage + 1) {
+                    issue();
+                    copy_wait<AHEAD>();
+                    __syncwarp();  // the other lanes' copies
+                    if (bulk >> at_slot & 1) {
+                        ok = wait(arrived + at_slot, parity >> at_slot & 1);
                         if (!ok) break;
-                        const uint8_t* const in = raw + at_slot * half_bytes;
-                        const int row0 = my * ROWS + half * HROWS;
+                        parity ^= 1u << at_slot, bulk &= ~(1u << at_slot);
+                    }
+                    if (round > 0) ok = wait(empty + stage, (round & 1) ^ 1);
+                    if (!ok) break;
+                    uint8_t* const to = pieces + stage * C::PIECE;
+                    const uint8_t* const in = raw + at_slot * raw_bytes;
 #pragma unroll
-                        for (int i0 = 0; i0 < COPIES; i0 += GROUP) {
-                            uint4 w[GROUP];
-                            uint32_t sc[GROUP];
+                    for (int i0 = 0; i0 < COPIES; i0 += GROUP) {
+                        uint4 w[GROUP];
+                        uint32_t sc[GROUP];
 #pragma unroll
-                            for (int i = 0; i < GROUP; ++i) {
-                                w[i] = lds128(in + ((i0 + i) * 32 + lane) * 16);
-                                if constexpr (KIND == kKvNvfp4) sc[i] = *reinterpret_cast<const uint16_t*>(in + HROWS * RB + ((i0 + i) * PER + sub) * SB + 2 * c);
-                            }
+                        for (int i = 0; i < GROUP; ++i) {
+                            w[i] = lds128(in + ((i0 + i) * 32 + lane) * 16);
+                            if constexpr (KIND == kKvNvfp4) sc[i] = *reinterpret_cast<const uint16_t*>(in + ROWS * RB + ((i0 + i) * PER + sub) * SB + 2 * c);
+                        }
 #pragma unroll
-                            for (int i = 0; i < GROUP; ++i) {
-                                const int r = row0 + (i0 + i) * PER + sub, e = (KIND == kKvFp8 ? 16 : 32) * c;
-                                uint8_t* const line = to + (e >> 6) * (TK * 128) + r * 128;
-                                const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                                auto put = [&](int n, uint4 v) { *reinterpret_cast<uint4*>(line + (((((e & 63) >> 3) + n) ^ (r & 7)) << 4)) = v; };
-                                if constexpr (KIND == kKvFp8) {
+                        for (int i = 0; i < GROUP; ++i) {
+                            const int r = my * ROWS + (i0 + i) * PER + sub, e = (KIND == kKvFp8 ? 16 : 32) * c;
+                            uint8_t* const line = to + (e >> 6) * (TK * 128) + r * 128;
+                            const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                            auto put = [&](int n, uint4 v) { *reinterpret_cast<uint4*>(line + (((((e & 63) >> 3) + n) ^ (r & 7)) << 4)) = v; };
+                            if constexpr (KIND == kKvFp8) {
 #pragma unroll
-                                    for (int h = 0; h < 2; ++h) {
-                                        uint32_t a[2], b[2];
-                                        e4m3x4_to_f16(words[2 * h], a);
-                                        e4m3x4_to_f16(words[2 * h + 1], b);
-                                        put(h, make_uint4(a[0], a[1], b[0], b[1]));
-                                    }
-                                } else {
+                                for (int h = 0; h < 2; ++h) {
+                                    uint32_t a[2], b[2];
+                                    e4m3x4_to_f16(words[2 * h], a);
+                                    e4m3x4_to_f16(words[2 * h + 1], b);
+                                    put(h, make_uint4(a[0], a[1], b[0], b[1]));
+                                }
+                            } else {
 #pragma unroll
-                                    for (int h = 0; h < 4; ++h) {
-                                        const uint32_t scale = ue4m3x2_to_f16((h < 2 ? sc[i] & 0xFFu : sc[i] >> 8) * 0x10001u);
-                                        uint32_t a[4];
-                                        e2m1x8_to_f16(words[h], a);
-                                        put(h, make_uint4(mul_f16x2(a[0], scale), mul_f16x2(a[1], scale), mul_f16x2(a[2], scale), mul_f16x2(a[3], scale)));
-                                    }
+                                for (int h = 0; h < 4; ++h) {
+                                    const uint32_t scale = ue4m3x2_to_f16((h < 2 ? sc[i] & 0xFFu : sc[i] >> 8) * 0x10001u);
+                                    uint32_t a[4];
+                                    e2m1x8_to_f16(words[h], a);
+                                    put(h, make_uint4(mul_f16x2(a[0], scale), mul_f16x2(a[1], scale), mul_f16x2(a[2], scale), mul_f16x2(a[3], scale)));
                                 }
                             }
                         }
-                        if constexpr (KIND == kKvFp8) {
-                            // (with V: the softmax that reads them ends before V's stage is free again)
-                            if (value && lane < HROWS) {
-                                float* const s = reinterpret_cast<float*>(smem + C::OFF_SCALES + stage * C::SCALES) + row0 + lane;
-                                const float scale = *reinterpret_cast<const float*>(in + HROWS * RB + lane * SB);
-                                s[0] = *reinterpret_cast<const float*>(in + HROWS * (RB + SB) + lane * SB);
-                                s[TK] = scale, s[2 * TK] = fmaxf(log2_approx(scale), -80.0f);
-                            }
-                        }
-                        if (++at_slot == C::HALVES) at_slot = 0;
-                        __syncwarp();  // (the half piece may be copied over)
                     }
-                    if (!ok) break;
+                    if constexpr (KIND == kKvFp8) {
+                        // (with V: the softmax that reads them ends before V's stage is free again)
+                        if (value && lane < ROWS) {
+                            float* const s = reinterpret_cast<float*>(smem + C::OFF_SCALES + stage * C::SCALES) + my * ROWS + lane;
+                            const float scale = *reinterpret_cast<const float*>(in + ROWS * RB + lane * SB);
+                            s[0] = *reinterpret_cast<const float*>(in + ROWS * (RB + SB) + lane * SB);
+                            s[TK] = scale, s[2 * TK] = fmaxf(log2_approx(scale), -80.0f);
+                        }
+                    }
+                    if (++at_slot == C::RAWS) at_slot = 0;
                     ptx::fence_proxy_async_smem();
                     ptx::mbar_arrive(full + stage);
+                    __syncwarp();  // (the slot may be copied over)
                 }
             }
             copy_wait<0>();
-            for (int i = 0; i < C::HALVES; ++i)  // (none are after the last tile)
+            for (int i = 0; i < C::RAWS; ++i)  // (none are after the last tile)
                 if (bulk >> i & 1) ptx::mbar_wait(arrived + i, parity >> i & 1);
         }
     } else if (working && warp == kMmaWarp) {
@@ -640,8 +634,8 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
         int it = 0, segment = 0;
         bool ok = true;
         auto scores = [&](int t) {  // S of tile t
-            const int stage = t % STAGES;
-            ok = wait(k_full + stage, (t / STAGES) & 1);
+            const int stage = t % C::K_STAGES;
+            ok = wait(k_full + stage, (t / C::K_STAGES) & 1);
             if (!ok) return;
             ptx::tc_fence_after();
             if (ptx::elect_one()) {
@@ -663,8 +657,8 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
             for (int j = 0; ok && j < n; ++j, ++it) {
                 if (j + kAhead < n) scores(it + kAhead);
                 if (!ok) break;
-                const int stage = it % STAGES, buf = it % C::BUFFERS, mine = GROUPS == 2 ? it & 1 : 0;
-                ok = wait(p_full + buf, (it / C::BUFFERS) & 1) && wait(v_full + stage, (it / STAGES) & 1);
+                const int stage = it % C::V_STAGES, buf = it % C::BUFFERS, mine = SLOTS == 2 ? it & 1 : 0;
+                ok = wait(p_full + buf, (it / C::BUFFERS) & 1) && wait(v_full + stage, (it / C::V_STAGES) & 1);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 if (ptx::elect_one()) {
@@ -675,7 +669,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
 #pragma unroll
                         for (int term = 0; term < 2; ++term)
                             ptx::tc_mma_f16_ts(o, w + 32 * (k >> 1) + 16 * term + 8 * (k & 1), v + (uint64_t)((k * 2048) >> 4), o_desc,
-                                               j >= GROUPS || k > 0 || term > 0);
+                                               j >= SLOTS || k > 0 || term > 0);
                     ptx::tc_commit(v_empty + stage);
                     ptx::tc_commit(o_done + mine);
                     if (j + 1 == n) ptx::tc_commit(unit_done);
