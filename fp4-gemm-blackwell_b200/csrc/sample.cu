@@ -17,8 +17,9 @@
 // one logit: its mass is its count times one weight, no element needs an
 // exponential, and a place in it is a place among equal logits, found by
 // counting.  Where a bin has more bits (FP16, FP32, and the logits nearest to
-// zero), elements add their weights to it, and the bin at hand is split again,
-// 8 bits at a time, until all its logits are one.
+// zero), elements add their weights to it, and the bin at hand is looked into: up to 512
+// candidates are listed and ranked one by one, more are split 8 bits at a time,
+// until they are few or all one logit.
 //
 // Bins.  bits 16 up of the logit as FP32: sign, exponent, 7 bits.  The weights
 // that matter lie within 46 of the maximum (e^-46 * 2^32 is below 2^-33, and u
@@ -27,13 +28,22 @@
 // them, and what lies below the range is in none.
 //
 // Sums.  Which token it is turns on sums over the whole row that lie next to a
-// border, so they are exact: a weight is exp() in FP64, rounded once to a whole
-// multiple of 2^-bits, bits the most that cannot overflow 64 (44 at 2^18
-// tokens), and sums of these do not depend on their order.
+// border, so they are exact: a weight is an exponential in FP64 (to about 1e-14),
+// rounded once to a whole multiple of 2^-bits, bits the most that cannot overflow
+// 64 (44 at 2^18 tokens), and sums of these do not depend on their order.
 //
 // A row belongs to a cluster of 1 to 8 CTAs, as many as give all rows' CTAs a
 // place on the GPU at once; each counts a slice, then merges its share of the
 // bins over distributed shared memory into the first CTA's, which walks them.
+// (Twice as many CTAs as fit at once: 64 x 131072 49 us where one wave takes 33.)
+//
+// Measured on B200, BF16: 256 x 131072 90 us, of which the bytes would take 10. The
+// row's phases follow one another in all CTAs alike: the maximum 5 us, the counting
+// 26 (an atomic of shared memory takes a warp 6 cycles, whose lanes meet in banks
+// 3 to 4 deep), the token's place by another reading 9, the rest waits: 4000
+// weights in FP64, scans, questions. 64 x 131072 33 us, 1 x 32768 15 (eight CTAs, five
+// meetings of the cluster of 0.5 us, three questions); FP32 with all filters, 7 x
+// 100003, 42 us (an exponential and two atomics an element, three lists).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -9,12 +9,17 @@ linear and the output linear when a model answers token by token.
         .append_qkv(q, k, v, positions, slots, rope)    norm + rotation + write, one pass; returns the queries
         .read(slots)                                    keys and values back in BF16
     decode_attention(q, cache, page_table, seq_lens)    one new token a sequence, split over the cache's length
+    shared_prefix_attention(q, cache, prefix_table, prefix_lens, page_table, seq_lens)
+                                                        the same where sequences share a prefix, which is read once
+    block_norm(x, residual, weight, ...)                norm after a block, gate, residual, norm before the next, one pass
+    sample(logits, u, temperature, top_k, top_p, min_p) the next tokens, from given uniform numbers
 
 (The linears' own form for few rows is ``fp4_gemm.fp4_cached_gemv``.)  Tensors are BF16 on one CUDA device; work is queued
 on PyTorch's current stream and nothing synchronises, so a decode step can be captured in a CUDA graph.  Inference only,
 like the rest of the library: no gradients.  Slots, positions, page tables and lengths live on the GPU; one out of
 range is never followed and shows in ``fp4_gemm.device_error()``: 11 a slot (nothing written, zeros read), 12 a position (no
-rotation), 13 a page (its keys count as rows of zeros: score 0, value 0) or a length (clamped to the table's pages).
+rotation), 13 a page (its keys count as rows of zeros: score 0, value 0) or a length (clamped to the table's pages).  14 there
+means that shared_prefix_attention's kernel gave up a wait: its results are not valid.
 """
 
 import ctypes
