@@ -548,7 +548,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         of those the ones with w >= min_p                      (0 or less: all; the first always),
 
     and the token is the first with which more than u of the kept ones' sum is reached.  A temperature of 0 gives the largest
-    logit's first index.  The sums are exact to 2^-44 and better of the largest weight, so the same call gives the same tokens.
+    logit's first index.  Weights are whole multiples of 2^-44 of the largest (vocabularies up to 2^18; one bit less for each
+    doubling) and their sums exact, so the same call gives the same tokens.
 
     Returns int64 [B], -1 for a row without candidates; with return_prob=True also fp32 [B], the share of the kept ones' sum
     that the token has (1 at temperature 0, 0 where there is none).
