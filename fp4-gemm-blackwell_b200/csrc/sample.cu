@@ -39,9 +39,9 @@
 //
 // Measured on B200, BF16: 256 x 131072 90 us, of which the bytes would take 10. The
 // row's phases follow one another in all CTAs alike: the maximum 5 us, the counting
-// 26 (an atomic of shared memory takes a warp 6 cycles, whose lanes meet in banks
-// 3 to 4 deep), the token's place by another reading 9, the rest waits: 4000
-// weights in FP64, scans, questions. 64 x 131072 33 us, 1 x 32768 15 (eight CTAs, five
+// 26 (42 instructions for 32 logits in all, half the issue slots in use, waits for
+// instructions among the rest), the token's place by another reading 9, then waits:
+// 4000 weights in FP64, scans, questions. 64 x 131072 33 us, 1 x 32768 15 (eight CTAs, five
 // meetings of the cluster of 0.5 us, three questions); FP32 with all filters, 7 x
 // 100003, 42 us (an exponential and two atomics an element, three lists).
 #include <cooperative_groups.h>
