@@ -72,20 +72,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     }
 }
 
-// The same for many threads: the timer, which is slow to read and slower for a
-// whole CTA at once, is looked at from the 64th attempt on only.
-__device__ __forceinline__ bool mbar_wait_many(uint64_t* bar, uint32_t parity) {
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 0) {
-            const uint64_t t = global_timer_ns();
-            if (t0 == 0) t0 = t;
-            else if (t - t0 > kSpinLimitNs) return false;
-        }
-    }
-}
-
 // ---------------------------------------------------------------- TMA / bulk copies
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y) {
     asm volatile(
