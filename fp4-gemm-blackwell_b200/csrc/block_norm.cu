@@ -254,8 +254,9 @@ __device__ __forceinline__ void norm_begin(Values<VEC>& r, const Pieces<VEC>& we
 template <int VEC, typename R, bool POST, bool GATE>
 __global__ void __launch_bounds__(Shape<VEC>::THREADS, Shape<VEC>::RESIDENT / Shape<VEC>::THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ Slots slots;
-    chain();
     const int ctas = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+    if (ctas > 1) ptx::cluster_start_arrive();
+    chain();
     const int warp = rank * (int)(blockDim.x >> 5) + (int)(threadIdx.x >> 5);
     const int at = (warp * 32 * Shape<VEC>::ITEMS + (int)(threadIdx.x & 31)) * VEC;  // the thread's first element
     const int each = (int)gridDim.x / ctas;  // rows at once
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(Shape<VEC>::THREADS, Shape<VEC>::RESIDENT / Sh
     };
     long row = blockIdx.x / ctas;
     load(row);
+    if (ctas > 1) ptx::cluster_start_wait();  // before the first sum goes to the other CTAs, behind the loads' starts
     for (; row < p.rows; row += each) {
         float factor = p.scale;  // what x is multiplied by besides the weights
         Pieces<VEC> weight;
