@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const long row = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+    if (ctas > 1) ptx::cluster_start_arrive();
     chain();
 
     // ---- this CTA's slice; a warp goes over a run of its own, 16 bytes a lane, in the order of the indices
@@ -368,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (lane == 0) s.warp_max[warp] = most;
     if (tid < 32) s.powers[tid] = exp2((double)tid / 32.0);
     __syncthreads();
+    if (ctas > 1) ptx::cluster_start_wait();  // the others have started: their shared memory is there
     if (warp == 0) {
         most = lane < kWarps ? s.warp_max[lane] : -INFINITY;
 #pragma unroll

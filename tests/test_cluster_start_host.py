@@ -52,3 +52,7 @@ def check(name):
 
 def test_block_norm():
     check("block_norm.cu")
+
+
+def test_sample():
+    check("sample.cu")
