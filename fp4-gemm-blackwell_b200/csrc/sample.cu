@@ -396,7 +396,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     {
         const uint32_t far = __float_as_uint(fmaf(-kReach, t, most)) & 0x7FFFFFFFu, top = __float_as_uint(most) & 0x7FFFFFFFu;
         const int octave = (int)(max(min(far, 0x7F800000u), top) >> 23);
-        r.lo = max(octave - (kOctaves - 1), 0) << 7;
+        // (an octave at least: zeros of both signs are in the bin between, as one)
+        r.lo = max(octave - (kOctaves - 1), 1) << 7;
     }
     const float least = p.min_p ? p.min_p[row] : p.min_p1;
     const bool has_least = least > 0.0f;

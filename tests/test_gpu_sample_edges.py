@@ -1,0 +1,46 @@
+"""fp4_decode.sample where its bins end: zeros of both signs under temperatures next to nothing."""
+import pytest
+import torch
+
+from tests.test_gpu_sample import TYPES, check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dec(cuda):
+    import fp4_decode
+    return fp4_decode
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1e-33, 1.6e-34, 1e-36, 1e-38, 1e-40])
+@pytest.mark.parametrize("v", [8, 256, 20000])
+def test_zeros_of_both_signs_are_equal(dec, cuda, dtype, temperature, v):
+    # all weights are 1, whatever the sign: token j for u in [j / V, (j + 1) / V)
+    b = min(v, 64)
+    at = torch.arange(b, device=cuda) * (v // b) + torch.arange(b, device=cuda) % (v // b)
+    u = ((at.double() + 0.5) / v).float()
+    logits = torch.zeros(b, v, device=cuda)
+    logits[:, ::2] = -0.0
+    logits[1::2, ::3] = 0.0
+    logits = logits.to(dtype)
+    assert check(dec, logits, u, temperature).tolist() == at.tolist()
+    check(dec, logits, u, temperature, 5, 1.0, 0.0)
+    check(dec, logits, u, temperature, 0, 0.3, 0.0)
+    check(dec, logits, u, temperature, v // 2 + 1, 0.7, 0.5)
+    assert check(dec, logits, u, temperature, 1).tolist() == [0] * b
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size,temperature", [(1e-36, 1e-36), (2.0 ** -112, 2.0 ** -114), (2.0 ** -126, 2.0 ** -128), (2.0 ** -133, 2.0 ** -133), (2.0 ** -120, 1e-40)])
+def test_logits_next_to_zero(dec, cuda, dtype, size, temperature):
+    # the bins' least magnitudes: small multiples of a small number (some of them subnormal) among zeros of both signs
+    g = torch.Generator(cuda).manual_seed(7)
+    b, v = 24, 3000
+    steps = torch.randint(-6, 4, (b, v), generator=g, device=cuda)
+    logits = (steps * size).to(dtype)
+    logits[steps == 0] *= torch.where(torch.rand(int((steps == 0).sum()), generator=g, device=cuda) < 0.5, -1.0, 1.0).to(dtype)
+    u = torch.rand(b, generator=g, device=cuda)
+    check(dec, logits, u, temperature)
+    check(dec, logits, u, temperature, 900, 0.8, 0.01)
