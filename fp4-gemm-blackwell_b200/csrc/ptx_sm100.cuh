@@ -72,6 +72,34 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     }
 }
 
+__device__ __forceinline__ void mbar_arrive_many(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+
+// Stages of a ring that copies of one warp fill: which of them may be under way, and in
+// which phase of their barriers.  The warp makes all of a barrier's arrivals itself, so
+// that waiting for its copies to land (before a CTA that gives up frees the memory they
+// go to) needs nobody else.
+struct Flights {
+    uint32_t stages = 0, phases = 0;
+    // Before the copies into `stage` start: `bytes` of them, in phase `phase & 1` of a barrier of `arrivals` (two or more).
+    __device__ __forceinline__ void begin(uint64_t* bars, int stage, uint32_t phase, uint32_t bytes, uint32_t arrivals, int lane) {
+        stages |= 1u << stage;
+        phases = (phases & ~(1u << stage)) | (phase & 1u) << stage;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bars + stage, bytes);  // (the bytes keep the phase from ending)
+            mbar_arrive_many(bars + stage, arrivals - 1);
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ bool land(uint64_t* bars, int count) {
+        bool ok = true;
+        for (int i = 0; i < count; ++i)
+            if (stages >> i & 1) ok = mbar_wait(bars + i, phases >> i & 1) && ok;
+        return ok;
+    }
+};
+
 // ---------------------------------------------------------------- TMA / bulk copies
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y) {
     asm volatile(

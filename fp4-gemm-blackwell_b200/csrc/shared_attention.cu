@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
         uint8_t* const pieces = smem + (value ? C::OFF_V : C::OFF_K);
         const uint8_t* const from = static_cast<const uint8_t*>(value ? p.cache.v : p.cache.k);
         bool ok = true;
-        int t = 0, stage = 0;
+        int stage = 0;
         uint32_t round = 0;  // of the stages, its low bit the barriers' phase
         auto row_of = [&](int page, int key) {  // in the cache; -1: none to read
             if (page >= 0 && page < p.cache.num_pages)
@@ -446,6 +446,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
             // Whole tiles of whole pages come as boxes that TMA swizzles; others row by row,
             // each of which is handed on when the next one's copies are under way.
             int pending = -1;
+            ptx::Flights flights;
             auto hand_on = [&]() {
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(full + pending);
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                     return lane < p.runs && j < walk.r1 && key < walk.valid ? table[key >> p.page_shift] : 0;
                 };
                 int next = look(walk.r0);
-                for (int j = walk.r0; j < walk.r1; ++j, ++t, stage = stage + 1 == stages ? (++round, 0) : stage + 1) {
+                for (int j = walk.r0; j < walk.r1; ++j, stage = stage + 1 == stages ? (++round, 0) : stage + 1) {
                     const int key0 = j * TK, entry = next;
                     next = look(j + 1);
                     uint8_t* const to = pieces + stage * C::PIECE;
@@ -475,13 +476,13 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
                         break;
                     }
                     if (boxes) {
-                        if (my == 0 && lane == 0) ptx::mbar_arrive_expect_tx(full + stage, C::PIECE);
-                        else ptx::mbar_arrive(full + stage);
-                        __syncwarp();
-                        if (my == 0 && lane < p.runs)
+                        if (my == 0) {  // one warp's alone
+                            flights.begin(full, stage, round, C::PIECE, 32 * C::FEEDERS, lane);
+                            if (lane < p.runs)
 #pragma unroll
-                            for (int n = 0; n < D / 64; ++n)
-                                ptx::tma_load_2d(to + n * (TK * 128) + lane * run * 128, value ? &p.v_map : &p.k_map, full + stage, 128 * n, first);
+                                for (int n = 0; n < D / 64; ++n)
+                                    ptx::tma_load_2d(to + n * (TK * 128) + lane * run * 128, value ? &p.v_map : &p.k_map, full + stage, 128 * n, first);
+                        }
                     } else {
 #pragma unroll 1
                         for (int r0 = my * ROWS; r0 < (my + 1) * ROWS; r0 += min(ROWS, 32)) {
@@ -508,8 +509,7 @@ __global__ void __launch_bounds__(PrefixCfg<KIND, D>::THREADS, 1) prefix_attenti
             }
             copy_wait<0>();
             if (ok && pending >= 0) hand_on();
-            if (!ok)  // (what is under way has to end before shared memory goes)
-                for (int i = max(t - stages, 0); i < t; ++i) ptx::mbar_wait(full + i % stages, (i / stages) & 1);
+            if (!ok) flights.land(full, stages);  // (what is under way has to end before shared memory goes)
         } else {
             // Through a ring of the warp's own: bulk copies of whole pages' runs, or row by row
             // where they are not whole.

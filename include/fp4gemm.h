@@ -106,9 +106,10 @@ const char* fp4b_last_error(void);
 
 /* Non-zero if a kernel on the current device gave up on a bounded wait: the
  * first code recorded (GEMM 1 producer, 2 MMA, 3 epilogue, 4 fused-quantize
- * wait; 5 quantizer ring; 7 / 8 the self-test below; 9 fp4b_mma_rate's final
- * wait; 10 fp4b_peer_barrier; 11 slot, 12 position, 13 page or length out of
- * range in a decode-side operator); clear != 0 resets it.
+ * wait; 5 quantizer ring; 7 / 8 / 15 the self-tests below; 9 fp4b_mma_rate's
+ * final wait; 10 fp4b_peer_barrier; 11 slot, 12 position, 13 page or length
+ * out of range in a decode-side operator; 14 fp4b_shared_attention);
+ * clear != 0 resets it.
  * Synchronises the device. */
 int fp4b_device_error(int clear);
 
@@ -119,6 +120,12 @@ int fp4b_device_error(int clear);
  * device error word and the kernel returns, leaving the context usable.
  * Asynchronous on `stream`; 0, or -1 bad `which`, -4 launch failure. */
 int fp4b_selftest_bounded_wait(int which, void* stream);
+
+/* Self-test of what comes after such a wait: a warp whose partner has stopped
+ * waits for the copies that it started into a ring of shared memory, which
+ * takes no longer than they do.  Records 15 in the device error word where
+ * they were not there.  Asynchronous on `stream`; 0, or -4 launch failure. */
+int fp4b_selftest_flights(void* stream);
 
 /* Measured tensor-pipe rate of the block-scaled NVFP4 MMA (no counterpart in
  * the reference): launches one CTA pair per two SMs whose even CTA issues
