@@ -343,6 +343,8 @@ FP4B_EXPORT int fp4b_block_norm(const fp4b_norm* call, void* stream) {
         if (c.rows < 0 || c.rows > (1 << 28)) why = "rows must be 0 to 2^28";
         else if (c.width <= 0 || c.width > kMaxWidth) why = "the width must be 1 to 32768";
         else if (c.rows > 0 && (!c.residual || !c.weight || !c.normed || (c.x && !c.residual_out))) why = "null tensor";
+        else if (c.x && c.residual_out == c.residual && c.rows > 1 && c.residual_stride != c.width)
+            why = "a residual that is updated in place must have its rows one after another";  // (a row's r' would lie over another's r)
         else if (!c.x && (c.post_weight || c.gate)) why = "a gate and a norm after the block need the block's output";
         else if (!whole(c.x, 2) || !whole(c.residual, c.residual_fp32 ? 4 : 2) || !whole(c.gate, 2) || !whole(c.weight, 2) ||
                  !whole(c.post_weight, 2) || !whole(c.normed, 2) || !whole(c.residual_out, c.residual_fp32 ? 4 : 2))

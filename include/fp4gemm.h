@@ -400,7 +400,8 @@ int fp4b_shared_attention(const fp4b_shared* call, void* stream);
  * residual, residual_out is not written.  x, gate, weights and normed are BF16,
  * residual and residual_out BF16 or, with residual_fp32, fp32.  Strides of rows
  * in elements (gate_stride 0: one gate for all rows); outputs contiguous, not
- * overlapping the inputs but that residual_out may be the residual itself.
+ * overlapping the inputs but that residual_out may be the residual itself
+ * where that is contiguous too (rows 1, or residual_stride the width).
  * width 1 to 32768. */
 typedef struct fp4b_norm {
     const void* x;
