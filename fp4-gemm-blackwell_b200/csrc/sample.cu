@@ -135,8 +135,8 @@ struct Run {
 };
 
 struct Row {
-    float max, scale;  // of the weights: 1 / T in FP64
-    double inv;
+    float max;
+    double inv;        // 1 / T
     int lo;            // leading bits of the smallest magnitude with a bin of its own
     double one;        // 2^bits
     const double* powers;  // 2^(i / 32), i < 32, in shared memory
@@ -199,8 +199,7 @@ struct Shared {
     u64 near_mass;  // of the bin between, where the others have one logit each
     uint32_t warp_count[kWarps];
     u64 warp_mass[kWarps];
-    uint32_t least_count;  // candidates with w >= min_p, of the row
-    u64 least_mass;
+    u64 least_mass;  // of the row's candidates with w >= min_p
     u64 list[kList];  // key and what the index lacks of 2^32 - 1: larger ones come first
     u64 list_weight[kList];
     uint32_t listed;
@@ -365,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         s.hist[i] = 0;
         if (kMasses) my_mass[i] = 0;
     }
-    if (tid == 0) s.near_mass = 0, s.least_count = 0, s.least_mass = 0, s.token = 0x7fffffff;
+    if (tid == 0) s.near_mass = 0, s.least_mass = 0, s.token = 0x7fffffff;
     if (lane == 0) s.warp_max[warp] = most;
     if (tid < 32) s.powers[tid] = exp2((double)tid / 32.0);
     __syncthreads();
@@ -477,13 +476,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
 
     // ---- counts (and masses) of the slice's bins
-    uint32_t kept = 0;
     u64 kept_mass = 0;
     auto heavy = [&](int bin, float l) {  // of a bin of more than one logit
         const double w = r.share(l);
         const u64 m = r.whole(w);
         atomicAdd(kMasses ? &my_mass[bin] : &s.near_mass, m);
-        if (has_least && w >= (double)least) ++kept, kept_mass += m;
+        if (has_least && w >= (double)least) kept_mass += m;
     };
     if constexpr (TYPE == kBf16) {
         // infinities and NaN lie above these
@@ -531,13 +529,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (me != 0) {
             if (has_least) {
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    kept += __shfl_xor_sync(0xffffffffu, kept, o);
-                    kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
-                }
-                if (lane == 0 && kept) atomicAdd(&home->least_count, kept), atomicAdd(&home->least_mass, kept_mass);
+                for (int o = 16; o > 0; o >>= 1) kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
+                if (lane == 0 && kept_mass) atomicAdd(&home->least_mass, kept_mass);
             }
-            kept = 0, kept_mass = 0;
+            kept_mass = 0;
         }
         cluster.sync();
     }
@@ -615,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         } else {
             const double w = r.share(r.run(i).logit());
             bin_mass[k] = i == kSide ? (there ? s.near_mass : 0) : r.whole(w) * n;
-            if (has_least && i != kSide && w >= (double)least) kept += n, kept_mass += bin_mass[k];
+            if (has_least && i != kSide && w >= (double)least) kept_mass += bin_mass[k];
         }
         my_count += n, my_total += bin_mass[k];
     }
@@ -623,11 +618,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     scan(s, my_before, my_mass_before);
     if (has_least) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            kept += __shfl_xor_sync(0xffffffffu, kept, o);
-            kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
-        }
-        if (lane == 0 && kept) atomicAdd(&s.least_count, kept), atomicAdd(&s.least_mass, kept_mass);
+        for (int o = 16; o > 0; o >>= 1) kept_mass += __shfl_xor_sync(0xffffffffu, kept_mass, o);
+        if (lane == 0 && kept_mass) atomicAdd(&s.least_mass, kept_mass);
     }
     if (tid == kThreads - 1) s.place.before = my_before + my_count, s.place.mass_before = my_mass_before + my_total;
     __syncthreads();
