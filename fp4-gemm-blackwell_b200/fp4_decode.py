@@ -528,6 +528,8 @@ def _setting(v, rows: int, dtype, what: str, index: int):
     if v.get_device() != index or v.numel() != rows:
         raise ValueError(f"{what} must be a number or {rows} numbers on cuda:{index}, got {tuple(v.shape)} on {v.device}")
     if v.dtype is not dtype:
+        if v.dtype is torch.int64 and dtype is torch.int32:
+            v = v.clamp(-1 << 31, (1 << 31) - 1)  # (a cast alone keeps the low 32 bits)
         v = v.to(dtype)
     if not v.is_contiguous():
         v = v.contiguous()

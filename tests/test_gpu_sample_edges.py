@@ -44,3 +44,13 @@ def test_logits_next_to_zero(dec, cuda, dtype, size, temperature):
     u = torch.rand(b, generator=g, device=cuda)
     check(dec, logits, u, temperature)
     check(dec, logits, u, temperature, 900, 0.8, 0.01)
+
+
+def test_wide_counts_are_not_cut(dec, cuda):
+    # k as int64, beyond 32 bits either way: more than the vocabulary is all of it, less than 0 too
+    g = torch.Generator(cuda).manual_seed(8)
+    k = torch.tensor([1, 5, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 1, 2 ** 32 + 1, 2 ** 32 + 5, 2 ** 62 + 3, -1, -2 ** 31 - 1, -2 ** 32 + 5, -2 ** 62 + 1], device=cuda)
+    b, v = len(k), 500
+    logits, u = torch.randn(1, v, generator=g, device=cuda).expand(b, v), torch.full((b,), 0.93, device=cuda)
+    whole = [1, 5] + [0] * (b - 2)
+    assert torch.equal(dec.sample(logits, u, 1.0, k), dec.sample(logits, u, 1.0, torch.tensor(whole, dtype=torch.int32, device=cuda)))
