@@ -789,6 +789,7 @@ FP4B_EXPORT int fp4b_shared_attention(const fp4b_shared* call, void* stream) {
     const long rows = why || c.batch == 0 ? 0 : (long)(c.batch / s.prefixes) * (c.q_heads / cache->kv_heads), tiles = (rows + kTileRows - 1) / kTileRows;
     if (!why && rows && (((long)s.prefix_width * cache->page_size + 63) / 64 + 1) * s.prefixes > 0x7fffffffL / (cache->kv_heads * tiles))
         why = "more than 2^31 tiles of 64 keys in one call";
+    if (!why && need < 0) why = "no device, or one beyond those that the library knows";
     if (why) {
         set_last_error("fp4b_shared_attention: %s", why);
         return -1;
