@@ -228,6 +228,17 @@ __device__ __forceinline__ void scan(Shared& s, uint32_t& count, u64& mass) {
     count -= c0, mass -= m0;
 }
 
+// Adds to a sum in shared memory by its halves: where many threads meet at one sum (equal
+// logits, zeros of a mask or of a padded vocabulary) an addition of 64 bits, which is a loop
+// of comparisons and exchanges, goes round once for each of them.  (256 x 131072, all logits
+// equal: FP32 16.7 ms so, 0.94 by halves; half of BF16 logits zeros 8.2 and 0.40.)
+__device__ __forceinline__ void add_mass(u64* at, u64 m) {
+    uint32_t* const half = reinterpret_cast<uint32_t*>(at);
+    const uint32_t low = (uint32_t)m, old = atomicAdd(half, low);
+    const uint32_t high = (uint32_t)(m >> 32) + (old + low < low ? 1u : 0u);
+    if (high) atomicAdd(half + 1, high);
+}
+
 enum Kind { kByCount, kByMassBefore, kByMassWith };
 
 // The question of one crossing.  kByCount: the last of the first k.
@@ -476,11 +487,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
 
     // ---- counts (and masses) of the slice's bins
-    u64 kept_mass = 0;
+    u64 kept_mass = 0, near_mass = 0;
+    uint32_t near_count = 0, zeros = 0;  // (zeros, which a mask or a padded vocabulary has many of, share one weight)
     auto heavy = [&](int bin, float l) {  // of a bin of more than one logit
         const double w = r.share(l);
         const u64 m = r.whole(w);
-        atomicAdd(kMasses ? &my_mass[bin] : &s.near_mass, m);
+        if (kMasses) add_mass(&my_mass[bin], m);
+        else near_mass += m, ++near_count;
         if (has_least && w >= (double)least) kept_mass += m;
     };
     if constexpr (TYPE == kBf16) {
@@ -494,9 +507,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 const bool minus = h & 0x8000;
                 if (k >= 0) {
                     if (k < (minus ? most_minus : most_plus)) atomicAdd(&s.hist[minus ? kSide + 1 + k : kSide - 1 - k], 1u);
+                } else if ((h & 0x7FFF) == 0) {
+                    ++zeros;
                 } else {
-                    atomicAdd(&s.hist[kSide], 1u);
-                    heavy(kSide, __uint_as_float(tidy((uint32_t)h << 16)));
+                    heavy(kSide, __uint_as_float((uint32_t)h << 16));
                 }
             }
         });
@@ -506,12 +520,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             for (int e = 0; e < PER; ++e) {
                 const uint32_t b = bits(v, e);
                 if (b == 0xFF800000u) continue;
+                if (b == 0u) {
+                    ++zeros;
+                    continue;
+                }
                 const int bin = r.bin(b);
                 if (bin < 0) continue;
                 atomicAdd(&s.hist[bin], 1u);
                 heavy(bin, __uint_as_float(b));
             }
         });
+    }
+    if (zeros + near_count) {
+        const double w = r.share(0.0f);
+        const u64 m = r.whole(w) * zeros;
+        if (has_least && w >= (double)least) kept_mass += m;
+        atomicAdd(&s.hist[kSide], zeros + near_count);
+        add_mass(kMasses ? &my_mass[kSide] : &s.near_mass, near_mass + m);
     }
     if (ctas > 1) cluster.sync();
     else __syncthreads();
@@ -553,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 if (part > 255) continue;
                 if (run.size > 16 && r.bin(b) != kSide) continue;  // (the bin between is less than its power of two)
                 atomicAdd(&s.sub_count[part], 1u);
-                atomicAdd(&s.sub_mass[part], r.weight(__uint_as_float(b)));
+                add_mass(&s.sub_mass[part], r.weight(__uint_as_float(b)));
             }
         });
         cluster.sync();

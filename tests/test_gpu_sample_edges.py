@@ -54,3 +54,36 @@ def test_wide_counts_are_not_cut(dec, cuda):
     logits, u = torch.randn(1, v, generator=g, device=cuda).expand(b, v), torch.full((b,), 0.93, device=cuda)
     whole = [1, 5] + [0] * (b - 2)
     assert torch.equal(dec.sample(logits, u, 1.0, k), dec.sample(logits, u, 1.0, torch.tensor(whole, dtype=torch.int32, device=cuda)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_logits_in_one_bin_take_no_time_of_their_own(dec, cuda, dtype):
+    # zeros (a padded vocabulary, a mask by multiplication) and equal or nearly equal logits meet at one sum in shared memory:
+    # the tokens are right, and a row takes a few times an ordinary one's time, not a hundred times
+    g = torch.Generator(cuda).manual_seed(9)
+    b, v = 256, 65536
+    ordinary = (2.0 * torch.randn(b, v, generator=g, device=cuda) - 2.0).to(dtype)
+    zeros = ordinary.masked_fill(torch.rand(b, v, generator=g, device=cuda) < 0.5, 0.0)
+    close = (20.0 + 1e-3 * torch.randn(b, v, generator=g, device=cuda)).to(dtype)
+    equal = torch.full((b, v), 3.0, device=cuda).to(dtype)
+    u = torch.rand(b, generator=g, device=cuda)
+
+    def time(logits):
+        times = []
+        for _ in range(4):
+            began, ended = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda._sleep(1_000_000)
+            began.record()
+            for _ in range(3):
+                dec.sample(logits, u, 0.8, 0, 0.95)
+            ended.record()
+            torch.cuda.synchronize()
+            times.append(began.elapsed_time(ended))
+        return min(times)
+
+    usual = time(ordinary)
+    for what, logits in (("zeros", zeros), ("close", close), ("equal", equal)):
+        check(dec, logits[:8], u[:8], 0.8, what=what)
+        check(dec, logits[:8], u[:8], 0.8, 1000, 0.95, 0.01, what=what)
+        took = time(logits)
+        assert took < 15 * usual, (what, took, usual)
