@@ -19,11 +19,11 @@
 // rows do not start on 16 bytes or the width is not a multiple of 8, four of two or
 // eight single ones.
 //
-// Measured on B200 (copy bandwidth 6.57 TB/s): 8192 x 2880 with both norms 31.3 us =
-// 6.0 TB/s (each row by a CTA of its own, loads not ahead: 37.6; rows through a ring
+// Measured on B200 (copy bandwidth 6.57 TB/s): 8192 x 2880 with both norms 31.1 us =
+// 6.1 TB/s (each row by a CTA of its own, loads not ahead: 37.6; rows through a ring
 // of bulk copies in shared memory: 49), 1024 x 16384 27.9, 1021 x 5003 in single
 // elements 20 us = 3.6 TB/s, bound by their instructions (1021 x 5004 in pairs 13.9),
-// 33 x 16384 4.1 and 1 x 2880 2.2, launches and a chain of waits.
+// 33 x 16384 4.1 and 1 x 2880 1.8, launches and a chain of waits.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -40,10 +40,11 @@
 // Measured on B200, BF16: 256 x 131072 90 us, of which the bytes would take 10. The
 // row's phases follow one another in all CTAs alike: the maximum 5 us, the counting
 // 26 (42 instructions for 32 logits in all, half the issue slots in use, waits for
-// instructions among the rest), the token's place by another reading 9, then waits:
-// 4000 weights in FP64, scans, questions. 64 x 131072 33 us, 1 x 32768 15 (eight CTAs, five
-// meetings of the cluster of 0.5 us, three questions); FP32 with all filters, 7 x
-// 100003, 42 us (an exponential and two atomics an element, three lists).
+// instructions among the rest), the token's place by another reading 9; what the 4097
+// weights in FP64, the scans and the questions take of the rest was not measured apart.
+// 64 x 131072 33 us, 1 x 32768 15 (eight CTAs, five meetings of the cluster of 0.5 us,
+// three questions); FP32 with all filters, 7 x 100003, 42 us (an exponential and three
+// atomics an element, three lists). 256 x 131072 of FP16 194 us, of FP32 223.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -140,7 +141,7 @@ struct Row {
     int lo;            // leading bits of the smallest magnitude with a bin of its own
     double one;        // 2^bits
     const double* powers;  // 2^(i / 32), i < 32, in shared memory
-    // Weights: of the largest 1.  exp(x) = 2^(n / 32) exp(y), n the nearest whole number
+    // Weights: of the largest 1, by a table-driven exponential (Tang's method).  exp(x) = 2^(n / 32) exp(y), n the nearest whole number
     // to 32 x / ln 2, |y| <= ln 2 / 64, exp(y) by its series up to y^5 (the next term is
     // below 3e-15): to within about 1e-14, with a third of the library's instructions.
     __device__ __forceinline__ double share(float l) const {

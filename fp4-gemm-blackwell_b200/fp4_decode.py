@@ -10,7 +10,7 @@ linear and the output linear when a model answers token by token.
         .read(slots)                                    keys and values back in BF16
     decode_attention(q, cache, page_table, seq_lens)    one new token a sequence, split over the cache's length
     shared_prefix_attention(q, cache, prefix_table, prefix_lens, page_table, seq_lens)
-                                                        the same where sequences share a prefix, which is read once
+                                                        the same where sequences share a prefix, read together
     block_norm(x, residual, weight, ...)                norm after a block, gate, residual, norm before the next, one pass
     sample(logits, u, temperature, top_k, top_p, min_p) the next tokens, from given uniform numbers
 
@@ -401,10 +401,11 @@ def shared_prefix_attention(q: torch.Tensor, cache: PagedKVCache, prefix_table: 
     """
     ``decode_attention`` of sequences that share prefixes: one system prompt before all, or several answers to each prompt.
 
-    Each of the G prefixes is read once for all its sequences: prefix_table [G, W0] int32 and prefix_lens [G] int32 hold its
-    pages and length, and sequence b of q's B (a multiple of G) belongs to prefix b // (B // G).  page_table [B, W] and
-    seq_lens [B] are the sequence's own keys behind the prefix, on pages of their own from their first on; either length may
-    be 0.  One softmax goes over both.  q, scale, sinks, the result and its precision as in ``decode_attention`` (no window).
+    Each of the G prefixes is read once for every 128 of its rows (its sequences times a key head's query heads) instead of
+    once a sequence: prefix_table [G, W0] int32 and prefix_lens [G] int32 hold its pages and length, and sequence b of q's B
+    (a multiple of G) belongs to prefix b // (B // G).  page_table [B, W] and seq_lens [B] are the sequence's own keys behind
+    the prefix, on pages of their own from their first on; either length may be 0.  One softmax goes over both.  q, scale,
+    sinks, the result and its precision as in ``decode_attention`` (no window).
 
     It pays from a few sequences a prefix on; decode_attention over tables that repeat the prefix's pages gives the same.
     """

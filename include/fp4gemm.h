@@ -378,7 +378,8 @@ int fp4b_decode_attention(const fp4b_decode* call, void* stream);
  * prefix_lens[b / (batch / prefixes)] keys found through that row of
  * prefix_table (int32, row stride prefix_stride, prefix_width entries), then its
  * own as own.seq_lens and own.page_table say (own.window has to be 0), in one
- * softmax.  Every prefix is read once for all its sequences.  own.workspace:
+ * softmax.  Every prefix is read once for each 128 rows (its sequences times
+ * the query heads of a key head).  own.workspace:
  * fp4b_shared_attention_workspace bytes, as for fp4b_decode_attention.  A wait
  * inside the kernel that gives up (after 2 s) is recorded as 14 in the device
  * error word. */
